@@ -228,6 +228,104 @@ SSM_API size_t ssm_rmsnorm_workspace_bytes(const ssm_norm_params_t* p);
 SSM_API int ssm_rmsnorm_fwd(const ssm_norm_params_t* p, ssm_stream_t stream);
 SSM_API int ssm_rmsnorm_bwd(const ssm_norm_params_t* p, ssm_stream_t stream);
 
+/* ---- dropout with an activation and a residual (selectssm.py:355-362) ----
+ * y = residual + act(drop(x)) over rows of `dim` elements, and its gradient
+ * dx = drop(dy * act'(drop(x))).  drop() zeroes an element with probability
+ * drop / 65536 and multiplies the kept ones by 65536 / (65536 - drop).  Its
+ * mask is a function of (seed, offset, row, column) alone and is not stored:
+ * column c of row r takes the 16 bits number c % 8 of the 128 bits that
+ * Philox4x32-10 gives for the counter (r * ceil(dim / 8) + c / 8, offset)
+ * under the key seed, and is kept when they are >= drop.  A dropped element
+ * contributes act(0) and no gradient, whatever x holds there.  */
+typedef struct ssm_dropout_params {
+  int64_t rows;
+  int32_t dim;                          /* columns, >= 1 */
+  int32_t dtype;                        /* x, residual, y, dy, dx */
+  int32_t act;                          /* ssm_act */
+  int32_t drop;                         /* 0 .. 65536 */
+  uint64_t seed, offset;
+  const uint64_t* rng;                  /* device {seed, offset} used instead of the two above, or NULL */
+  int64_t x_stride, res_stride, dy_stride; /* row strides in elements, 0 = dim; y and dx are dense */
+  const void* x;                        /* backward: may be NULL when act is SSM_ACT_NONE */
+  const void* residual;                 /* or NULL */
+  void* y;
+  const void* dy;
+  void* dx;
+} ssm_dropout_params_t;
+
+SSM_API int ssm_dropout_act_fwd(const ssm_dropout_params_t* p, ssm_stream_t stream);
+SSM_API int ssm_dropout_act_bwd(const ssm_dropout_params_t* p, ssm_stream_t stream);
+
+/* ---- group norm with an activation, channels last ----
+ * flax.linen.GroupNorm of BidirectionalMamba (selectssm.py:306-313, norm_type
+ * "group") over x (batch, seqlen, dim): mean and variance of each of `groups`
+ * runs of dim / groups channels over the whole sequence, then
+ * y = act((x - mean) * rstd * scale + bias).  The backward writes dx, dscale
+ * and dbias; every sum is formed in a fixed order.  */
+typedef struct ssm_group_norm_params {
+  int64_t batch, seqlen;
+  int32_t dim, groups;                  /* groups divides dim */
+  int32_t dtype;                        /* x, y, dy, dx (dense) */
+  int32_t act;                          /* ssm_act */
+  float eps;                            /* flax default 1e-6 */
+  const void* x;
+  const float* scale;                   /* (dim) or NULL: ones */
+  const float* bias;                    /* (dim) or NULL: zeros */
+  void* y;
+  float* stats;                         /* (batch, groups, 2) mean and rstd: forward output, backward input */
+  const void* dy;
+  void* dx;
+  float* dscale;                        /* (dim) */
+  float* dbias;                         /* (dim) */
+  void* workspace;                      /* 256-byte aligned; the queries below give its bytes */
+  size_t workspace_bytes;
+} ssm_group_norm_params_t;
+
+SSM_API size_t ssm_group_norm_fwd_workspace_bytes(const ssm_group_norm_params_t* p);
+SSM_API size_t ssm_group_norm_bwd_workspace_bytes(const ssm_group_norm_params_t* p);
+SSM_API int ssm_group_norm_act_fwd(const ssm_group_norm_params_t* p, ssm_stream_t stream);
+SSM_API int ssm_group_norm_act_bwd(const ssm_group_norm_params_t* p, ssm_stream_t stream);
+
+/* ---- dense layer with its epilogue (selectssm.py:345-362) ----
+ * y = residual + act(drop(x W + bias)), x (rows, fin), W (fin, fout) as Flax's
+ * Dense kernel, drop() as in ssm_dropout_act_fwd over rows of fout columns.
+ * The backward writes those of dx, dkernel and dbias that are not NULL; the
+ * residual's gradient is dy itself.  Sums are held in fp32; with bf16 the
+ * operands of the products (x, W, and in the backward the gradient of the
+ * pre-activation) are bf16.  */
+typedef struct ssm_dense_params {
+  int64_t rows;
+  int32_t fin, fout;                    /* >= 1 */
+  int32_t dtype;                        /* x, kernel, residual, y, pre, dy, dx */
+  int32_t bias_dtype;                   /* bias, dbias */
+  int32_t dkernel_dtype;
+  int32_t act;                          /* ssm_act */
+  int32_t drop;                         /* 0 .. 65536 */
+  uint64_t seed, offset;
+  const uint64_t* rng;                  /* device {seed, offset} used instead of the two above, or NULL */
+  int64_t x_stride, res_stride, dy_stride; /* row strides in elements, 0 = dense; the rest is dense */
+  const void* x;
+  const void* kernel;                   /* (fin, fout) */
+  const void* bias;                     /* (fout) or NULL */
+  const void* residual;                 /* (rows, fout) or NULL */
+  void* y;
+  void* pre;                            /* (rows, fout) x W + bias: forward output (NULL: not written),
+                                           backward input, needed there unless act is SSM_ACT_NONE */
+  const void* dy;
+  void* dx;
+  void* dkernel;
+  void* dbias;
+  void* workspace;                      /* 256-byte aligned; the queries below give its bytes */
+  size_t workspace_bytes;
+  int32_t* status;                      /* optional device word: nonzero after a device-side
+                                           failure (bounded wait gave up)                 */
+} ssm_dense_params_t;
+
+SSM_API size_t ssm_dense_fwd_workspace_bytes(const ssm_dense_params_t* p);
+SSM_API size_t ssm_dense_bwd_workspace_bytes(const ssm_dense_params_t* p);
+SSM_API int ssm_dense_act_fwd(const ssm_dense_params_t* p, ssm_stream_t stream);
+SSM_API int ssm_dense_act_bwd(const ssm_dense_params_t* p, ssm_stream_t stream);
+
 /* Failure-path self-test: one tiny kernel waits, with the scan kernels'
  * bounded wait, on an mbarrier that nothing arrives on; after spin_limit polls
  * (1 .. 2^24) it writes SSM_ERR_TIMEOUT to *status (a device int32) and

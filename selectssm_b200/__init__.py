@@ -5,7 +5,10 @@ Public names follow the reference package (src/selectssm/__init__.py:1-2):
 ``BidirectionalMamba``; plus the fused op ``selective_scan`` and the
 conv preamble ``conv1d_act``.
 
-The PyTorch host layer (ops, modules, rcps) is imported on first use of one of
+``group_norm_act``, ``dropout_act`` and ``dense_act`` are the block's norm,
+dropout and dense layers with their epilogues.
+
+The PyTorch host layer (ops, block_ops, modules, rcps) is imported on first use of one of
 its names, so the JAX binding (``selectssm_b200.jax_ffi``) and the C-ABI loader
 (``selectssm_b200._lib``) import without PyTorch.
 """
@@ -17,6 +20,7 @@ __version__ = "0.1.0"
 _LAZY = {
     "conv1d_act": "ops", "dense_onto": "ops", "rmsnorm_residual": "ops", "selective_scan": "ops",
     "selective_scan_bidir": "ops", "ssm_chunked_scan": "ops", "ssm_recursive_scan": "ops", "ssm_scan": "ops",
+    "dense_act": "block_ops", "dropout_act": "block_ops", "group_norm_act": "block_ops",
     "BidirectionalMamba": "modules", "SelectiveSSM": "modules",
     "RCPSEmbedding": "rcps", "RCPSLMHead": "rcps", "RCPSNorm": "rcps", "RCPSWrapper": "rcps",
     "rc_conjugate": "rcps",

@@ -45,6 +45,10 @@ EXPORTED_SYMBOLS = (
     "ssm_rmsnorm_workspace_bytes", "ssm_rmsnorm_fwd", "ssm_rmsnorm_bwd", "ssm_selftest_wait_timeout",
     "ssm_bwd_bc_multicast", "ssm_bwd_workspace_bytes", "ssm_fwd_workspace_bytes",
     "ssm_selftest_lookback_timeout",
+    "ssm_dropout_act_fwd", "ssm_dropout_act_bwd",
+    "ssm_group_norm_fwd_workspace_bytes", "ssm_group_norm_bwd_workspace_bytes",
+    "ssm_group_norm_act_fwd", "ssm_group_norm_act_bwd",
+    "ssm_dense_fwd_workspace_bytes", "ssm_dense_bwd_workspace_bytes", "ssm_dense_act_fwd", "ssm_dense_act_bwd",
 )
 
 
@@ -96,6 +100,47 @@ class SSMNormParams(ctypes.Structure):
     ]
 
 
+class SSMDropoutParams(ctypes.Structure):
+    """Mirror of ``ssm_dropout_params_t``."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("act", ctypes.c_int32),
+        ("drop", ctypes.c_int32), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("rng", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64), ("res_stride", ctypes.c_int64), ("dy_stride", ctypes.c_int64),
+        ("x", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("y", ctypes.c_void_p), ("dy", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p),
+    ]
+
+
+class SSMGroupNormParams(ctypes.Structure):
+    """Mirror of ``ssm_group_norm_params_t``."""
+
+    _fields_ = [
+        ("batch", ctypes.c_int64), ("seqlen", ctypes.c_int64), ("dim", ctypes.c_int32), ("groups", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("act", ctypes.c_int32), ("eps", ctypes.c_float),
+        ("x", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("y", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p), ("dy", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("dscale", ctypes.c_void_p),
+        ("dbias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class SSMDenseParams(ctypes.Structure):
+    """Mirror of ``ssm_dense_params_t``."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("fin", ctypes.c_int32), ("fout", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32), ("dkernel_dtype", ctypes.c_int32), ("act", ctypes.c_int32),
+        ("drop", ctypes.c_int32), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("rng", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64), ("res_stride", ctypes.c_int64), ("dy_stride", ctypes.c_int64),
+        ("x", ctypes.c_void_p), ("kernel", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+        ("y", ctypes.c_void_p), ("pre", ctypes.c_void_p), ("dy", ctypes.c_void_p), ("dx", ctypes.c_void_p),
+        ("dkernel", ctypes.c_void_p), ("dbias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("status", ctypes.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -116,6 +161,7 @@ def load(path: str | None = None) -> ctypes.CDLL:
     P = ctypes.POINTER(SSMParams)
     CP = ctypes.POINTER(SSMConvParams)
     NP = ctypes.POINTER(SSMNormParams)
+    DP, GP, LP = (ctypes.POINTER(c) for c in (SSMDropoutParams, SSMGroupNormParams, SSMDenseParams))
     sigs = {
         "ssm_workspace_bytes": (ctypes.c_size_t, [P]),
         "ssm_states_elems": (ctypes.c_size_t, [P]),
@@ -131,6 +177,16 @@ def load(path: str | None = None) -> ctypes.CDLL:
         "ssm_rmsnorm_workspace_bytes": (ctypes.c_size_t, [NP]),
         "ssm_rmsnorm_fwd": (ctypes.c_int, [NP, ctypes.c_void_p]),
         "ssm_rmsnorm_bwd": (ctypes.c_int, [NP, ctypes.c_void_p]),
+        "ssm_dropout_act_fwd": (ctypes.c_int, [DP, ctypes.c_void_p]),
+        "ssm_dropout_act_bwd": (ctypes.c_int, [DP, ctypes.c_void_p]),
+        "ssm_group_norm_fwd_workspace_bytes": (ctypes.c_size_t, [GP]),
+        "ssm_group_norm_bwd_workspace_bytes": (ctypes.c_size_t, [GP]),
+        "ssm_group_norm_act_fwd": (ctypes.c_int, [GP, ctypes.c_void_p]),
+        "ssm_group_norm_act_bwd": (ctypes.c_int, [GP, ctypes.c_void_p]),
+        "ssm_dense_fwd_workspace_bytes": (ctypes.c_size_t, [LP]),
+        "ssm_dense_bwd_workspace_bytes": (ctypes.c_size_t, [LP]),
+        "ssm_dense_act_fwd": (ctypes.c_int, [LP, ctypes.c_void_p]),
+        "ssm_dense_act_bwd": (ctypes.c_int, [LP, ctypes.c_void_p]),
         "ssm_selftest_wait_timeout": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p]),
         "ssm_selftest_lookback_timeout": (ctypes.c_int, [ctypes.POINTER(SSMParams), ctypes.c_uint32, ctypes.c_void_p]),
         "ssm_strerror": (ctypes.c_char_p, [ctypes.c_int]),

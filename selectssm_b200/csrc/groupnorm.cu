@@ -1,0 +1,556 @@
+// Group norm with an activation over channels-last x (batch, seqlen, dim)
+// (src/selectssm/selectssm.py:306-313, norm_type "group"; flax.linen.GroupNorm):
+// for each batch row and each run of dim / groups channels
+//
+//   mean, var over (seqlen, the run's channels);  rstd = 1 / sqrt(var + eps)
+//   xhat = (x - mean) rstd,  y = act(xhat scale + bias)
+// and with du = dy act'(xhat scale + bias), g = du scale, m the mean over the group
+//   dx = rstd (g - m(g) - xhat m(g xhat)),  dscale = sum du xhat,  dbias = sum du.
+//
+// All sums a group needs follow from sums per channel: m(g) is the sum over its
+// channels of scale * (sum of du), m(g xhat) of scale * (sum of du xhat).  So a
+// thread keeps a fixed run of channels, walks down the sequence, and no
+// group's width matters to the inner loops.
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+#include "vec8.cuh"
+#include "../../include/selectssm_b200.h"
+
+namespace ssm {
+
+int launch_error(const char* where, cudaError_t e);  // scan.cu
+int bind_device(const void* ptr);                      // scan.cu
+
+constexpr int kGnThreads = 256;
+
+// How a pass cuts (batch, seqlen, dim): column tiles of `ct` vectors of V
+// channels, `rt` rows at a time, chunks of `chunk` rows.
+struct GnGeom {
+  int64_t L;
+  int32_t B, D, G, cg;
+  int32_t nvec, ct, tiles, rt;
+  int32_t chunks;
+  int64_t chunk;
+};
+
+struct GnArgs {
+  GnGeom g;
+  float eps;
+  const void* x;
+  const void* dy;
+  const float* scale;
+  const float* bias;
+  float* stats;      // (B, G, 2) mean, rstd
+  float2* part;      // (B, chunks, D) per-channel partials: forward (mean, M2), backward (sum du, sum du xhat)
+  float2* sums;      // backward: (B, D) the same, summed over the chunks
+  float2* means;     // backward: (B, G) m(g), m(g xhat)
+  void* out;         // y or dx
+  float* dscale;
+  float* dbias;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
+  if constexpr (V == 8) load8(p, v);
+  else v[0] = Cvt<T>::to_f(*p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_v(T* p, const float (&v)[V]) {
+  if constexpr (V == 8) store8(p, v);
+  else *p = Cvt<T>::from_f(v[0]);
+}
+
+// Per-channel constants of a thread's V channels.
+template <int V>
+struct GnChan {
+  float mean[V], rstd[V], scale[V], bias[V];
+  __device__ __forceinline__ void load(const GnArgs& p, int b, int c0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 s = reinterpret_cast<const float2*>(p.stats)[(int64_t)b * p.g.G + (c0 + i) / p.g.cg];
+      mean[i] = s.x;
+      rstd[i] = s.y;
+      scale[i] = p.scale ? p.scale[c0 + i] : 1.f;
+      bias[i] = p.bias ? p.bias[c0 + i] : 0.f;
+    }
+  }
+};
+
+struct GnPlace {
+  int b, chunk, vec, r0;
+  bool active;
+  int64_t l0, l1;
+};
+__device__ __forceinline__ GnPlace gn_place(const GnGeom& g, bool reversed) {
+  GnPlace q;
+  const unsigned n = gridDim.x * gridDim.y;
+  unsigned id = blockIdx.y * gridDim.x + blockIdx.x;  // (batch, chunk)
+  if (reversed) id = n - 1 - id;
+  q.b = id / g.chunks;
+  q.chunk = id - q.b * g.chunks;
+  q.vec = blockIdx.z * g.ct + threadIdx.x % g.ct;
+  q.r0 = threadIdx.x / g.ct;
+  q.active = q.r0 < g.rt && q.vec < g.nvec;
+  q.l0 = q.chunk * g.chunk;
+  q.l1 = min(q.l0 + g.chunk, g.L);
+  return q;
+}
+
+// Mean and sum of squared deviations per channel of a chunk.  Rows come in
+// batches of kRows: each batch's mean and deviations are formed from its own
+// values and merged into the running pair with Chan's update, so no large mean
+// is ever subtracted from a sum of squares.
+template <typename T, int V>
+__global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(const GnArgs p) {
+  extern __shared__ float sm[];
+  constexpr int kRows = 8;
+  const GnGeom& g = p.g;
+  const GnPlace q = gn_place(g, false);
+  const T* x = static_cast<const T*>(p.x) + (int64_t)q.b * g.L * g.D + (int64_t)q.vec * V;
+  float mean[V], m2[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) mean[i] = m2[i] = 0.f;
+  float n = 0.f;
+  if (q.active) {
+    int64_t l = q.l0 + q.r0;
+    for (; l + (int64_t)(kRows - 1) * g.rt < q.l1; l += (int64_t)kRows * g.rt) {
+      float v[kRows][V];
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) load_v<T, V>(x + (l + (int64_t)k * g.rt) * g.D, v[k]);
+      const float nn = n + kRows, w = kRows / nn;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float s = 0.f, d2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) s += v[k][i];
+        const float bm = s * (1.f / kRows);
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+          const float d = v[k][i] - bm;
+          d2 = fmaf(d, d, d2);
+        }
+        const float delta = bm - mean[i];
+        mean[i] = fmaf(delta, w, mean[i]);
+        m2[i] += d2 + delta * delta * n * w;
+      }
+      n = nn;
+    }
+    for (; l < q.l1; l += g.rt) {
+      float v[V];
+      load_v<T, V>(x + l * g.D, v);
+      n += 1.f;
+      const float w = 1.f / n;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float delta = v[i] - mean[i];
+        mean[i] = fmaf(delta, w, mean[i]);
+        m2[i] = fmaf(delta, v[i] - mean[i], m2[i]);
+      }
+    }
+  }
+  // merge the rt row lanes of each channel in order
+  const int width = g.ct * V, mine = (threadIdx.x % g.ct) * V;
+  float *smean = sm, *sm2 = sm + g.rt * width, *sn = sm + 2 * g.rt * width;
+  if (q.r0 < g.rt) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      smean[q.r0 * width + mine + i] = mean[i];
+      sm2[q.r0 * width + mine + i] = m2[i];
+    }
+    if (threadIdx.x % g.ct == 0) sn[q.r0] = q.active ? n : 0.f;
+  }
+  __syncthreads();
+  const float total = (float)(q.l1 - q.l0);
+  for (int c = threadIdx.x; c < width; c += kGnThreads) {
+    const int ch = blockIdx.z * width + c;
+    if (ch >= g.D) break;
+    float s = 0.f;
+    for (int r = 0; r < g.rt; ++r) s = fmaf(sn[r], smean[r * width + c], s);
+    const float mu = s / total;
+    float d2 = 0.f;
+    for (int r = 0; r < g.rt; ++r) {
+      const float d = smean[r * width + c] - mu;
+      d2 += sm2[r * width + c] + sn[r] * d * d;
+    }
+    p.part[((int64_t)q.b * g.chunks + q.chunk) * g.D + ch] = make_float2(mu, d2);
+  }
+}
+
+__device__ __forceinline__ float block_sum(float v, float* buf) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0.f;
+  for (int w = 0; w < kGnThreads / 32; ++w) s += buf[w];
+  return s;
+}
+
+// mean and rstd of one group from its chunks' and channels' partials
+__global__ void __launch_bounds__(kGnThreads) gn_merge_kernel(const GnArgs p) {
+  __shared__ float buf[kGnThreads / 32];
+  const GnGeom& g = p.g;
+  const int grp = blockIdx.x % g.G, b = blockIdx.x / g.G;
+  const float2* part = p.part + (int64_t)b * g.chunks * g.D + grp * g.cg;
+  const int items = g.chunks * g.cg;
+  const float count = (float)g.L * (float)g.cg;
+  float s = 0.f;
+  for (int i = threadIdx.x; i < items; i += kGnThreads) {
+    const int ck = i / g.cg, c = i - ck * g.cg;
+    const float n = (float)(min((ck + 1) * g.chunk, g.L) - ck * g.chunk);
+    s = fmaf(n / count, part[(int64_t)ck * g.D + c].x, s);
+  }
+  const float mu = block_sum(s, buf);
+  float d2 = 0.f;
+  for (int i = threadIdx.x; i < items; i += kGnThreads) {
+    const int ck = i / g.cg, c = i - ck * g.cg;
+    const float n = (float)(min((ck + 1) * g.chunk, g.L) - ck * g.chunk);
+    const float2 v = part[(int64_t)ck * g.D + c];
+    d2 += v.y + n * (v.x - mu) * (v.x - mu);
+  }
+  const float var = block_sum(d2, buf) / count;
+  if (threadIdx.x == 0) reinterpret_cast<float2*>(p.stats)[blockIdx.x] = make_float2(mu, 1.f / sqrtf(var + p.eps));
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(const GnArgs p) {
+  constexpr int kRows = 4;
+  const GnGeom& g = p.g;
+  const GnPlace q = gn_place(g, true);
+  if (!q.active) return;
+  GnChan<V> c;
+  c.load(p, q.b, q.vec * V);
+  float a[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) a[i] = c.rstd[i] * c.scale[i];
+  const int64_t base = (int64_t)q.b * g.L * g.D + (int64_t)q.vec * V;
+  const T* x = static_cast<const T*>(p.x) + base;
+  T* y = static_cast<T*>(p.out) + base;
+  for (int64_t l = q.l0 + q.r0; l < q.l1; l += (int64_t)kRows * g.rt) {
+    float v[kRows][V];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k)
+      if (l + (int64_t)k * g.rt < q.l1) load_v<T, V>(x + (l + (int64_t)k * g.rt) * g.D, v[k]);
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (l + (int64_t)k * g.rt >= q.l1) break;
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[k][i] = act_f(fmaf(v[k][i] - c.mean[i], a[i], c.bias[i]), ACT);
+      store_v<T, V>(y + (l + (int64_t)k * g.rt) * g.D, v[k]);
+    }
+  }
+}
+
+// Sums over a chunk of du and du xhat per channel.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kGnThreads) gn_sums_kernel(const GnArgs p) {
+  extern __shared__ float sm[];
+  constexpr int kRows = 2;
+  const GnGeom& g = p.g;
+  const GnPlace q = gn_place(g, false);
+  float s1[V], s2[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+  if (q.active) {
+    GnChan<V> c;
+    c.load(p, q.b, q.vec * V);
+    const int64_t base = (int64_t)q.b * g.L * g.D + (int64_t)q.vec * V;
+    const T* x = static_cast<const T*>(p.x) + base;
+    const T* dy = static_cast<const T*>(p.dy) + base;
+    for (int64_t l = q.l0 + q.r0; l < q.l1; l += (int64_t)kRows * g.rt) {
+      float v[kRows][V], d[kRows][V];
+#pragma unroll
+      for (int k = 0; k < kRows; ++k)
+        if (l + (int64_t)k * g.rt < q.l1) {
+          load_v<T, V>(x + (l + (int64_t)k * g.rt) * g.D, v[k]);
+          load_v<T, V>(dy + (l + (int64_t)k * g.rt) * g.D, d[k]);
+        }
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        if (l + (int64_t)k * g.rt >= q.l1) break;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float xh = (v[k][i] - c.mean[i]) * c.rstd[i];
+          const float du = ACT ? d[k][i] * act_grad_f(fmaf(xh, c.scale[i], c.bias[i]), ACT) : d[k][i];
+          s1[i] += du;
+          s2[i] = fmaf(du, xh, s2[i]);
+        }
+      }
+    }
+  }
+  const int width = g.ct * V, mine = (threadIdx.x % g.ct) * V;
+  float *a1 = sm, *a2 = sm + g.rt * width;
+  if (q.r0 < g.rt) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      a1[q.r0 * width + mine + i] = s1[i];
+      a2[q.r0 * width + mine + i] = s2[i];
+    }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < width; c += kGnThreads) {
+    const int ch = blockIdx.z * width + c;
+    if (ch >= g.D) break;
+    float t1 = 0.f, t2 = 0.f;
+    for (int r = 0; r < g.rt; ++r) {
+      t1 += a1[r * width + c];
+      t2 += a2[r * width + c];
+    }
+    p.part[((int64_t)q.b * g.chunks + q.chunk) * g.D + ch] = make_float2(t1, t2);
+  }
+}
+
+// One group of one batch row: its channels' sums over the chunks (kept for
+// dscale and dbias) and the two means that dx needs.
+__global__ void __launch_bounds__(kGnThreads) gn_means_kernel(const GnArgs p) {
+  __shared__ float buf[kGnThreads / 32];
+  const GnGeom& g = p.g;
+  const int grp = blockIdx.x % g.G, b = blockIdx.x / g.G;
+  const float2* part = p.part + (int64_t)b * g.chunks * g.D;
+  float m1 = 0.f, m2 = 0.f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int c = grp * g.cg + warp; c < (grp + 1) * g.cg; c += kGnThreads / 32) {  // a warp per channel
+    float s1 = 0.f, s2 = 0.f;
+    for (int ck = lane; ck < g.chunks; ck += 32) {
+      const float2 v = part[(int64_t)ck * g.D + c];
+      s1 += v.x;
+      s2 += v.y;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+      s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+    }
+    if (lane == 0) {
+      p.sums[(int64_t)b * g.D + c] = make_float2(s1, s2);
+      const float w = p.scale ? p.scale[c] : 1.f;
+      m1 = fmaf(w, s1, m1);
+      m2 = fmaf(w, s2, m2);
+    }
+  }
+  const float t1 = block_sum(m1, buf), t2 = block_sum(m2, buf);
+  const float count = (float)g.L * (float)g.cg;
+  if (threadIdx.x == 0) p.means[blockIdx.x] = make_float2(t1 / count, t2 / count);
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kGnThreads) gn_dx_kernel(const GnArgs p) {
+  constexpr int kRows = 2;
+  const GnGeom& g = p.g;
+  const GnPlace q = gn_place(g, true);
+  if (!q.active) return;
+  GnChan<V> c;
+  c.load(p, q.b, q.vec * V);
+  float m1[V], m2[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float2 m = p.means[(int64_t)q.b * g.G + (q.vec * V + i) / g.cg];
+    m1[i] = m.x;
+    m2[i] = m.y;
+  }
+  const int64_t base = (int64_t)q.b * g.L * g.D + (int64_t)q.vec * V;
+  const T* x = static_cast<const T*>(p.x) + base;
+  const T* dy = static_cast<const T*>(p.dy) + base;
+  T* dx = static_cast<T*>(p.out) + base;
+  for (int64_t l = q.l0 + q.r0; l < q.l1; l += (int64_t)kRows * g.rt) {
+    float v[kRows][V], d[kRows][V];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k)
+      if (l + (int64_t)k * g.rt < q.l1) {
+        load_v<T, V>(x + (l + (int64_t)k * g.rt) * g.D, v[k]);
+        load_v<T, V>(dy + (l + (int64_t)k * g.rt) * g.D, d[k]);
+      }
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (l + (int64_t)k * g.rt >= q.l1) break;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float xh = (v[k][i] - c.mean[i]) * c.rstd[i];
+        const float du = ACT ? d[k][i] * act_grad_f(fmaf(xh, c.scale[i], c.bias[i]), ACT) : d[k][i];
+        v[k][i] = c.rstd[i] * (du * c.scale[i] - m1[i] - xh * m2[i]);
+      }
+      store_v<T, V>(dx + (l + (int64_t)k * g.rt) * g.D, v[k]);
+    }
+  }
+}
+
+// dscale and dbias: the batch rows' sums in order
+__global__ void gn_param_kernel(const GnArgs p) {
+  const int c = blockIdx.x * blockDim.x + threadIdx.x;
+  if (c >= p.g.D) return;
+  float s1 = 0.f, s2 = 0.f;
+  for (int b = 0; b < p.g.B; ++b) {
+    const float2 v = p.sums[(int64_t)b * p.g.D + c];
+    s1 += v.x;
+    s2 += v.y;
+  }
+  if (p.dbias) p.dbias[c] = s1;
+  if (p.dscale) p.dscale[c] = s2;
+}
+
+static int check_gn(const ssm_group_norm_params_t* p) {
+  if (!p) return SSM_ERR_NULL;
+  if (p->batch < 0 || p->seqlen < 0 || p->dim < 1 || p->groups < 1 || p->dim % p->groups || p->dim > (1 << 20) ||
+      p->batch > 65535 || p->seqlen > (1ll << 40) || p->act < SSM_ACT_NONE || p->act > SSM_ACT_RELU)
+    return SSM_ERR_SHAPE;
+  if (p->dtype != SSM_F32 && p->dtype != SSM_BF16) return SSM_ERR_DTYPE;
+  return SSM_OK;
+}
+
+static bool gn_vector(const ssm_group_norm_params_t* p) { return p->dim % 8 == 0; }
+
+static GnGeom gn_geom(const ssm_group_norm_params_t* p) {
+  GnGeom g;
+  g.B = (int)p->batch;
+  g.L = p->seqlen;
+  g.D = p->dim;
+  g.G = p->groups;
+  g.cg = p->dim / p->groups;
+  const int V = gn_vector(p) ? 8 : 1;
+  g.nvec = g.D / V;
+  g.tiles = (g.nvec + kGnThreads - 1) / kGnThreads;
+  g.ct = (g.nvec + g.tiles - 1) / g.tiles;
+  g.rt = kGnThreads / g.ct;
+  const int64_t want = 8 * 148;  // CTAs
+  const int64_t per_b = (want + (int64_t)g.B * g.tiles - 1) / ((int64_t)g.B * g.tiles);
+  int64_t chunk = (g.L + per_b - 1) / per_b;
+  const int64_t least = (int64_t)g.rt * 8;
+  chunk = chunk < least ? least : (chunk + least - 1) / least * least;
+  g.chunk = chunk;
+  g.chunks = (int)((g.L + chunk - 1) / chunk);
+  return g;
+}
+
+static size_t gn_round(size_t v) { return (v + 255) / 256 * 256; }
+static size_t gn_part_bytes(const GnGeom& g) { return gn_round((size_t)g.B * g.chunks * g.D * sizeof(float2)); }
+static size_t gn_sums_bytes(const GnGeom& g) { return gn_round((size_t)g.B * g.D * sizeof(float2)); }
+static size_t gn_means_bytes(const GnGeom& g) { return gn_round((size_t)g.B * g.G * sizeof(float2)); }
+
+template <typename T, int V, int ACT>
+static void gn_fwd_launch(const GnArgs& a, cudaStream_t s) {
+  const GnGeom& g = a.g;
+  const dim3 grid(g.chunks, g.B, g.tiles);
+  const size_t smem = (2 * (size_t)g.rt * g.ct * V + g.rt) * sizeof(float);
+  gn_stats_kernel<T, V><<<grid, kGnThreads, smem, s>>>(a);
+  gn_merge_kernel<<<g.B * g.G, kGnThreads, 0, s>>>(a);
+  gn_apply_kernel<T, V, ACT><<<grid, kGnThreads, 0, s>>>(a);
+  note_launches(3);
+}
+
+template <typename T, int V, int ACT>
+static void gn_bwd_launch(const GnArgs& a, cudaStream_t s) {
+  const GnGeom& g = a.g;
+  const dim3 grid(g.chunks, g.B, g.tiles);
+  const size_t smem = 2 * (size_t)g.rt * g.ct * V * sizeof(float);
+  gn_sums_kernel<T, V, ACT><<<grid, kGnThreads, smem, s>>>(a);
+  gn_means_kernel<<<g.B * g.G, kGnThreads, 0, s>>>(a);
+  gn_dx_kernel<T, V, ACT><<<grid, kGnThreads, 0, s>>>(a);
+  gn_param_kernel<<<(g.D + 127) / 128, 128, 0, s>>>(a);
+  note_launches(4);
+}
+
+template <typename T, int V>
+static void gn_launch(const GnArgs& a, int act, bool bwd, cudaStream_t s) {
+  switch (act) {
+    case SSM_ACT_SILU: return bwd ? gn_bwd_launch<T, V, SSM_ACT_SILU>(a, s) : gn_fwd_launch<T, V, SSM_ACT_SILU>(a, s);
+    case SSM_ACT_GELU: return bwd ? gn_bwd_launch<T, V, SSM_ACT_GELU>(a, s) : gn_fwd_launch<T, V, SSM_ACT_GELU>(a, s);
+    case SSM_ACT_RELU: return bwd ? gn_bwd_launch<T, V, SSM_ACT_RELU>(a, s) : gn_fwd_launch<T, V, SSM_ACT_RELU>(a, s);
+    default: return bwd ? gn_bwd_launch<T, V, SSM_ACT_NONE>(a, s) : gn_fwd_launch<T, V, SSM_ACT_NONE>(a, s);
+  }
+}
+
+static int gn_dispatch(const ssm_group_norm_params_t* p, GnArgs& a, bool bwd, cudaStream_t s) {
+  const bool vec = gn_vector(p);
+  if (p->dtype == SSM_BF16) {
+    if (vec) gn_launch<__nv_bfloat16, 8>(a, p->act, bwd, s);
+    else gn_launch<__nv_bfloat16, 1>(a, p->act, bwd, s);
+  } else {
+    if (vec) gn_launch<float, 8>(a, p->act, bwd, s);
+    else gn_launch<float, 1>(a, p->act, bwd, s);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? SSM_OK : launch_error("launch group norm kernel", e);
+}
+
+}  // namespace ssm
+
+using namespace ssm;
+
+extern "C" {
+
+size_t ssm_group_norm_fwd_workspace_bytes(const ssm_group_norm_params_t* p) {
+  if (check_gn(p) || p->batch == 0 || p->seqlen == 0) return 0;
+  return gn_part_bytes(gn_geom(p));
+}
+
+size_t ssm_group_norm_bwd_workspace_bytes(const ssm_group_norm_params_t* p) {
+  if (check_gn(p) || p->batch == 0 || p->seqlen == 0) return 0;
+  const GnGeom g = gn_geom(p);
+  return gn_part_bytes(g) + gn_sums_bytes(g) + gn_means_bytes(g);
+}
+
+int ssm_group_norm_act_fwd(const ssm_group_norm_params_t* p, ssm_stream_t stream) {
+  int st = check_gn(p);
+  if (st) return st;
+  if (p->batch == 0 || p->seqlen == 0) return SSM_OK;
+  if (!p->x || !p->y || !p->stats) return SSM_ERR_NULL;
+  if (gn_vector(p) && (!aligned16(p->x) || !aligned16(p->y))) return SSM_ERR_ALIGN;
+  if (!p->workspace || p->workspace_bytes < ssm_group_norm_fwd_workspace_bytes(p)) return SSM_ERR_WORKSPACE;
+  st = bind_device(p->x);
+  if (st) return st;
+  GnArgs a = {};
+  a.g = gn_geom(p);
+  a.eps = p->eps;
+  a.x = p->x;
+  a.scale = p->scale;
+  a.bias = p->bias;
+  a.stats = p->stats;
+  a.part = static_cast<float2*>(p->workspace);
+  a.out = p->y;
+  return gn_dispatch(p, a, false, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int ssm_group_norm_act_bwd(const ssm_group_norm_params_t* p, ssm_stream_t stream) {
+  int st = check_gn(p);
+  if (st) return st;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (p->batch == 0 || p->seqlen == 0) {
+    for (float* d : {p->dscale, p->dbias}) {
+      if (!d) continue;
+      st = bind_device(d);
+      if (st) return st;
+      const cudaError_t e = cudaMemsetAsync(d, 0, (size_t)p->dim * sizeof(float), s);
+      if (e != cudaSuccess) return launch_error("cudaMemsetAsync(group norm sums)", e);
+    }
+    return SSM_OK;
+  }
+  if (!p->x || !p->dy || !p->dx || !p->stats) return SSM_ERR_NULL;
+  if (gn_vector(p) && (!aligned16(p->x) || !aligned16(p->dy) || !aligned16(p->dx))) return SSM_ERR_ALIGN;
+  if (!p->workspace || p->workspace_bytes < ssm_group_norm_bwd_workspace_bytes(p)) return SSM_ERR_WORKSPACE;
+  st = bind_device(p->x);
+  if (st) return st;
+  GnArgs a = {};
+  a.g = gn_geom(p);
+  a.x = p->x;
+  a.dy = p->dy;
+  a.scale = p->scale;
+  a.bias = p->bias;
+  a.stats = p->stats;
+  char* w = static_cast<char*>(p->workspace);
+  a.part = reinterpret_cast<float2*>(w);
+  w += gn_part_bytes(a.g);
+  a.sums = reinterpret_cast<float2*>(w);
+  w += gn_sums_bytes(a.g);
+  a.means = reinterpret_cast<float2*>(w);
+  a.out = p->dx;
+  a.dscale = p->dscale;
+  a.dbias = p->dbias;
+  return gn_dispatch(p, a, true, s);
+}
+
+}  // extern "C"
