@@ -13,6 +13,11 @@ namespace ssm {
 
 // Adds n to the library's count of kernels launched (ssm_launch_count).
 void note_launches(unsigned n);
+// Encodes a 3-D tiled TMA map over (d0 innermost, d1, d2) of bf16 or fp32
+// elements with row strides in bytes; false (with a recorded message) on failure.
+bool make_map(CUtensorMap* m, const void* base, bool bf16, uint64_t d0, uint64_t d1, uint64_t d2,
+              uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
+              CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_NONE);
 
 constexpr int kChunk = 16;        // steps per TMA stage
 constexpr int kCk = 8;            // forward checkpoint spacing (backward register block)

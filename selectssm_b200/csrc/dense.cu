@@ -3,15 +3,19 @@
 //   pre = x W + bias,  u = keep * f * pre,  y = residual + act(u)
 //   dpre = keep * f * dy * act'(u),  dx = dpre W^T,  dW = x^T dpre,  dbias = sum over rows of dpre
 //
-// keep and f are dropout's (philox.cuh), recomputed in both directions.
+// keep and f are dropout's (philox.cuh), recomputed in both directions.  The
+// three products run on the tensor cores (dense_mma.cuh) over bf16 planes: a
+// bf16 operand whose rows TMA can address is read where it lies; an fp32 one is
+// split into three planes, and rows TMA cannot address (a stride or start that
+// is not a multiple of 16 bytes) are copied to padded ones, by one pass over it.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include "common.cuh"
-#include "philox.cuh"
-#include "vec8.cuh"
+#include <algorithm>
+
+#include "dense_mma.cuh"
 #include "../../include/selectssm_b200.h"
 
 namespace ssm {
@@ -19,134 +23,138 @@ namespace ssm {
 int launch_error(const char* where, cudaError_t e);  // scan.cu
 int bind_device(const void* ptr);                      // scan.cu
 
-struct Epilogue {
-  const void* bias;
-  int32_t bias_dtype;
-  const void* residual;
-  int64_t res_stride;
-  void* pre;
-  DropRng rng;
-  int32_t act;
-  int32_t per_row;  // dropout blocks in a row
-};
-
-// C = A B with A (M, K) and B (K, N) at any strides; one 64 x 64 tile per CTA,
-// 4 x 4 values per thread, fp32 FMA.
-constexpr int kTile = 64, kDepth = 16;
-
-template <typename T, typename TO, bool EPI>
-__global__ void __launch_bounds__(256) dense_simt_kernel(const T* A, const T* B, TO* C, int64_t M, int64_t N, int64_t K,
-                                                         int64_t sam, int64_t sak, int64_t sbk, int64_t sbn,
-                                                         const Epilogue e) {
-  __shared__ float as[kDepth][kTile + 4], bs[kDepth][kTile + 4];
-  const int64_t m0 = (int64_t)blockIdx.y * kTile, n0 = (int64_t)blockIdx.x * kTile;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < K; k0 += kDepth) {
+// ---------------------------------------------------------------- operands
+// Splits v into bf16 values that sum to it exactly: each takes the leading 8
+// bits of what is left.  A value that would round to infinity is cut instead.
+__device__ __forceinline__ void split3(float v, float (&h)[3]) {
 #pragma unroll
-    for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-      const int ak = sak == 1 ? i % kDepth : i / kTile, am = sak == 1 ? i / kDepth : i % kTile;
-      as[ak][am] = m0 + am < M && k0 + ak < K ? Cvt<T>::to_f(A[(m0 + am) * sam + (k0 + ak) * sak]) : 0.f;
-      const int bk = sbk == 1 ? i % kDepth : i / kTile, bn = sbk == 1 ? i / kDepth : i % kTile;
-      bs[bk][bn] = n0 + bn < N && k0 + bk < K ? Cvt<T>::to_f(B[(k0 + bk) * sbk + (n0 + bn) * sbn]) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kDepth; ++k) {
-      float a[4], b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = as[k][ty * 4 + i];
-        b[i] = bs[k][tx * 4 + i];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-    }
-    __syncthreads();
+  for (int p = 0; p < 3; ++p) {
+    float r = __bfloat162float(__float2bfloat16_rn(v));
+    if (isinf(r) && !isinf(v)) r = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+    h[p] = r;
+    v = isinf(v) ? 0.f : v - r;
   }
-  PhiloxKey key = {};
-  float f = 1.f;
-  if (EPI && e.rng.drop) {
-    key = philox_key(e.rng);
-    f = keep_factor(e.rng.drop);
-  }
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + ty * 4 + i;
-    if (m >= M) break;
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = n0 + tx * 4 + j;
-      if (n >= N) break;
-      float v = acc[i][j];
-      if (EPI) {
-        if (e.bias)
-          v += e.bias_dtype == SSM_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[n])
-                                        : static_cast<const float*>(e.bias)[n];
-        if (e.pre) static_cast<T*>(e.pre)[m * N + n] = Cvt<T>::from_f(v);
-        if (e.rng.drop) {
-          const uint32_t bits = keep_bits8(m * e.per_row + n / 8, key, e.rng.drop);
-          v = bits >> (n & 7) & 1 ? v * f : 0.f;
-        }
-        v = act_f(v, e.act);
-        if (e.residual) v += Cvt<T>::to_f(static_cast<const T*>(e.residual)[m * e.res_stride + n]);
-      }
-      C[m * N + n] = Cvt<TO>::from_f(v);
+}
+
+template <int PLANES>
+__device__ __forceinline__ void store_planes(__nv_bfloat16* dst, int64_t plane, const float (&v)[8]) {
+  if (PLANES == 1) {
+    store8(dst, v);
+  } else {
+    float h[8][3], t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split3(v[i], h[i]);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = h[i][p];
+      store8(dst + p * plane, t);
     }
   }
 }
 
-// dpre, rounded to the operand type of the two products that follow, and the
-// column sums of its unrounded values over a run of rows.
-constexpr int kDpreCols = 32, kDpreLanes = 8;
-template <typename T>
-__global__ void __launch_bounds__(kDpreCols* kDpreLanes)
-    dense_dpre_kernel(const T* dy, int64_t dy_stride, const T* pre, T* dpre, float* part, int64_t M, int N,
-                      int64_t run, int act, DropRng rng, int per_row) {
-  __shared__ float red[kDpreLanes][kDpreCols];
-  const int n = blockIdx.x * kDpreCols + threadIdx.x % kDpreCols, lane = threadIdx.x / kDpreCols;
-  const int64_t m0 = (int64_t)blockIdx.y * run, m1 = m0 + run < M ? m0 + run : M;
+// (rows, cols) at row stride `stride` to planes of row length ld, a multiple of
+// 8; columns beyond cols become zeros.  Eight columns a thread.
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(256) dense_pack_kernel(const T* src, int64_t stride, int64_t rows, int cols, int ld,
+                                                         __nv_bfloat16* dst, bool vec) {
+  const int per = ld / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * per) return;
+  const int64_t r = i / per;
+  const int c = (int)(i - r * per) * 8;
+  float v[8];
+  get8<T>(src, r * stride + c, cols - c, vec && c + 8 <= cols, v);
+  store_planes<PLANES>(dst + r * ld + c, rows * ld, v);
+}
+
+// dpre as planes for the two products that follow, and the column sums of its
+// unrounded values over a run of rows.  A thread keeps eight columns (one
+// dropout counter each row) and walks down the rows.
+template <typename T, int PLANES, bool WRITE>
+__global__ void __launch_bounds__(256)
+    dense_dpre_kernel(const T* dy, int64_t dy_stride, const T* pre, __nv_bfloat16* dpre, int ld, float* part, int64_t M,
+                      int N, int64_t run, int cb, int act, DropRng rng, bool vec_dy, bool vec_pre) {
+  extern __shared__ float red[];
+  const int per_row = (N + 7) / 8, rl = 256 / cb;
+  const int lane = threadIdx.x / cb, blk = blockIdx.x * cb + threadIdx.x % cb, n = blk * 8;
+  const int64_t m0 = (int64_t)blockIdx.y * run, m1 = min(m0 + run, M);
   PhiloxKey key = {};
   float f = 1.f;
   if (rng.drop) {
     key = philox_key(rng);
     f = keep_factor(rng.drop);
   }
-  float sum = 0.f;
-  if (n < N)
-    for (int64_t m = m0 + lane; m < m1; m += kDpreLanes) {
-      float d = Cvt<T>::to_f(dy[m * dy_stride + n]);
-      bool keep = true;
-      if (rng.drop) keep = keep_bits8(m * per_row + n / 8, key, rng.drop) >> (n & 7) & 1;
-      if (act != SSM_ACT_NONE) d *= act_grad_f(keep ? Cvt<T>::to_f(pre[m * N + n]) * f : 0.f, act);
-      d = keep ? d * f : 0.f;
-      sum += d;
-      dpre[m * N + n] = Cvt<T>::from_f(d);
-    }
-  red[lane][threadIdx.x % kDpreCols] = sum;
-  __syncthreads();
-  if (lane == 0 && n < N) {
-    float s = 0.f;
+  float sum[8] = {};
+  if (lane < rl && blk < per_row) {
+    const int cnt = min(8, N - n);
+    for (int64_t m = m0 + lane; m < m1; m += rl) {
+      float d[8], u[8];
+      get8<T>(dy, m * dy_stride + n, cnt, vec_dy, d);
+      if (act) get8<T>(pre, m * N + n, cnt, vec_pre, u);
+      uint32_t bits = 0xff;
+      if (rng.drop) bits = keep_bits8(m * per_row + blk, key, rng.drop);
+      switch (act) {
+        case 1:
 #pragma unroll
-    for (int i = 0; i < kDpreLanes; ++i) s += red[i][threadIdx.x];
-    part[(int64_t)blockIdx.y * N + n] = s;
+          for (int i = 0; i < 8; ++i) d[i] *= act_grad_f(u[i] * f, 1);
+          break;
+        case 2:
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[i] *= act_grad_f(u[i] * f, 2);
+          break;
+        case 3:
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[i] *= act_grad_f(u[i] * f, 3);
+          break;
+        default: break;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        d[i] = bits >> i & 1 ? d[i] * f : 0.f;
+        sum[i] += d[i];
+      }
+      if (WRITE) store_planes<PLANES>(dpre + m * ld + n, M * ld, d);
+    }
+  }
+  if (!part) return;
+  if (lane < rl)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) red[(lane * cb + threadIdx.x % cb) * 8 + i] = sum[i];
+  __syncthreads();
+  for (int c = threadIdx.x; c < cb * 8; c += 256) {
+    const int col = blockIdx.x * cb * 8 + c;
+    if (col >= N) break;
+    float s = 0.f;
+    for (int i = 0; i < rl; ++i) s += red[i * cb * 8 + c];
+    part[(int64_t)blockIdx.y * N + col] = s;
   }
 }
 
-__global__ void dense_dbias_kernel(const float* part, int parts, int N, void* dbias, int dtype) {
-  const int n = blockIdx.x * blockDim.x + threadIdx.x;
-  if (n >= N) return;
+// dbias: the runs' sums in a fixed order, 32 lanes a column
+__global__ void __launch_bounds__(1024) dense_dbias_kernel(const float* part, int parts, int N, void* dbias, int dtype) {
+  __shared__ float red[32][33];
+  const int col = threadIdx.x & 31, lane = threadIdx.x >> 5, n = blockIdx.x * 32 + col;
   float s = 0.f;
-  for (int i = 0; i < parts; ++i) s += part[(int64_t)i * N + n];
-  if (dtype == SSM_BF16) static_cast<__nv_bfloat16*>(dbias)[n] = __float2bfloat16_rn(s);
-  else static_cast<float*>(dbias)[n] = s;
+  if (n < N)
+    for (int i = lane; i < parts; i += 32) s += part[(int64_t)i * N + n];
+  red[lane][col] = s;
+  __syncthreads();
+  if (lane == 0 && n < N) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t += red[i][col];
+    if (dtype == SSM_BF16) static_cast<__nv_bfloat16*>(dbias)[n] = __float2bfloat16_rn(t);
+    else static_cast<float*>(dbias)[n] = t;
+  }
 }
 
+// ---------------------------------------------------------------- checks and sizes
 static bool known(int dtype) { return dtype == SSM_F32 || dtype == SSM_BF16; }
 
 static int check_dense(const ssm_dense_params_t* p) {
   if (!p) return SSM_ERR_NULL;
-  if (p->rows < 0 || p->rows > 0x7fffffff || p->fin < 1 || p->fout < 1 || p->fin > (1 << 24) || p->fout > (1 << 24) ||
+  if (p->rows < 0 || p->rows > 0x7fffff00 || p->fin < 1 || p->fout < 1 || p->fin > (1 << 24) || p->fout > (1 << 24) ||
       p->drop < 0 || p->drop > 65536 || p->act < SSM_ACT_NONE || p->act > SSM_ACT_RELU)
     return SSM_ERR_SHAPE;
   if ((p->x_stride && p->x_stride < p->fin) || (p->res_stride && p->res_stride < p->fout) ||
@@ -159,13 +167,10 @@ static int check_dense(const ssm_dense_params_t* p) {
 static size_t round256(size_t v) { return (v + 255) / 256 * 256; }
 static size_t elem_bytes(int dtype) { return dtype == SSM_BF16 ? 2 : 4; }
 static DropRng drop_rng(const ssm_dense_params_t* p) { return {p->seed, p->offset, p->rng, (uint32_t)p->drop}; }
-
-// rows of dpre that one CTA sums for dbias
-static int64_t dpre_run(const ssm_dense_params_t* p) {
-  const int64_t tiles = (p->fout + kDpreCols - 1) / kDpreCols, want = (8 * 148 + tiles - 1) / tiles;
-  const int64_t run = (p->rows + want - 1) / want;
-  return run < 32 ? 32 : run;
-}
+static int pad8(int n) { return (n + 7) / 8 * 8; }
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+static int planes_of(const ssm_dense_params_t* p) { return p->dtype == SSM_BF16 ? 1 : 3; }
+static int64_t stride_or(int64_t s, int64_t dense) { return s ? s : dense; }
 
 static int launched(const char* where, unsigned n) {
   note_launches(n);
@@ -173,63 +178,243 @@ static int launched(const char* where, unsigned n) {
   return e == cudaSuccess ? SSM_OK : launch_error(where, e);
 }
 
-template <typename T>
-static int dense_fwd(const ssm_dense_params_t* p, cudaStream_t s) {
-  Epilogue e;
-  e.bias = p->bias;
-  e.bias_dtype = p->bias_dtype;
-  e.residual = p->residual;
-  e.res_stride = p->res_stride ? p->res_stride : p->fout;
-  e.pre = p->pre;
-  e.rng = drop_rng(p);
-  e.act = p->act;
-  e.per_row = (p->fout + 7) / 8;
-  const dim3 grid((p->fout + kTile - 1) / kTile, (unsigned)((p->rows + kTile - 1) / kTile));
-  if (grid.y > 65535) return SSM_ERR_SHAPE;
-  dense_simt_kernel<T, T, true><<<grid, 256, 0, s>>>(
-      static_cast<const T*>(p->x), static_cast<const T*>(p->kernel), static_cast<T*>(p->y), p->rows, p->fout, p->fin,
-      p->x_stride ? p->x_stride : p->fin, 1, p->fout, 1, e);
-  return launched("launch dense kernel", 1);
+// An operand of a product: (rows, cols), cols contiguous.
+struct Operand {
+  const void* src;
+  int64_t stride, rows;
+  int cols;
+  bool bf16;
+  // read in place: bf16 rows TMA can address (a null pointer counts as aligned)
+  bool direct() const { return bf16 && stride % 8 == 0 && aligned16(src); }
+  size_t bytes() const { return direct() ? 0 : round256((size_t)rows * pad8(cols) * 2 * (bf16 ? 1 : 3)); }
+};
+
+static Operand x_operand(const ssm_dense_params_t* p) {
+  return {p->x, stride_or(p->x_stride, p->fin), p->rows, p->fin, p->dtype == SSM_BF16};
+}
+static Operand kernel_operand(const ssm_dense_params_t* p) {
+  return {p->kernel, p->fout, p->fin, p->fout, p->dtype == SSM_BF16};
 }
 
-template <typename T>
+// The planes of an operand, packed into `*ws` (advanced) where it cannot be read in place.
+static int planes(const Operand& o, bool k_major, char** ws, cudaStream_t s, Planes* out) {
+  out->k_major = k_major;
+  if (o.direct()) {
+    *out = {static_cast<const __nv_bfloat16*>(o.src), 0, o.stride, k_major};
+    return SSM_OK;
+  }
+  const int ld = pad8(o.cols);
+  __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(*ws);
+  *ws += o.bytes();
+  *out = {dst, o.rows * ld, ld, k_major};
+  const int64_t grid = ceil_div(o.rows * (ld / 8), 256);
+  if (grid > 0x7fffffff) return SSM_ERR_SHAPE;
+  const bool vec = aligned16(o.src) && o.stride % (o.bf16 ? 8 : 4) == 0;
+  if (o.bf16)
+    dense_pack_kernel<__nv_bfloat16, 1><<<(unsigned)grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(o.src), o.stride,
+                                                                      o.rows, o.cols, ld, dst, vec);
+  else
+    dense_pack_kernel<float, 3><<<(unsigned)grid, 256, 0, s>>>(static_cast<const float*>(o.src), o.stride, o.rows, o.cols,
+                                                               ld, dst, vec);
+  return launched("launch dense pack kernel", 1);
+}
+
+// ---------------------------------------------------------------- one product
+constexpr int kSms = 148;
+
+struct Plan {
+  int bn;
+  DenseWork w;
+  size_t part_bytes;
+};
+
+static Plan plan_product(int64_t M, int64_t N, int64_t K, int planes) {
+  Plan q;
+  q.w.tiles_m = (int)ceil_div(M, kBM);
+  q.w.kblocks = (int)ceil_div(K, kBK);
+  q.w.steps = q.w.kblocks * (planes == 3 ? 6 : 1);
+  q.bn = N <= 128 || q.w.tiles_m * ceil_div(N, 256) < kSms ? 128 : 256;
+  q.w.tiles_n = (int)ceil_div(N, q.bn);
+  // too few tiles for the SMs: cut the K loop, in parts of at least 8 steps
+  const int64_t tiles = (int64_t)q.w.tiles_m * q.w.tiles_n;
+  q.w.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / tiles, q.w.steps / 8));
+  q.part_bytes = q.w.splits > 1 ? round256((size_t)q.w.splits * M * N * sizeof(float)) : 0;
+  return q;
+}
+
+static bool operand_map(CUtensorMap* m, const Planes& o, int64_t rows, int64_t cols, int planes, int box_rows) {
+  const uint64_t ld = (uint64_t)o.ld * 2;
+  return make_map(m, o.base, true, cols, rows, planes, ld, planes == 3 ? (uint64_t)o.plane * 2 : ld, kBK,
+                  o.k_major ? box_rows : kBK, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <bool A_MN, bool B_MN, int BN>
+static int launch_mma(const DenseEpi& e, const Plan& q, const CUtensorMap& ma, const CUtensorMap& mb, int32_t* status,
+                      cudaStream_t s) {
+  const auto kernel = dense_mma_kernel<A_MN, B_MN, BN>;
+  const cudaError_t err =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MmaSmem<BN>::kBytes);
+  if (err != cudaSuccess) return launch_error("cudaFuncSetAttribute(dense)", err);
+  const int items = q.w.tiles_m * q.w.tiles_n * q.w.splits;
+  kernel<<<std::min(items, kSms), kMmaThreads, MmaSmem<BN>::kBytes, s>>>(ma, mb, e, q.w, status);
+  return launched("launch dense product kernel", 1);
+}
+
+// e.M, e.N, e.K, e.a, e.b and the epilogue are set; `part` holds plan_product's part_bytes.
+template <bool A_MN, bool B_MN>
+static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
+  const Plan q = plan_product(e.M, e.N, e.K, e.planes);
+  if ((int64_t)q.w.tiles_m * q.w.tiles_n * q.w.splits > 0x7fffffff) return SSM_ERR_SHAPE;
+  CUtensorMap ma, mb;
+  if (!operand_map(&ma, e.a, A_MN ? e.K : e.M, A_MN ? e.M : e.K, e.planes, kBM) ||
+      !operand_map(&mb, e.b, B_MN ? e.K : e.N, B_MN ? e.N : e.K, e.planes, q.bn))
+    return SSM_ERR_LAUNCH;
+  DenseEpi first = e;
+  if (q.w.splits > 1) {
+    first.out = part;
+    first.out_kind = kOutPartial;
+    first.pre = nullptr;
+  }
+  int st = q.bn == 256 ? launch_mma<A_MN, B_MN, 256>(first, q, ma, mb, status, s)
+                       : launch_mma<A_MN, B_MN, 128>(first, q, ma, mb, status, s);
+  if (st || q.w.splits == 1) return st;
+  const int64_t blocks = e.M * ((e.N + 7) / 8);
+  dense_join_kernel<<<(unsigned)ceil_div(blocks, 256), 256, 0, s>>>(part, q.w.splits, e);
+  return launched("launch dense join kernel", 1);
+}
+
+// ---------------------------------------------------------------- forward and backward
+static int dense_fwd(const ssm_dense_params_t* p, cudaStream_t s) {
+  char* ws = static_cast<char*>(p->workspace);
+  DenseEpi e = {};
+  int st = planes(x_operand(p), true, &ws, s, &e.a);
+  if (st) return st;
+  st = planes(kernel_operand(p), false, &ws, s, &e.b);
+  if (st) return st;
+  e.M = p->rows;
+  e.N = p->fout;
+  e.K = p->fin;
+  e.planes = planes_of(p);
+  e.out_kind = p->dtype == SSM_BF16 ? kOutBF16 : kOutF32;
+  e.out = p->y;
+  e.bias = p->bias;
+  e.bias_bf16 = p->bias_dtype == SSM_BF16;
+  e.act = p->act;
+  e.residual = p->residual;
+  e.res_stride = stride_or(p->res_stride, p->fout);
+  e.pre = p->pre;
+  e.per_row = (p->fout + 7) / 8;
+  e.rng = drop_rng(p);
+  return product<false, true>(e, reinterpret_cast<float*>(ws), p->status, s);
+}
+
+// How the dpre pass cuts (rows, fout): cb blocks of eight columns a CTA, `run` rows.
+struct DpreGeom {
+  int cb, tiles, parts;
+  int64_t run;
+};
+static DpreGeom dpre_geom(const ssm_dense_params_t* p) {
+  DpreGeom g;
+  const int per_row = (p->fout + 7) / 8;
+  g.tiles = (int)ceil_div(per_row, 32);
+  g.cb = (int)ceil_div(per_row, g.tiles);
+  const int rl = 256 / g.cb;
+  const int64_t want = ceil_div(6 * kSms, g.tiles);
+  g.run = std::max<int64_t>(ceil_div(p->rows, want), 2 * rl);
+  g.run = std::max(g.run, ceil_div(p->rows, 65535));
+  g.parts = (int)ceil_div(p->rows, g.run);
+  return g;
+}
+
+// dy serves as dpre itself
+static bool dpre_is_dy(const ssm_dense_params_t* p) {
+  return p->dtype == SSM_BF16 && p->act == SSM_ACT_NONE && p->drop == 0 && stride_or(p->dy_stride, p->fout) % 8 == 0 &&
+         aligned16(p->dy);
+}
+
+template <typename T, int PLANES>
+static int launch_dpre(const ssm_dense_params_t* p, __nv_bfloat16* dpre, float* part, cudaStream_t s) {
+  const DpreGeom g = dpre_geom(p);
+  const dim3 grid(g.tiles, g.parts);
+  const size_t smem = (size_t)(256 / g.cb) * g.cb * 8 * sizeof(float);
+  const int64_t ds = stride_or(p->dy_stride, p->fout);
+  const bool even = p->fout % 8 == 0;
+  const bool vec_dy = even && ds % 8 == 0 && aligned16(p->dy), vec_pre = even && aligned16(p->pre);
+  const T *dy = static_cast<const T*>(p->dy), *pre = static_cast<const T*>(p->pre);
+  if (dpre)
+    dense_dpre_kernel<T, PLANES, true><<<grid, 256, smem, s>>>(dy, ds, pre, dpre, pad8(p->fout), part, p->rows, p->fout,
+                                                               g.run, g.cb, p->act, drop_rng(p), vec_dy, vec_pre);
+  else
+    dense_dpre_kernel<T, PLANES, false><<<grid, 256, smem, s>>>(dy, ds, pre, dpre, pad8(p->fout), part, p->rows, p->fout,
+                                                                g.run, g.cb, p->act, drop_rng(p), vec_dy, vec_pre);
+  return launched("launch dense dpre kernel", 1);
+}
+
+struct BwdBytes {
+  size_t dpre, sums, x, kernel, part;
+  size_t all() const { return dpre + sums + x + kernel + part; }
+};
+static BwdBytes bwd_bytes(const ssm_dense_params_t* p) {
+  const int pl = planes_of(p);
+  BwdBytes b;
+  b.dpre = round256((size_t)p->rows * pad8(p->fout) * 2 * pl);  // also when dy serves: pointers may be unknown here
+  b.sums = round256((size_t)dpre_geom(p).parts * p->fout * sizeof(float));
+  b.x = x_operand(p).bytes();
+  b.kernel = kernel_operand(p).bytes();
+  b.part = std::max(plan_product(p->rows, p->fin, p->fout, pl).part_bytes,
+                    plan_product(p->fin, p->fout, p->rows, pl).part_bytes);
+  return b;
+}
+
 static int dense_bwd(const ssm_dense_params_t* p, cudaStream_t s) {
-  const int64_t M = p->rows, run = dpre_run(p);
-  const int N = p->fout, K = p->fin, parts = (int)((M + run - 1) / run);
-  char* w = static_cast<char*>(p->workspace);
-  T* dpre = reinterpret_cast<T*>(w);
-  float* part = reinterpret_cast<float*>(w + round256((size_t)M * N * sizeof(T)));
-  dense_dpre_kernel<T><<<dim3((N + kDpreCols - 1) / kDpreCols, parts), kDpreCols * kDpreLanes, 0, s>>>(
-      static_cast<const T*>(p->dy), p->dy_stride ? p->dy_stride : N, static_cast<const T*>(p->pre), dpre, part, M, N, run,
-      p->act, drop_rng(p), (N + 7) / 8);
-  int st = launched("launch dense dpre kernel", 1);
+  const int pl = planes_of(p), N = p->fout, K = p->fin, ld = pad8(N);
+  const BwdBytes bytes = bwd_bytes(p);
+  char* ws = static_cast<char*>(p->workspace);
+  __nv_bfloat16* dpre = reinterpret_cast<__nv_bfloat16*>(ws);
+  float* sums = reinterpret_cast<float*>(ws + bytes.dpre);
+  ws += bytes.dpre + bytes.sums;
+  const bool same = dpre_is_dy(p);
+  int st = SSM_OK;
+  if (!same || p->dbias)
+    st = pl == 1 ? launch_dpre<__nv_bfloat16, 1>(p, same ? nullptr : dpre, p->dbias ? sums : nullptr, s)
+                 : launch_dpre<float, 3>(p, dpre, p->dbias ? sums : nullptr, s);
   if (st) return st;
   if (p->dbias) {
-    dense_dbias_kernel<<<(N + 127) / 128, 128, 0, s>>>(part, parts, N, p->dbias, p->bias_dtype);
+    dense_dbias_kernel<<<(unsigned)ceil_div(N, 32), 1024, 0, s>>>(sums, dpre_geom(p).parts, N, p->dbias, p->bias_dtype);
     st = launched("launch dense dbias kernel", 1);
     if (st) return st;
   }
-  const Epilogue none = {};
-  const int64_t xs = p->x_stride ? p->x_stride : K;
-  if (p->dx) {
-    const dim3 grid((K + kTile - 1) / kTile, (unsigned)((M + kTile - 1) / kTile));
-    dense_simt_kernel<T, T, false><<<grid, 256, 0, s>>>(dpre, static_cast<const T*>(p->kernel), static_cast<T*>(p->dx), M,
-                                                        K, N, N, 1, 1, N, none);
-    st = launched("launch dense dx kernel", 1);
+  const Planes d = same ? Planes{static_cast<const __nv_bfloat16*>(p->dy), 0, stride_or(p->dy_stride, N), true}
+                        : Planes{dpre, p->rows * ld, ld, true};
+  DenseEpi e = {};
+  e.planes = pl;
+  if (p->dx) {  // (rows, fout) (fin, fout)^T
+    char* w = ws + bytes.x;
+    e.a = d;
+    st = planes(kernel_operand(p), true, &w, s, &e.b);
+    if (st) return st;
+    e.M = p->rows;
+    e.N = K;
+    e.K = N;
+    e.out_kind = p->dtype == SSM_BF16 ? kOutBF16 : kOutF32;
+    e.out = p->dx;
+    st = product<false, false>(e, reinterpret_cast<float*>(w), p->status, s);
     if (st) return st;
   }
-  if (p->dkernel) {
-    const dim3 grid((N + kTile - 1) / kTile, (K + kTile - 1) / kTile);
-    if (p->dkernel_dtype == SSM_BF16)
-      dense_simt_kernel<T, __nv_bfloat16, false><<<grid, 256, 0, s>>>(
-          static_cast<const T*>(p->x), dpre, static_cast<__nv_bfloat16*>(p->dkernel), K, N, M, 1, xs, N, 1, none);
-    else
-      dense_simt_kernel<T, float, false><<<grid, 256, 0, s>>>(static_cast<const T*>(p->x), dpre,
-                                                              static_cast<float*>(p->dkernel), K, N, M, 1, xs, N, 1, none);
-    st = launched("launch dense dkernel kernel", 1);
+  if (p->dkernel) {  // (rows, fin)^T (rows, fout)
+    char* w = ws;
+    st = planes(x_operand(p), false, &w, s, &e.a);
     if (st) return st;
+    e.b = d;
+    e.b.k_major = false;
+    e.M = K;
+    e.N = N;
+    e.K = p->rows;
+    e.out_kind = p->dkernel_dtype == SSM_BF16 ? kOutBF16 : kOutF32;
+    e.out = p->dkernel;
+    st = product<true, true>(e, reinterpret_cast<float*>(ws + bytes.x + bytes.kernel), p->status, s);
   }
-  return SSM_OK;
+  return st;
 }
 
 }  // namespace ssm
@@ -238,12 +423,15 @@ using namespace ssm;
 
 extern "C" {
 
-size_t ssm_dense_fwd_workspace_bytes(const ssm_dense_params_t* p) { return check_dense(p) ? 0 : 0; }
+size_t ssm_dense_fwd_workspace_bytes(const ssm_dense_params_t* p) {
+  if (check_dense(p) || p->rows == 0) return 0;
+  return x_operand(p).bytes() + kernel_operand(p).bytes() +
+         plan_product(p->rows, p->fout, p->fin, planes_of(p)).part_bytes;
+}
 
 size_t ssm_dense_bwd_workspace_bytes(const ssm_dense_params_t* p) {
   if (check_dense(p) || p->rows == 0) return 0;
-  const int64_t run = dpre_run(p), parts = (p->rows + run - 1) / run;
-  return round256((size_t)p->rows * p->fout * elem_bytes(p->dtype)) + round256((size_t)parts * p->fout * sizeof(float));
+  return bwd_bytes(p).all();
 }
 
 int ssm_dense_act_fwd(const ssm_dense_params_t* p, ssm_stream_t stream) {
@@ -251,11 +439,12 @@ int ssm_dense_act_fwd(const ssm_dense_params_t* p, ssm_stream_t stream) {
   if (st) return st;
   if (p->rows == 0) return SSM_OK;
   if (!p->x || !p->kernel || !p->y) return SSM_ERR_NULL;
-  if (p->workspace_bytes < ssm_dense_fwd_workspace_bytes(p)) return SSM_ERR_WORKSPACE;
+  const size_t need = ssm_dense_fwd_workspace_bytes(p);
+  if (need && (!p->workspace || p->workspace_bytes < need)) return SSM_ERR_WORKSPACE;
   st = bind_device(p->x);
   if (st) return st;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return p->dtype == SSM_BF16 ? dense_fwd<__nv_bfloat16>(p, s) : dense_fwd<float>(p, s);
+  return dense_fwd(p, s);
 }
 
 int ssm_dense_act_bwd(const ssm_dense_params_t* p, ssm_stream_t stream) {
@@ -280,7 +469,7 @@ int ssm_dense_act_bwd(const ssm_dense_params_t* p, ssm_stream_t stream) {
   if (!p->workspace || p->workspace_bytes < ssm_dense_bwd_workspace_bytes(p)) return SSM_ERR_WORKSPACE;
   st = bind_device(p->dy);
   if (st) return st;
-  return p->dtype == SSM_BF16 ? dense_bwd<__nv_bfloat16>(p, s) : dense_bwd<float>(p, s);
+  return dense_bwd(p, s);
 }
 
 }  // extern "C"

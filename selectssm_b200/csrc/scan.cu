@@ -134,9 +134,10 @@ static EncodeTiledFn encode_fn() {  // resolved once, read-only afterwards
   return fn;
 }
 
-// 3-D tiled map over (d0 innermost, d1, d2) with row strides in bytes.
-static bool make_map(CUtensorMap* m, const void* base, bool bf16, uint64_t d0, uint64_t d1, uint64_t d2,
-                     uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1) {
+// 3-D tiled map over (d0 innermost, d1, d2) with row strides in bytes (common.cuh).
+bool make_map(CUtensorMap* m, const void* base, bool bf16, uint64_t d0, uint64_t d1, uint64_t d2,
+              uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
+              CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) {
     snprintf(g_last_error, sizeof(g_last_error), "cuTensorMapEncodeTiled not available from the driver");
@@ -148,7 +149,7 @@ static bool make_map(CUtensorMap* m, const void* base, bool bf16, uint64_t d0, u
   const cuuint32_t es[3] = {1, 1, 1};
   const CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3,
                         const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     snprintf(g_last_error, sizeof(g_last_error),
