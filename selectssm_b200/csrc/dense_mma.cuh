@@ -94,8 +94,20 @@ struct EpiConst {
   }
 };
 
+// bias of columns n .. n+7, zeros where there is none
+__device__ __forceinline__ void dense_bias8(const DenseEpi& e, int n, float (&b)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    b[i] = 0.f;
+    if (e.bias && n + i < e.N)
+      b[i] = e.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[n + i])
+                         : static_cast<const float*>(e.bias)[n + i];
+  }
+}
+
 // Columns n .. n+7 (those below N) of row m from the summed products v.
-__device__ __forceinline__ void dense_epilogue8(const DenseEpi& e, const EpiConst& c, int64_t m, int n, float (&v)[8]) {
+__device__ __forceinline__ void dense_epilogue8(const DenseEpi& e, const EpiConst& c, int64_t m, int n,
+                                                const float (&bias)[8], float (&v)[8]) {
   const int cnt = min(8, e.N - n);
   if (e.planes == 3) {
     // An infinite operand has no finite planes besides its first, and infinity
@@ -110,13 +122,8 @@ __device__ __forceinline__ void dense_epilogue8(const DenseEpi& e, const EpiCons
       }
   }
   const int64_t off = m * e.N + n;
-  if (e.bias) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < cnt)
-        v[i] += e.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[n + i])
-                            : static_cast<const float*>(e.bias)[n + i];
-  }
+  for (int i = 0; i < 8; ++i) v[i] += bias[i];
   if (e.pre) {
     if (e.out_kind == kOutBF16) put8<__nv_bfloat16>(e.pre, off, cnt, c.vec_out, v);
     else put8<float>(e.pre, off, cnt, c.vec_out, v);
@@ -195,7 +202,8 @@ template <int BN>
 struct MmaSmem {
   static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
   static constexpr int kStages = BN == 256 ? 4 : 6;
-  static constexpr int kBytes = kStages * kStage + 1024;  // and alignment
+  static constexpr int kEpi = kEpiWarps * 4096;  // 32 x 32 fp32 for each epilogue warp
+  static constexpr int kBytes = kStages * kStage + kEpi + 1024;  // and alignment
 };
 
 // plane pairs (of A, of B), smallest products first
@@ -336,11 +344,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   } else if (warp >= 4) {
     const EpiConst c(e);
     const int quarter = warp & 3, half = (warp - 4) >> 2;
+    uint4* stage = reinterpret_cast<uint4*>(tiles + S::kStages * S::kStage) + (warp - 4) * 256;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
       const int n0 = item % w.tiles_n * BN, rest = item / w.tiles_n;
-      const int64_t m = (int64_t)(rest % w.tiles_m) * kBM + quarter * 32 + lane;
+      const int64_t m0 = (int64_t)(rest % w.tiles_m) * kBM + quarter * 32;
       const int split = rest / w.tiles_m;
       if (!__all_sync(0xffffffffu, wait(&acc_full[acc], acc_phase))) break;
       tmem_fence_after_sync();
@@ -349,24 +358,37 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       for (int j = 0; j < BN / 2; j += 32) {
         const int n = n0 + half * (BN / 2) + j;
         if (n >= e.N) break;
+        // A lane reads 32 columns of its own row of the accumulator; through
+        // shared memory (16-byte pieces, swizzled by row) it gets eight
+        // columns of four rows, so that four lanes cover 32 columns of a row
+        // in global memory and the eight share one dropout counter.
         uint32_t r[2][16];
         tmem_ld16(src + j, r[0]);
         tmem_ld16(src + j + 16, r[1]);
+        const int nl = n + (lane & 3) * 8;
+        float bias[8];
+        dense_bias8(e, nl, bias);
         tmem_wait_ld();
-        if (m < e.M) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (n + 8 * q >= e.N) break;
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[q >> 1][(q & 1) * 8 + i]);
-            if (e.out_kind == kOutPartial)
-              put8<float>(e.out, ((int64_t)split * e.M + m) * e.N + n + 8 * q, min(8, e.N - n - 8 * q), c.vec_out, v);
-            else
-              dense_epilogue8(e, c, m, n + 8 * q, v);
-          }
-        }
         __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          stage[lane * 8 + (q ^ (lane & 7))] = make_uint4(r[q >> 2][(q & 3) * 4], r[q >> 2][(q & 3) * 4 + 1],
+                                                          r[q >> 2][(q & 3) * 4 + 2], r[q >> 2][(q & 3) * 4 + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int row = q * 8 + (lane >> 2);
+          const int64_t m = m0 + row;
+          const uint4 lo = stage[row * 8 + (((lane & 3) * 2) ^ (row & 7))];
+          const uint4 hi = stage[row * 8 + (((lane & 3) * 2 + 1) ^ (row & 7))];
+          float v[8] = {__uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w),
+                        __uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w)};
+          if (m >= e.M || nl >= e.N) continue;
+          if (e.out_kind == kOutPartial)
+            put8<float>(e.out, ((int64_t)split * e.M + m) * e.N + nl, min(8, e.N - nl), c.vec_out, v);
+          else
+            dense_epilogue8(e, c, m, nl, bias, v);
+        }
       }
       tmem_fence_before_sync();
       if (lane == 0) mbar_arrive(&acc_empty[acc]);
@@ -400,7 +422,9 @@ __global__ void __launch_bounds__(256) dense_join_kernel(const float* part, int 
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] += t[k];
   }
-  dense_epilogue8(e, c, m, n, v);
+  float bias[8];
+  dense_bias8(e, n, bias);
+  dense_epilogue8(e, c, m, n, bias, v);
 }
 
 }  // namespace ssm
