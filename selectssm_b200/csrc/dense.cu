@@ -68,6 +68,15 @@ __global__ void __launch_bounds__(256) dense_pack_kernel(const T* src, int64_t s
   store_planes<PLANES>(dst + r * ld + c, rows * ld, v);
 }
 
+constexpr int kDpreRows = 2;
+template <int ACT>
+__device__ __forceinline__ void slope_rows(float (&d)[kDpreRows][8], const float (&u)[kDpreRows][8], float f) {
+#pragma unroll
+  for (int q = 0; q < kDpreRows; ++q)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[q][i] *= act_grad_f(u[q][i] * f, ACT);
+}
+
 // dpre as planes for the two products that follow, and the column sums of its
 // unrounded values over a run of rows.  A thread keeps eight columns (one
 // dropout counter each row) and walks down the rows.
@@ -88,33 +97,33 @@ __global__ void __launch_bounds__(256)
   float sum[8] = {};
   if (lane < rl && blk < per_row) {
     const int cnt = min(8, N - n);
-    for (int64_t m = m0 + lane; m < m1; m += rl) {
-      float d[8], u[8];
-      get8<T>(dy, m * dy_stride + n, cnt, vec_dy, d);
-      if (act) get8<T>(pre, m * N + n, cnt, vec_pre, u);
-      uint32_t bits = 0xff;
-      if (rng.drop) bits = keep_bits8(m * per_row + blk, key, rng.drop);
+    for (int64_t m = m0 + lane; m < m1; m += kDpreRows * rl) {
+      float d[kDpreRows][8] = {}, u[kDpreRows][8] = {};
+      uint32_t bits[kDpreRows];
+#pragma unroll
+      for (int q = 0; q < kDpreRows; ++q)
+        if (m + q * rl < m1) {
+          get8<T>(dy, (m + q * rl) * dy_stride + n, cnt, vec_dy, d[q]);
+          if (act) get8<T>(pre, (m + q * rl) * N + n, cnt, vec_pre, u[q]);
+        }
+#pragma unroll
+      for (int q = 0; q < kDpreRows; ++q)
+        bits[q] = rng.drop ? keep_bits8((m + q * rl) * per_row + blk, key, rng.drop) : 0xff;
       switch (act) {
-        case 1:
-#pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] *= act_grad_f(u[i] * f, 1);
-          break;
-        case 2:
-#pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] *= act_grad_f(u[i] * f, 2);
-          break;
-        case 3:
-#pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] *= act_grad_f(u[i] * f, 3);
-          break;
+        case 1: slope_rows<1>(d, u, f); break;
+        case 2: slope_rows<2>(d, u, f); break;
+        case 3: slope_rows<3>(d, u, f); break;
         default: break;
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        d[i] = bits >> i & 1 ? d[i] * f : 0.f;
-        sum[i] += d[i];
+      for (int q = 0; q < kDpreRows; ++q) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          d[q][i] = bits[q] >> i & 1 ? d[q][i] * f : 0.f;
+          if (m + q * rl < m1) sum[i] += d[q][i];
+        }
+        if (WRITE && m + q * rl < m1) store_planes<PLANES>(dpre + (m + q * rl) * ld + n, M * ld, d[q]);
       }
-      if (WRITE) store_planes<PLANES>(dpre + m * ld + n, M * ld, d);
     }
   }
   if (!part) return;
@@ -223,63 +232,88 @@ static int planes(const Operand& o, bool k_major, char** ws, cudaStream_t s, Pla
 constexpr int kSms = 148;
 
 struct Plan {
-  int bn;
+  bool pair;
   DenseWork w;
   size_t part_bytes;
 };
 
+// Tile (128 x 128 by one CTA, 256 x 256 by a pair) and cuts of the K loop: the
+// choice with the least estimated time.  The terms are measured: a 64-deep step
+// takes about 0.3 us in either, an item about 3 us around its steps, and joining
+// cut products a launch and their partials' way through memory.
 static Plan plan_product(int64_t M, int64_t N, int64_t K, int planes) {
-  Plan q;
-  q.w.tiles_m = (int)ceil_div(M, kBM);
-  q.w.kblocks = (int)ceil_div(K, kBK);
-  q.w.steps = q.w.kblocks * (planes == 3 ? 6 : 1);
-  q.bn = N <= 128 || q.w.tiles_m * ceil_div(N, 256) < kSms ? 128 : 256;
-  q.w.tiles_n = (int)ceil_div(N, q.bn);
-  // too few tiles for the SMs: cut the K loop, in parts of at least 8 steps
-  const int64_t tiles = (int64_t)q.w.tiles_m * q.w.tiles_n;
-  q.w.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / tiles, q.w.steps / 8));
-  q.part_bytes = q.w.splits > 1 ? round256((size_t)q.w.splits * M * N * sizeof(float)) : 0;
-  return q;
+  Plan best = {};
+  double least = 0;
+  for (int pair = 0; pair < 2; ++pair) {
+    DenseWork w;
+    w.tiles_m = (int)ceil_div(M, pair ? Tile<true>::kM : Tile<false>::kM);
+    w.tiles_n = (int)ceil_div(N, pair ? Tile<true>::kN : Tile<false>::kN);
+    w.kblocks = (int)ceil_div(K, kBK);
+    w.steps = w.kblocks * (planes == 3 ? 6 : 1);
+    const int64_t tiles = (int64_t)w.tiles_m * w.tiles_n, teams = pair ? kSms / 2 : kSms;
+    for (w.splits = 1; w.splits == 1 || (w.splits * tiles <= 2 * teams && w.splits * 4 <= w.steps); ++w.splits) {
+      const double rounds = (double)ceil_div(tiles * w.splits, teams);
+      double us = rounds * (ceil_div(w.steps, w.splits) * (pair ? 0.38 : 0.3) + 3);
+      if (w.splits > 1) us += 4.0 + 2.0 * w.splits * (double)M * N * 4 / 5e6;
+      if (least == 0 || us < least) {
+        best.pair = pair;
+        best.w = w;
+        least = us;
+      }
+    }
+  }
+  best.part_bytes = best.w.splits > 1 ? round256((size_t)best.w.splits * M * N * sizeof(float)) : 0;
+  return best;
 }
 
-static bool operand_map(CUtensorMap* m, const Planes& o, int64_t rows, int64_t cols, int planes, int box_rows) {
+static bool operand_map(CUtensorMap* m, const Planes& o, int64_t rows, int64_t cols, int planes) {
   const uint64_t ld = (uint64_t)o.ld * 2;
   return make_map(m, o.base, true, cols, rows, planes, ld, planes == 3 ? (uint64_t)o.plane * 2 : ld, kBK,
-                  o.k_major ? box_rows : kBK, CU_TENSOR_MAP_SWIZZLE_128B);
+                  o.k_major ? 128 : kBK, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <bool A_MN, bool B_MN, int BN>
+template <bool A_MN, bool B_MN, bool PAIR, typename T>
 static int launch_mma(const DenseEpi& e, const Plan& q, const CUtensorMap& ma, const CUtensorMap& mb, int32_t* status,
                       cudaStream_t s) {
-  const auto kernel = dense_mma_kernel<A_MN, B_MN, BN>;
-  const cudaError_t err =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MmaSmem<BN>::kBytes);
+  const auto kernel = dense_mma_kernel<A_MN, B_MN, PAIR, T>;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<PAIR>::kBytes);
   if (err != cudaSuccess) return launch_error("cudaFuncSetAttribute(dense)", err);
   const int items = q.w.tiles_m * q.w.tiles_n * q.w.splits;
-  kernel<<<std::min(items, kSms), kMmaThreads, MmaSmem<BN>::kBytes, s>>>(ma, mb, e, q.w, status);
-  return launched("launch dense product kernel", 1);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(PAIR ? 2 * std::min(items, kSms / 2) : std::min(items, kSms));
+  cfg.blockDim = dim3(kMmaThreads);
+  cfg.dynamicSmemBytes = Tile<PAIR>::kBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  err = cudaLaunchKernelEx(&cfg, kernel, ma, mb, e, q.w, status);
+  note_launches(1);
+  return err == cudaSuccess ? SSM_OK : launch_error("launch dense product kernel", err);
 }
 
 // e.M, e.N, e.K, e.a, e.b and the epilogue are set; `part` holds plan_product's part_bytes.
-template <bool A_MN, bool B_MN>
+template <bool A_MN, bool B_MN, typename T>
 static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
   const Plan q = plan_product(e.M, e.N, e.K, e.planes);
   if ((int64_t)q.w.tiles_m * q.w.tiles_n * q.w.splits > 0x7fffffff) return SSM_ERR_SHAPE;
   CUtensorMap ma, mb;
-  if (!operand_map(&ma, e.a, A_MN ? e.K : e.M, A_MN ? e.M : e.K, e.planes, kBM) ||
-      !operand_map(&mb, e.b, B_MN ? e.K : e.N, B_MN ? e.N : e.K, e.planes, q.bn))
+  if (!operand_map(&ma, e.a, A_MN ? e.K : e.M, A_MN ? e.M : e.K, e.planes) ||
+      !operand_map(&mb, e.b, B_MN ? e.K : e.N, B_MN ? e.N : e.K, e.planes))
     return SSM_ERR_LAUNCH;
   DenseEpi first = e;
   if (q.w.splits > 1) {
-    first.out = part;
-    first.out_kind = kOutPartial;
-    first.pre = nullptr;
+    first.partial = part;
+    first.residual = first.bias = nullptr;
   }
-  int st = q.bn == 256 ? launch_mma<A_MN, B_MN, 256>(first, q, ma, mb, status, s)
-                       : launch_mma<A_MN, B_MN, 128>(first, q, ma, mb, status, s);
+  int st = q.pair ? launch_mma<A_MN, B_MN, true, T>(first, q, ma, mb, status, s)
+                  : launch_mma<A_MN, B_MN, false, T>(first, q, ma, mb, status, s);
   if (st || q.w.splits == 1) return st;
   const int64_t blocks = e.M * ((e.N + 7) / 8);
-  dense_join_kernel<<<(unsigned)ceil_div(blocks, 256), 256, 0, s>>>(part, q.w.splits, e);
+  dense_join_kernel<T><<<(unsigned)ceil_div(blocks, 256), 256, 0, s>>>(part, q.w.splits, e);
   return launched("launch dense join kernel", 1);
 }
 
@@ -295,7 +329,6 @@ static int dense_fwd(const ssm_dense_params_t* p, cudaStream_t s) {
   e.N = p->fout;
   e.K = p->fin;
   e.planes = planes_of(p);
-  e.out_kind = p->dtype == SSM_BF16 ? kOutBF16 : kOutF32;
   e.out = p->y;
   e.bias = p->bias;
   e.bias_bf16 = p->bias_dtype == SSM_BF16;
@@ -305,7 +338,9 @@ static int dense_fwd(const ssm_dense_params_t* p, cudaStream_t s) {
   e.pre = p->pre;
   e.per_row = (p->fout + 7) / 8;
   e.rng = drop_rng(p);
-  return product<false, true>(e, reinterpret_cast<float*>(ws), p->status, s);
+  float* part = reinterpret_cast<float*>(ws);
+  return p->dtype == SSM_BF16 ? product<false, true, __nv_bfloat16>(e, part, p->status, s)
+                              : product<false, true, float>(e, part, p->status, s);
 }
 
 // How the dpre pass cuts (rows, fout): cb blocks of eight columns a CTA, `run` rows.
@@ -320,7 +355,7 @@ static DpreGeom dpre_geom(const ssm_dense_params_t* p) {
   g.cb = (int)ceil_div(per_row, g.tiles);
   const int rl = 256 / g.cb;
   const int64_t want = ceil_div(6 * kSms, g.tiles);
-  g.run = std::max<int64_t>(ceil_div(p->rows, want), 2 * rl);
+  g.run = std::max<int64_t>(ceil_div(p->rows, want), kDpreRows * rl);
   g.run = std::max(g.run, ceil_div(p->rows, 65535));
   g.parts = (int)ceil_div(p->rows, g.run);
   return g;
@@ -396,9 +431,10 @@ static int dense_bwd(const ssm_dense_params_t* p, cudaStream_t s) {
     e.M = p->rows;
     e.N = K;
     e.K = N;
-    e.out_kind = p->dtype == SSM_BF16 ? kOutBF16 : kOutF32;
     e.out = p->dx;
-    st = product<false, false>(e, reinterpret_cast<float*>(w), p->status, s);
+    float* part = reinterpret_cast<float*>(w);
+    st = p->dtype == SSM_BF16 ? product<false, false, __nv_bfloat16>(e, part, p->status, s)
+                              : product<false, false, float>(e, part, p->status, s);
     if (st) return st;
   }
   if (p->dkernel) {  // (rows, fin)^T (rows, fout)
@@ -410,9 +446,10 @@ static int dense_bwd(const ssm_dense_params_t* p, cudaStream_t s) {
     e.M = K;
     e.N = N;
     e.K = p->rows;
-    e.out_kind = p->dkernel_dtype == SSM_BF16 ? kOutBF16 : kOutF32;
     e.out = p->dkernel;
-    st = product<true, true>(e, reinterpret_cast<float*>(ws + bytes.x + bytes.kernel), p->status, s);
+    float* part = reinterpret_cast<float*>(ws + bytes.x + bytes.kernel);
+    st = p->dkernel_dtype == SSM_BF16 ? product<true, true, __nv_bfloat16>(e, part, p->status, s)
+                                      : product<true, true, float>(e, part, p->status, s);
   }
   return st;
 }

@@ -21,8 +21,6 @@
 
 namespace ssm {
 
-enum DenseOut { kOutF32 = 0, kOutBF16 = 1, kOutPartial = 2 };
-
 // bf16 planes of an operand, element (row, col) of plane p at
 // base[p * plane + row * ld + col]; `cols` is its contiguous axis.
 struct Planes {
@@ -40,8 +38,8 @@ struct DenseEpi {
   int32_t N;
   int32_t planes;      // 1 or 3
   Planes a, b;
-  int32_t out_kind;    // DenseOut
-  void* out;           // (M, N) dense, or partials (splits, M, N) fp32
+  void* out;           // (M, N) dense, of the kernel's type T
+  float* partial;      // not null: the sums go here, (splits, M, N), and nothing else is done
   // the forward's epilogue; all absent for the gradients' products
   const void* bias;
   int32_t bias_bf16;
@@ -94,6 +92,20 @@ struct EpiConst {
   }
 };
 
+template <int ACT, int R>
+__device__ __forceinline__ void act_rows(float (&v)[R][8]) {
+#pragma unroll
+  for (int q = 0; q < R; ++q)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[q][i] = act_f(v[q][i], ACT);
+}
+
+__device__ __noinline__ float dense_again(const DenseEpi& e, int64_t m, int n) {
+  float s = 0.f;
+  for (int64_t k = 0; k < e.K; ++k) s = fmaf(e.a.at(m, k), e.b.at(n, k), s);
+  return s;
+}
+
 // bias of columns n .. n+7, zeros where there is none
 __device__ __forceinline__ void dense_bias8(const DenseEpi& e, int n, float (&b)[8]) {
 #pragma unroll
@@ -105,63 +117,69 @@ __device__ __forceinline__ void dense_bias8(const DenseEpi& e, int n, float (&b)
   }
 }
 
-// Columns n .. n+7 (those below N) of row m from the summed products v.
-__device__ __forceinline__ void dense_epilogue8(const DenseEpi& e, const EpiConst& c, int64_t m, int n,
-                                                const float (&bias)[8], float (&v)[8]) {
+// What an epilogue does to columns n .. n+7 of R rows, from the summed products
+// v: written stage by stage over all rows, with stores as the only conditional
+// part, so that the rows' chains (ten dependent rounds of the generator, the
+// activation) overlap.  `res` holds the residual's values; rows beyond M are
+// marked by m < 0.
+template <typename T, int R>
+__device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst& c, const int64_t (&m)[R], int n,
+                                               const float (&bias)[8], const float (&res)[R][8], float (&v)[R][8]) {
   const int cnt = min(8, e.N - n);
-  if (e.planes == 3) {
+  if (sizeof(T) == 4) {
     // An infinite operand has no finite planes besides its first, and infinity
     // times the other operand's planes gives NaN where the product is infinite.
     // Such elements are summed again from the fp32 values.
+    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < cnt && isnan(v[i])) {
-        float s = 0.f;
-        for (int64_t k = 0; k < e.K; ++k) s = fmaf(e.a.at(m, k), e.b.at(n + i, k), s);
-        v[i] = s;
-      }
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) bad |= isnan(v[q][i]);
+    if (bad) {
+#pragma unroll
+      for (int q = 0; q < R; ++q)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (isnan(v[q][i]) && m[q] >= 0 && i < cnt) v[q][i] = dense_again(e, m[q], n + i);
+    }
   }
-  const int64_t off = m * e.N + n;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] += bias[i];
+  for (int q = 0; q < R; ++q)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[q][i] += bias[i];
   if (e.pre) {
-    if (e.out_kind == kOutBF16) put8<__nv_bfloat16>(e.pre, off, cnt, c.vec_out, v);
-    else put8<float>(e.pre, off, cnt, c.vec_out, v);
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      if (m[q] >= 0) put8<T>(e.pre, m[q] * e.N + n, cnt, c.vec_out, v[q]);
   }
   if (e.rng.drop) {
-    const uint32_t bits = keep_bits8(m * e.per_row + n / 8, c.key, e.rng.drop);
+    uint32_t bits[R];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = bits >> i & 1 ? v[i] * c.f : 0.f;
+    for (int q = 0; q < R; ++q) bits[q] = keep_bits8(m[q] * e.per_row + n / 8, c.key, e.rng.drop);
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[q][i] = bits[q] >> i & 1 ? v[q][i] * c.f : 0.f;
   }
   switch (e.act) {
-    case 1:
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_f(v[i], 1);
-      break;
-    case 2:
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_f(v[i], 2);
-      break;
-    case 3:
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_f(v[i], 3);
-      break;
+    case 1: act_rows<1, R>(v); break;
+    case 2: act_rows<2, R>(v); break;
+    case 3: act_rows<3, R>(v); break;
     default: break;
   }
   if (e.residual) {
-    float r[8];
-    const int64_t ro = m * e.res_stride + n;
-    if (e.out_kind == kOutBF16) get8<__nv_bfloat16>(e.residual, ro, cnt, c.vec_res, r);
-    else get8<float>(e.residual, ro, cnt, c.vec_res, r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += r[i];
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[q][i] += res[q][i];
   }
-  if (e.out_kind == kOutBF16) put8<__nv_bfloat16>(e.out, off, cnt, c.vec_out, v);
-  else put8<float>(e.out, off, cnt, c.vec_out, v);
+#pragma unroll
+  for (int q = 0; q < R; ++q)
+    if (m[q] >= 0) put8<T>(e.out, m[q] * e.N + n, cnt, c.vec_out, v[q]);
 }
 
 // ---------------------------------------------------------------- tensor-core pieces
-constexpr int kBM = 128, kBK = 64;
+constexpr int kBM = 128, kBK = 64;  // rows of a CTA's tile, depth of a step
 constexpr int kMmaThreads = 384;
 constexpr int kEpiWarps = 8;
 // Polls before a wait gives up; a tile takes microseconds, so this is far above any wait that ends.
@@ -175,21 +193,90 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
   constexpr uint64_t kLead = 8192 >> 4, kStep = 1024 >> 4;
   return (uint64_t)((addr >> 4) & 0x3fff) | kLead << 16 | kStep << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-// bf16 x bf16 -> fp32, M rows, N columns
+// bf16 x bf16 -> fp32, m rows, n columns
 constexpr uint32_t mma_idesc(int m, int n, bool a_mn, bool b_mn) {
   return 1u << 4 | 1u << 7 | 1u << 10 | (a_mn ? 1u : 0u) << 15 | (b_mn ? 1u : 0u) << 16 | (uint32_t)(n >> 3) << 17 |
          (uint32_t)(m >> 4) << 24;
 }
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
+
+// The instructions that differ between a CTA of its own and a pair of CTAs (a
+// cluster of two) that share one product: the pair's first CTA issues for both.
+template <bool PAIR>
+struct Mma {
+  __device__ __forceinline__ static void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (PAIR)
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+          "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+          "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+          : "memory");
+    else
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+          "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+          "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+          : "memory");
+  }
+  // arrives on `bar` (of both CTAs of a pair) when the products issued so far are done
+  __device__ __forceinline__ static void commit(uint64_t* bar) {
+    if constexpr (PAIR)
+      asm volatile(
+          "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+              smem_u32(bar)),
+          "h"((uint16_t)3)
+          : "memory");
+    else
+      asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                   : "memory");
+  }
+  __device__ __forceinline__ static void alloc(uint32_t* dst, uint32_t ncols) {
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(ncols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(dst, ncols);
+    }
+  }
+  __device__ __forceinline__ static void dealloc(uint32_t t, uint32_t ncols) {
+    if constexpr (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(ncols) : "memory");
+    else
+      tmem_dealloc(t, ncols);
+  }
+  // a box to this CTA's `dst`, counted on `bar`: an address in the cluster's
+  // shared memory, for a pair that of the first CTA's barrier
+  __device__ __forceinline__ static void load(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+    if constexpr (PAIR)
+      asm volatile(
+          "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+          " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+          "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+          : "memory");
+    else
+      asm volatile(
+          "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+          " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+          "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+          : "memory");
+  }
+};
+// the same shared-memory address in the cluster's CTA 0
+__device__ __forceinline__ uint32_t in_first_cta(const void* p) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+  return r;
 }
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
 }
 
 struct DenseWork {
@@ -198,10 +285,16 @@ struct DenseWork {
   int32_t steps;    // kblocks * plane pairs
 };
 
-template <int BN>
-struct MmaSmem {
-  static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
-  static constexpr int kStages = BN == 256 ? 4 : 6;
+// A CTA of its own makes a tile of 128 x 128, a pair one of 256 x 256: each CTA
+// of it holds 128 rows of A and 128 columns of B and accumulates its 128 rows
+// of all 256 columns, so a step moves 32 KB into each SM for twice the products
+// that 32 KB give a single CTA.
+template <bool PAIR>
+struct Tile {
+  static constexpr int kM = PAIR ? 256 : 128, kN = PAIR ? 256 : 128;  // of the item
+  static constexpr int kBoxA = 128, kBoxB = 128;                      // rows or columns one CTA loads
+  static constexpr int kA = kBoxA * kBK * 2, kB = kBoxB * kBK * 2, kStage = kA + kB;
+  static constexpr int kStages = 6;
   static constexpr int kEpi = kEpiWarps * 4096;  // 32 x 32 fp32 for each epilogue warp
   static constexpr int kBytes = kStages * kStage + kEpi + 1024;  // and alignment
 };
@@ -216,17 +309,20 @@ __device__ __forceinline__ void plane_pair(int planes, int seg, int& pa, int& pb
   pb = 0x010210 >> (4 * seg) & 15;  // 0 1 2 0 1 0
 }
 
-template <bool A_MN, bool B_MN, int BN>
+template <bool A_MN, bool B_MN, bool PAIR, typename T>
 __global__ void __launch_bounds__(kMmaThreads, 1)
     dense_mma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                      const __grid_constant__ DenseEpi e, const DenseWork w, int32_t* status) {
-  using S = MmaSmem<BN>;
+  using S = Tile<PAIR>;
+  using I = Mma<PAIR>;
+  constexpr int BN = S::kN;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base;
   __shared__ volatile int dead;
   uint8_t* tiles = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = PAIR ? (int)cluster_rank() : 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&full[i], 1);
@@ -234,19 +330,22 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], kEpiWarps);
+      mbar_init(&acc_empty[i], PAIR ? 2 * kEpiWarps : kEpiWarps);
     }
     dead = 0;
     fence_mbar_init();
     tma_prefetch_desc(&map_a);
     tma_prefetch_desc(&map_b);
   }
-  if (warp == 2) tmem_alloc(&tmem_base, 2 * BN);
+  __syncthreads();
+  if constexpr (PAIR) cluster_barrier();
+  if (warp == 2) I::alloc(&tmem_base, 2 * BN);
   tmem_fence_before_sync();
   __syncthreads();
   tmem_fence_after_sync();
   const uint32_t tmem = tmem_base;
   const int items = w.tiles_m * w.tiles_n * w.splits;
+  const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
 
   // Bounded wait; a role that gives up (or sees that another did) stops.
   const auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -263,9 +362,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-      const int n0 = item % w.tiles_n * BN, rest = item / w.tiles_n;
-      const int m0 = rest % w.tiles_m * kBM, split = rest / w.tiles_m;
+    for (int item = first; ok && item < items; item += stride) {
+      const int rest = item / w.tiles_n, split = rest / w.tiles_m;
+      const int n0 = item % w.tiles_n * BN + (PAIR ? rank * 128 : 0);
+      const int m0 = rest % w.tiles_m * S::kM + (PAIR ? rank * 128 : 0);
       const int t0 = (int)((int64_t)w.steps * split / w.splits), t1 = (int)((int64_t)w.steps * (split + 1) / w.splits);
       for (int t = t0; t < t1; ++t) {
         if (!wait(&empty[stage], phase ^ 1)) {
@@ -277,18 +377,19 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         plane_pair(e.planes, seg, pa, pb);
         uint8_t* sa = tiles + stage * S::kStage;
         uint8_t* sb = sa + S::kA;
-        mbar_arrive_expect_tx(&full[stage], S::kStage);
+        const uint32_t bar = PAIR ? in_first_cta(&full[stage]) : smem_u32(&full[stage]);
+        if (rank == 0) mbar_arrive_expect_tx(&full[stage], PAIR ? 2 * S::kStage : S::kStage);
         if (A_MN) {
 #pragma unroll
-          for (int j = 0; j < kBM / 64; ++j) tma_load_3d(sa + j * 8192, &map_a, &full[stage], m0 + 64 * j, k0, pa);
+          for (int j = 0; j < S::kBoxA / 64; ++j) I::load(sa + j * 8192, &map_a, bar, m0 + 64 * j, k0, pa);
         } else {
-          tma_load_3d(sa, &map_a, &full[stage], k0, m0, pa);
+          I::load(sa, &map_a, bar, k0, m0, pa);
         }
         if (B_MN) {
 #pragma unroll
-          for (int j = 0; j < BN / 64; ++j) tma_load_3d(sb + j * 8192, &map_b, &full[stage], n0 + 64 * j, k0, pb);
+          for (int j = 0; j < S::kBoxB / 64; ++j) I::load(sb + j * 8192, &map_b, bar, n0 + 64 * j, k0, pb);
         } else {
-          tma_load_3d(sb, &map_b, &full[stage], k0, n0, pb);
+          I::load(sb, &map_b, bar, k0, n0, pb);
         }
         if (++stage == S::kStages) {
           stage = 0;
@@ -298,7 +399,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     }
     // Loads still in flight when the products stopped early: wait for the last
     // ones so that none lands after the CTA has gone.
-    if (!ok)
+    if (!ok && rank == 0)
       for (int i = 0; i < S::kStages; ++i) {
         mbar_wait_bounded(&full[stage], phase ^ 1, 1u << 16);
         if (++stage == S::kStages) {
@@ -306,13 +407,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           phase ^= 1;
         }
       }
-  } else if (warp == 1 && lane == 0) {
-    constexpr uint32_t idesc = mma_idesc(kBM, BN, A_MN, B_MN);
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    constexpr uint32_t idesc = mma_idesc(S::kM, BN, A_MN, B_MN);
     constexpr uint32_t kStepA = (A_MN ? 2048 : 32) >> 4, kStepB = (B_MN ? 2048 : 32) >> 4;
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
-    for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+    for (int item = first; ok && item < items; item += stride) {
       const int split = item / w.tiles_n / w.tiles_m;
       const int t0 = (int)((int64_t)w.steps * split / w.splits), t1 = (int)((int64_t)w.steps * (split + 1) / w.splits);
       if (!wait(&acc_empty[acc], acc_phase ^ 1)) break;
@@ -327,14 +428,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         const uint32_t sa = smem_u32(tiles + stage * S::kStage);
         const uint64_t da = smem_desc(sa), db = smem_desc(sa + S::kA);
 #pragma unroll
-        for (int k = 0; k < kBK / 16; ++k) mma_f16(d, da + k * kStepA, db + k * kStepB, idesc, t > t0 || k > 0);
-        mma_commit(&empty[stage]);
+        for (int k = 0; k < kBK / 16; ++k) I::mma(d, da + k * kStepA, db + k * kStepB, idesc, t > t0 || k > 0);
+        I::commit(&empty[stage]);
         if (++stage == S::kStages) {
           stage = 0;
           phase ^= 1;
         }
       }
-      mma_commit(&acc_full[acc]);
+      I::commit(&acc_full[acc]);
       if (!ok) mbar_wait_bounded(&acc_full[acc], acc_phase, 1u << 16);  // products still running use the buffers
       if (++acc == 2) {
         acc = 0;
@@ -347,16 +448,21 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     uint4* stage = reinterpret_cast<uint4*>(tiles + S::kStages * S::kStage) + (warp - 4) * 256;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-      const int n0 = item % w.tiles_n * BN, rest = item / w.tiles_n;
-      const int64_t m0 = (int64_t)(rest % w.tiles_m) * kBM + quarter * 32;
-      const int split = rest / w.tiles_m;
+    for (int item = first; item < items; item += stride) {
+      const int rest = item / w.tiles_n, split = rest / w.tiles_m;
+      const int n0 = item % w.tiles_n * BN + half * (BN / 2);
+      const int64_t m0 = (int64_t)(rest % w.tiles_m) * S::kM + rank * 128 + quarter * 32;
+      if (e.residual && m0 + lane < e.M) {  // on its way to L2 while the products run
+        const char* r = static_cast<const char*>(e.residual) + ((m0 + lane) * e.res_stride + n0) * sizeof(T);
+        const int bytes = min(BN / 2, e.N - n0) * (int)sizeof(T);
+        for (int o = 0; o < bytes; o += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(r + o));
+      }
       if (!__all_sync(0xffffffffu, wait(&acc_full[acc], acc_phase))) break;
       tmem_fence_after_sync();
       const uint32_t src = tmem + acc * BN + half * (BN / 2) + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
       for (int j = 0; j < BN / 2; j += 32) {
-        const int n = n0 + half * (BN / 2) + j;
+        const int n = n0 + j;
         if (n >= e.N) break;
         // A lane reads 32 columns of its own row of the accumulator; through
         // shared memory (16-byte pieces, swizzled by row) it gets eight
@@ -366,8 +472,16 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         tmem_ld16(src + j, r[0]);
         tmem_ld16(src + j + 16, r[1]);
         const int nl = n + (lane & 3) * 8;
-        float bias[8];
+        const bool in = nl < e.N;
+        float bias[8], res[4][8] = {};
+        int64_t m[4];
         dense_bias8(e, nl, bias);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          m[q] = m0 + q * 8 + (lane >> 2);
+          if (m[q] >= e.M || !in) m[q] = -1;
+          if (e.residual && m[q] >= 0) get8<T>(e.residual, m[q] * e.res_stride + nl, e.N - nl, c.vec_res, res[q]);
+        }
         tmem_wait_ld();
         __syncwarp();
 #pragma unroll
@@ -375,23 +489,31 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           stage[lane * 8 + (q ^ (lane & 7))] = make_uint4(r[q >> 2][(q & 3) * 4], r[q >> 2][(q & 3) * 4 + 1],
                                                           r[q >> 2][(q & 3) * 4 + 2], r[q >> 2][(q & 3) * 4 + 3]);
         __syncwarp();
+        float v[4][8];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int row = q * 8 + (lane >> 2);
-          const int64_t m = m0 + row;
           const uint4 lo = stage[row * 8 + (((lane & 3) * 2) ^ (row & 7))];
           const uint4 hi = stage[row * 8 + (((lane & 3) * 2 + 1) ^ (row & 7))];
-          float v[8] = {__uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w),
-                        __uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w)};
-          if (m >= e.M || nl >= e.N) continue;
-          if (e.out_kind == kOutPartial)
-            put8<float>(e.out, ((int64_t)split * e.M + m) * e.N + nl, min(8, e.N - nl), c.vec_out, v);
-          else
-            dense_epilogue8(e, c, m, nl, bias, v);
+          v[q][0] = __uint_as_float(lo.x); v[q][1] = __uint_as_float(lo.y);
+          v[q][2] = __uint_as_float(lo.z); v[q][3] = __uint_as_float(lo.w);
+          v[q][4] = __uint_as_float(hi.x); v[q][5] = __uint_as_float(hi.y);
+          v[q][6] = __uint_as_float(hi.z); v[q][7] = __uint_as_float(hi.w);
+        }
+        if (e.partial) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (m[q] >= 0)
+              put8<float>(e.partial, ((int64_t)split * e.M + m[q]) * e.N + nl, min(8, e.N - nl), e.N % 8 == 0, v[q]);
+        } else {
+          dense_epilogue<T, 4>(e, c, m, nl, bias, res, v);
         }
       }
       tmem_fence_before_sync();
-      if (lane == 0) mbar_arrive(&acc_empty[acc]);
+      if (lane == 0) {
+        if constexpr (PAIR) arrive_cluster(in_first_cta(&acc_empty[acc]));
+        else mbar_arrive(&acc_empty[acc]);
+      }
       __syncwarp();
       if (++acc == 2) {
         acc = 0;
@@ -402,29 +524,31 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   __syncwarp();
   tmem_fence_before_sync();
   __syncthreads();
+  if constexpr (PAIR) cluster_barrier();  // the other CTA's products, loads and arrivals reach into this one
   tmem_fence_after_sync();
-  if (warp == 2) tmem_dealloc(tmem, 2 * BN);
+  if (warp == 2) I::dealloc(tmem, 2 * BN);
 }
 
 // The epilogue of a product whose K loop was cut: the parts summed in order.
+template <typename T>
 __global__ void __launch_bounds__(256) dense_join_kernel(const float* part, int splits, const __grid_constant__ DenseEpi e) {
   const EpiConst c(e);
   const int64_t blocks = e.M * ((e.N + 7) / 8), per = (e.N + 7) / 8;
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= blocks) return;
-  const int64_t m = i / per;
-  const int n = (int)(i - m * per) * 8, cnt = min(8, e.N - n);
+  const int64_t m[1] = {i / per};
+  const int n = (int)(i - m[0] * per) * 8, cnt = min(8, e.N - n);
   const bool vec = e.N % 8 == 0;
-  float v[8], t[8];
-  get8<float>(part, m * e.N + n, cnt, vec, v);
+  float v[1][8], t[8], bias[8], res[1][8] = {};
+  get8<float>(part, m[0] * e.N + n, cnt, vec, v[0]);
   for (int s = 1; s < splits; ++s) {
-    get8<float>(part, ((int64_t)s * e.M + m) * e.N + n, cnt, vec, t);
+    get8<float>(part, ((int64_t)s * e.M + m[0]) * e.N + n, cnt, vec, t);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] += t[k];
+    for (int k = 0; k < 8; ++k) v[0][k] += t[k];
   }
-  float bias[8];
   dense_bias8(e, n, bias);
-  dense_epilogue8(e, c, m, n, bias, v);
+  if (e.residual) get8<T>(e.residual, m[0] * e.res_stride + n, cnt, c.vec_res, res[0]);
+  dense_epilogue<T, 1>(e, c, m, n, bias, res, v);
 }
 
 }  // namespace ssm
