@@ -367,14 +367,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const int n0 = item % w.tiles_n * BN + (PAIR ? rank * 128 : 0);
       const int m0 = rest % w.tiles_m * S::kM + (PAIR ? rank * 128 : 0);
       const int t0 = (int)((int64_t)w.steps * split / w.splits), t1 = (int)((int64_t)w.steps * (split + 1) / w.splits);
+      int seg = t0 / w.kblocks, kb = t0 - seg * w.kblocks, pa, pb;
+      plane_pair(e.planes, seg, pa, pb);
       for (int t = t0; t < t1; ++t) {
         if (!wait(&empty[stage], phase ^ 1)) {
           ok = false;
           break;
         }
-        int pa, pb;
-        const int seg = t / w.kblocks, k0 = (t - seg * w.kblocks) * kBK;
-        plane_pair(e.planes, seg, pa, pb);
+        const int k0 = kb * kBK;
         uint8_t* sa = tiles + stage * S::kStage;
         uint8_t* sb = sa + S::kA;
         const uint32_t bar = PAIR ? in_first_cta(&full[stage]) : smem_u32(&full[stage]);
@@ -390,6 +390,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           for (int j = 0; j < S::kBoxB / 64; ++j) I::load(sb + j * 8192, &map_b, bar, n0 + 64 * j, k0, pb);
         } else {
           I::load(sb, &map_b, bar, k0, n0, pb);
+        }
+        if (++kb == w.kblocks) {
+          kb = 0;
+          plane_pair(e.planes, ++seg, pa, pb);
         }
         if (++stage == S::kStages) {
           stage = 0;
@@ -419,21 +423,28 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       if (!wait(&acc_empty[acc], acc_phase ^ 1)) break;
       tmem_fence_after_sync();
       const uint32_t d = tmem + acc * BN;
+      bool ready = false;
       for (int t = t0; t < t1; ++t) {
-        if (!wait(&full[stage], phase)) {
+        if (!ready && !wait(&full[stage], phase)) {
           ok = false;
           break;
         }
         tmem_fence_after_sync();
         const uint32_t sa = smem_u32(tiles + stage * S::kStage);
         const uint64_t da = smem_desc(sa), db = smem_desc(sa + S::kA);
-#pragma unroll
-        for (int k = 0; k < kBK / 16; ++k) I::mma(d, da + k * kStepA, db + k * kStepB, idesc, t > t0 || k > 0);
-        I::commit(&empty[stage]);
+        uint64_t* const used = &empty[stage];
         if (++stage == S::kStages) {
           stage = 0;
           phase ^= 1;
         }
+        // The queue of products is short: a barrier asked about after the last
+        // one is issued leaves the tensor core idle for the answer's 250
+        // cycles of every 510, so the next step's is asked about before.
+        I::mma(d, da, db, idesc, t > t0);
+        ready = t + 1 < t1 && mbar_try_wait(&full[stage], phase);
+#pragma unroll
+        for (int k = 1; k < kBK / 16; ++k) I::mma(d, da + k * kStepA, db + k * kStepB, idesc, 1);
+        I::commit(used);
       }
       I::commit(&acc_full[acc]);
       if (!ok) mbar_wait_bounded(&acc_full[acc], acc_phase, 1u << 16);  // products still running use the buffers
