@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256)
     const int cnt = min(8, N - n);
     for (int64_t m = m0 + lane; m < m1; m += kDpreRows * rl) {
       float d[kDpreRows][8] = {}, u[kDpreRows][8] = {};
-      uint32_t bits[kDpreRows];
+      uint4 w[kDpreRows];
 #pragma unroll
       for (int q = 0; q < kDpreRows; ++q)
         if (m + q * rl < m1) {
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(256)
         }
 #pragma unroll
       for (int q = 0; q < kDpreRows; ++q)
-        bits[q] = rng.drop ? keep_bits8((m + q * rl) * per_row + blk, key, rng.drop) : 0xff;
+        if (rng.drop) w[q] = philox4x32_10((m + q * rl) * per_row + blk, key);
       switch (act) {
         case 1: slope_rows<1>(d, u, f); break;
         case 2: slope_rows<2>(d, u, f); break;
@@ -117,11 +117,9 @@ __global__ void __launch_bounds__(256)
       }
 #pragma unroll
       for (int q = 0; q < kDpreRows; ++q) {
+        if (rng.drop) drop8(w[q], rng.drop, f, d[q]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          d[q][i] = bits[q] >> i & 1 ? d[q][i] * f : 0.f;
-          if (m + q * rl < m1) sum[i] += d[q][i];
-        }
+        for (int i = 0; i < 8; ++i) sum[i] += d[q][i];  // rows past the end hold zeros
         if (WRITE && m + q * rl < m1) store_planes<PLANES>(dpre + (m + q * rl) * ld + n, M * ld, d[q]);
       }
     }
@@ -246,8 +244,8 @@ static Plan plan_product(int64_t M, int64_t N, int64_t K, int planes) {
   double least = 0;
   for (int pair = 0; pair < 2; ++pair) {
     DenseWork w;
-    w.tiles_m = (int)ceil_div(M, pair ? Tile<true>::kM : Tile<false>::kM);
-    w.tiles_n = (int)ceil_div(N, pair ? Tile<true>::kN : Tile<false>::kN);
+    w.tiles_m = (int)ceil_div(M, pair ? Tile<true, float>::kM : Tile<false, float>::kM);
+    w.tiles_n = (int)ceil_div(N, pair ? Tile<true, float>::kN : Tile<false, float>::kN);
     w.kblocks = (int)ceil_div(K, kBK);
     w.steps = w.kblocks * (planes == 3 ? 6 : 1);
     const int64_t tiles = (int64_t)w.tiles_m * w.tiles_n, teams = pair ? kSms / 2 : kSms;
@@ -276,13 +274,13 @@ template <bool A_MN, bool B_MN, bool PAIR, typename T>
 static int launch_mma(const DenseEpi& e, const Plan& q, const CUtensorMap& ma, const CUtensorMap& mb, int32_t* status,
                       cudaStream_t s) {
   const auto kernel = dense_mma_kernel<A_MN, B_MN, PAIR, T>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<PAIR>::kBytes);
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<PAIR, T>::kBytes);
   if (err != cudaSuccess) return launch_error("cudaFuncSetAttribute(dense)", err);
   const int items = q.w.tiles_m * q.w.tiles_n * q.w.splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(PAIR ? 2 * std::min(items, kSms / 2) : std::min(items, kSms));
   cfg.blockDim = dim3(kMmaThreads);
-  cfg.dynamicSmemBytes = Tile<PAIR>::kBytes;
+  cfg.dynamicSmemBytes = Tile<PAIR, T>::kBytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

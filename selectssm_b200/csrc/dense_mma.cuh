@@ -7,7 +7,7 @@
 // in and only the last K / 16 steps round at the size of the result.
 //
 // A persistent CTA walks over items (tile of 128 x BN, part of the K loop).
-// Warp 0 moves 64-deep slices of the operands to shared memory by TMA (128-byte
+// Warps 0 and 3 move 64-deep slices of A and of B to shared memory by TMA (128-byte
 // swizzle), warp 1 issues the products, and warps 4 to 11 read the finished
 // accumulator from tensor memory, apply the epilogue and store; two
 // accumulators let the epilogue of one tile overlap the products of the next.
@@ -77,7 +77,7 @@ __device__ __forceinline__ void get8(const void* base, int64_t off, int cnt, boo
 struct EpiConst {
   PhiloxKey key;
   float f;
-  bool vec_out, vec_res;
+  bool vec_out, vec_res, vec_bias;
   __device__ __forceinline__ explicit EpiConst(const DenseEpi& e) {
     key = {};
     f = 1.f;
@@ -88,6 +88,7 @@ struct EpiConst {
     // rows of a multiple of 8 elements from a 16-byte aligned start
     const auto a16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     vec_out = e.N % 8 == 0 && a16(e.out) && a16(e.pre);
+    vec_bias = e.N % 8 == 0 && a16(e.bias);
     vec_res = e.residual && e.N % 8 == 0 && e.res_stride % 8 == 0 && a16(e.residual);
   }
 };
@@ -107,14 +108,12 @@ __device__ __noinline__ float dense_again(const DenseEpi& e, int64_t m, int n) {
 }
 
 // bias of columns n .. n+7, zeros where there is none
-__device__ __forceinline__ void dense_bias8(const DenseEpi& e, int n, float (&b)[8]) {
+__device__ __forceinline__ void dense_bias8(const DenseEpi& e, const EpiConst& c, int n, float (&b)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    b[i] = 0.f;
-    if (e.bias && n + i < e.N)
-      b[i] = e.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[n + i])
-                         : static_cast<const float*>(e.bias)[n + i];
-  }
+  for (int i = 0; i < 8; ++i) b[i] = 0.f;
+  if (!e.bias || n >= e.N) return;
+  if (e.bias_bf16) get8<__nv_bfloat16>(e.bias, n, e.N - n, c.vec_bias, b);
+  else get8<float>(e.bias, n, e.N - n, c.vec_bias, b);
 }
 
 // What an epilogue does to columns n .. n+7 of R rows, from the summed products
@@ -153,13 +152,11 @@ __device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst
       if (m[q] >= 0) put8<T>(e.pre, m[q] * e.N + n, cnt, c.vec_out, v[q]);
   }
   if (e.rng.drop) {
-    uint32_t bits[R];
+    uint4 w[R];
 #pragma unroll
-    for (int q = 0; q < R; ++q) bits[q] = keep_bits8(m[q] * e.per_row + n / 8, c.key, e.rng.drop);
+    for (int q = 0; q < R; ++q) w[q] = philox4x32_10(m[q] * e.per_row + n / 8, c.key);
 #pragma unroll
-    for (int q = 0; q < R; ++q)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[q][i] = bits[q] >> i & 1 ? v[q][i] * c.f : 0.f;
+    for (int q = 0; q < R; ++q) drop8(w[q], e.rng.drop, c.f, v[q]);
   }
   switch (e.act) {
     case 1: act_rows<1, R>(v); break;
@@ -289,13 +286,18 @@ struct DenseWork {
 // of it holds 128 rows of A and 128 columns of B and accumulates its 128 rows
 // of all 256 columns, so a step moves 32 KB into each SM for twice the products
 // that 32 KB give a single CTA.
-template <bool PAIR>
+template <bool PAIR, typename T>
 struct Tile {
   static constexpr int kM = PAIR ? 256 : 128, kN = PAIR ? 256 : 128;  // of the item
   static constexpr int kBoxA = 128, kBoxB = 128;                      // rows or columns one CTA loads
   static constexpr int kA = kBoxA * kBK * 2, kB = kBoxB * kBK * 2, kStage = kA + kB;
   static constexpr int kStages = 6;
   static constexpr int kEpi = kEpiWarps * 4096;  // 32 x 32 fp32 for each epilogue warp
+  static constexpr int kChunks = kN / 64;        // of 32 columns, for an epilogue warp
+  // Two chunks of residual, 32 x 32 bf16 each, in the place of the last stage
+  // (not for fp32, where an item's products take six times as long).
+  static constexpr int kAhead = sizeof(T) == 2 ? 2 : 0;
+  static_assert(kEpiWarps * kAhead * 2048 <= kStage);
   static constexpr int kBytes = kStages * kStage + kEpi + 1024;  // and alignment
 };
 
@@ -313,7 +315,7 @@ template <bool A_MN, bool B_MN, bool PAIR, typename T>
 __global__ void __launch_bounds__(kMmaThreads, 1)
     dense_mma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                      const __grid_constant__ DenseEpi e, const DenseWork w, int32_t* status) {
-  using S = Tile<PAIR>;
+  using S = Tile<PAIR, T>;
   using I = Mma<PAIR>;
   constexpr int BN = S::kN;
   extern __shared__ uint8_t raw[];
@@ -345,6 +347,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   tmem_fence_after_sync();
   const uint32_t tmem = tmem_base;
   const int items = w.tiles_m * w.tiles_n * w.splits;
+  const bool ahead = S::kAhead && e.residual && EpiConst(e).vec_res;
+  const int stages = ahead ? S::kStages - 1 : S::kStages;
   const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
 
   // Bounded wait; a role that gives up (or sees that another did) stops.
@@ -358,7 +362,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     return false;
   };
 
-  if (warp == 0 && lane == 0) {
+  if ((warp == 0 || warp == 3) && lane == 0) {
+    // Warp 0 loads A, warp 3 loads B: the time from a slice's release to its
+    // next load is on the path that bounds the products.
+    const bool of_a = warp == 0;
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -378,14 +385,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         uint8_t* sa = tiles + stage * S::kStage;
         uint8_t* sb = sa + S::kA;
         const uint32_t bar = PAIR ? in_first_cta(&full[stage]) : smem_u32(&full[stage]);
-        if (rank == 0) mbar_arrive_expect_tx(&full[stage], PAIR ? 2 * S::kStage : S::kStage);
-        if (A_MN) {
+        if (rank == 0 && of_a) mbar_arrive_expect_tx(&full[stage], PAIR ? 2 * S::kStage : S::kStage);
+        if (of_a) {
+          if (A_MN) {
 #pragma unroll
-          for (int j = 0; j < S::kBoxA / 64; ++j) I::load(sa + j * 8192, &map_a, bar, m0 + 64 * j, k0, pa);
-        } else {
-          I::load(sa, &map_a, bar, k0, m0, pa);
-        }
-        if (B_MN) {
+            for (int j = 0; j < S::kBoxA / 64; ++j) I::load(sa + j * 8192, &map_a, bar, m0 + 64 * j, k0, pa);
+          } else {
+            I::load(sa, &map_a, bar, k0, m0, pa);
+          }
+        } else if (B_MN) {
 #pragma unroll
           for (int j = 0; j < S::kBoxB / 64; ++j) I::load(sb + j * 8192, &map_b, bar, n0 + 64 * j, k0, pb);
         } else {
@@ -395,7 +403,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           kb = 0;
           plane_pair(e.planes, ++seg, pa, pb);
         }
-        if (++stage == S::kStages) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1;
         }
@@ -404,9 +412,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     // Loads still in flight when the products stopped early: wait for the last
     // ones so that none lands after the CTA has gone.
     if (!ok && rank == 0)
-      for (int i = 0; i < S::kStages; ++i) {
+      for (int i = 0; i < stages; ++i) {
         mbar_wait_bounded(&full[stage], phase ^ 1, 1u << 16);
-        if (++stage == S::kStages) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1;
         }
@@ -433,7 +441,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         const uint32_t sa = smem_u32(tiles + stage * S::kStage);
         const uint64_t da = smem_desc(sa), db = smem_desc(sa + S::kA);
         uint64_t* const used = &empty[stage];
-        if (++stage == S::kStages) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1;
         }
@@ -457,24 +465,48 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     const EpiConst c(e);
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     uint4* stage = reinterpret_cast<uint4*>(tiles + S::kStages * S::kStage) + (warp - 4) * 256;
+    // The slices that TMA has asked for keep the SM's way from L2 busy: a plain
+    // load issued now is answered some 4000 cycles later, as long as a chunk
+    // takes.  So the residual is fetched to shared memory two chunks ahead, each
+    // lane its own pieces.
+    uint4* held = reinterpret_cast<uint4*>(tiles + (S::kStages - 1) * S::kStage) + (warp - 4) * 256;
+    int f_item = first, f_chunk = 0, slot = 0;  // next to fetch; where it goes and the oldest one is
+    const auto fetch = [&]() {
+      if (!ahead) return;
+      if (f_item < items) {
+        const int n = f_item % w.tiles_n * BN + half * (BN / 2) + f_chunk * 32 + (lane & 3) * 8;
+        const int64_t m = (int64_t)(f_item / w.tiles_n % w.tiles_m) * S::kM + rank * 128 + quarter * 32 + (lane >> 2);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (m + q * 8 < e.M && n < e.N)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(held + slot * 128 + q * 32 + lane)),
+                         "l"(static_cast<const T*>(e.residual) + (m + q * 8) * e.res_stride + n)
+                         : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      slot ^= 1;
+      if (++f_chunk == S::kChunks) {
+        f_chunk = 0;
+        f_item += stride;
+      }
+    };
+    for (int i = 0; i < S::kAhead; ++i) fetch();
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int item = first; item < items; item += stride) {
       const int rest = item / w.tiles_n, split = rest / w.tiles_m;
       const int n0 = item % w.tiles_n * BN + half * (BN / 2);
       const int64_t m0 = (int64_t)(rest % w.tiles_m) * S::kM + rank * 128 + quarter * 32;
-      if (e.residual && m0 + lane < e.M) {  // on its way to L2 while the products run
-        const char* r = static_cast<const char*>(e.residual) + ((m0 + lane) * e.res_stride + n0) * sizeof(T);
-        const int bytes = min(BN / 2, e.N - n0) * (int)sizeof(T);
-        for (int o = 0; o < bytes; o += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(r + o));
-      }
       if (!__all_sync(0xffffffffu, wait(&acc_full[acc], acc_phase))) break;
       tmem_fence_after_sync();
       const uint32_t src = tmem + acc * BN + half * (BN / 2) + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
-      for (int j = 0; j < BN / 2; j += 32) {
-        const int n = n0 + j;
-        if (n >= e.N) break;
+      for (int chunk = 0; chunk < S::kChunks; ++chunk) {
+        const int j = chunk * 32, n = n0 + j;
+        if (n >= e.N) {
+          fetch();
+          continue;
+        }
         // A lane reads 32 columns of its own row of the accumulator; through
         // shared memory (16-byte pieces, swizzled by row) it gets eight
         // columns of four rows, so that four lanes cover 32 columns of a row
@@ -486,12 +518,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         const bool in = nl < e.N;
         float bias[8], res[4][8] = {};
         int64_t m[4];
-        dense_bias8(e, nl, bias);
+        dense_bias8(e, c, nl, bias);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           m[q] = m0 + q * 8 + (lane >> 2);
           if (m[q] >= e.M || !in) m[q] = -1;
-          if (e.residual && m[q] >= 0) get8<T>(e.residual, m[q] * e.res_stride + nl, e.N - nl, c.vec_res, res[q]);
+          if (e.residual && !ahead && m[q] >= 0)
+            get8<T>(e.residual, m[q] * e.res_stride + nl, e.N - nl, c.vec_res, res[q]);
         }
         tmem_wait_ld();
         __syncwarp();
@@ -517,7 +550,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
             if (m[q] >= 0)
               put8<float>(e.partial, ((int64_t)split * e.M + m[q]) * e.N + nl, min(8, e.N - nl), e.N % 8 == 0, v[q]);
         } else {
+          if (ahead) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+#pragma unroll
+            for (int q = 0; q < 4; ++q) unpack8(held[slot * 128 + q * 32 + lane], res[q]);
+          }
           dense_epilogue<T, 4>(e, c, m, nl, bias, res, v);
+          fetch();
         }
       }
       tmem_fence_before_sync();
@@ -531,6 +570,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         acc_phase ^= 1;
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   __syncwarp();
   tmem_fence_before_sync();
@@ -557,7 +597,7 @@ __global__ void __launch_bounds__(256) dense_join_kernel(const float* part, int 
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[0][k] += t[k];
   }
-  dense_bias8(e, n, bias);
+  dense_bias8(e, c, n, bias);
   if (e.residual) get8<T>(e.residual, m[0] * e.res_stride + n, cnt, c.vec_res, res[0]);
   dense_epilogue<T, 1>(e, c, m, n, bias, res, v);
 }

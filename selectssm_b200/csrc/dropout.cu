@@ -76,10 +76,12 @@ __global__ void __launch_bounds__(kDropThreads) dropout_vec_kernel(const DropArg
   for (int u = 0; u < UNROLL; ++u) {
     const int64_t blk = first + u * kDropThreads;
     if (blk >= p.blocks) break;
-    const uint32_t m = keep_bits8(blk, key, p.rng.drop);
     float o[8];
+    const auto one = [&](int i, bool keep) { o[i] = drop_elem<BWD, ACT>(a[u][i], HAS_B ? b[u][i] : 0.f, keep, f); };
+    if (p.rng.drop) for_kept8(philox4x32_10(blk, key), p.rng.drop, one);
+    else
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = drop_elem<BWD, ACT>(a[u][i], HAS_B ? b[u][i] : 0.f, m >> i & 1, f);
+      for (int i = 0; i < 8; ++i) one(i, true);
     store8(out + blk * 8, o);
   }
 }
@@ -100,7 +102,8 @@ __global__ void __launch_bounds__(kDropThreads) dropout_any_kernel(const DropArg
     row = blk / p.per_row;
     col = (int)(blk - row * p.per_row) * 8;
     cnt = min(8, p.dim - col);
-    m = keep_bits8(blk, key, p.rng.drop);
+    if (p.rng.drop) for_kept8(philox4x32_10(blk, key), p.rng.drop, [&](int i, bool keep) { m |= (uint32_t)keep << i; });
+    else m = 0xff;
   }
   float a[8], b[8];
 #pragma unroll

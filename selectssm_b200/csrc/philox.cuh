@@ -50,17 +50,22 @@ __device__ __forceinline__ uint4 philox4x32_10(uint64_t counter, const PhiloxKey
   return make_uint4(c0, c1, c2, c3);
 }
 
-// bit i of the result: column i of the block is kept
-__device__ __forceinline__ uint32_t keep_bits8(uint64_t block, const PhiloxKey& key, uint32_t drop) {
-  const uint4 w = philox4x32_10(block, key);
+// Calls f(i, kept) for the block's eight columns.  A 16-bit draw is at least
+// drop (1 .. 65536) exactly when it exceeds drop - 1; with the draw in the upper
+// half of a word both compare as they stand, whatever the lower half holds.
+template <typename F>
+__device__ __forceinline__ void for_kept8(uint4 w, uint32_t drop, F f) {
+  const uint32_t over = (drop << 16) - 1u;  // drop 65536: nothing exceeds it
   const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-  uint32_t m = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if ((v[j] & 0xffffu) >= drop) m |= 1u << (2 * j);
-    if ((v[j] >> 16) >= drop) m |= 2u << (2 * j);
+    f(2 * j, v[j] << 16 > over);
+    f(2 * j + 1, v[j] > over);
   }
-  return m;
+}
+// v[i] * factor where column i is kept, else 0
+__device__ __forceinline__ void drop8(uint4 w, uint32_t drop, float factor, float (&v)[8]) {
+  for_kept8(w, drop, [&](int i, bool keep) { v[i] = keep ? v[i] * factor : 0.f; });
 }
 
 // Factor of a kept value; 0 when everything is dropped.

@@ -15,14 +15,17 @@ __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
   v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 r = __ldcs(reinterpret_cast<const uint4*>(p));
+// eight bf16 values held in 16 bytes
+__device__ __forceinline__ void unpack8(const uint4& r, float (&v)[8]) {
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     v[2 * j] = __uint_as_float(w[j] << 16);
     v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
   }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+  unpack8(__ldcs(reinterpret_cast<const uint4*>(p)), v);
 }
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
