@@ -68,22 +68,22 @@ __global__ void __launch_bounds__(256) dense_pack_kernel(const T* src, int64_t s
   store_planes<PLANES>(dst + r * ld + c, rows * ld, v);
 }
 
-constexpr int kDpreRows = 2;
 template <int ACT>
-__device__ __forceinline__ void slope_rows(float (&d)[kDpreRows][8], const float (&u)[kDpreRows][8], float f) {
-#pragma unroll
-  for (int q = 0; q < kDpreRows; ++q)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) d[q][i] *= act_grad_f(u[q][i] * f, ACT);
+__device__ __forceinline__ void slope_row(float (&d)[8], float (&u)[8], float f) {
+  scale8(u, f);
+  slope8<ACT>(d, u);
 }
 
 // dpre as planes for the two products that follow, and the column sums of its
 // unrounded values over a run of rows.  A thread keeps eight columns (one
-// dropout counter each row) and walks down the rows.
+// dropout counter each row) and takes ROWS rows at a time, whose loads it issues
+// together: the pass is bound by memory, and a loop that loads, computes and
+// stores row by row left it at half the rate.
 template <typename T, int PLANES, bool WRITE>
 __global__ void __launch_bounds__(256)
     dense_dpre_kernel(const T* dy, int64_t dy_stride, const T* pre, __nv_bfloat16* dpre, int ld, float* part, int64_t M,
-                      int N, int64_t run, int cb, int act, DropRng rng, bool vec_dy, bool vec_pre) {
+                      int N, int64_t run, int cb, int act, DropRng rng, bool vec) {
+  constexpr int ROWS = sizeof(T) == 2 ? 4 : 2;
   extern __shared__ float red[];
   const int per_row = (N + 7) / 8, rl = 256 / cb;
   const int lane = threadIdx.x / cb, blk = blockIdx.x * cb + threadIdx.x % cb, n = blk * 8;
@@ -97,30 +97,41 @@ __global__ void __launch_bounds__(256)
   float sum[8] = {};
   if (lane < rl && blk < per_row) {
     const int cnt = min(8, N - n);
-    for (int64_t m = m0 + lane; m < m1; m += kDpreRows * rl) {
-      float d[kDpreRows][8] = {}, u[kDpreRows][8] = {};
-      uint4 w[kDpreRows];
+    for (int64_t m = m0 + lane; m < m1; m += ROWS * rl) {
+      Raw8<T> rd[ROWS], ru[ROWS];
+      if (vec) {
 #pragma unroll
-      for (int q = 0; q < kDpreRows; ++q)
-        if (m + q * rl < m1) {
-          get8<T>(dy, (m + q * rl) * dy_stride + n, cnt, vec_dy, d[q]);
-          if (act) get8<T>(pre, (m + q * rl) * N + n, cnt, vec_pre, u[q]);
-        }
-#pragma unroll
-      for (int q = 0; q < kDpreRows; ++q)
-        if (rng.drop) w[q] = philox4x32_10((m + q * rl) * per_row + blk, key);
-      switch (act) {
-        case 1: slope_rows<1>(d, u, f); break;
-        case 2: slope_rows<2>(d, u, f); break;
-        case 3: slope_rows<3>(d, u, f); break;
-        default: break;
+        for (int q = 0; q < ROWS; ++q)
+          if (m + q * rl < m1) {
+            rd[q].load(dy + (m + q * rl) * dy_stride + n);
+            if (act) ru[q].load(pre + (m + q * rl) * N + n);
+          }
       }
 #pragma unroll
-      for (int q = 0; q < kDpreRows; ++q) {
-        if (rng.drop) drop8(w[q], rng.drop, f, d[q]);
+      for (int q = 0; q < ROWS; ++q) {
+        const int64_t row = m + q * rl;
+        if (row >= m1) break;
+        float d[8], u[8];
+        if (vec) {
+          rd[q].get(d);
+          if (act) ru[q].get(u);
+        } else {
+          get8<T>(dy, row * dy_stride + n, cnt, false, d);
+          if (act) get8<T>(pre, row * N + n, cnt, false, u);
+        }
+        switch (act) {
+          case 1: slope_row<1>(d, u, f); break;
+          case 2: slope_row<2>(d, u, f); break;
+          case 3: slope_row<3>(d, u, f); break;
+          default: break;
+        }
+        if (rng.drop) {
+          scale8(d, f);
+          keep8(philox4x32_10(row * per_row + blk, key), rng.drop, d);
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] += d[q][i];  // rows past the end hold zeros
-        if (WRITE && m + q * rl < m1) store_planes<PLANES>(dpre + (m + q * rl) * ld + n, M * ld, d[q]);
+        for (int i = 0; i < 8; ++i) sum[i] += d[i];
+        if (WRITE) store_planes<PLANES>(dpre + row * ld + n, M * ld, d);
       }
     }
   }
@@ -352,9 +363,9 @@ static DpreGeom dpre_geom(const ssm_dense_params_t* p) {
   g.tiles = (int)ceil_div(per_row, 32);
   g.cb = (int)ceil_div(per_row, g.tiles);
   const int rl = 256 / g.cb;
-  const int64_t want = ceil_div(6 * kSms, g.tiles);
-  g.run = std::max<int64_t>(ceil_div(p->rows, want), kDpreRows * rl);
-  g.run = std::max(g.run, ceil_div(p->rows, 65535));
+  // one round of the rows' loads a CTA, more where that made over 1024 parts of each column's sum
+  const int64_t round = (int64_t)rl * (p->dtype == SSM_BF16 ? 4 : 2);
+  g.run = round * ceil_div(p->rows, 1024 * round);
   g.parts = (int)ceil_div(p->rows, g.run);
   return g;
 }
@@ -372,14 +383,14 @@ static int launch_dpre(const ssm_dense_params_t* p, __nv_bfloat16* dpre, float* 
   const size_t smem = (size_t)(256 / g.cb) * g.cb * 8 * sizeof(float);
   const int64_t ds = stride_or(p->dy_stride, p->fout);
   const bool even = p->fout % 8 == 0;
-  const bool vec_dy = even && ds % 8 == 0 && aligned16(p->dy), vec_pre = even && aligned16(p->pre);
+  const bool vec = even && ds % 8 == 0 && aligned16(p->dy) && aligned16(p->pre);
   const T *dy = static_cast<const T*>(p->dy), *pre = static_cast<const T*>(p->pre);
   if (dpre)
     dense_dpre_kernel<T, PLANES, true><<<grid, 256, smem, s>>>(dy, ds, pre, dpre, pad8(p->fout), part, p->rows, p->fout,
-                                                               g.run, g.cb, p->act, drop_rng(p), vec_dy, vec_pre);
+                                                               g.run, g.cb, p->act, drop_rng(p), vec);
   else
     dense_dpre_kernel<T, PLANES, false><<<grid, 256, smem, s>>>(dy, ds, pre, dpre, pad8(p->fout), part, p->rows, p->fout,
-                                                                g.run, g.cb, p->act, drop_rng(p), vec_dy, vec_pre);
+                                                                g.run, g.cb, p->act, drop_rng(p), vec);
   return launched("launch dense dpre kernel", 1);
 }
 

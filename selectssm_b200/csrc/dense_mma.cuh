@@ -15,6 +15,7 @@
 
 #include <cstdint>
 
+#include "act8.cuh"
 #include "common.cuh"
 #include "philox.cuh"
 #include "vec8.cuh"
@@ -96,9 +97,7 @@ struct EpiConst {
 template <int ACT, int R>
 __device__ __forceinline__ void act_rows(float (&v)[R][8]) {
 #pragma unroll
-  for (int q = 0; q < R; ++q)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[q][i] = act_f(v[q][i], ACT);
+  for (int q = 0; q < R; ++q) act8<ACT>(v[q]);
 }
 
 __device__ __noinline__ float dense_again(const DenseEpi& e, int64_t m, int n) {
@@ -156,7 +155,10 @@ __device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst
 #pragma unroll
     for (int q = 0; q < R; ++q) w[q] = philox4x32_10(m[q] * e.per_row + n / 8, c.key);
 #pragma unroll
-    for (int q = 0; q < R; ++q) drop8(w[q], e.rng.drop, c.f, v[q]);
+    for (int q = 0; q < R; ++q) {
+      scale8(v[q], c.f);
+      keep8(w[q], e.rng.drop, v[q]);
+    }
   }
   switch (e.act) {
     case 1: act_rows<1, R>(v); break;

@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "act8.cuh"
 #include "common.cuh"
 #include "philox.cuh"
 #include "vec8.cuh"
@@ -28,7 +29,7 @@ namespace ssm {
 int launch_error(const char* where, cudaError_t e);  // scan.cu
 int bind_device(const void* ptr);                      // scan.cu
 
-constexpr int kDropThreads = 256;
+constexpr int kDropThreads = 128;
 
 struct DropArgs {
   int64_t blocks, rows;   // blocks of eight columns, all rows
@@ -40,11 +41,25 @@ struct DropArgs {
   DropRng rng;
 };
 
-// One element.  Forward: a = x, b = residual.  Backward: a = dy, b = x.
-template <bool BWD, int ACT>
-__device__ __forceinline__ float drop_elem(float a, float b, bool keep, float f) {
-  if (BWD) return keep ? (ACT ? a * act_grad_f(b * f, ACT) : a) * f : 0.f;
-  return (keep ? act_f(a * f, ACT) : 0.f) + b;  // every activation here maps 0 to 0
+// Eight elements of a block.  Forward: a = x, b = residual.  Backward: a = dy,
+// b = x.  The mask enters by selection only, so that what a dropped place holds
+// (NaN and infinities among it) has no effect; every activation here maps 0 to 0.
+template <bool BWD, int ACT, bool HAS_B, typename KEEP>
+__device__ __forceinline__ void drop_block(float (&a)[8], float (&b)[8], float f, KEEP keep) {
+  scale8(a, f);
+  if (BWD) {
+    if (ACT) {
+      scale8(b, f);
+      slope8<ACT>(a, b);
+    }
+    keep(a);
+  } else {
+    keep(a);
+    act8<ACT>(a);
+    if (HAS_B)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] += b[i];
+  }
 }
 
 template <typename T, bool BWD, int ACT, bool HAS_B, int UNROLL>
@@ -54,9 +69,15 @@ __global__ void __launch_bounds__(kDropThreads) dropout_vec_kernel(const DropArg
   const T* A = static_cast<const T*>(p.a);
   const T* B = static_cast<const T*>(p.b);
   T* out = static_cast<T*>(p.out);
-  const int64_t first = (int64_t)blockIdx.x * (kDropThreads * UNROLL) + threadIdx.x;
+  // A CTA's blocks are an aligned run of a power of two, so their counters
+  // share the upper word, and with it the two of the generator's products that
+  // depend on no other part of the counter.
+  static_assert((kDropThreads * UNROLL & (kDropThreads * UNROLL - 1)) == 0);
+  const int64_t run = (int64_t)blockIdx.x * (kDropThreads * UNROLL);
+  const int64_t first = run + threadIdx.x;
+  const uint32_t upper = (uint32_t)(run >> 32);
   const bool dense = p.a_stride == p.dim && (!HAS_B || p.b_stride == p.dim);
-  float a[UNROLL][8], b[UNROLL][8];
+  Raw8<T> a[UNROLL], b[UNROLL];
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
     const int64_t blk = first + u * kDropThreads;
@@ -68,21 +89,21 @@ __global__ void __launch_bounds__(kDropThreads) dropout_vec_kernel(const DropArg
         ao = row * p.a_stride + col;
         bo = row * p.b_stride + col;
       }
-      load8(A + ao, a[u]);
-      if (HAS_B) load8(B + bo, b[u]);
+      a[u].load(A + ao);
+      if (HAS_B) b[u].load(B + bo);
     }
   }
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
     const int64_t blk = first + u * kDropThreads;
     if (blk >= p.blocks) break;
-    float o[8];
-    const auto one = [&](int i, bool keep) { o[i] = drop_elem<BWD, ACT>(a[u][i], HAS_B ? b[u][i] : 0.f, keep, f); };
-    if (p.rng.drop) for_kept8(philox4x32_10(blk, key), p.rng.drop, one);
-    else
-#pragma unroll
-      for (int i = 0; i < 8; ++i) one(i, true);
-    store8(out + blk * 8, o);
+    float x[8], r[8];
+    a[u].get(x);
+    if (HAS_B) b[u].get(r);
+    drop_block<BWD, ACT, HAS_B>(x, r, f, [&](float (&v)[8]) {
+      if (p.rng.drop) keep8(philox4x32_10((uint32_t)blk, upper, key), p.rng.drop, v);
+    });
+    store8(out + blk * 8, x);
   }
 }
 
@@ -115,14 +136,20 @@ __global__ void __launch_bounds__(kDropThreads) dropout_any_kernel(const DropArg
     a[j] = ok ? Cvt<T>::to_f(A[r * p.a_stride + c]) : 0.f;
     b[j] = HAS_B && ok ? Cvt<T>::to_f(B[r * p.b_stride + c]) : 0.f;
   }
+  uint32_t kept = 0;  // bit j: this lane's element of blocks 4 j ..
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    kept |= (__shfl_sync(0xffffffffu, m, 4 * j + (lane >> 3)) >> (lane & 7) & 1) << j;
+  drop_block<BWD, ACT, HAS_B>(a, b, f, [&](float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = kept >> j & 1 ? v[j] : 0.f;
+  });
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int src = 4 * j + (lane >> 3), i = lane & 7;
     const int64_t r = __shfl_sync(0xffffffffu, row, src);
     const int c = __shfl_sync(0xffffffffu, col, src) + i;
-    const bool ok = i < __shfl_sync(0xffffffffu, cnt, src);
-    const uint32_t bits = __shfl_sync(0xffffffffu, m, src);
-    if (ok) out[r * p.dim + c] = Cvt<T>::from_f(drop_elem<BWD, ACT>(a[j], b[j], bits >> i & 1, f));
+    if (i < __shfl_sync(0xffffffffu, cnt, src)) out[r * p.dim + c] = Cvt<T>::from_f(a[j]);
   }
 }
 
@@ -130,7 +157,7 @@ template <typename T, bool BWD, int ACT, bool HAS_B>
 static int launch_drop(const DropArgs& p, cudaStream_t s) {
   const bool vec = p.dim % 8 == 0 && aligned16(p.a) && aligned16(p.out) && (!HAS_B || aligned16(p.b)) &&
                    p.a_stride * sizeof(T) % 16 == 0 && (!HAS_B || p.b_stride * sizeof(T) % 16 == 0);
-  constexpr int kUnroll = 2;
+  constexpr int kUnroll = sizeof(T) == 2 ? 4 : 2;  // 64 bytes of each input in flight a thread
   const int64_t per = vec ? kDropThreads * kUnroll : kDropThreads;
   const int64_t grid = (p.blocks + per - 1) / per;
   if (grid > 0x7fffffff) return SSM_ERR_SHAPE;

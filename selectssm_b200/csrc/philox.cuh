@@ -34,8 +34,8 @@ __device__ __forceinline__ PhiloxKey philox_key(const DropRng& r) {
   return {(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)off, (uint32_t)(off >> 32)};
 }
 
-__device__ __forceinline__ uint4 philox4x32_10(uint64_t counter, const PhiloxKey& key) {
-  uint32_t c0 = (uint32_t)counter, c1 = (uint32_t)(counter >> 32), c2 = key.c2, c3 = key.c3;
+__device__ __forceinline__ uint4 philox4x32_10(uint32_t c0, uint32_t c1, const PhiloxKey& key) {
+  uint32_t c2 = key.c2, c3 = key.c3;
   uint32_t k0 = key.k0, k1 = key.k1;
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
@@ -48,6 +48,10 @@ __device__ __forceinline__ uint4 philox4x32_10(uint64_t counter, const PhiloxKey
     k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
+}
+
+__device__ __forceinline__ uint4 philox4x32_10(uint64_t counter, const PhiloxKey& key) {
+  return philox4x32_10((uint32_t)counter, (uint32_t)(counter >> 32), key);
 }
 
 // Calls f(i, kept) for the block's eight columns.  A 16-bit draw is at least
@@ -63,9 +67,9 @@ __device__ __forceinline__ void for_kept8(uint4 w, uint32_t drop, F f) {
     f(2 * j + 1, v[j] > over);
   }
 }
-// v[i] * factor where column i is kept, else 0
-__device__ __forceinline__ void drop8(uint4 w, uint32_t drop, float factor, float (&v)[8]) {
-  for_kept8(w, drop, [&](int i, bool keep) { v[i] = keep ? v[i] * factor : 0.f; });
+// v[i] where column i is kept, else 0
+__device__ __forceinline__ void keep8(uint4 w, uint32_t drop, float (&v)[8]) {
+  for_kept8(w, drop, [&](int i, bool keep) { v[i] = keep ? v[i] : 0.f; });
 }
 
 // Factor of a kept value; 0 when everything is dropped.
