@@ -68,22 +68,19 @@ __global__ void __launch_bounds__(256) dense_pack_kernel(const T* src, int64_t s
   store_planes<PLANES>(dst + r * ld + c, rows * ld, v);
 }
 
-template <int ACT>
-__device__ __forceinline__ void slope_row(float (&d)[8], float (&u)[8], float f) {
-  scale8(u, f);
-  slope8<ACT>(d, u);
-}
+template <typename T>
+constexpr int kDpreRows = sizeof(T) == 2 ? 4 : 2;
 
 // dpre as planes for the two products that follow, and the column sums of its
 // unrounded values over a run of rows.  A thread keeps eight columns (one
 // dropout counter each row) and takes ROWS rows at a time, whose loads it issues
 // together: the pass is bound by memory, and a loop that loads, computes and
 // stores row by row left it at half the rate.
-template <typename T, int PLANES, bool WRITE>
-__global__ void __launch_bounds__(256)
+template <typename T, int PLANES, bool WRITE, int ACT>
+__global__ void __launch_bounds__(256, 3)
     dense_dpre_kernel(const T* dy, int64_t dy_stride, const T* pre, __nv_bfloat16* dpre, int ld, float* part, int64_t M,
-                      int N, int64_t run, int cb, int act, DropRng rng, bool vec) {
-  constexpr int ROWS = sizeof(T) == 2 ? 4 : 2;
+                      int N, int64_t run, int cb, DropRng rng, bool vec) {
+  constexpr int ROWS = kDpreRows<T>;
   extern __shared__ float red[];
   const int per_row = (N + 7) / 8, rl = 256 / cb;
   const int lane = threadIdx.x / cb, blk = blockIdx.x * cb + threadIdx.x % cb, n = blk * 8;
@@ -97,42 +94,48 @@ __global__ void __launch_bounds__(256)
   float sum[8] = {};
   if (lane < rl && blk < per_row) {
     const int cnt = min(8, N - n);
-    for (int64_t m = m0 + lane; m < m1; m += ROWS * rl) {
+    const T* pd = dy + (m0 + lane) * dy_stride + n;
+    const T* pp = ACT ? pre + (m0 + lane) * N + n : nullptr;
+    __nv_bfloat16* po = dpre + (m0 + lane) * ld + n;
+    int64_t counter = (m0 + lane) * per_row + blk;
+    int left = m1 > m0 + lane ? (int)((m1 - m0 - lane + rl - 1) / rl) : 0;  // rows of this thread
+    for (; left > 0; left -= ROWS) {
       Raw8<T> rd[ROWS], ru[ROWS];
       if (vec) {
 #pragma unroll
         for (int q = 0; q < ROWS; ++q)
-          if (m + q * rl < m1) {
-            rd[q].load(dy + (m + q * rl) * dy_stride + n);
-            if (act) ru[q].load(pre + (m + q * rl) * N + n);
+          if (q < left) {
+            rd[q].load(pd + q * rl * dy_stride);
+            if (ACT) ru[q].load(pp + (int64_t)q * rl * N);
           }
       }
 #pragma unroll
       for (int q = 0; q < ROWS; ++q) {
-        const int64_t row = m + q * rl;
-        if (row >= m1) break;
+        if (q >= left) break;
         float d[8], u[8];
         if (vec) {
           rd[q].get(d);
-          if (act) ru[q].get(u);
+          if (ACT) ru[q].get(u);
         } else {
-          get8<T>(dy, row * dy_stride + n, cnt, false, d);
-          if (act) get8<T>(pre, row * N + n, cnt, false, u);
+          get8<T>(pd, q * rl * dy_stride, cnt, false, d);
+          if (ACT) get8<T>(pp, (int64_t)q * rl * N, cnt, false, u);
         }
-        switch (act) {
-          case 1: slope_row<1>(d, u, f); break;
-          case 2: slope_row<2>(d, u, f); break;
-          case 3: slope_row<3>(d, u, f); break;
-          default: break;
+        if (ACT) {
+          scale8(u, f);
+          slope8<ACT>(d, u);
         }
         if (rng.drop) {
           scale8(d, f);
-          keep8(philox4x32_10(row * per_row + blk, key), rng.drop, d);
+          keep8(philox4x32_10(counter + q * rl * per_row, key), rng.drop, d);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[i] += d[i];
-        if (WRITE) store_planes<PLANES>(dpre + row * ld + n, M * ld, d);
+        if (WRITE) store_planes<PLANES>(po + (int64_t)q * rl * ld, M * ld, d);
       }
+      pd += ROWS * rl * dy_stride;
+      if (ACT) pp += (int64_t)ROWS * rl * N;
+      po += (int64_t)ROWS * rl * ld;
+      counter += (int64_t)ROWS * rl * per_row;
     }
   }
   if (!part) return;
@@ -363,9 +366,9 @@ static DpreGeom dpre_geom(const ssm_dense_params_t* p) {
   g.tiles = (int)ceil_div(per_row, 32);
   g.cb = (int)ceil_div(per_row, g.tiles);
   const int rl = 256 / g.cb;
-  // one round of the rows' loads a CTA, more where that made over 1024 parts of each column's sum
-  const int64_t round = (int64_t)rl * (p->dtype == SSM_BF16 ? 4 : 2);
-  g.run = round * ceil_div(p->rows, 1024 * round);
+  // one round of the rows' loads a CTA, more where that made over 256 parts of each column's sum
+  const int64_t round = (int64_t)rl * (p->dtype == SSM_BF16 ? kDpreRows<__nv_bfloat16> : kDpreRows<float>);
+  g.run = round * ceil_div(p->rows, 256 * round);
   g.parts = (int)ceil_div(p->rows, g.run);
   return g;
 }
@@ -376,22 +379,30 @@ static bool dpre_is_dy(const ssm_dense_params_t* p) {
          aligned16(p->dy);
 }
 
-template <typename T, int PLANES>
-static int launch_dpre(const ssm_dense_params_t* p, __nv_bfloat16* dpre, float* part, cudaStream_t s) {
+template <typename T, int PLANES, int ACT>
+static int launch_dpre_act(const ssm_dense_params_t* p, __nv_bfloat16* dpre, float* part, cudaStream_t s) {
   const DpreGeom g = dpre_geom(p);
   const dim3 grid(g.tiles, g.parts);
   const size_t smem = (size_t)(256 / g.cb) * g.cb * 8 * sizeof(float);
   const int64_t ds = stride_or(p->dy_stride, p->fout);
-  const bool even = p->fout % 8 == 0;
-  const bool vec = even && ds % 8 == 0 && aligned16(p->dy) && aligned16(p->pre);
+  const bool vec = p->fout % 8 == 0 && ds % 8 == 0 && aligned16(p->dy) && aligned16(p->pre);
   const T *dy = static_cast<const T*>(p->dy), *pre = static_cast<const T*>(p->pre);
   if (dpre)
-    dense_dpre_kernel<T, PLANES, true><<<grid, 256, smem, s>>>(dy, ds, pre, dpre, pad8(p->fout), part, p->rows, p->fout,
-                                                               g.run, g.cb, p->act, drop_rng(p), vec);
+    dense_dpre_kernel<T, PLANES, true, ACT><<<grid, 256, smem, s>>>(dy, ds, pre, dpre, pad8(p->fout), part, p->rows,
+                                                                    p->fout, g.run, g.cb, drop_rng(p), vec);
   else
-    dense_dpre_kernel<T, PLANES, false><<<grid, 256, smem, s>>>(dy, ds, pre, dpre, pad8(p->fout), part, p->rows, p->fout,
-                                                                g.run, g.cb, p->act, drop_rng(p), vec);
+    dense_dpre_kernel<T, PLANES, false, ACT><<<grid, 256, smem, s>>>(dy, ds, pre, dpre, pad8(p->fout), part, p->rows,
+                                                                     p->fout, g.run, g.cb, drop_rng(p), vec);
   return launched("launch dense dpre kernel", 1);
+}
+template <typename T, int PLANES>
+static int launch_dpre(const ssm_dense_params_t* p, __nv_bfloat16* dpre, float* part, cudaStream_t s) {
+  switch (p->act) {
+    case SSM_ACT_SILU: return launch_dpre_act<T, PLANES, SSM_ACT_SILU>(p, dpre, part, s);
+    case SSM_ACT_GELU: return launch_dpre_act<T, PLANES, SSM_ACT_GELU>(p, dpre, part, s);
+    case SSM_ACT_RELU: return launch_dpre_act<T, PLANES, SSM_ACT_RELU>(p, dpre, part, s);
+    default: return launch_dpre_act<T, PLANES, SSM_ACT_NONE>(p, dpre, part, s);
+  }
 }
 
 struct BwdBytes {
