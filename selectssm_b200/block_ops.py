@@ -25,7 +25,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _dense, _dtype_code, _ptr, _require_cuda, ctypes_byref
+from .ops import _DT, _dense, _dtype_code, _ptr, _require_cuda, ctypes_byref
 
 __all__ = ["group_norm_act", "dropout_act", "dense_act"]
 
@@ -61,41 +61,39 @@ def _rng_of(rng, drop, device):
     return int(seed) & _U64, int(offset) & _U64, None
 
 
-def _same_device(x, **others):
-    _require_cuda(x, *others.values())
-    for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+def _check_devices(x, *others):
+    _require_cuda(x, *others)
+    device = x.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError(f"operands on {t.device} and {device}")
 
 
-def _matrix(t):
-    """(2-D view with unit stride along the last axis, row stride); copies only
-    when the leading axes do not collapse to one stride."""
+def _rows_of(t):
+    """(t, row stride) as rows of the last axis with unit stride in it; copies
+    only when the leading axes do not collapse to one stride."""
     cols = t.shape[-1]
-    rows = t.numel() // cols if cols else 0
-    if t.numel() == 0 or t.is_contiguous():
-        return t.reshape(rows, cols), cols
+    if t.is_contiguous():
+        return t, cols
     if t.stride(-1) == 1 or cols == 1:
         # axes of one element have no stride of their own
         lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1]
         if all(a[1] == b[0] * b[1] for a, b in zip(lead, lead[1:])):
             step = lead[-1][1] if lead else cols
             if step >= cols:
-                return t.as_strided((rows, cols), (step, 1)), step
-    return t.reshape(rows, cols).contiguous(), cols
+                return t, step
+    return t.contiguous(), cols
 
 
 def _stream_of(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
-def _workspace(nbytes, device):
-    return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+def _workspace(nbytes, t):
+    return torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
 
 
 def _residual_of(residual, shape, dtype):
-    if residual is None:
-        return None
     if residual.shape != shape:
         try:
             residual = residual.expand(shape)  # autograd sums a broadcast residual's gradient
@@ -104,47 +102,52 @@ def _residual_of(residual, shape, dtype):
     return residual.to(dtype)
 
 
+def _records(*tensors):
+    """Whether autograd will ask for a gradient."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# Each operator has a plain function that makes the call and an autograd
+# function around it; without a gradient to record the former is called
+# directly, which halves the host's time for a single token.
+
 # ----------------------------------------------------------------------------- dropout
+def _dropout_forward(x, residual, drop, rng, act):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if not x.numel():
+        return y
+    x, xs = _rows_of(x)
+    res, rs = (None, 0) if residual is None else _rows_of(residual)
+    dim = x.shape[-1]
+    p = _lib.SSMDropoutParams(x.numel() // dim, dim, _DT[x.dtype], act, drop, rng[0], rng[1], _ptr(rng[2]), xs, rs, 0,
+                              x.data_ptr(), _ptr(res), y.data_ptr())
+    _lib.check(_lib.load().ssm_dropout_act_fwd(ctypes_byref(p), _stream_of(x)), "ssm_dropout_act_fwd")
+    return y
+
+
 class _DropoutActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, drop, rng, act):
-        seed, offset, rng_t = rng
-        x2, xs = _matrix(x)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        p = _drop_params(x2, drop, seed, offset, rng_t, act)
-        p.x, p.x_stride, p.y = x2.data_ptr(), xs, y.data_ptr()
-        if residual is not None:
-            r2, p.res_stride = _matrix(residual)
-            p.residual = r2.data_ptr()
-        if x.numel():
-            _lib.check(_lib.load().ssm_dropout_act_fwd(ctypes_byref(p), _stream_of(x)), "ssm_dropout_act_fwd")
-        ctx.save_for_backward(x2 if act else None, rng_t)
-        ctx.cfg = (x.shape, x.dtype, drop, seed, offset, act, xs)
-        return y
+        ctx.save_for_backward(x if act else None, rng[2])
+        ctx.cfg = (drop, rng[:2], act)
+        return _dropout_forward(x, residual, drop, rng, act)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x2, rng_t = ctx.saved_tensors
-        shape, dtype, drop, seed, offset, act, xs = ctx.cfg
+        x, rng_t = ctx.saved_tensors
+        drop, rng, act = ctx.cfg
         dx = None
         if ctx.needs_input_grad[0]:
-            dx = torch.empty(shape, dtype=dtype, device=dy.device)
+            dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
             if dx.numel():
-                d2, ds = _matrix(dy.to(dtype))
-                p = _drop_params(d2, drop, seed, offset, rng_t, act)
-                p.x, p.x_stride = _ptr(x2), xs
-                p.dy, p.dy_stride, p.dx = d2.data_ptr(), ds, dx.data_ptr()
+                d, ds = _rows_of(dy)
+                x, xs = _rows_of(x) if act else (None, 0)
+                dim = dy.shape[-1]
+                p = _lib.SSMDropoutParams(dy.numel() // dim, dim, _DT[dy.dtype], act, drop, *rng, _ptr(rng_t), xs, 0, ds,
+                                          _ptr(x), None, None, d.data_ptr(), dx.data_ptr())
                 _lib.check(_lib.load().ssm_dropout_act_bwd(ctypes_byref(p), _stream_of(dy)), "ssm_dropout_act_bwd")
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
-
-
-def _drop_params(x2, drop, seed, offset, rng_t, act):
-    p = _lib.SSMDropoutParams()
-    p.rows, p.dim = x2.shape
-    p.dtype, p.act, p.drop = _dtype_code(x2), act, drop
-    p.seed, p.offset, p.rng = seed, offset, _ptr(rng_t)
-    return p
 
 
 def dropout_act(x, rate, rng, activation=None, residual=None):
@@ -153,62 +156,67 @@ def dropout_act(x, rate, rng, activation=None, residual=None):
     x: (..., dim), float32 or bfloat16, rows at any stride.  ``rate`` in [0, 1]
     is taken to the nearest 65536th, kept values are divided by the keep
     probability that leaves.  ``residual`` broadcasts to x."""
-    _same_device(x, residual=residual)
+    _check_devices(x, residual)
     _dtype_code(x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must have a last axis of at least one element, got {tuple(x.shape)}")
     act, drop = _act_code(activation), _drop_of(rate)
     rng = _rng_of(rng, drop, x.device)
-    return _DropoutActFn.apply(x, _residual_of(residual, x.shape, x.dtype), drop, rng, act)
+    if residual is not None:
+        residual = _residual_of(residual, x.shape, x.dtype)
+    if _records(x, residual):
+        return _DropoutActFn.apply(x, residual, drop, rng, act)
+    return _dropout_forward(x, residual, drop, rng, act)
 
 
 # ----------------------------------------------------------------------------- group norm
+def _gn_params(x, scale, bias, y, stats, groups, eps, act):
+    batch, dim = x.shape[0], x.shape[-1]
+    seqlen = x.numel() // (batch * dim) if batch else 0
+    return _lib.SSMGroupNormParams(batch, seqlen, dim, groups, _DT[x.dtype], act, eps, x.data_ptr(), _ptr(scale),
+                                   _ptr(bias), _ptr(y), stats.data_ptr())
+
+
+def _group_norm_forward(x, scale, bias, groups, eps, act):
+    """y and the statistics; x, scale and bias are dense, the latter float32."""
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
+    if x.numel():
+        p = _gn_params(x, scale, bias, y, stats, groups, eps, act)
+        lib, ref = _lib.load(), ctypes_byref(p)
+        ws = _workspace(lib.ssm_group_norm_fwd_workspace_bytes(ref), x)
+        if ws is not None:
+            p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+        _lib.check(lib.ssm_group_norm_act_fwd(ref, _stream_of(x)), "ssm_group_norm_act_fwd")
+    return y, stats
+
+
 class _GroupNormActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, scale, bias, groups, eps, act):
-        x3 = _dense(x).view(x.shape[0], -1, x.shape[-1]) if x.numel() else x.reshape(x.shape[0], 0, x.shape[-1])
-        scale32 = None if scale is None else _dense(scale.float())
-        bias32 = None if bias is None else _dense(bias.float())
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
-        p = _gn_params(x3, scale32, bias32, stats, groups, eps, act)
-        p.y = y.data_ptr()
-        lib = _lib.load()
-        if x.numel():
-            ws = _workspace(lib.ssm_group_norm_fwd_workspace_bytes(ctypes_byref(p)), x.device)
-            p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
-            _lib.check(lib.ssm_group_norm_act_fwd(ctypes_byref(p), _stream_of(x)), "ssm_group_norm_act_fwd")
-        ctx.save_for_backward(x3, scale32, bias32, stats)
-        ctx.cfg = (x.shape, groups, eps, act)
-        ctx.dtypes = (None if scale is None else scale.dtype, None if bias is None else bias.dtype)
+        x = _dense(x)
+        y, stats = _group_norm_forward(x, scale, bias, groups, eps, act)
+        ctx.save_for_backward(x, scale, bias, stats)
+        ctx.cfg = (groups, eps, act)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x3, scale32, bias32, stats = ctx.saved_tensors
-        shape, groups, eps, act = ctx.cfg
-        dim = x3.shape[2]
-        dy = _dense(dy.to(x3.dtype))
-        dx = torch.empty(shape, dtype=x3.dtype, device=x3.device)
-        dscale, dbias = (torch.empty(dim, dtype=torch.float32, device=x3.device) for _ in range(2))
-        p = _gn_params(x3, scale32, bias32, stats, groups, eps, act)
-        p.dy, p.dx, p.dscale, p.dbias = dy.data_ptr(), dx.data_ptr(), dscale.data_ptr(), dbias.data_ptr()
-        lib = _lib.load()
-        ws = _workspace(lib.ssm_group_norm_bwd_workspace_bytes(ctypes_byref(p)), x3.device)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
-        _lib.check(lib.ssm_group_norm_act_bwd(ctypes_byref(p), _stream_of(x3)), "ssm_group_norm_act_bwd")
-        del ws
-        sdt, bdt = ctx.dtypes
-        return (dx, None if sdt is None else dscale.to(sdt), None if bdt is None else dbias.to(bdt), None, None, None)
-
-
-def _gn_params(x3, scale32, bias32, stats, groups, eps, act):
-    p = _lib.SSMGroupNormParams()
-    p.batch, p.seqlen, p.dim = x3.shape
-    p.groups, p.dtype, p.act, p.eps = groups, _dtype_code(x3), act, eps
-    p.x, p.scale, p.bias, p.stats = x3.data_ptr(), _ptr(scale32), _ptr(bias32), stats.data_ptr()
-    return p
+        x, scale, bias, stats = ctx.saved_tensors
+        groups, eps, act = ctx.cfg
+        dim = x.shape[-1]
+        dy = _dense(dy)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        sums = torch.empty((2, dim), dtype=torch.float32, device=x.device)
+        p = _gn_params(x, scale, bias, None, stats, groups, eps, act)
+        p.dy, p.dx, p.dscale, p.dbias = dy.data_ptr(), dx.data_ptr(), sums.data_ptr(), sums.data_ptr() + 4 * dim
+        lib, ref = _lib.load(), ctypes_byref(p)
+        ws = _workspace(lib.ssm_group_norm_bwd_workspace_bytes(ref), x)
+        if ws is not None:
+            p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+        _lib.check(lib.ssm_group_norm_act_bwd(ref, _stream_of(x)), "ssm_group_norm_act_bwd")
+        return dx, None if scale is None else sums[0], None if bias is None else sums[1], None, None, None
 
 
 def group_norm_act(x, scale=None, bias=None, groups=32, eps=1e-6, activation=None):
@@ -217,7 +225,7 @@ def group_norm_act(x, scale=None, bias=None, groups=32, eps=1e-6, activation=Non
     x: (batch, ..., dim), float32 or bfloat16.  Each batch row's mean and
     variance are taken over all middle axes and the dim / groups channels of a
     group.  ``scale`` and ``bias``: (dim,) or None for ones and zeros."""
-    _same_device(x, scale=scale, bias=bias)
+    _check_devices(x, scale, bias)
     _dtype_code(x)
     if x.dim() < 2 or x.shape[-1] < 1:
         raise ValueError(f"x must be (batch, ..., dim), got {tuple(x.shape)}")
@@ -227,33 +235,53 @@ def group_norm_act(x, scale=None, bias=None, groups=32, eps=1e-6, activation=Non
     for name, t in (("scale", scale), ("bias", bias)):
         if t is not None and t.shape != (dim,):
             raise ValueError(f"{name} must be ({dim},), got {tuple(t.shape)}")
-    return _GroupNormActFn.apply(x, scale, bias, int(groups), float(eps), _act_code(activation))
+    # converted outside, so that autograd returns the gradients in their types
+    scale = scale if scale is None else _dense(scale.float())
+    bias = bias if bias is None else _dense(bias.float())
+    if _records(x, scale, bias):
+        return _GroupNormActFn.apply(x, scale, bias, groups, eps, _act_code(activation))
+    return _group_norm_forward(_dense(x), scale, bias, groups, eps, _act_code(activation))[0]
 
 
 # ----------------------------------------------------------------------------- dense layer
+def _dense_params(x, xs, w, b, drop, rng, act):
+    code = _DT[x.dtype]
+    fin, fout = w.shape
+    return _lib.SSMDenseParams(x.numel() // fin, fin, fout, code, code if b is None else _DT[b.dtype], code, act, drop,
+                               rng[0], rng[1], _ptr(rng[2]), xs, 0, 0, x.data_ptr(), w.data_ptr(), _ptr(b))
+
+
+def _dense_forward(x, w, bias, residual, act, drop, rng, keep_pre):
+    """y and, with keep_pre, the activation's input; w and bias are dense, w of x's type."""
+    shape = (*x.shape[:-1], w.shape[1])
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    pre = torch.empty(shape, dtype=x.dtype, device=x.device) if keep_pre else None
+    if y.numel():
+        x, xs = _rows_of(x)
+        p = _dense_params(x, xs, w, bias, drop, rng, act)
+        p.y = y.data_ptr()
+        if keep_pre:
+            p.pre = pre.data_ptr()
+        if residual is not None:
+            residual, p.res_stride = _rows_of(residual)
+            p.residual = residual.data_ptr()
+        lib, ref = _lib.load(), ctypes_byref(p)
+        ws = _workspace(lib.ssm_dense_fwd_workspace_bytes(ref), x)
+        if ws is not None:
+            p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+        _lib.check(lib.ssm_dense_act_fwd(ref, _stream_of(x)), "ssm_dense_act_fwd")
+    return y, pre
+
+
 class _DenseActFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, kernel, bias, residual, act, drop, rng, grad):
-        seed, offset, rng_t = rng
-        x2, xs = _matrix(x)
+    def forward(ctx, x, kernel, bias, residual, act, drop, rng):
         w = _dense(kernel.to(x.dtype))
-        b = None if bias is None else _dense(bias)
-        out_shape = (*x.shape[:-1], kernel.shape[1])
-        y = torch.empty(out_shape, dtype=x.dtype, device=x.device)
-        pre = torch.empty((x2.shape[0], kernel.shape[1]), dtype=x.dtype, device=x.device) if grad and act else None
-        p = _dense_params(x2, xs, w, b, drop, seed, offset, rng_t, act)
-        p.y, p.pre = y.data_ptr(), _ptr(pre)
-        if residual is not None:
-            r2, p.res_stride = _matrix(residual)
-            p.residual = r2.data_ptr()
-        lib = _lib.load()
-        if y.numel():
-            ws = _workspace(lib.ssm_dense_fwd_workspace_bytes(ctypes_byref(p)), x.device)
-            p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
-            _lib.check(lib.ssm_dense_act_fwd(ctypes_byref(p), _stream_of(x)), "ssm_dense_act_fwd")
-        if grad:
-            ctx.save_for_backward(x2, w, b, pre, rng_t)
-        ctx.cfg = (x.shape, xs, drop, seed, offset, act, kernel.dtype)
+        need = any(ctx.needs_input_grad[:3])
+        y, pre = _dense_forward(x, w, bias, residual, act, drop, rng, need and act != 0)
+        if need:
+            ctx.save_for_backward(x, w, bias, pre, rng[2])
+        ctx.cfg = (drop, rng[:2], act, kernel.dtype)
         return y
 
     @staticmethod
@@ -261,34 +289,24 @@ class _DenseActFn(torch.autograd.Function):
     def backward(ctx, dy):
         dres = dy if ctx.needs_input_grad[3] else None
         if not any(ctx.needs_input_grad[:3]):
-            return None, None, None, dres, None, None, None, None
-        x2, w, b, pre, rng_t = ctx.saved_tensors
-        shape, xs, drop, seed, offset, act, kdtype = ctx.cfg
-        d2, ds = _matrix(dy.to(x2.dtype))
-        p = _dense_params(x2, xs, w, b, drop, seed, offset, rng_t, act)
-        p.pre, p.dy, p.dy_stride = _ptr(pre), d2.data_ptr(), ds
-        p.dkernel_dtype = _lib.SSM_BF16 if kdtype == torch.bfloat16 else _lib.SSM_F32
-        dx = torch.empty(shape, dtype=x2.dtype, device=x2.device) if ctx.needs_input_grad[0] else None
-        dw = torch.empty(w.shape, dtype=kdtype, device=x2.device) if ctx.needs_input_grad[1] else None
-        db = torch.empty_like(b) if ctx.needs_input_grad[2] else None
+            return None, None, None, dres, None, None, None
+        x, w, bias, pre, rng_t = ctx.saved_tensors
+        drop, rng, act, kdtype = ctx.cfg
+        d, ds = _rows_of(dy)
+        xc, xs = _rows_of(x)
+        p = _dense_params(xc, xs, w, bias, drop, (*rng, rng_t), act)
+        p.pre, p.dy, p.dy_stride = _ptr(pre), d.data_ptr(), ds
+        p.dkernel_dtype = _DT[kdtype]
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
+        dw = torch.empty(w.shape, dtype=kdtype, device=x.device) if ctx.needs_input_grad[1] else None
+        db = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
         p.dx, p.dkernel, p.dbias = _ptr(dx), _ptr(dw), _ptr(db)
-        lib = _lib.load()
-        ws = _workspace(lib.ssm_dense_bwd_workspace_bytes(ctypes_byref(p)), x2.device)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
-        _lib.check(lib.ssm_dense_act_bwd(ctypes_byref(p), _stream_of(x2)), "ssm_dense_act_bwd")
-        del ws
-        return dx, dw, db, dres, None, None, None, None
-
-
-def _dense_params(x2, xs, w, b, drop, seed, offset, rng_t, act):
-    p = _lib.SSMDenseParams()
-    p.rows, p.fin = x2.shape
-    p.fout = w.shape[1]
-    p.dtype, p.act, p.drop = _dtype_code(x2), act, drop
-    p.bias_dtype = p.dkernel_dtype = p.dtype if b is None else _dtype_code(b)
-    p.seed, p.offset, p.rng = seed, offset, _ptr(rng_t)
-    p.x, p.x_stride, p.kernel, p.bias = x2.data_ptr(), xs, w.data_ptr(), _ptr(b)
-    return p
+        lib, ref = _lib.load(), ctypes_byref(p)
+        ws = _workspace(lib.ssm_dense_bwd_workspace_bytes(ref), x)
+        if ws is not None:
+            p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+        _lib.check(lib.ssm_dense_act_bwd(ref, _stream_of(x)), "ssm_dense_act_bwd")
+        return dx, dw, db, dres, None, None, None
 
 
 def dense_act(x, kernel, bias=None, activation=None, residual=None, rate=0.0, rng=None):
@@ -300,7 +318,7 @@ def dense_act(x, kernel, bias=None, activation=None, residual=None, rate=0.0, rn
     keep fp32 accuracy.  ``rate`` and ``rng`` as in :func:`dropout_act`, over
     rows of fout columns.  For the backward an activation's input is kept in
     x's type."""
-    _same_device(x, kernel=kernel, bias=bias, residual=residual)
+    _check_devices(x, kernel, bias, residual)
     _dtype_code(x), _dtype_code(kernel)
     if kernel.dim() != 2 or x.dim() < 1 or x.shape[-1] != kernel.shape[0] or min(kernel.shape) < 1:
         raise ValueError(f"x {tuple(x.shape)} and kernel {tuple(kernel.shape)} do not match (..., fin) @ (fin, fout)")
@@ -309,8 +327,11 @@ def dense_act(x, kernel, bias=None, activation=None, residual=None, rate=0.0, rn
         _dtype_code(bias)
         if bias.shape != (fout,):
             raise ValueError(f"bias must be ({fout},), got {tuple(bias.shape)}")
+        bias = bias if bias.is_contiguous() else bias.contiguous()
     act, drop = _act_code(activation), _drop_of(rate)
     rng = _rng_of(rng, drop, x.device)
-    residual = _residual_of(residual, (*x.shape[:-1], fout), x.dtype)
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, kernel, bias))
-    return _DenseActFn.apply(x, kernel, bias, residual, act, drop, rng, grad)
+    if residual is not None:
+        residual = _residual_of(residual, (*x.shape[:-1], fout), x.dtype)
+    if _records(x, kernel, bias, residual):
+        return _DenseActFn.apply(x, kernel, bias, residual, act, drop, rng)
+    return _dense_forward(x, _dense(kernel.to(x.dtype)), bias, residual, act, drop, rng, False)[0]

@@ -18,7 +18,7 @@ LIB = os.path.join(HERE, "libselectssm_b200.so")
 SOURCES = ["scan.cu", "conv1d.cu", "noalloc.cu", "rmsnorm.cu", "selftest.cu", "dropout.cu", "groupnorm.cu",
            "dense.cu"]
 HEADERS = ["common.cuh", "scan_kernels.cuh", "scan_bwd.cuh", "scan_fwd.cuh", "scan_fwd_lane.cuh", "philox.cuh", "vec8.cuh",
-           "dense_mma.cuh", "act8.cuh"]
+           "dense_mma.cuh", "act8.cuh", "dense_few.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

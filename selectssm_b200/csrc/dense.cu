@@ -15,6 +15,7 @@
 
 #include <algorithm>
 
+#include "dense_few.cuh"
 #include "dense_mma.cuh"
 #include "../../include/selectssm_b200.h"
 
@@ -330,17 +331,65 @@ static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
 }
 
 // ---------------------------------------------------------------- forward and backward
+static bool few_rows(const ssm_dense_params_t* p) { return p->rows <= kFewRows && p->fin <= kFewMaxFin; }
+
+template <typename T, int R, int CT>
+static int launch_few(const ssm_dense_params_t* p, const DenseEpi& e, cudaStream_t s) {
+  const int tiles = (int)ceil_div(p->fout, CT);
+  // parts of fin: enough CTAs for the SMs, and at least 64 rows of the kernel each
+  // (and few enough for x's part to fit: 16384 rows of 16 values need all eight)
+  const int64_t useful = std::min<int64_t>({8, ceil_div(kSms, tiles), p->fin / 64});
+  const int parts = (int)std::max<int64_t>({1, useful, ceil_div((int64_t)p->fin * R * sizeof(float), 128 * 1024)});
+  const size_t smem = (size_t)ceil_div(p->fin, parts) * R * sizeof(float) + R * sizeof(float);
+  const auto kernel = dense_few_kernel<T, R, CT>;
+  cudaError_t err;
+  if (smem > 16 * 1024) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (err != cudaSuccess) return launch_error("cudaFuncSetAttribute(dense few rows)", err);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(parts * tiles);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const bool vec = p->fout % 8 == 0 && aligned16(p->kernel);
+  err = cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(p->x), stride_or(p->x_stride, p->fin),
+                           static_cast<const T*>(p->kernel), e, parts, vec);
+  note_launches(1);
+  return err == cudaSuccess ? SSM_OK : launch_error("launch dense few rows kernel", err);
+}
+template <typename T, int R>
+static int launch_few_ct(const ssm_dense_params_t* p, const DenseEpi& e, cudaStream_t s) {
+  // 64 columns read 128 bytes of bf16 a row; 32 where that leaves SMs without work
+  return ceil_div(p->fout, 64) * 8 >= kSms ? launch_few<T, R, 64>(p, e, s) : launch_few<T, R, 32>(p, e, s);
+}
+template <typename T>
+static int dense_few(const ssm_dense_params_t* p, const DenseEpi& e, cudaStream_t s) {
+  if (p->rows == 1) return launch_few_ct<T, 1>(p, e, s);
+  return p->rows <= 4 ? launch_few_ct<T, 4>(p, e, s) : launch_few_ct<T, 16>(p, e, s);
+}
+
 static int dense_fwd(const ssm_dense_params_t* p, cudaStream_t s) {
   char* ws = static_cast<char*>(p->workspace);
   DenseEpi e = {};
-  int st = planes(x_operand(p), true, &ws, s, &e.a);
-  if (st) return st;
-  st = planes(kernel_operand(p), false, &ws, s, &e.b);
-  if (st) return st;
+  int st = SSM_OK;
+  const bool few = few_rows(p);
+  if (!few) {
+    st = planes(x_operand(p), true, &ws, s, &e.a);
+    if (st) return st;
+    st = planes(kernel_operand(p), false, &ws, s, &e.b);
+    if (st) return st;
+  }
   e.M = p->rows;
   e.N = p->fout;
   e.K = p->fin;
-  e.planes = planes_of(p);
+  e.planes = few ? 0 : planes_of(p);
   e.out = p->y;
   e.bias = p->bias;
   e.bias_bf16 = p->bias_dtype == SSM_BF16;
@@ -350,6 +399,7 @@ static int dense_fwd(const ssm_dense_params_t* p, cudaStream_t s) {
   e.pre = p->pre;
   e.per_row = (p->fout + 7) / 8;
   e.rng = drop_rng(p);
+  if (few) return p->dtype == SSM_BF16 ? dense_few<__nv_bfloat16>(p, e, s) : dense_few<float>(p, e, s);
   float* part = reinterpret_cast<float*>(ws);
   return p->dtype == SSM_BF16 ? product<false, true, __nv_bfloat16>(e, part, p->status, s)
                               : product<false, true, float>(e, part, p->status, s);
@@ -481,7 +531,7 @@ using namespace ssm;
 extern "C" {
 
 size_t ssm_dense_fwd_workspace_bytes(const ssm_dense_params_t* p) {
-  if (check_dense(p) || p->rows == 0) return 0;
+  if (check_dense(p) || p->rows == 0 || few_rows(p)) return 0;
   return x_operand(p).bytes() + kernel_operand(p).bytes() +
          plan_product(p->rows, p->fout, p->fin, planes_of(p)).part_bytes;
 }

@@ -124,7 +124,7 @@ template <typename T, int R>
 __device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst& c, const int64_t (&m)[R], int n,
                                                const float (&bias)[8], const float (&res)[R][8], float (&v)[R][8]) {
   const int cnt = min(8, e.N - n);
-  if (sizeof(T) == 4) {
+  if (sizeof(T) == 4 && e.planes == 3) {
     // An infinite operand has no finite planes besides its first, and infinity
     // times the other operand's planes gives NaN where the product is infinite.
     // Such elements are summed again from the fp32 values.

@@ -107,13 +107,13 @@ def test_rate_and_rng_rules():
     assert block_ops._rng_of(None, 0, None) == (0, 0, None)
 
 
-def test_matrix_views():
+def test_row_views():
     """Leading axes collapse without a copy exactly when one stride serves them."""
     t = torch.arange(2 * 3 * 40.0).view(2, 3, 40)
-    m, step = block_ops._matrix(t[..., 4:20])
-    assert step == 40 and m.data_ptr() == t[..., 4:20].data_ptr() and torch.equal(m, t[..., 4:20].reshape(6, 16))
-    for view in (t.transpose(0, 1), t[:, :2], t[..., ::2], t[:1].expand(4, 3, 40), t[:, :, :1], t.new_zeros(0, 7),
-                 torch.arange(5.0), t[0, 0].expand(6, 40)):
-        m, step = block_ops._matrix(view)
-        assert torch.equal(m, view.reshape(-1, view.shape[-1])) and (m.shape[0] < 2 or m.stride(0) == step)
-        assert step >= view.shape[-1]
+    m, step = block_ops._rows_of(t[..., 4:20])
+    assert step == 40 and m.data_ptr() == t[..., 4:20].data_ptr()
+    for view in (t, t[..., 4:20], t.transpose(0, 1), t[:, :2], t[..., ::2], t[:1].expand(4, 3, 40), t[:, :, :1],
+                 t.new_zeros(0, 7), torch.arange(5.0), t[0, 0].expand(6, 40)):
+        m, step = block_ops._rows_of(view)
+        rows = view.reshape(-1, view.shape[-1])
+        assert step >= view.shape[-1] and torch.equal(m.as_strided(rows.shape, (step, 1)), rows)
