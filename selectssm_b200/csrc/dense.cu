@@ -333,7 +333,7 @@ static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
 // ---------------------------------------------------------------- forward and backward
 static bool few_rows(const ssm_dense_params_t* p) { return p->rows <= kFewRows && p->fin <= kFewMaxFin; }
 
-template <typename T, int R, int CT>
+template <typename T, int R, int CT, int V>
 static int launch_few(const ssm_dense_params_t* p, const DenseEpi& e, cudaStream_t s) {
   const int tiles = (int)ceil_div(p->fout, CT);
   // parts of fin: enough CTAs for the SMs, and at least 64 rows of the kernel each
@@ -341,7 +341,7 @@ static int launch_few(const ssm_dense_params_t* p, const DenseEpi& e, cudaStream
   const int64_t useful = std::min<int64_t>({8, ceil_div(kSms, tiles), p->fin / 64});
   const int parts = (int)std::max<int64_t>({1, useful, ceil_div((int64_t)p->fin * R * sizeof(float), 128 * 1024)});
   const size_t smem = (size_t)ceil_div(p->fin, parts) * R * sizeof(float) + R * sizeof(float);
-  const auto kernel = dense_few_kernel<T, R, CT>;
+  const auto kernel = dense_few_kernel<T, R, CT, V>;
   cudaError_t err;
   if (smem > 16 * 1024) {
     err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -358,21 +358,18 @@ static int launch_few(const ssm_dense_params_t* p, const DenseEpi& e, cudaStream
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const bool vec = p->fout % 8 == 0 && aligned16(p->kernel);
+  const bool vec = p->fout % V == 0 && reinterpret_cast<uintptr_t>(p->kernel) % std::min<size_t>(16, V * sizeof(T)) == 0;
   err = cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(p->x), stride_or(p->x_stride, p->fin),
                            static_cast<const T*>(p->kernel), e, parts, vec);
   note_launches(1);
   return err == cudaSuccess ? SSM_OK : launch_error("launch dense few rows kernel", err);
 }
-template <typename T, int R>
-static int launch_few_ct(const ssm_dense_params_t* p, const DenseEpi& e, cudaStream_t s) {
-  // 64 columns read 128 bytes of bf16 a row; 32 where that leaves SMs without work
-  return ceil_div(p->fout, 64) * 8 >= kSms ? launch_few<T, R, 64>(p, e, s) : launch_few<T, R, 32>(p, e, s);
-}
 template <typename T>
 static int dense_few(const ssm_dense_params_t* p, const DenseEpi& e, cudaStream_t s) {
-  if (p->rows == 1) return launch_few_ct<T, 1>(p, e, s);
-  return p->rows <= 4 ? launch_few_ct<T, 4>(p, e, s) : launch_few_ct<T, 16>(p, e, s);
+  if (p->rows > 4) return launch_few<T, 16, 64, 2>(p, e, s);
+  if (p->rows > 1) return launch_few<T, 4, 64, 2>(p, e, s);
+  // 64 columns read 128 bytes of bf16 a row; 32 where that leaves SMs without work
+  return ceil_div(p->fout, 64) * 8 >= kSms ? launch_few<T, 1, 64, 8>(p, e, s) : launch_few<T, 1, 32, 8>(p, e, s);
 }
 
 static int dense_fwd(const ssm_dense_params_t* p, cudaStream_t s) {
