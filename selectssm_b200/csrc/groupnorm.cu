@@ -11,11 +11,21 @@
 // channels of scale * (sum of du), m(g xhat) of scale * (sum of du xhat).  So a
 // thread keeps a fixed run of channels, walks down the sequence, and no
 // group's width matters to the inner loops.
+//
+// Two forms.  Held: a cluster of up to eight CTAs keeps some groups of one batch
+// row in its shared memory between the statistics and their use, so each input
+// is read once and the call is one kernel (and a small one for dscale and
+// dbias).  Split, where a single group is too long for that: one pass for the
+// sums per chunk of the sequence, a small kernel that joins them, and a second
+// pass over the inputs.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
+#include "act8.cuh"
 #include "common.cuh"
 #include "vec8.cuh"
 #include "../../include/selectssm_b200.h"
@@ -200,12 +210,13 @@ __global__ void __launch_bounds__(kGnThreads) gn_merge_kernel(const GnArgs p) {
   const int items = g.chunks * g.cg;
   const float count = (float)g.L * (float)g.cg;
   float s = 0.f;
+  const float ref = part[0].x;  // so that equal means merge to themselves
   for (int i = threadIdx.x; i < items; i += kGnThreads) {
     const int ck = i / g.cg, c = i - ck * g.cg;
     const float n = (float)(min((ck + 1) * g.chunk, g.L) - ck * g.chunk);
-    s = fmaf(n / count, part[(int64_t)ck * g.D + c].x, s);
+    s = fmaf(n / count, part[(int64_t)ck * g.D + c].x - ref, s);
   }
-  const float mu = block_sum(s, buf);
+  const float mu = block_sum(s, buf) + ref;
   float d2 = 0.f;
   for (int i = threadIdx.x; i < items; i += kGnThreads) {
     const int ck = i / g.cg, c = i - ck * g.cg;
@@ -379,18 +390,335 @@ __global__ void __launch_bounds__(kGnThreads) gn_dx_kernel(const GnArgs p) {
   }
 }
 
-// dscale and dbias: the batch rows' sums in order
-__global__ void gn_param_kernel(const GnArgs p) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= p.g.D) return;
-  float s1 = 0.f, s2 = 0.f;
-  for (int b = 0; b < p.g.B; ++b) {
-    const float2 v = p.sums[(int64_t)b * p.g.D + c];
-    s1 += v.x;
-    s2 += v.y;
+// dscale and dbias: `rows` partial sums of every channel in a fixed order
+__global__ void __launch_bounds__(1024) gn_param_kernel(const float2* sums, int rows, int D, float* dscale, float* dbias) {
+  __shared__ float2 red[32][33];
+  const int col = threadIdx.x & 31, lane = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
+  float2 s = make_float2(0.f, 0.f);
+  if (c < D)
+    for (int r = lane; r < rows; r += 32) s = fadd2(s, sums[(int64_t)r * D + c]);
+  red[lane][col] = s;
+  __syncthreads();
+  if (lane == 0 && c < D) {
+    float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t = fadd2(t, red[i][col]);
+    if (dbias) dbias[c] = t.x;
+    if (dscale) dscale[c] = t.y;
   }
-  if (p.dbias) p.dbias[c] = s1;
-  if (p.dscale) p.dscale[c] = s2;
+}
+
+// ---------------------------------------------------------------- held form
+// A job: `gpj` groups (W channels) of one batch row, `ctas` CTAs with `rows`
+// rows each.  nv vectors of V channels by rt row lanes; each thread keeps
+// `slots` vectors of its own in shared memory.
+struct GnHold {
+  int32_t W, gpj, jobs, ctas, nv, rt, slots;
+  int64_t rows;
+  size_t smem;
+};
+
+template <typename T, int V>
+struct GnVec;  // V values as they lie in shared memory
+template <> struct GnVec<float, 4> {
+  float4 r;
+  __device__ __forceinline__ void get(float (&v)[4]) const { v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w; }
+  __device__ __forceinline__ static void put(float* p, const float (&v)[4]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+};
+template <> struct GnVec<__nv_bfloat16, 8> {
+  uint4 r;
+  __device__ __forceinline__ void get(float (&v)[8]) const { unpack8(r, v); }
+  __device__ __forceinline__ static void put(__nv_bfloat16* p, const float (&v)[8]) { store8(p, v); }
+};
+template <typename T> struct GnVec<T, 1> {
+  T r;
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = Cvt<T>::to_f(r); }
+  __device__ __forceinline__ static void put(T* p, const float (&v)[1]) { *p = Cvt<T>::from_f(v[0]); }
+};
+
+__device__ __forceinline__ void gn_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void gn_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float2 gn_peer(const float2* p, int cta) {
+  uint32_t at;
+  float2 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(cta));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+
+// du of V elements from d = dy and xh = xhat (d is overwritten)
+template <int V, int ACT>
+__device__ __forceinline__ void gn_du(float (&d)[V], const float (&xh)[V], const float (&scale)[V], const float (&bias)[V]) {
+  if constexpr (ACT == 0) return;
+  float u[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) u[i] = fmaf(xh[i], scale[i], bias[i]);
+  if constexpr (V == 1) {
+    d[0] *= slope2<ACT>(make_float2(u[0], 0.f)).x;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 y = fmul2(make_float2(d[i], d[i + 1]), slope2<ACT>(make_float2(u[i], u[i + 1])));
+      d[i] = y.x;
+      d[i + 1] = y.y;
+    }
+  }
+}
+template <int V, int ACT>
+__device__ __forceinline__ void gn_act(float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = act2<ACT>(make_float2(v[0], 0.f)).x;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 y = act2<ACT>(make_float2(v[i], v[i + 1]));
+      v[i] = y.x;
+      v[i + 1] = y.y;
+    }
+  }
+}
+
+template <typename T, int V, int ACT, bool BWD>
+__global__ void __launch_bounds__(kGnThreads) gn_hold_kernel(const GnArgs p, const GnHold h) {
+  using Vec = GnVec<T, V>;
+  constexpr int kWarps = kGnThreads / 32;
+  extern __shared__ __align__(16) uint8_t raw[];
+  const GnGeom& g = p.g;
+  Vec* hx = reinterpret_cast<Vec*>(raw);
+  Vec* hd = hx + (BWD ? h.slots * kGnThreads : 0);
+  float* red = reinterpret_cast<float*>(raw + ((size_t)h.slots * kGnThreads * sizeof(Vec) * (BWD ? 2 : 1) + 15) / 16 * 16);
+  float2* own = reinterpret_cast<float2*>(red + kGnThreads * V * (BWD ? 2 : 1));  // this CTA's pair of each group
+  float2* all = own + h.gpj;                                                       // the job's
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int rank = 0;
+  if (h.ctas > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int job = blockIdx.x / h.ctas, b = job / h.jobs, g0 = job % h.jobs * h.gpj;
+  const int ng = min(h.gpj, g.G - g0), width = ng * g.cg, c0 = g0 * g.cg;
+  const int cv = tid % h.nv, rl = tid / h.nv;
+  const bool active = rl < h.rt && cv * V < width;
+  const int64_t l0 = rank * h.rows, l1 = min(l0 + h.rows, g.L);
+  const int mine = active && l0 + rl < l1 ? (int)((l1 - l0 - rl + h.rt - 1) / h.rt) : 0;  // vectors of this thread
+  const int64_t base = ((int64_t)b * g.L + l0 + rl) * g.D + c0 + cv * V, step = (int64_t)h.rt * g.D;
+  const T* x = static_cast<const T*>(p.x) + base;
+  const T* dy = BWD ? static_cast<const T*>(p.dy) + base : nullptr;
+
+  for (int i = 0; i < mine; ++i) {
+    if constexpr (sizeof(Vec) == 16) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hx + i * kGnThreads + tid)), "l"(x + i * step)
+                   : "memory");
+      if (BWD)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hd + i * kGnThreads + tid)),
+                     "l"(dy + i * step)
+                     : "memory");
+    } else {
+      hx[i * kGnThreads + tid].r = x[i * step];
+      if (BWD) hd[i * kGnThreads + tid].r = dy[i * step];
+    }
+  }
+  float scale[V], bias[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    scale[i] = active && p.scale ? p.scale[c0 + cv * V + i] : 1.f;
+    bias[i] = active && p.bias ? p.bias[c0 + cv * V + i] : 0.f;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");  // a thread reads only what it fetched itself
+
+  const float total = (float)g.L * (float)g.cg;
+  T* out = static_cast<T*>(p.out) + base;
+  // Per-thread values to sums over each group, in a fixed order; the result in
+  // `dst[group].x` or `.y`.  Vectors that lie in one group are summed first.
+  const bool single = g.cg % V == 0;
+  const int unit = single ? V : 1, per = g.cg / unit, units = h.nv * V / unit;
+  const auto group_sums = [&](const float (&s)[V], auto finish) {
+    if (active) {
+      if (single) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) t += s[i];
+        red[rl * units + cv] = t;
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) red[rl * units + cv * V + i] = s[i];
+      }
+    }
+    __syncthreads();
+    for (int q = warp; q < ng; q += kWarps) {
+      float t = 0.f;
+      for (int i = lane; i < h.rt * per; i += 32) {
+        const int r = i / per;
+        t += red[r * units + q * per + (i - r * per)];
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      if (lane == 0) finish(q, t);
+    }
+    __syncthreads();
+  };
+
+  if constexpr (!BWD) {
+    const float n = (float)max(l1 - l0, (int64_t)0) * (float)g.cg;  // this CTA's values of a group
+    float s[V] = {}, mean[V];
+    for (int i = 0; i < mine; ++i) {
+      float v[V];
+      hx[i * kGnThreads + tid].get(v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[j] += v[j];
+    }
+    group_sums(s, [&](int q, float t) { own[q].x = n > 0.f ? t / n : 0.f; });
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      mean[j] = active ? own[(cv * V + j) / g.cg].x : 0.f;
+      s[j] = 0.f;
+    }
+    for (int i = 0; i < mine; ++i) {
+      float v[V];
+      hx[i * kGnThreads + tid].get(v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = v[j] - mean[j];
+        s[j] = fmaf(d, d, s[j]);
+      }
+    }
+    group_sums(s, [&](int q, float t) { own[q].y = t; });
+    // the CTAs' means and squared deviations, merged about the common mean
+    if (h.ctas > 1) {
+      gn_cluster_arrive();
+      gn_cluster_wait();
+    }
+    for (int q = tid; q < ng; q += kGnThreads) {
+      // (from the first one's mean, so that equal means merge to themselves)
+      float mu = 0.f, m2 = 0.f;
+      float2 each[8];
+      float cnt[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        cnt[r] = 0.f;
+        if (r < h.ctas) {
+          each[r] = h.ctas > 1 ? gn_peer(own + q, r) : own[q];
+          cnt[r] = (float)max(min((r + 1) * h.rows, g.L) - r * h.rows, (int64_t)0) * (float)g.cg;
+          mu = fmaf(cnt[r] / total, each[r].x - each[0].x, mu);
+        }
+      }
+      mu += each[0].x;
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < h.ctas) {
+          const float d = each[r].x - mu;
+          m2 += each[r].y + cnt[r] * d * d;
+        }
+      all[q] = make_float2(mu, 1.f / sqrtf(m2 / total + p.eps));
+      if (rank == 0) reinterpret_cast<float2*>(p.stats)[(int64_t)b * g.G + g0 + q] = all[q];
+    }
+    __syncthreads();
+    if (h.ctas > 1) gn_cluster_arrive();
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 st = active ? all[(cv * V + j) / g.cg] : make_float2(0.f, 0.f);
+      mean[j] = st.x;
+      scale[j] *= st.y;
+    }
+    for (int i = 0; i < mine; ++i) {
+      float v[V];
+      hx[i * kGnThreads + tid].get(v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = fmaf(v[j] - mean[j], scale[j], bias[j]);
+      gn_act<V, ACT>(v);
+      Vec::put(out + i * step, v);
+    }
+  } else {
+    float mean[V], rstd[V], s1[V] = {}, s2[V] = {};
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 st = active ? reinterpret_cast<const float2*>(p.stats)[(int64_t)b * g.G + g0 + (cv * V + j) / g.cg]
+                               : make_float2(0.f, 0.f);
+      mean[j] = st.x;
+      rstd[j] = st.y;
+    }
+    for (int i = 0; i < mine; ++i) {
+      float xh[V], d[V];
+      hx[i * kGnThreads + tid].get(xh);
+      hd[i * kGnThreads + tid].get(d);
+#pragma unroll
+      for (int j = 0; j < V; ++j) xh[j] = (xh[j] - mean[j]) * rstd[j];
+      gn_du<V, ACT>(d, xh, scale, bias);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        s1[j] += d[j];
+        s2[j] = fmaf(d[j], xh[j], s2[j]);
+      }
+    }
+    // sums per channel, for dscale and dbias, and from them the groups' means
+    float* red2 = red + kGnThreads * V;
+    const int chs = h.nv * V;
+    if (active)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        red[rl * chs + cv * V + j] = s1[j];
+        red2[rl * chs + cv * V + j] = s2[j];
+      }
+    __syncthreads();
+    for (int c = tid; c < width; c += kGnThreads) {
+      float t1 = 0.f, t2 = 0.f;
+      for (int r = 0; r < h.rt; ++r) {
+        t1 += red[r * chs + c];
+        t2 += red2[r * chs + c];
+      }
+      p.sums[((int64_t)b * h.ctas + rank) * g.D + c0 + c] = make_float2(t1, t2);
+      const float w = p.scale ? p.scale[c0 + c] : 1.f;
+      red[c] = w * t1;  // this thread alone reads and writes column c of row 0
+      red2[c] = w * t2;
+    }
+    __syncthreads();
+    for (int q = warp; q < ng; q += kWarps) {
+      float t1 = 0.f, t2 = 0.f;
+      for (int c = lane; c < g.cg; c += 32) {
+        t1 += red[q * g.cg + c];
+        t2 += red2[q * g.cg + c];
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        t1 += __shfl_xor_sync(0xffffffffu, t1, o);
+        t2 += __shfl_xor_sync(0xffffffffu, t2, o);
+      }
+      if (lane == 0) own[q] = make_float2(t1, t2);
+    }
+    __syncthreads();
+    if (h.ctas > 1) {
+      gn_cluster_arrive();
+      gn_cluster_wait();
+    }
+    for (int q = tid; q < ng; q += kGnThreads) {
+      float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < h.ctas) t = fadd2(t, h.ctas > 1 ? gn_peer(own + q, r) : own[q]);
+      all[q] = make_float2(t.x / total, t.y / total);
+    }
+    __syncthreads();
+    if (h.ctas > 1) gn_cluster_arrive();
+    float m1[V], m2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 m = active ? all[(cv * V + j) / g.cg] : make_float2(0.f, 0.f);
+      m1[j] = m.x;
+      m2[j] = m.y;
+    }
+    for (int i = 0; i < mine; ++i) {
+      float xh[V], d[V];
+      hx[i * kGnThreads + tid].get(xh);
+      hd[i * kGnThreads + tid].get(d);
+#pragma unroll
+      for (int j = 0; j < V; ++j) xh[j] = (xh[j] - mean[j]) * rstd[j];
+      gn_du<V, ACT>(d, xh, scale, bias);
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[j] = rstd[j] * (d[j] * scale[j] - m1[j] - xh[j] * m2[j]);
+      Vec::put(out + i * step, d);
+    }
+  }
+  __syncwarp();
+  if (h.ctas > 1) gn_cluster_wait();  // the others read this CTA's pairs
 }
 
 static int check_gn(const ssm_group_norm_params_t* p) {
@@ -426,6 +754,53 @@ static GnGeom gn_geom(const ssm_group_norm_params_t* p) {
   return g;
 }
 
+// The held form's cut, or false where a group is too long for it.  Jobs are
+// sized so that four CTAs share an SM (one's loads overlap another's sums), rows
+// read at least 128 bytes where the groups allow it, and small calls spread over
+// the SMs.
+constexpr size_t kHoldTile = 48 * 1024, kHoldMost = 96 * 1024;
+static bool gn_hold(const ssm_group_norm_params_t* p, bool bwd, GnHold* h, int* V) {
+  const int es = p->dtype == SSM_BF16 ? 2 : 4, cg = p->dim / p->groups;
+  const int wide = 16 / es;
+  const bool vec = p->dim % wide == 0 && aligned16(p->x) && aligned16(bwd ? p->dx : p->y) && (!bwd || aligned16(p->dy));
+  // the fewest groups that make whole vectors (all of them do)
+  int least = 1;
+  *V = vec ? wide : 1;
+  while (least * cg % *V) ++least;
+  bool found = false;
+  for (int ctas = 1; ctas <= 8; ctas *= 2) {
+    if (ctas > 1 && p->seqlen < ctas * 4) break;
+    const int64_t rows = (p->seqlen + ctas - 1) / ctas;
+    if (rows > 65536) continue;
+    const auto fits = [&](int gpj, size_t tile) {
+      return (size_t)rows * gpj * cg * es * (bwd ? 2 : 1) <= tile && gpj * cg / *V <= kGnThreads;
+    };
+    if (!fits(least, kHoldMost)) continue;
+    int gpj = least;
+    while (gpj + least <= p->groups &&
+           (fits(gpj + least, kHoldTile) || (gpj * cg * es < 128 && fits(gpj + least, kHoldMost))))
+      gpj += least;
+    const auto count = [&](int q) { return p->batch * ((p->groups + q - 1) / q) * ctas; };
+    while (gpj > least && gpj * cg * es > 128 && count(gpj) < 2 * 148) gpj -= least;
+    GnHold c;
+    c.gpj = gpj;
+    c.W = gpj * cg;
+    c.jobs = (p->groups + gpj - 1) / gpj;
+    c.ctas = ctas;
+    c.rows = rows;
+    c.nv = c.W / *V;
+    c.rt = kGnThreads / c.nv;
+    c.slots = (int)((rows + c.rt - 1) / c.rt);
+    c.smem = ((size_t)c.slots * kGnThreads * *V * es * (bwd ? 2 : 1) + 15) / 16 * 16 +
+             (size_t)kGnThreads * *V * 4 * (bwd ? 2 : 1) + 2 * (size_t)gpj * sizeof(float2);
+    if (c.smem > 200 * 1024 || (int64_t)c.jobs * p->batch * ctas > 0x7fffffff) continue;
+    *h = c;
+    found = true;
+    if (count(gpj) >= 2 * 148 && c.smem <= kHoldTile + 24 * 1024) break;
+  }
+  return found;
+}
+
 static size_t gn_round(size_t v) { return (v + 255) / 256 * 256; }
 static size_t gn_part_bytes(const GnGeom& g) { return gn_round((size_t)g.B * g.chunks * g.D * sizeof(float2)); }
 static size_t gn_sums_bytes(const GnGeom& g) { return gn_round((size_t)g.B * g.D * sizeof(float2)); }
@@ -450,7 +825,7 @@ static void gn_bwd_launch(const GnArgs& a, cudaStream_t s) {
   gn_sums_kernel<T, V, ACT><<<grid, kGnThreads, smem, s>>>(a);
   gn_means_kernel<<<g.B * g.G, kGnThreads, 0, s>>>(a);
   gn_dx_kernel<T, V, ACT><<<grid, kGnThreads, 0, s>>>(a);
-  gn_param_kernel<<<(g.D + 127) / 128, 128, 0, s>>>(a);
+  gn_param_kernel<<<(g.D + 31) / 32, 1024, 0, s>>>(a.sums, g.B, g.D, a.dscale, a.dbias);
   note_launches(4);
 }
 
@@ -464,7 +839,57 @@ static void gn_launch(const GnArgs& a, int act, bool bwd, cudaStream_t s) {
   }
 }
 
+template <typename T, int V, int ACT, bool BWD>
+static cudaError_t gn_hold_launch(const GnArgs& a, const GnHold& h, cudaStream_t s) {
+  const auto kernel = gn_hold_kernel<T, V, ACT, BWD>;
+  if (h.smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)h.smem);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.g.B * h.jobs * h.ctas));
+  cfg.blockDim = dim3(kGnThreads);
+  cfg.dynamicSmemBytes = h.smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = h.ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, h);
+  note_launches(1);
+  if (BWD && e == cudaSuccess && (a.dscale || a.dbias)) {
+    gn_param_kernel<<<(a.g.D + 31) / 32, 1024, 0, s>>>(a.sums, a.g.B * h.ctas, a.g.D, a.dscale, a.dbias);
+    note_launches(1);
+  }
+  return e;
+}
+template <typename T, int V, bool BWD>
+static cudaError_t gn_hold_act(const GnArgs& a, const GnHold& h, int act, cudaStream_t s) {
+  switch (act) {
+    case SSM_ACT_SILU: return gn_hold_launch<T, V, SSM_ACT_SILU, BWD>(a, h, s);
+    case SSM_ACT_GELU: return gn_hold_launch<T, V, SSM_ACT_GELU, BWD>(a, h, s);
+    case SSM_ACT_RELU: return gn_hold_launch<T, V, SSM_ACT_RELU, BWD>(a, h, s);
+    default: return gn_hold_launch<T, V, SSM_ACT_NONE, BWD>(a, h, s);
+  }
+}
+template <bool BWD>
+static cudaError_t gn_hold_run(const ssm_group_norm_params_t* p, const GnArgs& a, const GnHold& h, int V, cudaStream_t s) {
+  if (p->dtype == SSM_BF16)
+    return V == 1 ? gn_hold_act<__nv_bfloat16, 1, BWD>(a, h, p->act, s) : gn_hold_act<__nv_bfloat16, 8, BWD>(a, h, p->act, s);
+  return V == 1 ? gn_hold_act<float, 1, BWD>(a, h, p->act, s) : gn_hold_act<float, 4, BWD>(a, h, p->act, s);
+}
+
 static int gn_dispatch(const ssm_group_norm_params_t* p, GnArgs& a, bool bwd, cudaStream_t s) {
+  GnHold h;
+  int V;
+  if (gn_hold(p, bwd, &h, &V)) {
+    a.sums = reinterpret_cast<float2*>(p->workspace);
+    cudaError_t e = bwd ? gn_hold_run<true>(p, a, h, V, s) : gn_hold_run<false>(p, a, h, V, s);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    return e == cudaSuccess ? SSM_OK : launch_error("launch group norm kernel", e);
+  }
   const bool vec = gn_vector(p);
   if (p->dtype == SSM_BF16) {
     if (vec) gn_launch<__nv_bfloat16, 8>(a, p->act, bwd, s);
@@ -485,13 +910,17 @@ extern "C" {
 
 size_t ssm_group_norm_fwd_workspace_bytes(const ssm_group_norm_params_t* p) {
   if (check_gn(p) || p->batch == 0 || p->seqlen == 0) return 0;
-  return gn_part_bytes(gn_geom(p));
+  GnHold h;
+  int V;
+  // without the pointers their alignment, which has a say in the form, is unknown
+  return p->x && p->y && gn_hold(p, false, &h, &V) ? 0 : gn_part_bytes(gn_geom(p));
 }
 
 size_t ssm_group_norm_bwd_workspace_bytes(const ssm_group_norm_params_t* p) {
   if (check_gn(p) || p->batch == 0 || p->seqlen == 0) return 0;
   const GnGeom g = gn_geom(p);
-  return gn_part_bytes(g) + gn_sums_bytes(g) + gn_means_bytes(g);
+  const size_t split = gn_part_bytes(g) + gn_sums_bytes(g) + gn_means_bytes(g);
+  return std::max(split, gn_round((size_t)g.B * 8 * g.D * sizeof(float2)));  // of either form, whatever its cut
 }
 
 int ssm_group_norm_act_fwd(const ssm_group_norm_params_t* p, ssm_stream_t stream) {
@@ -500,7 +929,8 @@ int ssm_group_norm_act_fwd(const ssm_group_norm_params_t* p, ssm_stream_t stream
   if (p->batch == 0 || p->seqlen == 0) return SSM_OK;
   if (!p->x || !p->y || !p->stats) return SSM_ERR_NULL;
   if (gn_vector(p) && (!aligned16(p->x) || !aligned16(p->y))) return SSM_ERR_ALIGN;
-  if (!p->workspace || p->workspace_bytes < ssm_group_norm_fwd_workspace_bytes(p)) return SSM_ERR_WORKSPACE;
+  const size_t need = ssm_group_norm_fwd_workspace_bytes(p);
+  if (need && (!p->workspace || p->workspace_bytes < need)) return SSM_ERR_WORKSPACE;
   st = bind_device(p->x);
   if (st) return st;
   GnArgs a = {};
