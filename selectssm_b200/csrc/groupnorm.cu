@@ -74,22 +74,6 @@ __device__ __forceinline__ void store_v(T* p, const float (&v)[V]) {
   else *p = Cvt<T>::from_f(v[0]);
 }
 
-// Per-channel constants of a thread's V channels.
-template <int V>
-struct GnChan {
-  float mean[V], rstd[V], scale[V], bias[V];
-  __device__ __forceinline__ void load(const GnArgs& p, int b, int c0) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float2 s = reinterpret_cast<const float2*>(p.stats)[(int64_t)b * p.g.G + (c0 + i) / p.g.cg];
-      mean[i] = s.x;
-      rstd[i] = s.y;
-      scale[i] = p.scale ? p.scale[c0 + i] : 1.f;
-      bias[i] = p.bias ? p.bias[c0 + i] : 0.f;
-    }
-  }
-};
-
 struct GnPlace {
   int b, chunk, vec, r0;
   bool active;
@@ -110,56 +94,152 @@ __device__ __forceinline__ GnPlace gn_place(const GnGeom& g, bool reversed) {
   return q;
 }
 
-// Mean and sum of squared deviations per channel of a chunk.  Rows come in
-// batches of kRows: each batch's mean and deviations are formed from its own
-// values and merged into the running pair with Chan's update, so no large mean
-// is ever subtracted from a sum of squares.
+// Elementwise on V values, two at a time.
+template <int V, typename F>
+__device__ __forceinline__ void gn_pairs(float (&a)[V], F f) {
+  if constexpr (V == 1) {
+    a[0] = f(make_float2(a[0], 0.f), 0).x;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 r = f(make_float2(a[i], a[i + 1]), i);
+      a[i] = r.x;
+      a[i + 1] = r.y;
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ float2 gn_at(const float (&a)[V], int i) {
+  return make_float2(a[i], V == 1 ? 0.f : a[i + (V > 1)]);
+}
+template <int V>
+__device__ __forceinline__ void gn_add(float (&a)[V], const float (&b)[V]) {
+  gn_pairs<V>(a, [&](float2 x, int i) { return fadd2(x, gn_at<V>(b, i)); });
+}
+template <int V>
+__device__ __forceinline__ void gn_sub(float (&a)[V], const float (&b)[V]) {
+  gn_pairs<V>(a, [&](float2 x, int i) { return fsub2(x, gn_at<V>(b, i)); });
+}
+template <int V>
+__device__ __forceinline__ void gn_mul(float (&a)[V], const float (&b)[V]) {
+  gn_pairs<V>(a, [&](float2 x, int i) { return fmul2(x, gn_at<V>(b, i)); });
+}
+template <int V>  // a += b c
+__device__ __forceinline__ void gn_fma(float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  gn_pairs<V>(a, [&](float2 x, int i) { return ffma2(gn_at<V>(b, i), gn_at<V>(c, i), x); });
+}
+template <int V>  // a = a b + c
+__device__ __forceinline__ void gn_muladd(float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  gn_pairs<V>(a, [&](float2 x, int i) { return ffma2(x, gn_at<V>(b, i), gn_at<V>(c, i)); });
+}
+
+// du of V elements from d = dy and xh = xhat (d is overwritten)
+template <int V, int ACT>
+__device__ __forceinline__ void gn_du(float (&d)[V], const float (&xh)[V], const float (&scale)[V], const float (&bias)[V]) {
+  if constexpr (ACT != 0) {
+    float u[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) u[i] = xh[i];
+    gn_muladd<V>(u, scale, bias);
+    gn_pairs<V>(d, [&](float2 x, int i) { return fmul2(x, slope2<ACT>(gn_at<V>(u, i))); });
+  }
+}
+
+// ---------------------------------------------------------------- split form
+// Rows that a thread loads before it uses them: 64 bytes of each input in
+// flight, and few enough registers for four CTAs an SM, whose warps then stand
+// at different points of their loops.  (With eight rows and two CTAs the sums of
+// 64 x 2048 x 768 bf16 ran at 4.0 TB/s.)
+template <typename T, int V> constexpr int kGnRows = V == 1 ? 8 : sizeof(T) == 2 ? 4 : 2;
+
 template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(const GnArgs p) {
+struct GnRaw;  // V values as they lie in global memory
+template <typename T> struct GnRaw<T, 8> : Raw8<T> {};
+template <typename T> struct GnRaw<T, 1> {
+  T r;
+  __device__ __forceinline__ void load(const T* p) { r = *p; }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = Cvt<T>::to_f(r); }
+};
+
+// A thread's walk over its rows: f(v) for every row's V values, of x alone or of x and dy.
+template <typename T, int V, typename F>
+__device__ __forceinline__ void gn_walk(const T* x, int64_t step, int rows, F f) {
+  constexpr int R = kGnRows<T, V>;
+  for (; rows > 0; rows -= R, x += R * step) {
+    GnRaw<T, V> raw[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+      if (k < rows) raw[k].load(x + k * step);
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      if (k >= rows) break;
+      float v[V];
+      raw[k].get(v);
+      f(k * step, v);
+    }
+  }
+}
+template <typename T, int V, typename F>
+__device__ __forceinline__ void gn_walk2(const T* x, const T* dy, int64_t step, int rows, F f) {
+  constexpr int R = kGnRows<T, V>;
+  for (; rows > 0; rows -= R, x += R * step, dy += R * step) {
+    GnRaw<T, V> raw[R], rd[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+      if (k < rows) {
+        raw[k].load(x + k * step);
+        rd[k].load(dy + k * step);
+      }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      if (k >= rows) break;
+      float v[V], d[V];
+      raw[k].get(v);
+      rd[k].get(d);
+      f(k * step, v, d);
+    }
+  }
+}
+
+// Mean and sum of squared deviations per channel of a chunk.  The values are
+// summed about the thread's first one of each channel, runs of 64 rows at a time
+// whose mean and deviations are merged into the running pair with Chan's update:
+// a far-off first value costs digits of one run only, and no large mean is ever
+// subtracted from a sum of squares.
+template <typename T, int V>
+__global__ void __launch_bounds__(kGnThreads, 3) gn_stats_kernel(const GnArgs p) {
   extern __shared__ float sm[];
-  constexpr int kRows = 8;
   const GnGeom& g = p.g;
   const GnPlace q = gn_place(g, false);
-  const T* x = static_cast<const T*>(p.x) + (int64_t)q.b * g.L * g.D + (int64_t)q.vec * V;
   float mean[V], m2[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) mean[i] = m2[i] = 0.f;
   float n = 0.f;
   if (q.active) {
-    int64_t l = q.l0 + q.r0;
-    for (; l + (int64_t)(kRows - 1) * g.rt < q.l1; l += (int64_t)kRows * g.rt) {
-      float v[kRows][V];
+    const int64_t step = (int64_t)g.rt * g.D;
+    const T* x = static_cast<const T*>(p.x) + ((int64_t)q.b * g.L + q.l0 + q.r0) * g.D + (int64_t)q.vec * V;
+    int64_t rows = (q.l1 - q.l0 - q.r0 + g.rt - 1) / g.rt;
+    for (; rows > 0; rows -= 64, x += 64 * step) {
+      const int run = (int)min(rows, (int64_t)64);
+      float ref[V], s[V], ss[V];
+      GnRaw<T, V> first;
+      first.load(x);
+      first.get(ref);
 #pragma unroll
-      for (int k = 0; k < kRows; ++k) load_v<T, V>(x + (l + (int64_t)k * g.rt) * g.D, v[k]);
-      const float nn = n + kRows, w = kRows / nn;
+      for (int i = 0; i < V; ++i) s[i] = ss[i] = 0.f;
+      gn_walk<T, V>(x, step, run, [&](int64_t, float (&v)[V]) {
+        gn_sub<V>(v, ref);
+        gn_add<V>(s, v);
+        gn_fma<V>(ss, v, v);
+      });
+      const float inv = 1.f / (float)run, nn = n + (float)run, w = (float)run / nn;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float s = 0.f, d2 = 0.f;
-#pragma unroll
-        for (int k = 0; k < kRows; ++k) s += v[k][i];
-        const float bm = s * (1.f / kRows);
-#pragma unroll
-        for (int k = 0; k < kRows; ++k) {
-          const float d = v[k][i] - bm;
-          d2 = fmaf(d, d, d2);
-        }
-        const float delta = bm - mean[i];
+        const float off = s[i] * inv, dev = fmaxf(fmaf(-s[i], off, ss[i]), 0.f), delta = ref[i] + off - mean[i];
         mean[i] = fmaf(delta, w, mean[i]);
-        m2[i] += d2 + delta * delta * n * w;
+        m2[i] += fmaf(delta * delta, n * w, dev);
       }
       n = nn;
-    }
-    for (; l < q.l1; l += g.rt) {
-      float v[V];
-      load_v<T, V>(x + l * g.D, v);
-      n += 1.f;
-      const float w = 1.f / n;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float delta = v[i] - mean[i];
-        mean[i] = fmaf(delta, w, mean[i]);
-        m2[i] = fmaf(delta, v[i] - mean[i], m2[i]);
-      }
     }
   }
   // merge the rt row lanes of each channel in order
@@ -178,9 +258,10 @@ __global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(const GnArgs p) {
   for (int c = threadIdx.x; c < width; c += kGnThreads) {
     const int ch = blockIdx.z * width + c;
     if (ch >= g.D) break;
+    const float ref = smean[c];
     float s = 0.f;
-    for (int r = 0; r < g.rt; ++r) s = fmaf(sn[r], smean[r * width + c], s);
-    const float mu = s / total;
+    for (int r = 1; r < g.rt; ++r) s = fmaf(sn[r], smean[r * width + c] - ref, s);
+    const float mu = ref + s / total;
     float d2 = 0.f;
     for (int r = 0; r < g.rt; ++r) {
       const float d = smean[r * width + c] - mu;
@@ -201,98 +282,114 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
   return s;
 }
 
+// Calls f(chunk, channel) for every partial of a group, dealt out over the
+// CTA's threads: neighbouring threads take neighbouring channels.
+template <typename F>
+__device__ __forceinline__ void gn_each_part(const GnGeom& g, F f) {
+  if (g.cg <= kGnThreads) {
+    const int at_once = kGnThreads / g.cg, k = threadIdx.x / g.cg, c = threadIdx.x - k * g.cg;
+    if (k < at_once)
+      for (int ck = k; ck < g.chunks; ck += at_once) f(ck, c);
+  } else {
+    for (int ck = 0; ck < g.chunks; ++ck)
+      for (int c = threadIdx.x; c < g.cg; c += kGnThreads) f(ck, c);
+  }
+}
+
 // mean and rstd of one group from its chunks' and channels' partials
 __global__ void __launch_bounds__(kGnThreads) gn_merge_kernel(const GnArgs p) {
   __shared__ float buf[kGnThreads / 32];
   const GnGeom& g = p.g;
   const int grp = blockIdx.x % g.G, b = blockIdx.x / g.G;
   const float2* part = p.part + (int64_t)b * g.chunks * g.D + grp * g.cg;
-  const int items = g.chunks * g.cg;
-  const float count = (float)g.L * (float)g.cg;
+  const float inv = 1.f / ((float)g.L * (float)g.cg), ref = part[0].x;  // so that equal means merge to themselves
+  const auto size = [&](int ck) { return (float)(min((ck + 1) * g.chunk, g.L) - ck * g.chunk); };
   float s = 0.f;
-  const float ref = part[0].x;  // so that equal means merge to themselves
-  for (int i = threadIdx.x; i < items; i += kGnThreads) {
-    const int ck = i / g.cg, c = i - ck * g.cg;
-    const float n = (float)(min((ck + 1) * g.chunk, g.L) - ck * g.chunk);
-    s = fmaf(n / count, part[(int64_t)ck * g.D + c].x - ref, s);
-  }
+  gn_each_part(g, [&](int ck, int c) { s = fmaf(size(ck) * inv, part[(int64_t)ck * g.D + c].x - ref, s); });
   const float mu = block_sum(s, buf) + ref;
   float d2 = 0.f;
-  for (int i = threadIdx.x; i < items; i += kGnThreads) {
-    const int ck = i / g.cg, c = i - ck * g.cg;
-    const float n = (float)(min((ck + 1) * g.chunk, g.L) - ck * g.chunk);
+  gn_each_part(g, [&](int ck, int c) {
     const float2 v = part[(int64_t)ck * g.D + c];
-    d2 += v.y + n * (v.x - mu) * (v.x - mu);
-  }
-  const float var = block_sum(d2, buf) / count;
-  if (threadIdx.x == 0) reinterpret_cast<float2*>(p.stats)[blockIdx.x] = make_float2(mu, 1.f / sqrtf(var + p.eps));
+    d2 += v.y + size(ck) * (v.x - mu) * (v.x - mu);
+  });
+  const float var = block_sum(d2, buf) * inv;
+  if (threadIdx.x == 0) reinterpret_cast<float2*>(p.stats)[blockIdx.x] = make_float2(mu, rsqrtf(var + p.eps));
 }
 
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(const GnArgs p) {
-  constexpr int kRows = 4;
+// A thread's constants: one pair of statistics where its channels share a group
+// (ONE), else one a channel.
+template <int V, bool ONE>
+struct GnStat {
+  float a[ONE ? 1 : V], b[ONE ? 1 : V];
+  __device__ __forceinline__ void load(const float2* from, int b_, const GnGeom& g, int c0) {
+#pragma unroll
+    for (int i = 0; i < (ONE ? 1 : V); ++i) {
+      const float2 s = from[(int64_t)b_ * g.G + (c0 + i) / g.cg];
+      a[i] = s.x;
+      b[i] = s.y;
+    }
+  }
+  __device__ __forceinline__ float2 a2(int i) const { return ONE ? dup2(a[0]) : gn_at<ONE ? 1 : V>(a, ONE ? 0 : i); }
+  __device__ __forceinline__ float2 b2(int i) const { return ONE ? dup2(b[0]) : gn_at<ONE ? 1 : V>(b, ONE ? 0 : i); }
+};
+template <int V>
+__device__ __forceinline__ void gn_affine(const GnArgs& p, int c0, float (&scale)[V], float (&bias)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    scale[i] = p.scale ? p.scale[c0 + i] : 1.f;
+    bias[i] = p.bias ? p.bias[c0 + i] : 0.f;
+  }
+}
+
+template <typename T, int V, int ACT, bool ONE>
+__global__ void __launch_bounds__(kGnThreads, 3) gn_apply_kernel(const GnArgs p) {
   const GnGeom& g = p.g;
   const GnPlace q = gn_place(g, true);
   if (!q.active) return;
-  GnChan<V> c;
-  c.load(p, q.b, q.vec * V);
-  float a[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) a[i] = c.rstd[i] * c.scale[i];
-  const int64_t base = (int64_t)q.b * g.L * g.D + (int64_t)q.vec * V;
+  float scale[V], bias[V];
+  gn_affine<V>(p, q.vec * V, scale, bias);
+  GnStat<V, ONE> st;
+  st.load(reinterpret_cast<const float2*>(p.stats), q.b, g, q.vec * V);
+  gn_pairs<V>(scale, [&](float2 x, int i) { return fmul2(x, st.b2(i)); });
+  const int64_t base = ((int64_t)q.b * g.L + q.l0 + q.r0) * g.D + (int64_t)q.vec * V, step = (int64_t)g.rt * g.D;
   const T* x = static_cast<const T*>(p.x) + base;
   T* y = static_cast<T*>(p.out) + base;
-  for (int64_t l = q.l0 + q.r0; l < q.l1; l += (int64_t)kRows * g.rt) {
-    float v[kRows][V];
-#pragma unroll
-    for (int k = 0; k < kRows; ++k)
-      if (l + (int64_t)k * g.rt < q.l1) load_v<T, V>(x + (l + (int64_t)k * g.rt) * g.D, v[k]);
-#pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      if (l + (int64_t)k * g.rt >= q.l1) break;
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[k][i] = act_f(fmaf(v[k][i] - c.mean[i], a[i], c.bias[i]), ACT);
-      store_v<T, V>(y + (l + (int64_t)k * g.rt) * g.D, v[k]);
+  constexpr int R = kGnRows<T, V>;
+  int count = 0;
+  gn_walk<T, V>(x, step, (int)((q.l1 - q.l0 - q.r0 + g.rt - 1) / g.rt), [&](int64_t at, float (&v)[V]) {
+    gn_pairs<V>(v, [&](float2 t, int i) {
+      return act2<ACT>(ffma2(fsub2(t, st.a2(i)), gn_at<V>(scale, i), gn_at<V>(bias, i)));
+    });
+    store_v<T, V>(y + at, v);
+    if (++count == R) {
+      count = 0;
+      y += R * step;
     }
-  }
+  });
 }
 
 // Sums over a chunk of du and du xhat per channel.
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kGnThreads) gn_sums_kernel(const GnArgs p) {
+template <typename T, int V, int ACT, bool ONE>
+__global__ void __launch_bounds__(kGnThreads, 2) gn_sums_kernel(const GnArgs p) {
   extern __shared__ float sm[];
-  constexpr int kRows = 2;
   const GnGeom& g = p.g;
   const GnPlace q = gn_place(g, false);
   float s1[V], s2[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
   if (q.active) {
-    GnChan<V> c;
-    c.load(p, q.b, q.vec * V);
-    const int64_t base = (int64_t)q.b * g.L * g.D + (int64_t)q.vec * V;
-    const T* x = static_cast<const T*>(p.x) + base;
-    const T* dy = static_cast<const T*>(p.dy) + base;
-    for (int64_t l = q.l0 + q.r0; l < q.l1; l += (int64_t)kRows * g.rt) {
-      float v[kRows][V], d[kRows][V];
-#pragma unroll
-      for (int k = 0; k < kRows; ++k)
-        if (l + (int64_t)k * g.rt < q.l1) {
-          load_v<T, V>(x + (l + (int64_t)k * g.rt) * g.D, v[k]);
-          load_v<T, V>(dy + (l + (int64_t)k * g.rt) * g.D, d[k]);
-        }
-#pragma unroll
-      for (int k = 0; k < kRows; ++k) {
-        if (l + (int64_t)k * g.rt >= q.l1) break;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float xh = (v[k][i] - c.mean[i]) * c.rstd[i];
-          const float du = ACT ? d[k][i] * act_grad_f(fmaf(xh, c.scale[i], c.bias[i]), ACT) : d[k][i];
-          s1[i] += du;
-          s2[i] = fmaf(du, xh, s2[i]);
-        }
-      }
-    }
+    float scale[V], bias[V];
+    gn_affine<V>(p, q.vec * V, scale, bias);
+    GnStat<V, ONE> st;
+    st.load(reinterpret_cast<const float2*>(p.stats), q.b, g, q.vec * V);
+    const int64_t base = ((int64_t)q.b * g.L + q.l0 + q.r0) * g.D + (int64_t)q.vec * V, step = (int64_t)g.rt * g.D;
+    gn_walk2<T, V>(static_cast<const T*>(p.x) + base, static_cast<const T*>(p.dy) + base, step,
+                   (int)((q.l1 - q.l0 - q.r0 + g.rt - 1) / g.rt), [&](int64_t, float (&v)[V], float (&d)[V]) {
+                     gn_pairs<V>(v, [&](float2 t, int i) { return fmul2(fsub2(t, st.a2(i)), st.b2(i)); });
+                     gn_du<V, ACT>(d, v, scale, bias);
+                     gn_add<V>(s1, d);
+                     gn_fma<V>(s2, d, v);
+                   });
   }
   const int width = g.ct * V, mine = (threadIdx.x % g.ct) * V;
   float *a1 = sm, *a2 = sm + g.rt * width;
@@ -349,45 +446,34 @@ __global__ void __launch_bounds__(kGnThreads) gn_means_kernel(const GnArgs p) {
   if (threadIdx.x == 0) p.means[blockIdx.x] = make_float2(t1 / count, t2 / count);
 }
 
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kGnThreads) gn_dx_kernel(const GnArgs p) {
-  constexpr int kRows = 2;
+template <typename T, int V, int ACT, bool ONE>
+__global__ void __launch_bounds__(kGnThreads, 2) gn_dx_kernel(const GnArgs p) {
   const GnGeom& g = p.g;
   const GnPlace q = gn_place(g, true);
   if (!q.active) return;
-  GnChan<V> c;
-  c.load(p, q.b, q.vec * V);
-  float m1[V], m2[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float2 m = p.means[(int64_t)q.b * g.G + (q.vec * V + i) / g.cg];
-    m1[i] = m.x;
-    m2[i] = m.y;
-  }
-  const int64_t base = (int64_t)q.b * g.L * g.D + (int64_t)q.vec * V;
-  const T* x = static_cast<const T*>(p.x) + base;
-  const T* dy = static_cast<const T*>(p.dy) + base;
+  float scale[V], bias[V];
+  gn_affine<V>(p, q.vec * V, scale, bias);
+  GnStat<V, ONE> st, mm;
+  st.load(reinterpret_cast<const float2*>(p.stats), q.b, g, q.vec * V);
+  mm.load(p.means, q.b, g, q.vec * V);
+  const int64_t base = ((int64_t)q.b * g.L + q.l0 + q.r0) * g.D + (int64_t)q.vec * V, step = (int64_t)g.rt * g.D;
   T* dx = static_cast<T*>(p.out) + base;
-  for (int64_t l = q.l0 + q.r0; l < q.l1; l += (int64_t)kRows * g.rt) {
-    float v[kRows][V], d[kRows][V];
-#pragma unroll
-    for (int k = 0; k < kRows; ++k)
-      if (l + (int64_t)k * g.rt < q.l1) {
-        load_v<T, V>(x + (l + (int64_t)k * g.rt) * g.D, v[k]);
-        load_v<T, V>(dy + (l + (int64_t)k * g.rt) * g.D, d[k]);
-      }
-#pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      if (l + (int64_t)k * g.rt >= q.l1) break;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float xh = (v[k][i] - c.mean[i]) * c.rstd[i];
-        const float du = ACT ? d[k][i] * act_grad_f(fmaf(xh, c.scale[i], c.bias[i]), ACT) : d[k][i];
-        v[k][i] = c.rstd[i] * (du * c.scale[i] - m1[i] - xh * m2[i]);
-      }
-      store_v<T, V>(dx + (l + (int64_t)k * g.rt) * g.D, v[k]);
-    }
-  }
+  constexpr int R = kGnRows<T, V>;
+  int count = 0;
+  gn_walk2<T, V>(static_cast<const T*>(p.x) + base, static_cast<const T*>(p.dy) + base, step,
+                 (int)((q.l1 - q.l0 - q.r0 + g.rt - 1) / g.rt), [&](int64_t at, float (&v)[V], float (&d)[V]) {
+                   gn_pairs<V>(v, [&](float2 t, int i) { return fmul2(fsub2(t, st.a2(i)), st.b2(i)); });
+                   gn_du<V, ACT>(d, v, scale, bias);
+                   gn_pairs<V>(d, [&](float2 t, int i) {  // rstd (du scale - m1 - xhat m2)
+                     const float2 r = fsub2(fmul2(t, gn_at<V>(scale, i)), mm.a2(i));
+                     return fmul2(fsub2(r, fmul2(gn_at<V>(v, i), mm.b2(i))), st.b2(i));
+                   });
+                   store_v<T, V>(dx + at, d);
+                   if (++count == R) {
+                     count = 0;
+                     dx += R * step;
+                   }
+                 });
 }
 
 // dscale and dbias: `rows` partial sums of every channel in a fixed order
@@ -412,8 +498,9 @@ __global__ void __launch_bounds__(1024) gn_param_kernel(const float2* sums, int 
 // A job: `gpj` groups (W channels) of one batch row, `ctas` CTAs with `rows`
 // rows each.  nv vectors of V channels by rt row lanes; each thread keeps
 // `slots` vectors of its own in shared memory.
+constexpr int kHoldThreads = 256;  // at most
 struct GnHold {
-  int32_t W, gpj, jobs, ctas, nv, rt, slots;
+  int32_t threads, W, gpj, jobs, ctas, nv, rt, slots;
   int64_t rows;
   size_t smem;
 };
@@ -448,48 +535,18 @@ __device__ __forceinline__ float2 gn_peer(const float2* p, int cta) {
   return v;
 }
 
-// du of V elements from d = dy and xh = xhat (d is overwritten)
-template <int V, int ACT>
-__device__ __forceinline__ void gn_du(float (&d)[V], const float (&xh)[V], const float (&scale)[V], const float (&bias)[V]) {
-  if constexpr (ACT == 0) return;
-  float u[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) u[i] = fmaf(xh[i], scale[i], bias[i]);
-  if constexpr (V == 1) {
-    d[0] *= slope2<ACT>(make_float2(u[0], 0.f)).x;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i += 2) {
-      const float2 y = fmul2(make_float2(d[i], d[i + 1]), slope2<ACT>(make_float2(u[i], u[i + 1])));
-      d[i] = y.x;
-      d[i + 1] = y.y;
-    }
-  }
-}
-template <int V, int ACT>
-__device__ __forceinline__ void gn_act(float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = act2<ACT>(make_float2(v[0], 0.f)).x;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i += 2) {
-      const float2 y = act2<ACT>(make_float2(v[i], v[i + 1]));
-      v[i] = y.x;
-      v[i + 1] = y.y;
-    }
-  }
-}
-
 template <typename T, int V, int ACT, bool BWD>
-__global__ void __launch_bounds__(kGnThreads) gn_hold_kernel(const GnArgs p, const GnHold h) {
+__global__ void __launch_bounds__(kHoldThreads, 3) gn_hold_kernel(const GnArgs p, const GnHold h) {
   using Vec = GnVec<T, V>;
-  constexpr int kWarps = kGnThreads / 32;
   extern __shared__ __align__(16) uint8_t raw[];
+  __shared__ float parts[kHoldThreads / 32];
   const GnGeom& g = p.g;
+  const int threads = blockDim.x, warps = threads >> 5;
   Vec* hx = reinterpret_cast<Vec*>(raw);
-  Vec* hd = hx + (BWD ? h.slots * kGnThreads : 0);
-  float* red = reinterpret_cast<float*>(raw + ((size_t)h.slots * kGnThreads * sizeof(Vec) * (BWD ? 2 : 1) + 15) / 16 * 16);
-  float2* own = reinterpret_cast<float2*>(red + kGnThreads * V * (BWD ? 2 : 1));  // this CTA's pair of each group
+  Vec* hd = hx + (BWD ? h.slots * threads : 0);
+  float* red = reinterpret_cast<float*>(raw + ((size_t)h.slots * threads * sizeof(Vec) * (BWD ? 2 : 1) + 15) / 16 * 16);
+  float2* chan = reinterpret_cast<float2*>(red + threads * (BWD || g.cg % V ? V : 2));  // backward: sums per channel
+  float2* own = chan + (BWD ? h.W : 0);  // this CTA's pair of each group
   float2* all = own + h.gpj;                                                       // the job's
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int rank = 0;
@@ -504,17 +561,27 @@ __global__ void __launch_bounds__(kGnThreads) gn_hold_kernel(const GnArgs p, con
   const T* x = static_cast<const T*>(p.x) + base;
   const T* dy = BWD ? static_cast<const T*>(p.dy) + base : nullptr;
 
+#pragma unroll 4
   for (int i = 0; i < mine; ++i) {
     if constexpr (sizeof(Vec) == 16) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hx + i * kGnThreads + tid)), "l"(x + i * step)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hx + i * threads + tid)), "l"(x + i * step)
                    : "memory");
       if (BWD)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hd + i * kGnThreads + tid)),
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hd + i * threads + tid)),
                      "l"(dy + i * step)
                      : "memory");
     } else {
-      hx[i * kGnThreads + tid].r = x[i * step];
-      if (BWD) hd[i * kGnThreads + tid].r = dy[i * step];
+      hx[i * threads + tid].r = x[i * step];
+      if (BWD) hd[i * threads + tid].r = dy[i * step];
+    }
+  }
+  int grp[V];  // of the job's groups
+#pragma unroll
+  for (int j = 0, q = cv * V / g.cg, left = (q + 1) * g.cg - cv * V; j < V; ++j) {
+    grp[j] = active ? q : 0;
+    if (--left == 0) {
+      ++q;
+      left = g.cg;
     }
   }
   float scale[V], bias[V];
@@ -525,61 +592,72 @@ __global__ void __launch_bounds__(kGnThreads) gn_hold_kernel(const GnArgs p, con
   }
   asm volatile("cp.async.wait_all;" ::: "memory");  // a thread reads only what it fetched itself
 
-  const float total = (float)g.L * (float)g.cg;
+  const float per_group = 1.f / ((float)g.L * (float)g.cg);
   T* out = static_cast<T*>(p.out) + base;
-  // Per-thread values to sums over each group, in a fixed order; the result in
-  // `dst[group].x` or `.y`.  Vectors that lie in one group are summed first.
+  // Per-thread values to sums over each group, in a fixed order, handed to
+  // finish(group, sum).  Vectors that lie in one group are summed first.  A
+  // group's values lie together, so that as many warps as there are for each
+  // group walk over them without a division.
   const bool single = g.cg % V == 0;
-  const int unit = single ? V : 1, per = g.cg / unit, units = h.nv * V / unit;
+  const int unit = single ? V : 1, entries = g.cg / unit * h.rt;
+  const int share = max(warps / ng, 1);  // warps for a group
   const auto group_sums = [&](const float (&s)[V], auto finish) {
     if (active) {
       if (single) {
         float t = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) t += s[i];
-        red[rl * units + cv] = t;
+        red[cv * h.rt + rl] = t;
       } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) red[rl * units + cv * V + i] = s[i];
+        for (int i = 0; i < V; ++i) red[(cv * V + i) * h.rt + rl] = s[i];
       }
     }
     __syncthreads();
-    for (int q = warp; q < ng; q += kWarps) {
+    for (int w = warp; w < ng * share; w += warps) {
+      const int q = w / share, part = w - q * share;
+      const float* from = red + q * entries;
       float t = 0.f;
-      for (int i = lane; i < h.rt * per; i += 32) {
-        const int r = i / per;
-        t += red[r * units + q * per + (i - r * per)];
-      }
+      for (int i = part * 32 + lane; i < entries; i += 32 * share) t += from[i];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      if (lane == 0) finish(q, t);
+      if (lane == 0) {
+        if (share == 1) finish(q, t);
+        else parts[w] = t;
+      }
     }
     __syncthreads();
+    if (share > 1) {
+      if (tid < ng) {
+        float t = 0.f;
+        for (int i = 0; i < share; ++i) t += parts[tid * share + i];
+        finish(tid, t);
+      }
+      __syncthreads();
+    }
   };
 
   if constexpr (!BWD) {
     const float n = (float)max(l1 - l0, (int64_t)0) * (float)g.cg;  // this CTA's values of a group
     float s[V] = {}, mean[V];
+#pragma unroll 4
     for (int i = 0; i < mine; ++i) {
       float v[V];
-      hx[i * kGnThreads + tid].get(v);
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[j] += v[j];
+      hx[i * threads + tid].get(v);
+      gn_add<V>(s, v);
     }
     group_sums(s, [&](int q, float t) { own[q].x = n > 0.f ? t / n : 0.f; });
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      mean[j] = active ? own[(cv * V + j) / g.cg].x : 0.f;
+      mean[j] = own[grp[j]].x;
       s[j] = 0.f;
     }
+#pragma unroll 4
     for (int i = 0; i < mine; ++i) {
       float v[V];
-      hx[i * kGnThreads + tid].get(v);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = v[j] - mean[j];
-        s[j] = fmaf(d, d, s[j]);
-      }
+      hx[i * threads + tid].get(v);
+      gn_sub<V>(v, mean);
+      gn_fma<V>(s, v, v);
     }
     group_sums(s, [&](int q, float t) { own[q].y = t; });
     // the CTAs' means and squared deviations, merged about the common mean
@@ -587,95 +665,98 @@ __global__ void __launch_bounds__(kGnThreads) gn_hold_kernel(const GnArgs p, con
       gn_cluster_arrive();
       gn_cluster_wait();
     }
-    for (int q = tid; q < ng; q += kGnThreads) {
-      // (from the first one's mean, so that equal means merge to themselves)
-      float mu = 0.f, m2 = 0.f;
-      float2 each[8];
-      float cnt[8];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        cnt[r] = 0.f;
-        if (r < h.ctas) {
-          each[r] = h.ctas > 1 ? gn_peer(own + q, r) : own[q];
-          cnt[r] = (float)max(min((r + 1) * h.rows, g.L) - r * h.rows, (int64_t)0) * (float)g.cg;
-          mu = fmaf(cnt[r] / total, each[r].x - each[0].x, mu);
-        }
+    // (from the first one's mean, so that equal means merge to themselves); a
+    // lane for each CTA
+    for (int q = warp; q < ng; q += warps) {
+      float2 each = own[q];
+      float cnt = n;
+      if (h.ctas > 1) {
+        const int r = min(lane, h.ctas - 1);
+        each = gn_peer(own + q, r);
+        cnt = lane < h.ctas ? (float)((int)max(min((r + 1) * h.rows, g.L) - r * h.rows, (int64_t)0) * g.cg) : 0.f;
+      } else if (lane) {
+        cnt = 0.f;
       }
-      mu += each[0].x;
+      const float ref = __shfl_sync(0xffffffffu, each.x, 0);
+      float mu = cnt * (each.x - ref);
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r < h.ctas) {
-          const float d = each[r].x - mu;
-          m2 += each[r].y + cnt[r] * d * d;
-        }
-      all[q] = make_float2(mu, 1.f / sqrtf(m2 / total + p.eps));
-      if (rank == 0) reinterpret_cast<float2*>(p.stats)[(int64_t)b * g.G + g0 + q] = all[q];
+      for (int o = 4; o > 0; o >>= 1) mu += __shfl_xor_sync(0xffffffffu, mu, o, 8);
+      mu = fmaf(mu, per_group, ref);
+      const float d = each.x - mu;
+      float m2 = cnt > 0.f ? fmaf(cnt * d, d, each.y) : 0.f;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o, 8);
+      if (lane == 0) {
+        const float2 st = make_float2(mu, rsqrtf(fmaf(m2, per_group, p.eps)));
+        all[q] = st;
+        if (rank == 0) reinterpret_cast<float2*>(p.stats)[(int64_t)b * g.G + g0 + q] = st;
+      }
     }
     __syncthreads();
     if (h.ctas > 1) gn_cluster_arrive();
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float2 st = active ? all[(cv * V + j) / g.cg] : make_float2(0.f, 0.f);
+      const float2 st = all[grp[j]];
       mean[j] = st.x;
       scale[j] *= st.y;
     }
+#pragma unroll 4
     for (int i = 0; i < mine; ++i) {
       float v[V];
-      hx[i * kGnThreads + tid].get(v);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = fmaf(v[j] - mean[j], scale[j], bias[j]);
-      gn_act<V, ACT>(v);
+      hx[i * threads + tid].get(v);
+      gn_sub<V>(v, mean);
+      gn_muladd<V>(v, scale, bias);
+      gn_pairs<V>(v, [](float2 x, int) { return act2<ACT>(x); });
       Vec::put(out + i * step, v);
     }
   } else {
     float mean[V], rstd[V], s1[V] = {}, s2[V] = {};
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float2 st = active ? reinterpret_cast<const float2*>(p.stats)[(int64_t)b * g.G + g0 + (cv * V + j) / g.cg]
-                               : make_float2(0.f, 0.f);
+      const float2 st = reinterpret_cast<const float2*>(p.stats)[(int64_t)b * g.G + g0 + grp[j]];
       mean[j] = st.x;
       rstd[j] = st.y;
     }
+#pragma unroll 4
     for (int i = 0; i < mine; ++i) {
       float xh[V], d[V];
-      hx[i * kGnThreads + tid].get(xh);
-      hd[i * kGnThreads + tid].get(d);
-#pragma unroll
-      for (int j = 0; j < V; ++j) xh[j] = (xh[j] - mean[j]) * rstd[j];
+      hx[i * threads + tid].get(xh);
+      hd[i * threads + tid].get(d);
+      gn_sub<V>(xh, mean);
+      gn_mul<V>(xh, rstd);
       gn_du<V, ACT>(d, xh, scale, bias);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        s1[j] += d[j];
-        s2[j] = fmaf(d[j], xh[j], s2[j]);
-      }
+      gn_add<V>(s1, d);
+      gn_fma<V>(s2, d, xh);
     }
-    // sums per channel, for dscale and dbias, and from them the groups' means
-    float* red2 = red + kGnThreads * V;
-    const int chs = h.nv * V;
-    if (active)
+    // sums per channel, for dscale and dbias, and from them the groups' means; a
+    // thread a channel where its row lanes are few, a warp where they are many
+    const int step_c = h.rt <= 8 ? 1 : 32;
+    const auto channel_sums = [&](const float (&s)[V], auto finish) {
+      if (active)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        red[rl * chs + cv * V + j] = s1[j];
-        red2[rl * chs + cv * V + j] = s2[j];
+        for (int j = 0; j < V; ++j) red[(cv * V + j) * h.rt + rl] = s[j];
+      __syncthreads();
+      for (int c = step_c == 1 ? tid : warp; c < width; c += step_c == 1 ? threads : warps) {
+        float t = 0.f;
+        for (int r = step_c == 1 ? 0 : lane; r < h.rt; r += step_c) t += red[c * h.rt + r];
+        if (step_c > 1)
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        if (step_c == 1 || lane == 0) finish(c, t);
       }
-    __syncthreads();
-    for (int c = tid; c < width; c += kGnThreads) {
-      float t1 = 0.f, t2 = 0.f;
-      for (int r = 0; r < h.rt; ++r) {
-        t1 += red[r * chs + c];
-        t2 += red2[r * chs + c];
-      }
-      p.sums[((int64_t)b * h.ctas + rank) * g.D + c0 + c] = make_float2(t1, t2);
-      const float w = p.scale ? p.scale[c0 + c] : 1.f;
-      red[c] = w * t1;  // this thread alone reads and writes column c of row 0
-      red2[c] = w * t2;
-    }
-    __syncthreads();
-    for (int q = warp; q < ng; q += kWarps) {
+      __syncthreads();
+    };
+    channel_sums(s1, [&](int c, float t) { chan[c].x = t; });
+    channel_sums(s2, [&](int c, float t) {
+      p.sums[((int64_t)b * h.ctas + rank) * g.D + c0 + c] = make_float2(chan[c].x, t);
+      chan[c].y = t;
+    });
+    for (int q = warp; q < ng; q += warps) {
       float t1 = 0.f, t2 = 0.f;
       for (int c = lane; c < g.cg; c += 32) {
-        t1 += red[q * g.cg + c];
-        t2 += red2[q * g.cg + c];
+        const float w = p.scale ? p.scale[c0 + q * g.cg + c] : 1.f;
+        t1 = fmaf(w, chan[q * g.cg + c].x, t1);
+        t2 = fmaf(w, chan[q * g.cg + c].y, t2);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -689,31 +770,39 @@ __global__ void __launch_bounds__(kGnThreads) gn_hold_kernel(const GnArgs p, con
       gn_cluster_arrive();
       gn_cluster_wait();
     }
-    for (int q = tid; q < ng; q += kGnThreads) {
-      float2 t = make_float2(0.f, 0.f);
+    for (int q = warp; q < ng; q += warps) {
+      float2 t = own[q];
+      if (h.ctas > 1) {
+        t = lane < h.ctas ? gn_peer(own + q, lane) : make_float2(0.f, 0.f);
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r < h.ctas) t = fadd2(t, h.ctas > 1 ? gn_peer(own + q, r) : own[q]);
-      all[q] = make_float2(t.x / total, t.y / total);
+        for (int o = 4; o > 0; o >>= 1) {
+          t.x += __shfl_xor_sync(0xffffffffu, t.x, o, 8);
+          t.y += __shfl_xor_sync(0xffffffffu, t.y, o, 8);
+        }
+      }
+      if (lane == 0) all[q] = make_float2(t.x * per_group, t.y * per_group);
     }
     __syncthreads();
     if (h.ctas > 1) gn_cluster_arrive();
     float m1[V], m2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float2 m = active ? all[(cv * V + j) / g.cg] : make_float2(0.f, 0.f);
+      const float2 m = all[grp[j]];
       m1[j] = m.x;
-      m2[j] = m.y;
+      m2[j] = -m.y;
     }
+#pragma unroll 4
     for (int i = 0; i < mine; ++i) {
       float xh[V], d[V];
-      hx[i * kGnThreads + tid].get(xh);
-      hd[i * kGnThreads + tid].get(d);
-#pragma unroll
-      for (int j = 0; j < V; ++j) xh[j] = (xh[j] - mean[j]) * rstd[j];
+      hx[i * threads + tid].get(xh);
+      hd[i * threads + tid].get(d);
+      gn_sub<V>(xh, mean);
+      gn_mul<V>(xh, rstd);
       gn_du<V, ACT>(d, xh, scale, bias);
-#pragma unroll
-      for (int j = 0; j < V; ++j) d[j] = rstd[j] * (d[j] * scale[j] - m1[j] - xh[j] * m2[j]);
+      gn_mul<V>(d, scale);
+      gn_sub<V>(d, m1);
+      gn_fma<V>(d, xh, m2);  // m2 holds its negative
+      gn_mul<V>(d, rstd);
       Vec::put(out + i * step, d);
     }
   }
@@ -755,48 +844,51 @@ static GnGeom gn_geom(const ssm_group_norm_params_t* p) {
 }
 
 // The held form's cut, or false where a group is too long for it.  Jobs are
-// sized so that four CTAs share an SM (one's loads overlap another's sums), rows
-// read at least 128 bytes where the groups allow it, and small calls spread over
-// the SMs.
-constexpr size_t kHoldTile = 48 * 1024, kHoldMost = 96 * 1024;
+// sized so that three CTAs share an SM (one's loads overlap another's sums), that
+// rows read 64 bytes or more (with 16 a call of 16 x 4096 x 256 bf16 took 39 us
+// for 24), and that small calls spread over the SMs.
+constexpr size_t kHoldSmem = 74 * 1024;
 static bool gn_hold(const ssm_group_norm_params_t* p, bool bwd, GnHold* h, int* V) {
   const int es = p->dtype == SSM_BF16 ? 2 : 4, cg = p->dim / p->groups;
   const int wide = 16 / es;
   const bool vec = p->dim % wide == 0 && aligned16(p->x) && aligned16(bwd ? p->dx : p->y) && (!bwd || aligned16(p->dy));
-  // the fewest groups that make whole vectors (all of them do)
+  // the fewest groups that make whole vectors (all of them do) and 64 bytes
   int least = 1;
   *V = vec ? wide : 1;
-  while (least * cg % *V) ++least;
+  while (least < p->groups && (least * cg % *V || least * cg * es < 64)) ++least;
   bool found = false;
   for (int ctas = 1; ctas <= 8; ctas *= 2) {
     if (ctas > 1 && p->seqlen < ctas * 4) break;
     const int64_t rows = (p->seqlen + ctas - 1) / ctas;
     if (rows > 65536) continue;
-    const auto fits = [&](int gpj, size_t tile) {
-      return (size_t)rows * gpj * cg * es * (bwd ? 2 : 1) <= tile && gpj * cg / *V <= kGnThreads;
-    };
-    if (!fits(least, kHoldMost)) continue;
-    int gpj = least;
-    while (gpj + least <= p->groups &&
-           (fits(gpj + least, kHoldTile) || (gpj * cg * es < 128 && fits(gpj + least, kHoldMost))))
-      gpj += least;
-    const auto count = [&](int q) { return p->batch * ((p->groups + q - 1) / q) * ctas; };
-    while (gpj > least && gpj * cg * es > 128 && count(gpj) < 2 * 148) gpj -= least;
     GnHold c;
-    c.gpj = gpj;
-    c.W = gpj * cg;
-    c.jobs = (p->groups + gpj - 1) / gpj;
     c.ctas = ctas;
     c.rows = rows;
-    c.nv = c.W / *V;
-    c.rt = kGnThreads / c.nv;
-    c.slots = (int)((rows + c.rt - 1) / c.rt);
-    c.smem = ((size_t)c.slots * kGnThreads * *V * es * (bwd ? 2 : 1) + 15) / 16 * 16 +
-             (size_t)kGnThreads * *V * 4 * (bwd ? 2 : 1) + 2 * (size_t)gpj * sizeof(float2);
-    if (c.smem > 200 * 1024 || (int64_t)c.jobs * p->batch * ctas > 0x7fffffff) continue;
+    const auto cut = [&](int gpj) {  // the job of gpj groups; whether it fits
+      const size_t bytes = (size_t)rows * gpj * cg * es * (bwd ? 2 : 1);
+      c.gpj = gpj;
+      c.W = gpj * cg;
+      c.jobs = (p->groups + gpj - 1) / gpj;
+      c.nv = c.W / *V;
+      if (c.nv > kHoldThreads) return false;
+      c.threads = bytes > 4096 ? 256 : 128;
+      while (c.threads < c.nv) c.threads *= 2;
+      c.rt = c.threads / c.nv;
+      c.slots = (int)((rows + c.rt - 1) / c.rt);
+      c.smem = ((size_t)c.slots * c.threads * *V * es * (bwd ? 2 : 1) + 15) / 16 * 16 +
+               (size_t)c.threads * 4 * (bwd || cg % *V ? *V : 2) + (bwd ? (size_t)c.W : 0) * sizeof(float2) +
+               2 * (size_t)gpj * sizeof(float2);
+      return c.smem <= kHoldSmem && (int64_t)c.jobs * p->batch * ctas <= 0x7fffffff;
+    };
+    if (!cut(least)) continue;
+    int gpj = least;
+    while (gpj + least <= p->groups && cut(gpj + least)) gpj += least;
+    const auto count = [&](int q) { return p->batch * ((p->groups + q - 1) / q) * ctas; };
+    while (gpj > least && gpj * cg * es > 128 && count(gpj) < 2 * 148) gpj -= least;
+    cut(gpj);
     *h = c;
     found = true;
-    if (count(gpj) >= 2 * 148 && c.smem <= kHoldTile + 24 * 1024) break;
+    if (count(gpj) >= 2 * 148) break;
   }
   return found;
 }
@@ -813,20 +905,26 @@ static void gn_fwd_launch(const GnArgs& a, cudaStream_t s) {
   const size_t smem = (2 * (size_t)g.rt * g.ct * V + g.rt) * sizeof(float);
   gn_stats_kernel<T, V><<<grid, kGnThreads, smem, s>>>(a);
   gn_merge_kernel<<<g.B * g.G, kGnThreads, 0, s>>>(a);
-  gn_apply_kernel<T, V, ACT><<<grid, kGnThreads, 0, s>>>(a);
+  if (g.cg % V == 0) gn_apply_kernel<T, V, ACT, true><<<grid, kGnThreads, 0, s>>>(a);
+  else gn_apply_kernel<T, V, ACT, V == 1><<<grid, kGnThreads, 0, s>>>(a);
   note_launches(3);
 }
 
-template <typename T, int V, int ACT>
-static void gn_bwd_launch(const GnArgs& a, cudaStream_t s) {
+template <typename T, int V, int ACT, bool ONE>
+static void gn_bwd_launch_one(const GnArgs& a, cudaStream_t s) {
   const GnGeom& g = a.g;
   const dim3 grid(g.chunks, g.B, g.tiles);
   const size_t smem = 2 * (size_t)g.rt * g.ct * V * sizeof(float);
-  gn_sums_kernel<T, V, ACT><<<grid, kGnThreads, smem, s>>>(a);
+  gn_sums_kernel<T, V, ACT, ONE><<<grid, kGnThreads, smem, s>>>(a);
   gn_means_kernel<<<g.B * g.G, kGnThreads, 0, s>>>(a);
-  gn_dx_kernel<T, V, ACT><<<grid, kGnThreads, 0, s>>>(a);
+  gn_dx_kernel<T, V, ACT, ONE><<<grid, kGnThreads, 0, s>>>(a);
   gn_param_kernel<<<(g.D + 31) / 32, 1024, 0, s>>>(a.sums, g.B, g.D, a.dscale, a.dbias);
   note_launches(4);
+}
+template <typename T, int V, int ACT>
+static void gn_bwd_launch(const GnArgs& a, cudaStream_t s) {
+  if (a.g.cg % V == 0) gn_bwd_launch_one<T, V, ACT, true>(a, s);
+  else gn_bwd_launch_one<T, V, ACT, V == 1>(a, s);
 }
 
 template <typename T, int V>
@@ -848,7 +946,7 @@ static cudaError_t gn_hold_launch(const GnArgs& a, const GnHold& h, cudaStream_t
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.g.B * h.jobs * h.ctas));
-  cfg.blockDim = dim3(kGnThreads);
+  cfg.blockDim = dim3(h.threads);
   cfg.dynamicSmemBytes = h.smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
