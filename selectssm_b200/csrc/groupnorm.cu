@@ -64,11 +64,6 @@ struct GnArgs {
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
-  if constexpr (V == 8) load8(p, v);
-  else v[0] = Cvt<T>::to_f(*p);
-}
-template <typename T, int V>
 __device__ __forceinline__ void store_v(T* p, const float (&v)[V]) {
   if constexpr (V == 8) store8(p, v);
   else *p = Cvt<T>::from_f(v[0]);
@@ -146,58 +141,80 @@ __device__ __forceinline__ void gn_du(float (&d)[V], const float (&xh)[V], const
 }
 
 // ---------------------------------------------------------------- split form
-// Rows that a thread loads before it uses them: 64 bytes of each input in
-// flight, and few enough registers for four CTAs an SM, whose warps then stand
-// at different points of their loops.  (With eight rows and two CTAs the sums of
-// 64 x 2048 x 768 bf16 ran at 4.0 TB/s.)
-template <typename T, int V> constexpr int kGnRows = V == 1 ? 8 : sizeof(T) == 2 ? 4 : 2;
+// A thread's walk over its rows of x, and of dy with IN = 2: f(offset, v, d) for
+// every row's V values (d only with IN = 2).  Rows on their way wait in a ring of
+// the thread's own places in shared memory, `kGnAhead` deep, filled by cp.async:
+// 128 bytes a thread in flight at any time, without a register or a scoreboard
+// held for them.  (Four rows of loads into registers, then their use, then the
+// next four: 3.8 TB/s; asking for each register's next row as it empties: 2.1,
+// because a wait for one load waits for younger ones too.)
+template <int IN> constexpr int kGnAhead = IN == 1 ? 8 : 4;
+template <typename T, int V, int IN>
+constexpr size_t kGnRing = V == 1 ? 0 : (size_t)kGnThreads * kGnAhead<IN> * IN * V * sizeof(T);
 
-template <typename T, int V>
-struct GnRaw;  // V values as they lie in global memory
-template <typename T> struct GnRaw<T, 8> : Raw8<T> {};
-template <typename T> struct GnRaw<T, 1> {
-  T r;
-  __device__ __forceinline__ void load(const T* p) { r = *p; }
-  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = Cvt<T>::to_f(r); }
-};
-
-// A thread's walk over its rows: f(v) for every row's V values, of x alone or of x and dy.
-template <typename T, int V, typename F>
-__device__ __forceinline__ void gn_walk(const T* x, int64_t step, int rows, F f) {
-  constexpr int R = kGnRows<T, V>;
-  for (; rows > 0; rows -= R, x += R * step) {
-    GnRaw<T, V> raw[R];
+template <typename T, int V, int IN, typename F>
+__device__ __forceinline__ void gn_walk(uint8_t* ring, const T* x, const T* dy, int64_t step, int rows, F f) {
+  if constexpr (V == 1) {
+    constexpr int R = 8;  // rows loaded together
+    for (; rows > 0; rows -= R, x += R * step, dy += IN == 2 ? R * step : 0) {
+      T a[R], b[R];
 #pragma unroll
-    for (int k = 0; k < R; ++k)
-      if (k < rows) raw[k].load(x + k * step);
+      for (int k = 0; k < R; ++k)
+        if (k < rows) {
+          a[k] = x[k * step];
+          if (IN == 2) b[k] = dy[k * step];
+        }
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      if (k >= rows) break;
-      float v[V];
-      raw[k].get(v);
-      f(k * step, v);
-    }
-  }
-}
-template <typename T, int V, typename F>
-__device__ __forceinline__ void gn_walk2(const T* x, const T* dy, int64_t step, int rows, F f) {
-  constexpr int R = kGnRows<T, V>;
-  for (; rows > 0; rows -= R, x += R * step, dy += R * step) {
-    GnRaw<T, V> raw[R], rd[R];
-#pragma unroll
-    for (int k = 0; k < R; ++k)
-      if (k < rows) {
-        raw[k].load(x + k * step);
-        rd[k].load(dy + k * step);
+      for (int k = 0; k < R; ++k) {
+        if (k >= rows) break;
+        float v[1] = {Cvt<T>::to_f(a[k])}, d[1] = {0.f};
+        if (IN == 2) d[0] = Cvt<T>::to_f(b[k]);
+        f(v, d);
       }
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      if (k >= rows) break;
-      float v[V], d[V];
-      raw[k].get(v);
-      rd[k].get(d);
-      f(k * step, v, d);
     }
+  } else {
+    constexpr int S = kGnAhead<IN>, P = sizeof(T) * V / 16;  // 16-byte pieces of a vector
+    uint4* mine = reinterpret_cast<uint4*>(ring) + threadIdx.x;
+    const auto ask = [&](int row, int slot) {
+      if (row < rows)
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                           smem_u32(mine + ((slot * IN) * P + q) * kGnThreads)),
+                       "l"(reinterpret_cast<const uint4*>(x + row * step) + q)
+                       : "memory");
+          if (IN == 2)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                             smem_u32(mine + ((slot * IN + 1) * P + q) * kGnThreads)),
+                         "l"(reinterpret_cast<const uint4*>(dy + row * step) + q)
+                         : "memory");
+        }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const auto take = [&](int slot, int in, float (&v)[V]) {
+      if constexpr (P == 1) {
+        unpack8(mine[(slot * IN + in) * kGnThreads], v);
+      } else {
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          const uint4 r = mine[((slot * IN + in) * P + q) * kGnThreads];
+          v[4 * q] = __uint_as_float(r.x); v[4 * q + 1] = __uint_as_float(r.y);
+          v[4 * q + 2] = __uint_as_float(r.z); v[4 * q + 3] = __uint_as_float(r.w);
+        }
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < S; ++k) ask(k, k);
+    for (int row = 0, slot = 0; row < rows; ++row) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");  // the oldest row's
+      float v[V], d[V];
+      take(slot, 0, v);
+      if constexpr (IN == 2) take(slot, 1, d);
+      f(v, d);
+      ask(row + S, slot);
+      slot = slot + 1 == S ? 0 : slot + 1;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
 }
 
@@ -207,8 +224,8 @@ __device__ __forceinline__ void gn_walk2(const T* x, const T* dy, int64_t step, 
 // a far-off first value costs digits of one run only, and no large mean is ever
 // subtracted from a sum of squares.
 template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads, 3) gn_stats_kernel(const GnArgs p) {
-  extern __shared__ float sm[];
+__global__ void __launch_bounds__(kGnThreads, 4) gn_stats_kernel(const GnArgs p) {
+  extern __shared__ __align__(16) float sm[];
   const GnGeom& g = p.g;
   const GnPlace q = gn_place(g, false);
   float mean[V], m2[V];
@@ -218,20 +235,10 @@ __global__ void __launch_bounds__(kGnThreads, 3) gn_stats_kernel(const GnArgs p)
   if (q.active) {
     const int64_t step = (int64_t)g.rt * g.D;
     const T* x = static_cast<const T*>(p.x) + ((int64_t)q.b * g.L + q.l0 + q.r0) * g.D + (int64_t)q.vec * V;
-    int64_t rows = (q.l1 - q.l0 - q.r0 + g.rt - 1) / g.rt;
-    for (; rows > 0; rows -= 64, x += 64 * step) {
-      const int run = (int)min(rows, (int64_t)64);
-      float ref[V], s[V], ss[V];
-      GnRaw<T, V> first;
-      first.load(x);
-      first.get(ref);
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = ss[i] = 0.f;
-      gn_walk<T, V>(x, step, run, [&](int64_t, float (&v)[V]) {
-        gn_sub<V>(v, ref);
-        gn_add<V>(s, v);
-        gn_fma<V>(ss, v, v);
-      });
+    const int rows = (int)((q.l1 - q.l0 - q.r0 + g.rt - 1) / g.rt);
+    float ref[V], s[V], ss[V];
+    int run = 0;
+    const auto close = [&] {
       const float inv = 1.f / (float)run, nn = n + (float)run, w = (float)run / nn;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -240,8 +247,24 @@ __global__ void __launch_bounds__(kGnThreads, 3) gn_stats_kernel(const GnArgs p)
         m2[i] += fmaf(delta * delta, n * w, dev);
       }
       n = nn;
-    }
+      run = 0;
+    };
+    gn_walk<T, V, 1>(reinterpret_cast<uint8_t*>(sm), x, x, step, rows, [&](float (&v)[V], float (&)[V]) {
+      if (run == 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          ref[i] = v[i];
+          s[i] = ss[i] = 0.f;
+        }
+      }
+      gn_sub<V>(v, ref);
+      gn_add<V>(s, v);
+      gn_fma<V>(ss, v, v);
+      if (++run == 64) close();
+    });
+    if (run) close();
   }
+  __syncthreads();  // the rings' memory serves below
   // merge the rt row lanes of each channel in order
   const int width = g.ct * V, mine = (threadIdx.x % g.ct) * V;
   float *smean = sm, *sm2 = sm + g.rt * width, *sn = sm + 2 * g.rt * width;
@@ -271,6 +294,7 @@ __global__ void __launch_bounds__(kGnThreads, 3) gn_stats_kernel(const GnArgs p)
   }
 }
 
+constexpr int kMergeThreads = 256;  // of the small kernels, a CTA a group
 __device__ __forceinline__ float block_sum(float v, float* buf) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -278,7 +302,7 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
   if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
   __syncthreads();
   float s = 0.f;
-  for (int w = 0; w < kGnThreads / 32; ++w) s += buf[w];
+  for (int w = 0; w < kMergeThreads / 32; ++w) s += buf[w];
   return s;
 }
 
@@ -286,19 +310,20 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
 // CTA's threads: neighbouring threads take neighbouring channels.
 template <typename F>
 __device__ __forceinline__ void gn_each_part(const GnGeom& g, F f) {
-  if (g.cg <= kGnThreads) {
-    const int at_once = kGnThreads / g.cg, k = threadIdx.x / g.cg, c = threadIdx.x - k * g.cg;
+  if (g.cg <= kMergeThreads) {
+    const int at_once = kMergeThreads / g.cg, k = threadIdx.x / g.cg, c = threadIdx.x - k * g.cg;
     if (k < at_once)
+#pragma unroll 8
       for (int ck = k; ck < g.chunks; ck += at_once) f(ck, c);
   } else {
     for (int ck = 0; ck < g.chunks; ++ck)
-      for (int c = threadIdx.x; c < g.cg; c += kGnThreads) f(ck, c);
+      for (int c = threadIdx.x; c < g.cg; c += kMergeThreads) f(ck, c);
   }
 }
 
 // mean and rstd of one group from its chunks' and channels' partials
-__global__ void __launch_bounds__(kGnThreads) gn_merge_kernel(const GnArgs p) {
-  __shared__ float buf[kGnThreads / 32];
+__global__ void __launch_bounds__(kMergeThreads) gn_merge_kernel(const GnArgs p) {
+  __shared__ float buf[kMergeThreads / 32];
   const GnGeom& g = p.g;
   const int grp = blockIdx.x % g.G, b = blockIdx.x / g.G;
   const float2* part = p.part + (int64_t)b * g.chunks * g.D + grp * g.cg;
@@ -342,7 +367,8 @@ __device__ __forceinline__ void gn_affine(const GnArgs& p, int c0, float (&scale
 }
 
 template <typename T, int V, int ACT, bool ONE>
-__global__ void __launch_bounds__(kGnThreads, 3) gn_apply_kernel(const GnArgs p) {
+__global__ void __launch_bounds__(kGnThreads, 4) gn_apply_kernel(const GnArgs p) {
+  extern __shared__ __align__(16) uint8_t ring[];
   const GnGeom& g = p.g;
   const GnPlace q = gn_place(g, true);
   if (!q.active) return;
@@ -354,24 +380,19 @@ __global__ void __launch_bounds__(kGnThreads, 3) gn_apply_kernel(const GnArgs p)
   const int64_t base = ((int64_t)q.b * g.L + q.l0 + q.r0) * g.D + (int64_t)q.vec * V, step = (int64_t)g.rt * g.D;
   const T* x = static_cast<const T*>(p.x) + base;
   T* y = static_cast<T*>(p.out) + base;
-  constexpr int R = kGnRows<T, V>;
-  int count = 0;
-  gn_walk<T, V>(x, step, (int)((q.l1 - q.l0 - q.r0 + g.rt - 1) / g.rt), [&](int64_t at, float (&v)[V]) {
+  gn_walk<T, V, 1>(ring, x, x, step, (int)((q.l1 - q.l0 - q.r0 + g.rt - 1) / g.rt), [&](float (&v)[V], float (&)[V]) {
     gn_pairs<V>(v, [&](float2 t, int i) {
       return act2<ACT>(ffma2(fsub2(t, st.a2(i)), gn_at<V>(scale, i), gn_at<V>(bias, i)));
     });
-    store_v<T, V>(y + at, v);
-    if (++count == R) {
-      count = 0;
-      y += R * step;
-    }
+    store_v<T, V>(y, v);
+    y += step;
   });
 }
 
 // Sums over a chunk of du and du xhat per channel.
 template <typename T, int V, int ACT, bool ONE>
-__global__ void __launch_bounds__(kGnThreads, 2) gn_sums_kernel(const GnArgs p) {
-  extern __shared__ float sm[];
+__global__ void __launch_bounds__(kGnThreads, 3) gn_sums_kernel(const GnArgs p) {
+  extern __shared__ __align__(16) float sm[];
   const GnGeom& g = p.g;
   const GnPlace q = gn_place(g, false);
   float s1[V], s2[V];
@@ -383,14 +404,15 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_sums_kernel(const GnArgs p) 
     GnStat<V, ONE> st;
     st.load(reinterpret_cast<const float2*>(p.stats), q.b, g, q.vec * V);
     const int64_t base = ((int64_t)q.b * g.L + q.l0 + q.r0) * g.D + (int64_t)q.vec * V, step = (int64_t)g.rt * g.D;
-    gn_walk2<T, V>(static_cast<const T*>(p.x) + base, static_cast<const T*>(p.dy) + base, step,
-                   (int)((q.l1 - q.l0 - q.r0 + g.rt - 1) / g.rt), [&](int64_t, float (&v)[V], float (&d)[V]) {
-                     gn_pairs<V>(v, [&](float2 t, int i) { return fmul2(fsub2(t, st.a2(i)), st.b2(i)); });
-                     gn_du<V, ACT>(d, v, scale, bias);
-                     gn_add<V>(s1, d);
-                     gn_fma<V>(s2, d, v);
-                   });
+    gn_walk<T, V, 2>(reinterpret_cast<uint8_t*>(sm), static_cast<const T*>(p.x) + base, static_cast<const T*>(p.dy) + base,
+                     step, (int)((q.l1 - q.l0 - q.r0 + g.rt - 1) / g.rt), [&](float (&v)[V], float (&d)[V]) {
+                       gn_pairs<V>(v, [&](float2 t, int i) { return fmul2(fsub2(t, st.a2(i)), st.b2(i)); });
+                       gn_du<V, ACT>(d, v, scale, bias);
+                       gn_add<V>(s1, d);
+                       gn_fma<V>(s2, d, v);
+                     });
   }
+  __syncthreads();  // the rings' memory serves below
   const int width = g.ct * V, mine = (threadIdx.x % g.ct) * V;
   float *a1 = sm, *a2 = sm + g.rt * width;
   if (q.r0 < g.rt) {
@@ -415,30 +437,33 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_sums_kernel(const GnArgs p) 
 
 // One group of one batch row: its channels' sums over the chunks (kept for
 // dscale and dbias) and the two means that dx needs.
-__global__ void __launch_bounds__(kGnThreads) gn_means_kernel(const GnArgs p) {
-  __shared__ float buf[kGnThreads / 32];
+__global__ void __launch_bounds__(kMergeThreads) gn_means_kernel(const GnArgs p) {
+  __shared__ float buf[kMergeThreads / 32];
   const GnGeom& g = p.g;
   const int grp = blockIdx.x % g.G, b = blockIdx.x / g.G;
-  const float2* part = p.part + (int64_t)b * g.chunks * g.D;
+  __shared__ float2 sums[kMergeThreads];
+  const float2* part = p.part + (int64_t)b * g.chunks * g.D + grp * g.cg;
   float m1 = 0.f, m2 = 0.f;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int c = grp * g.cg + warp; c < (grp + 1) * g.cg; c += kGnThreads / 32) {  // a warp per channel
-    float s1 = 0.f, s2 = 0.f;
-    for (int ck = lane; ck < g.chunks; ck += 32) {
-      const float2 v = part[(int64_t)ck * g.D + c];
-      s1 += v.x;
-      s2 += v.y;
+  const auto channel = [&](int c, float2 s) {  // a channel's sums over the chunks
+    p.sums[(int64_t)b * g.D + grp * g.cg + c] = s;
+    const float w = p.scale ? p.scale[grp * g.cg + c] : 1.f;
+    m1 = fmaf(w, s.x, m1);
+    m2 = fmaf(w, s.y, m2);
+  };
+  if (g.cg <= kMergeThreads) {
+    float2 s = make_float2(0.f, 0.f);
+    gn_each_part(g, [&](int ck, int c) { s = fadd2(s, part[(int64_t)ck * g.D + c]); });
+    sums[threadIdx.x] = s;  // of channel threadIdx.x % cg
+    __syncthreads();
+    if ((int)threadIdx.x < g.cg) {
+      for (int k = 1; k < kMergeThreads / g.cg; ++k) s = fadd2(s, sums[k * g.cg + threadIdx.x]);
+      channel(threadIdx.x, s);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      s1 += __shfl_xor_sync(0xffffffffu, s1, o);
-      s2 += __shfl_xor_sync(0xffffffffu, s2, o);
-    }
-    if (lane == 0) {
-      p.sums[(int64_t)b * g.D + c] = make_float2(s1, s2);
-      const float w = p.scale ? p.scale[c] : 1.f;
-      m1 = fmaf(w, s1, m1);
-      m2 = fmaf(w, s2, m2);
+  } else {
+    for (int c = threadIdx.x; c < g.cg; c += kMergeThreads) {
+      float2 s = make_float2(0.f, 0.f);
+      for (int ck = 0; ck < g.chunks; ++ck) s = fadd2(s, part[(int64_t)ck * g.D + c]);
+      channel(c, s);
     }
   }
   const float t1 = block_sum(m1, buf), t2 = block_sum(m2, buf);
@@ -447,7 +472,8 @@ __global__ void __launch_bounds__(kGnThreads) gn_means_kernel(const GnArgs p) {
 }
 
 template <typename T, int V, int ACT, bool ONE>
-__global__ void __launch_bounds__(kGnThreads, 2) gn_dx_kernel(const GnArgs p) {
+__global__ void __launch_bounds__(kGnThreads, 3) gn_dx_kernel(const GnArgs p) {
+  extern __shared__ __align__(16) uint8_t ring[];
   const GnGeom& g = p.g;
   const GnPlace q = gn_place(g, true);
   if (!q.active) return;
@@ -458,22 +484,17 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_dx_kernel(const GnArgs p) {
   mm.load(p.means, q.b, g, q.vec * V);
   const int64_t base = ((int64_t)q.b * g.L + q.l0 + q.r0) * g.D + (int64_t)q.vec * V, step = (int64_t)g.rt * g.D;
   T* dx = static_cast<T*>(p.out) + base;
-  constexpr int R = kGnRows<T, V>;
-  int count = 0;
-  gn_walk2<T, V>(static_cast<const T*>(p.x) + base, static_cast<const T*>(p.dy) + base, step,
-                 (int)((q.l1 - q.l0 - q.r0 + g.rt - 1) / g.rt), [&](int64_t at, float (&v)[V], float (&d)[V]) {
-                   gn_pairs<V>(v, [&](float2 t, int i) { return fmul2(fsub2(t, st.a2(i)), st.b2(i)); });
-                   gn_du<V, ACT>(d, v, scale, bias);
-                   gn_pairs<V>(d, [&](float2 t, int i) {  // rstd (du scale - m1 - xhat m2)
-                     const float2 r = fsub2(fmul2(t, gn_at<V>(scale, i)), mm.a2(i));
-                     return fmul2(fsub2(r, fmul2(gn_at<V>(v, i), mm.b2(i))), st.b2(i));
+  gn_walk<T, V, 2>(ring, static_cast<const T*>(p.x) + base, static_cast<const T*>(p.dy) + base, step,
+                   (int)((q.l1 - q.l0 - q.r0 + g.rt - 1) / g.rt), [&](float (&v)[V], float (&d)[V]) {
+                     gn_pairs<V>(v, [&](float2 t, int i) { return fmul2(fsub2(t, st.a2(i)), st.b2(i)); });
+                     gn_du<V, ACT>(d, v, scale, bias);
+                     gn_pairs<V>(d, [&](float2 t, int i) {  // rstd (du scale - m1 - xhat m2)
+                       const float2 r = fsub2(fmul2(t, gn_at<V>(scale, i)), mm.a2(i));
+                       return fmul2(fsub2(r, fmul2(gn_at<V>(v, i), mm.b2(i))), st.b2(i));
+                     });
+                     store_v<T, V>(dx, d);
+                     dx += step;
                    });
-                   store_v<T, V>(dx + at, d);
-                   if (++count == R) {
-                     count = 0;
-                     dx += R * step;
-                   }
-                 });
 }
 
 // dscale and dbias: `rows` partial sums of every channel in a fixed order
@@ -864,6 +885,11 @@ static bool gn_hold(const ssm_group_norm_params_t* p, bool bwd, GnHold* h, int* 
     GnHold c;
     c.ctas = ctas;
     c.rows = rows;
+    // The backward's held form keeps two inputs and runs the activation's slope
+    // twice between two barriers of the cluster: with more than two CTAs the
+    // split form's extra reads cost less (64 x 2048 x 768 bf16: 199 us for 338),
+    // unless the call is small enough that its launches count.
+    if (bwd && ctas > 2 && p->batch * p->seqlen * p->dim * es > (8 << 20)) break;
     const auto cut = [&](int gpj) {  // the job of gpj groups; whether it fits
       const size_t bytes = (size_t)rows * gpj * cg * es * (bwd ? 2 : 1);
       c.gpj = gpj;
@@ -902,11 +928,17 @@ template <typename T, int V, int ACT>
 static void gn_fwd_launch(const GnArgs& a, cudaStream_t s) {
   const GnGeom& g = a.g;
   const dim3 grid(g.chunks, g.B, g.tiles);
-  const size_t smem = (2 * (size_t)g.rt * g.ct * V + g.rt) * sizeof(float);
+  constexpr size_t ring = kGnRing<T, V, 1>;
+  const size_t smem = std::max(ring, (2 * (size_t)g.rt * g.ct * V + g.rt) * sizeof(float));
+  if (ring > 48 * 1024) {
+    cudaFuncSetAttribute(gn_stats_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring);
+    cudaFuncSetAttribute(gn_apply_kernel<T, V, ACT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring);
+    cudaFuncSetAttribute(gn_apply_kernel<T, V, ACT, V == 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring);
+  }
   gn_stats_kernel<T, V><<<grid, kGnThreads, smem, s>>>(a);
-  gn_merge_kernel<<<g.B * g.G, kGnThreads, 0, s>>>(a);
-  if (g.cg % V == 0) gn_apply_kernel<T, V, ACT, true><<<grid, kGnThreads, 0, s>>>(a);
-  else gn_apply_kernel<T, V, ACT, V == 1><<<grid, kGnThreads, 0, s>>>(a);
+  gn_merge_kernel<<<g.B * g.G, kMergeThreads, 0, s>>>(a);
+  if (g.cg % V == 0) gn_apply_kernel<T, V, ACT, true><<<grid, kGnThreads, ring, s>>>(a);
+  else gn_apply_kernel<T, V, ACT, V == 1><<<grid, kGnThreads, ring, s>>>(a);
   note_launches(3);
 }
 
@@ -914,10 +946,15 @@ template <typename T, int V, int ACT, bool ONE>
 static void gn_bwd_launch_one(const GnArgs& a, cudaStream_t s) {
   const GnGeom& g = a.g;
   const dim3 grid(g.chunks, g.B, g.tiles);
-  const size_t smem = 2 * (size_t)g.rt * g.ct * V * sizeof(float);
+  constexpr size_t ring = kGnRing<T, V, 2>;
+  const size_t smem = std::max(ring, 2 * (size_t)g.rt * g.ct * V * sizeof(float));
+  if (ring > 48 * 1024) {
+    cudaFuncSetAttribute(gn_sums_kernel<T, V, ACT, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring);
+    cudaFuncSetAttribute(gn_dx_kernel<T, V, ACT, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring);
+  }
   gn_sums_kernel<T, V, ACT, ONE><<<grid, kGnThreads, smem, s>>>(a);
-  gn_means_kernel<<<g.B * g.G, kGnThreads, 0, s>>>(a);
-  gn_dx_kernel<T, V, ACT, ONE><<<grid, kGnThreads, 0, s>>>(a);
+  gn_means_kernel<<<g.B * g.G, kMergeThreads, 0, s>>>(a);
+  gn_dx_kernel<T, V, ACT, ONE><<<grid, kGnThreads, ring, s>>>(a);
   gn_param_kernel<<<(g.D + 31) / 32, 1024, 0, s>>>(a.sums, g.B, g.D, a.dscale, a.dbias);
   note_launches(4);
 }

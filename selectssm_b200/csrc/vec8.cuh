@@ -45,12 +45,16 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
 }
 
 // Eight values as they lie in memory.
-template <typename T> struct Raw8;
+template <typename T> struct Raw8;  // load: read once; keep: to be read again soon
 template <> struct Raw8<float> {
   float4 lo, hi;
   __device__ __forceinline__ void load(const float* p) {
     lo = __ldcs(reinterpret_cast<const float4*>(p));
     hi = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+  }
+  __device__ __forceinline__ void keep(const float* p) {
+    lo = reinterpret_cast<const float4*>(p)[0];
+    hi = reinterpret_cast<const float4*>(p)[1];
   }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
@@ -60,6 +64,7 @@ template <> struct Raw8<float> {
 template <> struct Raw8<__nv_bfloat16> {
   uint4 r;
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { r = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void keep(const __nv_bfloat16* p) { r = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void get(float (&v)[8]) const { unpack8(r, v); }
 };
 
