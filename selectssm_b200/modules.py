@@ -30,7 +30,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import ops
+from . import block_ops, ops
 
 
 # ----------------------------------------------------------------------------- initialisers
@@ -275,15 +275,24 @@ class BidirectionalMamba(nn.Module):
     -> gate (concatenated or summed) -> out_proj -> residual (-> MLP).
 
     With ``concatenate_fwd_rev`` both SSM scans, their D skips and the gates run
-    in one kernel launch writing the concatenated (B, L, 2*ED) result."""
+    in one kernel launch writing the concatenated (B, L, 2*ED) result.
+
+    With ``fused_block`` the rest of the block runs in this package's kernels
+    too: the group norm (``norm_type="group"``), the projections with their
+    biases and residuals, and the MLP with dropout and activation in the
+    products' epilogues (:mod:`selectssm_b200.block_ops`).  Values agree with the
+    unfused block up to rounding; the dropout masks come from ``dropout_rng`` of
+    the call instead of PyTorch's generator."""
 
     def __init__(self, features: int, hidden_features: int, expansion_factor: float, dt_rank="auto",
                  complement: bool = False, tie_in_proj: bool = False, tie_gate: bool = False,
                  concatenate_fwd_rev: bool = True, activation: str = "silu", norm_type: str = "rms",
                  bn_momentum: float = 0.9, mlp_layer: bool = False, dense_expansion: int = 2,
-                 mlp_dropout_rate: float = 0.1, ssm_args: dict = None, diagnostics: dict = None, generator=None):
+                 mlp_dropout_rate: float = 0.1, ssm_args: dict = None, diagnostics: dict = None, generator=None,
+                 fused_block: bool = False):
         super().__init__()
         Din = features
+        self.fused_block = fused_block
         self.features, self.hidden_features, self.expansion_factor = Din, hidden_features, expansion_factor
         self.dt_rank = math.ceil(Din / 16) if dt_rank == "auto" else dt_rank   # :286-289
         self.complement, self.tie_in_proj, self.tie_gate = complement, tie_in_proj, tie_gate
@@ -316,18 +325,46 @@ class BidirectionalMamba(nn.Module):
             self.mlp_proj = _Dense(dense_expansion * Din, Din, generator=generator)                     # :360
         self.sown = {}
 
-    def forward(self, x, train: bool = False):
+    def _project(self, dense, x, **kw):
+        if self.fused_block:
+            return block_ops.dense_act(x, dense.kernel, dense.bias, **kw)
+        return dense(x)
+
+    def _mlp(self, x, train, dropout_rng):
+        """x + dropout(act(dropout(x W + b)) W' + b') in two products; the second
+        dropout takes the next offset."""
+        rate = self.mlp_dropout_rate if train else 0.0
+        first = second = None
+        if rate > 0:
+            first = dropout_rng
+            if first is None:  # as PyTorch's dropout: from its default (CPU) generator
+                first = tuple(torch.randint(0, 2 ** 62, (2,)).tolist())
+            if torch.is_tensor(first):
+                second = torch.stack((first[0], first[1] + 1))
+            else:
+                second = (first[0], first[1] + 1)
+        h = self._project(self.mlp, x, activation=self.activation, rate=rate, rng=first)
+        return self._project(self.mlp_proj, h, residual=x, rate=rate, rng=second)
+
+    def forward(self, x, train: bool = False, dropout_rng=None):
+        """x: (B, L, features).  ``dropout_rng``: (seed, offset) of this call's MLP
+        dropout with ``fused_block``, two integers or an int64 CUDA tensor of
+        them; a call uses offset and offset + 1.  Without it they are drawn from
+        PyTorch's default generator."""
         skip = x                                                                 # :300
         base = None
         if self.norm_type == "rms":  # one kernel: the norm and the residual base skip + out_proj.bias
             nm = getattr(self, self.norm_name)
             x, base = ops.rmsnorm_residual(x, nm.scale, self.out_proj.bias, nm.eps)
+        elif self.norm_type == "group" and self.fused_block:
+            nm = getattr(self, self.norm_name)
+            x = block_ops.group_norm_act(x, nm.scale, nm.bias, groups=nm.groups, eps=nm.eps)
         elif self.norm_name is not None:
             nm = getattr(self, self.norm_name)
             x = nm(x, train) if self.norm_type == "batch" else nm(x)
         ED = self.ED
         n_in = 1 if self.tie_in_proj else 2
-        proj = self.in_proj(x)
+        proj = self._project(self.in_proj, x)
         xf = proj[..., :ED]
         xr = xf if self.tie_in_proj else proj[..., ED:2 * ED]                   # :320
         zf = proj[..., n_in * ED:(n_in + 1) * ED]
@@ -345,11 +382,16 @@ class BidirectionalMamba(nn.Module):
             g = sf(xf, train, z=zf, gate_act=self.activation) + sr(xr, train, z=zr, gate_act=self.activation)
         if "gated" in self.diagnostics and train:
             self.sown["gated_mean"], self.sown["gated_sd"] = g.mean(), g.std()
-        if base is not None:                                                     # :345-352
+        if self.fused_block:                                                     # :345-352
+            bias = self.out_proj.bias if base is None else None
+            x = block_ops.dense_act(g, self.out_proj.kernel, bias, residual=skip if base is None else base)
+        elif base is not None:
             x = ops.dense_onto(base, g, self.out_proj.kernel)  # base + g W: GEMM with the residual as accumulator
         else:
             x = skip + self.out_proj(g)
-        if self.mlp_layer:                                                       # :355-362
+        if self.mlp_layer and self.fused_block:                                  # :355-362
+            x = self._mlp(x, train, dropout_rng)
+        elif self.mlp_layer:
             skip = x
             h = F.dropout(self.mlp(x), self.mlp_dropout_rate, training=train)
             h = _act(h, self.activation)
