@@ -252,8 +252,14 @@ struct Plan {
 
 // Tile (128 x 128 by one CTA, 256 x 256 by a pair) and cuts of the K loop: the
 // choice with the least estimated time.  The terms are measured: a 64-deep step
-// takes about 0.3 us in either, an item about 3 us around its steps, and joining
-// cut products a launch and their partials' way through memory.
+// takes about 0.3 us of a single CTA's and 0.38 of a pair's, an item about 3 us
+// around its steps, and joining cut products a launch and their partials' way
+// through memory.
+//
+// The tensor cores cut, not round, what an addition to the accumulator cannot
+// hold, so an error grows with the number of additions.  For fp32 operands the K
+// loop is therefore cut at 512: partial sums of 32 additions each are then added
+// in rounded fp32 (a sum of 2042 products is good to 6e-7 so, 2.4e-6 without).
 static Plan plan_product(int64_t M, int64_t N, int64_t K, int planes) {
   Plan best = {};
   double least = 0;
@@ -262,11 +268,16 @@ static Plan plan_product(int64_t M, int64_t N, int64_t K, int planes) {
     w.tiles_m = (int)ceil_div(M, pair ? Tile<true, float>::kM : Tile<false, float>::kM);
     w.tiles_n = (int)ceil_div(N, pair ? Tile<true, float>::kN : Tile<false, float>::kN);
     w.kblocks = (int)ceil_div(K, kBK);
-    w.steps = w.kblocks * (planes == 3 ? 6 : 1);
+    w.pairs = planes == 3 ? 6 : 1;
     const int64_t tiles = (int64_t)w.tiles_m * w.tiles_n, teams = pair ? kSms / 2 : kSms;
-    for (w.splits = 1; w.splits == 1 || (w.splits * tiles <= 2 * teams && w.splits * 4 <= w.steps); ++w.splits) {
+    // (in at most 1 GB of partial sums)
+    const int64_t room = std::max<int64_t>(1, ((int64_t)1 << 28) / (M * pad8((int)N)));
+    const int fewest = planes == 3 ? (int)std::min<int64_t>(ceil_div(w.kblocks, 8), room) : 1;
+    for (w.splits = fewest; w.splits == fewest || (w.splits * tiles <= 2 * teams &&
+                                                   w.splits * 4 <= w.kblocks * w.pairs && w.splits <= w.kblocks);
+         ++w.splits) {
       const double rounds = (double)ceil_div(tiles * w.splits, teams);
-      double us = rounds * (ceil_div(w.steps, w.splits) * (pair ? 0.38 : 0.3) + 3);
+      double us = rounds * (ceil_div(w.kblocks, w.splits) * w.pairs * (pair ? 0.38 : 0.3) + 3);
       if (w.splits > 1) us += 4.0 + 2.0 * w.splits * (double)M * N * 4 / 5e6;
       if (least == 0 || us < least) {
         best.pair = pair;
@@ -275,7 +286,7 @@ static Plan plan_product(int64_t M, int64_t N, int64_t K, int planes) {
       }
     }
   }
-  best.part_bytes = best.w.splits > 1 ? round256((size_t)best.w.splits * M * N * sizeof(float)) : 0;
+  best.part_bytes = best.w.splits > 1 ? round256((size_t)best.w.splits * M * pad8((int)N) * sizeof(float)) : 0;
   return best;
 }
 
@@ -312,7 +323,8 @@ static int launch_mma(const DenseEpi& e, const Plan& q, const CUtensorMap& ma, c
 template <bool A_MN, bool B_MN, typename T>
 static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
   const Plan q = plan_product(e.M, e.N, e.K, e.planes);
-  if ((int64_t)q.w.tiles_m * q.w.tiles_n * q.w.splits > 0x7fffffff) return SSM_ERR_SHAPE;
+  e.per_row = (e.N + 7) / 8;
+  if ((int64_t)q.w.tiles_m * q.w.tiles_n * q.w.splits > 0x7fffffff || ceil_div(e.M * e.per_row, 256) > 0x7fffffff) return SSM_ERR_SHAPE;
   CUtensorMap ma, mb;
   if (!operand_map(&ma, e.a, A_MN ? e.K : e.M, A_MN ? e.M : e.K, e.planes) ||
       !operand_map(&mb, e.b, B_MN ? e.K : e.N, B_MN ? e.N : e.K, e.planes))
@@ -325,8 +337,13 @@ static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
   int st = q.pair ? launch_mma<A_MN, B_MN, true, T>(first, q, ma, mb, status, s)
                   : launch_mma<A_MN, B_MN, false, T>(first, q, ma, mb, status, s);
   if (st || q.w.splits == 1) return st;
-  const int64_t blocks = e.M * ((e.N + 7) / 8);
-  dense_join_kernel<T><<<(unsigned)ceil_div(blocks, 256), 256, 0, s>>>(part, q.w.splits, e);
+  if (e.N % 8 == 0) {
+    dense_join_kernel<T, true><<<(unsigned)ceil_div(e.M * e.per_row, 256), 256, 0, s>>>(part, q.w.splits, e);
+  } else {
+    const int64_t grid = ceil_div(e.M * e.N, 256);
+    if (grid > 0x7fffffff) return SSM_ERR_SHAPE;
+    dense_join_kernel<T, false><<<(unsigned)grid, 256, 0, s>>>(part, q.w.splits, e);
+  }
   return launched("launch dense join kernel", 1);
 }
 

@@ -139,7 +139,8 @@ __global__ void __launch_bounds__(kFewThreads)
     }
     dense_bias8(e, c, n0 + col, bias);
     if (e.residual) get8<T>(e.residual, m[0] * e.res_stride + n0 + col, e.N - n0 - col, c.vec_res, res[0]);
-    dense_epilogue<T, 1>(e, c, m, n0 + col, bias, res, v);
+    dense_epilogue<T, 1>(e, c, m, n0 + col, bias, res, v,
+                         [&](void* base, const float (&u)[1][8]) { dense_put<T, 1>(e, c, base, m, n0 + col, u); });
   }
   __syncwarp();
   if (parts > 1) cluster_barrier();  // the others read this CTA's sums

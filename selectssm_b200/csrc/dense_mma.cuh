@@ -40,7 +40,7 @@ struct DenseEpi {
   int32_t planes;      // 1 or 3
   Planes a, b;
   void* out;           // (M, N) dense, of the kernel's type T
-  float* partial;      // not null: the sums go here, (splits, M, N), and nothing else is done
+  float* partial;      // not null: the sums go here, (splits, M, per_row * 8), and nothing else is done
   // the forward's epilogue; all absent for the gradients' products
   const void* bias;
   int32_t bias_bf16;
@@ -48,7 +48,7 @@ struct DenseEpi {
   const void* residual;
   int64_t res_stride;
   void* pre;
-  int32_t per_row;
+  int32_t per_row;     // blocks of eight columns in a row
   DropRng rng;
 };
 
@@ -119,10 +119,11 @@ __device__ __forceinline__ void dense_bias8(const DenseEpi& e, const EpiConst& c
 // v: written stage by stage over all rows, with stores as the only conditional
 // part, so that the rows' chains (ten dependent rounds of the generator, the
 // activation) overlap.  `res` holds the residual's values; rows beyond M are
-// marked by m < 0.
-template <typename T, int R>
+// marked by m < 0; put(base, v) stores to `pre` or `out`.
+template <typename T, int R, typename PUT>
 __device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst& c, const int64_t (&m)[R], int n,
-                                               const float (&bias)[8], const float (&res)[R][8], float (&v)[R][8]) {
+                                               const float (&bias)[8], const float (&res)[R][8], float (&v)[R][8],
+                                               PUT put) {
   const int cnt = min(8, e.N - n);
   if (sizeof(T) == 4 && e.planes == 3) {
     // An infinite operand has no finite planes besides its first, and infinity
@@ -145,11 +146,7 @@ __device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst
   for (int q = 0; q < R; ++q)
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[q][i] += bias[i];
-  if (e.pre) {
-#pragma unroll
-    for (int q = 0; q < R; ++q)
-      if (m[q] >= 0) put8<T>(e.pre, m[q] * e.N + n, cnt, c.vec_out, v[q]);
-  }
+  if (e.pre) put(e.pre, v);
   if (e.rng.drop) {
     uint4 w[R];
 #pragma unroll
@@ -172,13 +169,52 @@ __device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[q][i] += res[q][i];
   }
+  put(e.out, v);
+}
+// put of R rows of eight columns by the thread that holds them
+template <typename T, int R>
+__device__ __forceinline__ void dense_put(const DenseEpi& e, const EpiConst& c, void* base, const int64_t (&m)[R], int n,
+                                          const float (&v)[R][8]) {
 #pragma unroll
   for (int q = 0; q < R; ++q)
-    if (m[q] >= 0) put8<T>(e.out, m[q] * e.N + n, cnt, c.vec_out, v[q]);
+    if (m[q] >= 0) put8<T>(base, m[q] * e.N + n, min(8, e.N - n), c.vec_out, v[q]);
 }
 
+// A warp's 32 x 32 values in shared memory: 16-byte pieces, swizzled by row.
+// `put` and `get` move the epilogue's arrangement (eight columns of rows
+// lane / 4 + 8 q), `at` addresses a lane's own column.
+struct Stage32 {
+  uint4* s;
+  int lane;
+  __device__ __forceinline__ uint4& piece(int row, int p) const { return s[row * 8 + (p ^ (row & 7))]; }
+  __device__ __forceinline__ float& at(int row) const {
+    return reinterpret_cast<float*>(&piece(row, lane >> 2))[lane & 3];
+  }
+  __device__ __forceinline__ void get(float (&v)[4][8]) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int row = q * 8 + (lane >> 2);
+      const uint4 lo = piece(row, (lane & 3) * 2), hi = piece(row, (lane & 3) * 2 + 1);
+      v[q][0] = __uint_as_float(lo.x); v[q][1] = __uint_as_float(lo.y);
+      v[q][2] = __uint_as_float(lo.z); v[q][3] = __uint_as_float(lo.w);
+      v[q][4] = __uint_as_float(hi.x); v[q][5] = __uint_as_float(hi.y);
+      v[q][6] = __uint_as_float(hi.z); v[q][7] = __uint_as_float(hi.w);
+    }
+  }
+  __device__ __forceinline__ void put(const float (&v)[4][8]) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int row = q * 8 + (lane >> 2);
+      piece(row, (lane & 3) * 2) = make_uint4(__float_as_uint(v[q][0]), __float_as_uint(v[q][1]),
+                                              __float_as_uint(v[q][2]), __float_as_uint(v[q][3]));
+      piece(row, (lane & 3) * 2 + 1) = make_uint4(__float_as_uint(v[q][4]), __float_as_uint(v[q][5]),
+                                                  __float_as_uint(v[q][6]), __float_as_uint(v[q][7]));
+    }
+  }
+};
+
 // ---------------------------------------------------------------- tensor-core pieces
-constexpr int kBM = 128, kBK = 64;  // rows of a CTA's tile, depth of a step
+constexpr int kBK = 64;  // depth of a step
 constexpr int kMmaThreads = 384;
 constexpr int kEpiWarps = 8;
 // Polls before a wait gives up; a tile takes microseconds, so this is far above any wait that ends.
@@ -281,7 +317,9 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 struct DenseWork {
   int32_t tiles_m, tiles_n, splits;
   int32_t kblocks;  // ceil(K / 64)
-  int32_t steps;    // kblocks * plane pairs
+  int32_t pairs;    // plane pairs: 1 or 6
+  // the 64-deep blocks of a split: each runs through all plane pairs
+  __device__ __forceinline__ int block(int split) const { return (int)((int64_t)kblocks * split / splits); }
 };
 
 // A CTA of its own makes a tile of 128 x 128, a pair one of 256 x 256: each CTA
@@ -375,10 +413,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const int rest = item / w.tiles_n, split = rest / w.tiles_m;
       const int n0 = item % w.tiles_n * BN + (PAIR ? rank * 128 : 0);
       const int m0 = rest % w.tiles_m * S::kM + (PAIR ? rank * 128 : 0);
-      const int t0 = (int)((int64_t)w.steps * split / w.splits), t1 = (int)((int64_t)w.steps * (split + 1) / w.splits);
-      int seg = t0 / w.kblocks, kb = t0 - seg * w.kblocks, pa, pb;
+      const int kb0 = w.block(split), kb1 = w.block(split + 1);
+      int seg = 0, kb = kb0, pa, pb;
       plane_pair(e.planes, seg, pa, pb);
-      for (int t = t0; t < t1; ++t) {
+      for (int t = (kb1 - kb0) * w.pairs; t > 0; --t) {
         if (!wait(&empty[stage], phase ^ 1)) {
           ok = false;
           break;
@@ -401,8 +439,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         } else {
           I::load(sb, &map_b, bar, k0, n0, pb);
         }
-        if (++kb == w.kblocks) {
-          kb = 0;
+        if (++kb == kb1) {
+          kb = kb0;
           plane_pair(e.planes, ++seg, pa, pb);
         }
         if (++stage == stages) {
@@ -429,12 +467,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     bool ok = true;
     for (int item = first; ok && item < items; item += stride) {
       const int split = item / w.tiles_n / w.tiles_m;
-      const int t0 = (int)((int64_t)w.steps * split / w.splits), t1 = (int)((int64_t)w.steps * (split + 1) / w.splits);
+      const int t1 = (w.block(split + 1) - w.block(split)) * w.pairs;
       if (!wait(&acc_empty[acc], acc_phase ^ 1)) break;
       tmem_fence_after_sync();
       const uint32_t d = tmem + acc * BN;
       bool ready = false;
-      for (int t = t0; t < t1; ++t) {
+      for (int t = 0; t < t1; ++t) {
         if (!ready && !wait(&full[stage], phase)) {
           ok = false;
           break;
@@ -450,7 +488,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         // The queue of products is short: a barrier asked about after the last
         // one is issued leaves the tensor core idle for the answer's 250
         // cycles of every 510, so the next step's is asked about before.
-        I::mma(d, da, db, idesc, t > t0);
+        I::mma(d, da, db, idesc, t > 0);
         ready = t + 1 < t1 && mbar_try_wait(&full[stage], phase);
 #pragma unroll
         for (int k = 1; k < kBK / 16; ++k) I::mma(d, da + k * kStepA, db + k * kStepB, idesc, 1);
@@ -466,7 +504,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   } else if (warp >= 4) {
     const EpiConst c(e);
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    uint4* stage = reinterpret_cast<uint4*>(tiles + S::kStages * S::kStage) + (warp - 4) * 256;
+    const Stage32 st = {reinterpret_cast<uint4*>(tiles + S::kStages * S::kStage) + (warp - 4) * 256, lane};
     // The slices that TMA has asked for keep the SM's way from L2 busy: a plain
     // load issued now is answered some 4000 cycles later, as long as a chunk
     // takes.  So the residual is fetched to shared memory two chunks ahead, each
@@ -525,39 +563,49 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         for (int q = 0; q < 4; ++q) {
           m[q] = m0 + q * 8 + (lane >> 2);
           if (m[q] >= e.M || !in) m[q] = -1;
-          if (e.residual && !ahead && m[q] >= 0)
-            get8<T>(e.residual, m[q] * e.res_stride + nl, e.N - nl, c.vec_res, res[q]);
+          if (e.residual && c.vec_res && !ahead && m[q] >= 0)
+            get8<T>(e.residual, m[q] * e.res_stride + nl, 8, true, res[q]);
         }
         tmem_wait_ld();
         __syncwarp();
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-          stage[lane * 8 + (q ^ (lane & 7))] = make_uint4(r[q >> 2][(q & 3) * 4], r[q >> 2][(q & 3) * 4 + 1],
-                                                          r[q >> 2][(q & 3) * 4 + 2], r[q >> 2][(q & 3) * 4 + 3]);
+          st.piece(lane, q) = make_uint4(r[q >> 2][(q & 3) * 4], r[q >> 2][(q & 3) * 4 + 1], r[q >> 2][(q & 3) * 4 + 2],
+                                         r[q >> 2][(q & 3) * 4 + 3]);
         __syncwarp();
         float v[4][8];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int row = q * 8 + (lane >> 2);
-          const uint4 lo = stage[row * 8 + (((lane & 3) * 2) ^ (row & 7))];
-          const uint4 hi = stage[row * 8 + (((lane & 3) * 2 + 1) ^ (row & 7))];
-          v[q][0] = __uint_as_float(lo.x); v[q][1] = __uint_as_float(lo.y);
-          v[q][2] = __uint_as_float(lo.z); v[q][3] = __uint_as_float(lo.w);
-          v[q][4] = __uint_as_float(hi.x); v[q][5] = __uint_as_float(hi.y);
-          v[q][6] = __uint_as_float(hi.z); v[q][7] = __uint_as_float(hi.w);
-        }
+        st.get(v);
         if (e.partial) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            if (m[q] >= 0)
-              put8<float>(e.partial, ((int64_t)split * e.M + m[q]) * e.N + nl, min(8, e.N - nl), e.N % 8 == 0, v[q]);
+            if (m[q] >= 0) store8(e.partial + ((int64_t)split * e.M + m[q]) * (e.per_row * 8) + nl, v[q]);
         } else {
           if (ahead) {
             asm volatile("cp.async.wait_group 1;" ::: "memory");
 #pragma unroll
             for (int q = 0; q < 4; ++q) unpack8(held[slot * 128 + q * 32 + lane], res[q]);
+          } else if (e.residual && !c.vec_res) {
+            // rows that start anywhere: a lane a column, so that a warp's
+            // accesses lie together, and through shared memory from there
+            __syncwarp();
+            if (n + lane < e.N)
+              for (int row = 0; row < 32 && m0 + row < e.M; ++row)
+                st.at(row) = Cvt<T>::to_f(static_cast<const T*>(e.residual)[(m0 + row) * e.res_stride + n + lane]);
+            __syncwarp();
+            st.get(res);
           }
-          dense_epilogue<T, 4>(e, c, m, nl, bias, res, v);
+          dense_epilogue<T, 4>(e, c, m, nl, bias, res, v, [&](void* base, const float (&u)[4][8]) {
+            if (c.vec_out) {
+              dense_put<T, 4>(e, c, base, m, nl, u);
+              return;
+            }
+            __syncwarp();
+            st.put(u);
+            __syncwarp();
+            if (n + lane < e.N)
+              for (int row = 0; row < 32 && m0 + row < e.M; ++row)
+                static_cast<T*>(base)[(m0 + row) * e.N + n + lane] = Cvt<T>::from_f(st.at(row));
+          });
           fetch();
         }
       }
@@ -583,25 +631,52 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 }
 
 // The epilogue of a product whose K loop was cut: the parts summed in order.
-template <typename T>
+// Eight columns a thread where rows start on 16 bytes, one where they do not
+// (every element then draws its own block's bits again).
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dense_join_kernel(const float* part, int splits, const __grid_constant__ DenseEpi e) {
   const EpiConst c(e);
-  const int64_t blocks = e.M * ((e.N + 7) / 8), per = (e.N + 7) / 8;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= blocks) return;
-  const int64_t m[1] = {i / per};
-  const int n = (int)(i - m[0] * per) * 8, cnt = min(8, e.N - n);
-  const bool vec = e.N % 8 == 0;
-  float v[1][8], t[8], bias[8], res[1][8] = {};
-  get8<float>(part, m[0] * e.N + n, cnt, vec, v[0]);
-  for (int s = 1; s < splits; ++s) {
-    get8<float>(part, ((int64_t)s * e.M + m[0]) * e.N + n, cnt, vec, t);
+  const int64_t ld = (int64_t)e.per_row * 8, i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int64_t m[1] = {i / (VEC ? e.per_row : e.N)};
+  const int n = (int)(i - m[0] * (VEC ? e.per_row : e.N)) * (VEC ? 8 : 1), first = n & ~7, k = n & 7;
+  if (m[0] >= e.M) return;
+  float v[1][8] = {}, t[8], bias[8], res[1][8] = {};
+  for (int s = 0; s < splits; ++s) {
+    const float* from = part + ((int64_t)s * e.M + m[0]) * ld + n;
+    if (VEC) {
+      load8(from, t);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[0][k] += t[k];
+      for (int j = 0; j < 8; ++j) v[0][j] += t[j];
+    } else {
+      v[0][0] += *from;
+    }
   }
-  dense_bias8(e, c, n, bias);
-  if (e.residual) get8<T>(e.residual, m[0] * e.res_stride + n, cnt, c.vec_res, res[0]);
-  dense_epilogue<T, 1>(e, c, m, n, bias, res, v);
+  if (VEC) {
+    dense_bias8(e, c, n, bias);
+    if (e.residual) get8<T>(e.residual, m[0] * e.res_stride + n, 8, c.vec_res, res[0]);
+    dense_epilogue<T, 1>(e, c, m, n, bias, res, v,
+                         [&](void* base, const float (&u)[1][8]) { dense_put<T, 1>(e, c, base, m, n, u); });
+  } else {
+    // place the element where its block has it; the others hold zeros
+    float bk = 0.f;
+    if (e.bias)
+      bk = e.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[n])
+                       : static_cast<const float*>(e.bias)[n];
+    const float rk = e.residual ? Cvt<T>::to_f(static_cast<const T*>(e.residual)[m[0] * e.res_stride + n]) : 0.f;
+    const float x = v[0][0];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[0][j] = j == k ? x : 0.f;
+      bias[j] = j == k ? bk : 0.f;
+      res[0][j] = j == k ? rk : 0.f;
+    }
+    dense_epilogue<T, 1>(e, c, m, first, bias, res, v, [&](void* base, const float (&u)[1][8]) {
+      float y = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y = j == k ? u[0][j] : y;
+      static_cast<T*>(base)[m[0] * e.N + n] = Cvt<T>::from_f(y);
+    });
+  }
 }
 
 }  // namespace ssm
