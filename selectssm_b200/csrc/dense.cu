@@ -324,7 +324,7 @@ template <bool A_MN, bool B_MN, typename T>
 static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
   const Plan q = plan_product(e.M, e.N, e.K, e.planes);
   e.per_row = (e.N + 7) / 8;
-  if ((int64_t)q.w.tiles_m * q.w.tiles_n * q.w.splits > 0x7fffffff || ceil_div(e.M * e.per_row, 256) > 0x7fffffff) return SSM_ERR_SHAPE;
+  if ((int64_t)q.w.tiles_m * q.w.tiles_n * q.w.splits > 0x7fffffff) return SSM_ERR_SHAPE;
   CUtensorMap ma, mb;
   if (!operand_map(&ma, e.a, A_MN ? e.K : e.M, A_MN ? e.M : e.K, e.planes) ||
       !operand_map(&mb, e.b, B_MN ? e.K : e.N, B_MN ? e.N : e.K, e.planes))
@@ -337,13 +337,9 @@ static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
   int st = q.pair ? launch_mma<A_MN, B_MN, true, T>(first, q, ma, mb, status, s)
                   : launch_mma<A_MN, B_MN, false, T>(first, q, ma, mb, status, s);
   if (st || q.w.splits == 1) return st;
-  if (e.N % 8 == 0) {
-    dense_join_kernel<T, true><<<(unsigned)ceil_div(e.M * e.per_row, 256), 256, 0, s>>>(part, q.w.splits, e);
-  } else {
-    const int64_t grid = ceil_div(e.M * e.N, 256);
-    if (grid > 0x7fffffff) return SSM_ERR_SHAPE;
-    dense_join_kernel<T, false><<<(unsigned)grid, 256, 0, s>>>(part, q.w.splits, e);
-  }
+  const int64_t grid = ceil_div(ceil_div(e.M, 32) * ceil_div(e.N, 32), kJoinWarps);
+  if (grid > 0x7fffffff) return SSM_ERR_SHAPE;
+  dense_join_kernel<T><<<(unsigned)grid, 32 * kJoinWarps, 0, s>>>(part, q.w.splits, e);
   return launched("launch dense join kernel", 1);
 }
 

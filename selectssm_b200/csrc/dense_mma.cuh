@@ -213,6 +213,33 @@ struct Stage32 {
   }
 };
 
+// For rows that start anywhere: a warp's 32 x 32 chunk from row m0, column n,
+// one row at a time with a lane a column, so that its accesses lie together, and
+// through shared memory to or from the epilogue's arrangement.
+template <typename T>
+__device__ __forceinline__ void dense_stage_rows(const DenseEpi& e, const Stage32& st, int64_t m0, int n, float (&res)[4][8]) {
+  __syncwarp();
+  if (n + st.lane < e.N)
+    for (int row = 0; row < 32 && m0 + row < e.M; ++row)
+      st.at(row) = Cvt<T>::to_f(static_cast<const T*>(e.residual)[(m0 + row) * e.res_stride + n + st.lane]);
+  __syncwarp();
+  st.get(res);
+}
+template <typename T>
+__device__ __forceinline__ void dense_put_chunk(const DenseEpi& e, const EpiConst& c, const Stage32& st, void* base, int64_t m0,
+                                                int n, const int64_t (&m)[4], int nl, const float (&v)[4][8]) {
+  if (c.vec_out) {
+    dense_put<T, 4>(e, c, base, m, nl, v);
+    return;
+  }
+  __syncwarp();
+  st.put(v);
+  __syncwarp();
+  if (n + st.lane < e.N)
+    for (int row = 0; row < 32 && m0 + row < e.M; ++row)
+      static_cast<T*>(base)[(m0 + row) * e.N + n + st.lane] = Cvt<T>::from_f(st.at(row));
+}
+
 // ---------------------------------------------------------------- tensor-core pieces
 constexpr int kBK = 64;  // depth of a step
 constexpr int kMmaThreads = 384;
@@ -585,27 +612,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 #pragma unroll
             for (int q = 0; q < 4; ++q) unpack8(held[slot * 128 + q * 32 + lane], res[q]);
           } else if (e.residual && !c.vec_res) {
-            // rows that start anywhere: a lane a column, so that a warp's
-            // accesses lie together, and through shared memory from there
-            __syncwarp();
-            if (n + lane < e.N)
-              for (int row = 0; row < 32 && m0 + row < e.M; ++row)
-                st.at(row) = Cvt<T>::to_f(static_cast<const T*>(e.residual)[(m0 + row) * e.res_stride + n + lane]);
-            __syncwarp();
-            st.get(res);
+            dense_stage_rows<T>(e, st, m0, n, res);
           }
-          dense_epilogue<T, 4>(e, c, m, nl, bias, res, v, [&](void* base, const float (&u)[4][8]) {
-            if (c.vec_out) {
-              dense_put<T, 4>(e, c, base, m, nl, u);
-              return;
-            }
-            __syncwarp();
-            st.put(u);
-            __syncwarp();
-            if (n + lane < e.N)
-              for (int row = 0; row < 32 && m0 + row < e.M; ++row)
-                static_cast<T*>(base)[(m0 + row) * e.N + n + lane] = Cvt<T>::from_f(st.at(row));
-          });
+          dense_epilogue<T, 4>(e, c, m, nl, bias, res, v,
+                               [&](void* base, const float (&u)[4][8]) { dense_put_chunk<T>(e, c, st, base, m0, n, m, nl, u); });
           fetch();
         }
       }
@@ -630,53 +640,41 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   if (warp == 2) I::dealloc(tmem, 2 * BN);
 }
 
-// The epilogue of a product whose K loop was cut: the parts summed in order.
-// Eight columns a thread where rows start on 16 bytes, one where they do not
-// (every element then draws its own block's bits again).
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) dense_join_kernel(const float* part, int splits, const __grid_constant__ DenseEpi e) {
+// The epilogue of a product whose K loop was cut: the parts summed in order, a
+// 32 x 32 chunk a warp.
+constexpr int kJoinWarps = 4;
+template <typename T>
+__global__ void __launch_bounds__(32 * kJoinWarps)
+    dense_join_kernel(const float* part, int splits, const __grid_constant__ DenseEpi e) {
+  __shared__ uint4 staged[kJoinWarps][256];
   const EpiConst c(e);
-  const int64_t ld = (int64_t)e.per_row * 8, i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t m[1] = {i / (VEC ? e.per_row : e.N)};
-  const int n = (int)(i - m[0] * (VEC ? e.per_row : e.N)) * (VEC ? 8 : 1), first = n & ~7, k = n & 7;
-  if (m[0] >= e.M) return;
-  float v[1][8] = {}, t[8], bias[8], res[1][8] = {};
+  const Stage32 st = {staged[threadIdx.x >> 5], (int)threadIdx.x & 31};
+  const int64_t ld = (int64_t)e.per_row * 8, chunks_n = (e.N + 31) / 32;
+  const int64_t i = (int64_t)blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+  const int64_t m0 = i / chunks_n * 32;
+  const int n = (int)(i % chunks_n) * 32, nl = n + (st.lane & 3) * 8;
+  if (m0 >= e.M) return;
+  float v[4][8] = {}, bias[8], res[4][8] = {};
+  int64_t m[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    m[q] = m0 + q * 8 + (st.lane >> 2);
+    if (m[q] >= e.M || nl >= e.N) m[q] = -1;
+    if (e.residual && c.vec_res && m[q] >= 0) get8<T>(e.residual, m[q] * e.res_stride + nl, 8, true, res[q]);
+  }
   for (int s = 0; s < splits; ++s) {
-    const float* from = part + ((int64_t)s * e.M + m[0]) * ld + n;
-    if (VEC) {
-      load8(from, t);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[0][j] += t[j];
-    } else {
-      v[0][0] += *from;
+    for (int q = 0; q < 4; ++q) {
+      float t[8] = {};
+      if (m[q] >= 0) load8(part + ((int64_t)s * e.M + m[q]) * ld + nl, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[q][j] += t[j];
     }
   }
-  if (VEC) {
-    dense_bias8(e, c, n, bias);
-    if (e.residual) get8<T>(e.residual, m[0] * e.res_stride + n, 8, c.vec_res, res[0]);
-    dense_epilogue<T, 1>(e, c, m, n, bias, res, v,
-                         [&](void* base, const float (&u)[1][8]) { dense_put<T, 1>(e, c, base, m, n, u); });
-  } else {
-    // place the element where its block has it; the others hold zeros
-    float bk = 0.f;
-    if (e.bias)
-      bk = e.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[n])
-                       : static_cast<const float*>(e.bias)[n];
-    const float rk = e.residual ? Cvt<T>::to_f(static_cast<const T*>(e.residual)[m[0] * e.res_stride + n]) : 0.f;
-    const float x = v[0][0];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[0][j] = j == k ? x : 0.f;
-      bias[j] = j == k ? bk : 0.f;
-      res[0][j] = j == k ? rk : 0.f;
-    }
-    dense_epilogue<T, 1>(e, c, m, first, bias, res, v, [&](void* base, const float (&u)[1][8]) {
-      float y = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y = j == k ? u[0][j] : y;
-      static_cast<T*>(base)[m[0] * e.N + n] = Cvt<T>::from_f(y);
-    });
-  }
+  if (e.residual && !c.vec_res) dense_stage_rows<T>(e, st, m0, n, res);
+  dense_bias8(e, c, nl, bias);
+  dense_epilogue<T, 4>(e, c, m, nl, bias, res, v,
+                       [&](void* base, const float (&u)[4][8]) { dense_put_chunk<T>(e, c, st, base, m0, n, m, nl, u); });
 }
 
 }  // namespace ssm
