@@ -63,6 +63,14 @@ __device__ __forceinline__ void slope8(float (&d)[8], const float (&u)[8]) {
     d[i + 1] = y.y;
   }
 }
+__device__ __forceinline__ void add8(float (&v)[8], const float (&b)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const float2 y = fadd2(make_float2(v[i], v[i + 1]), make_float2(b[i], b[i + 1]));
+    v[i] = y.x;
+    v[i + 1] = y.y;
+  }
+}
 __device__ __forceinline__ void scale8(float (&v)[8], float f) {
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {

@@ -116,10 +116,10 @@ __global__ void __launch_bounds__(kFewThreads)
   // one block of eight columns of a row a thread, dealt out over the parts
   const EpiConst c(e);
   for (int i = threadIdx.x * parts + part; i < R * CT / 8; i += kFewThreads * parts) {
-    const int64_t m[1] = {i / (CT / 8)};
+    const int64_t m = i / (CT / 8);
     const int col = i % (CT / 8) * 8;
-    if (m[0] >= e.M || n0 + col >= e.N) continue;
-    float v[1][8] = {}, bias[8], res[1][8] = {};
+    if (m >= e.M || n0 + col >= e.N) continue;
+    float v[1][8] = {}, bias[8];
     for (int q = 0; q < parts; ++q) {
       const float* at = &sums[0][i / (CT / 8) * CT + col];
       float4 lo, hi;
@@ -134,13 +134,16 @@ __global__ void __launch_bounds__(kFewThreads)
         lo = *reinterpret_cast<const float4*>(at);
         hi = *reinterpret_cast<const float4*>(at + 4);
       }
-      v[0][0] += lo.x; v[0][1] += lo.y; v[0][2] += lo.z; v[0][3] += lo.w;
-      v[0][4] += hi.x; v[0][5] += hi.y; v[0][6] += hi.z; v[0][7] += hi.w;
+      const float t[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      add8(v[0], t);
     }
     dense_bias8(e, c, n0 + col, bias);
-    if (e.residual) get8<T>(e.residual, m[0] * e.res_stride + n0 + col, e.N - n0 - col, c.vec_res, res[0]);
-    dense_epilogue<T, 1>(e, c, m, n0 + col, bias, res, v,
-                         [&](void* base, const float (&u)[1][8]) { dense_put<T, 1>(e, c, base, m, n0 + col, u); });
+    dense_epilogue<T, 1>(
+        e, c, m, 1, n0 + col, bias, v,
+        [&](float (&res)[1][8]) {
+          get8<T>(e.residual, m * e.res_stride + n0 + col, e.N - n0 - col, c.vec_res, res[0]);
+        },
+        [&](void* base, const float (&u)[1][8]) { dense_put<T, 1>(e, c, base, m, 1, n0 + col, u); });
   }
   __syncwarp();
   if (parts > 1) cluster_barrier();  // the others read this CTA's sums

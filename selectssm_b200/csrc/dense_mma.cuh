@@ -78,7 +78,7 @@ __device__ __forceinline__ void get8(const void* base, int64_t off, int cnt, boo
 struct EpiConst {
   PhiloxKey key;
   float f;
-  bool vec_out, vec_res, vec_bias;
+  bool vec_out, vec_res, vec_bias, low;
   __device__ __forceinline__ explicit EpiConst(const DenseEpi& e) {
     key = {};
     f = 1.f;
@@ -89,6 +89,7 @@ struct EpiConst {
     // rows of a multiple of 8 elements from a 16-byte aligned start
     const auto a16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     vec_out = e.N % 8 == 0 && a16(e.out) && a16(e.pre);
+    low = e.M * e.per_row <= (int64_t)1 << 32;
     vec_bias = e.N % 8 == 0 && a16(e.bias);
     vec_res = e.residual && e.N % 8 == 0 && e.res_stride % 8 == 0 && a16(e.residual);
   }
@@ -115,16 +116,16 @@ __device__ __forceinline__ void dense_bias8(const DenseEpi& e, const EpiConst& c
   else get8<float>(e.bias, n, e.N - n, c.vec_bias, b);
 }
 
-// What an epilogue does to columns n .. n+7 of R rows, from the summed products
-// v: written stage by stage over all rows, with stores as the only conditional
-// part, so that the rows' chains (ten dependent rounds of the generator, the
-// activation) overlap.  `res` holds the residual's values; rows beyond M are
-// marked by m < 0; put(base, v) stores to `pre` or `out`.
-template <typename T, int R, typename PUT>
-__device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst& c, const int64_t (&m)[R], int n,
-                                               const float (&bias)[8], const float (&res)[R][8], float (&v)[R][8],
-                                               PUT put) {
-  const int cnt = min(8, e.N - n);
+// What an epilogue does to columns n .. n+7 of R rows (row, row + 8, ...) from
+// the summed products v.  Only the first `left` / 8 of the rows exist, and only
+// stores look at that: written stage by stage over all rows, the rows' chains
+// (ten dependent rounds of the generator, the activation) overlap.  The
+// instructions of this function are what an epilogue costs: issued beside the
+// warp that starts the tensor core's products, they delay it one for one.
+// get_res() gives the residual's values, put(base, v) stores to `pre` or `out`.
+template <typename T, int R, typename RES, typename PUT>
+__device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst& c, int64_t row, int left, int n,
+                                               const float (&bias)[8], float (&v)[R][8], RES get_res, PUT put) {
   if (sizeof(T) == 4 && e.planes == 3) {
     // An infinite operand has no finite planes besides its first, and infinity
     // times the other operand's planes gives NaN where the product is infinite.
@@ -139,18 +140,23 @@ __device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst
       for (int q = 0; q < R; ++q)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (isnan(v[q][i]) && m[q] >= 0 && i < cnt) v[q][i] = dense_again(e, m[q], n + i);
+          if (isnan(v[q][i]) && q * 8 < left && n + i < e.N) v[q][i] = dense_again(e, row + q * 8, n + i);
     }
   }
+  if (e.bias)
 #pragma unroll
-  for (int q = 0; q < R; ++q)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[q][i] += bias[i];
+    for (int q = 0; q < R; ++q) add8(v[q], bias);
   if (e.pre) put(e.pre, v);
   if (e.rng.drop) {
     uint4 w[R];
+    const int64_t block = row * e.per_row + n / 8;
+    if (c.low) {  // no counter passes 32 bits: the generator's first products are common to all
 #pragma unroll
-    for (int q = 0; q < R; ++q) w[q] = philox4x32_10(m[q] * e.per_row + n / 8, c.key);
+      for (int q = 0; q < R; ++q) w[q] = philox4x32_10((uint32_t)block + (uint32_t)(q * 8 * e.per_row), 0u, c.key);
+    } else {
+#pragma unroll
+      for (int q = 0; q < R; ++q) w[q] = philox4x32_10((uint64_t)(block + (int64_t)q * 8 * e.per_row), c.key);
+    }
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       scale8(v[q], c.f);
@@ -164,20 +170,21 @@ __device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst
     default: break;
   }
   if (e.residual) {
+    float res[R][8];
+    get_res(res);
 #pragma unroll
-    for (int q = 0; q < R; ++q)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[q][i] += res[q][i];
+    for (int q = 0; q < R; ++q) add8(v[q], res[q]);
   }
   put(e.out, v);
 }
 // put of R rows of eight columns by the thread that holds them
 template <typename T, int R>
-__device__ __forceinline__ void dense_put(const DenseEpi& e, const EpiConst& c, void* base, const int64_t (&m)[R], int n,
+__device__ __forceinline__ void dense_put(const DenseEpi& e, const EpiConst& c, void* base, int64_t row, int left, int n,
                                           const float (&v)[R][8]) {
+  T* p = static_cast<T*>(base) + row * e.N + n;
 #pragma unroll
   for (int q = 0; q < R; ++q)
-    if (m[q] >= 0) put8<T>(base, m[q] * e.N + n, min(8, e.N - n), c.vec_out, v[q]);
+    if (q * 8 < left) put8<T>(p, (int64_t)(q * 8) * e.N, min(8, e.N - n), c.vec_out, v[q]);
 }
 
 // A warp's 32 x 32 values in shared memory: 16-byte pieces, swizzled by row.
@@ -190,11 +197,13 @@ struct Stage32 {
   __device__ __forceinline__ float& at(int row) const {
     return reinterpret_cast<float*>(&piece(row, lane >> 2))[lane & 3];
   }
+  // this lane's two pieces of row lane / 4; those of the rows 8, 16 and 24 below are 64 pieces on
+  __device__ __forceinline__ uint4* mine(int half) const { return &piece(lane >> 2, (lane & 3) * 2 + half); }
   __device__ __forceinline__ void get(float (&v)[4][8]) const {
+    const uint4 *a = mine(0), *b = mine(1);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int row = q * 8 + (lane >> 2);
-      const uint4 lo = piece(row, (lane & 3) * 2), hi = piece(row, (lane & 3) * 2 + 1);
+      const uint4 lo = a[q * 64], hi = b[q * 64];
       v[q][0] = __uint_as_float(lo.x); v[q][1] = __uint_as_float(lo.y);
       v[q][2] = __uint_as_float(lo.z); v[q][3] = __uint_as_float(lo.w);
       v[q][4] = __uint_as_float(hi.x); v[q][5] = __uint_as_float(hi.y);
@@ -202,13 +211,13 @@ struct Stage32 {
     }
   }
   __device__ __forceinline__ void put(const float (&v)[4][8]) const {
+    uint4 *a = mine(0), *b = mine(1);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int row = q * 8 + (lane >> 2);
-      piece(row, (lane & 3) * 2) = make_uint4(__float_as_uint(v[q][0]), __float_as_uint(v[q][1]),
-                                              __float_as_uint(v[q][2]), __float_as_uint(v[q][3]));
-      piece(row, (lane & 3) * 2 + 1) = make_uint4(__float_as_uint(v[q][4]), __float_as_uint(v[q][5]),
-                                                  __float_as_uint(v[q][6]), __float_as_uint(v[q][7]));
+      a[q * 64] = make_uint4(__float_as_uint(v[q][0]), __float_as_uint(v[q][1]), __float_as_uint(v[q][2]),
+                             __float_as_uint(v[q][3]));
+      b[q * 64] = make_uint4(__float_as_uint(v[q][4]), __float_as_uint(v[q][5]), __float_as_uint(v[q][6]),
+                             __float_as_uint(v[q][7]));
     }
   }
 };
@@ -226,10 +235,10 @@ __device__ __forceinline__ void dense_stage_rows(const DenseEpi& e, const Stage3
   st.get(res);
 }
 template <typename T>
-__device__ __forceinline__ void dense_put_chunk(const DenseEpi& e, const EpiConst& c, const Stage32& st, void* base, int64_t m0,
-                                                int n, const int64_t (&m)[4], int nl, const float (&v)[4][8]) {
+__device__ __forceinline__ void dense_put_chunk(const DenseEpi& e, const EpiConst& c, const Stage32& st, void* base,
+                                                int64_t m0, int n, int left, const float (&v)[4][8]) {
   if (c.vec_out) {
-    dense_put<T, 4>(e, c, base, m, nl, v);
+    dense_put<T, 4>(e, c, base, m0 + (st.lane >> 2), left, n + (st.lane & 3) * 8, v);
     return;
   }
   __syncwarp();
@@ -238,6 +247,26 @@ __device__ __forceinline__ void dense_put_chunk(const DenseEpi& e, const EpiCons
   if (n + st.lane < e.N)
     for (int row = 0; row < 32 && m0 + row < e.M; ++row)
       static_cast<T*>(base)[(m0 + row) * e.N + n + st.lane] = Cvt<T>::from_f(st.at(row));
+}
+// The residual of a chunk by plain loads.
+template <typename T>
+__device__ __forceinline__ void dense_get_chunk(const DenseEpi& e, const EpiConst& c, const Stage32& st, int64_t m0, int n,
+                                                int left, float (&res)[4][8]) {
+  if (!c.vec_res) {
+    dense_stage_rows<T>(e, st, m0, n, res);
+    return;
+  }
+  const T* p = static_cast<const T*>(e.residual) + (m0 + (st.lane >> 2)) * e.res_stride + n + (st.lane & 3) * 8;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) res[q][i] = 0.f;
+    if (q * 8 < left) get8<T>(p, q * 8 * e.res_stride, 8, true, res[q]);
+  }
+}
+// rows of a chunk from m0 that this lane's places reach, times 8; 0 beyond the last column
+__device__ __forceinline__ int dense_left(const DenseEpi& e, int64_t m0, int n, int lane) {
+  return n + (lane & 3) * 8 < e.N ? (int)min(e.M - m0 - (lane >> 2), (int64_t)32) : 0;
 }
 
 // ---------------------------------------------------------------- tensor-core pieces
@@ -538,17 +567,26 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     // lane its own pieces.
     uint4* held = reinterpret_cast<uint4*>(tiles + (S::kStages - 1) * S::kStage) + (warp - 4) * 256;
     int f_item = first, f_chunk = 0, slot = 0;  // next to fetch; where it goes and the oldest one is
+    const T* f_from = nullptr;                  // this lane's first piece of the item
+    int f_left = 0, f_n = 0;
     const auto fetch = [&]() {
       if (!ahead) return;
       if (f_item < items) {
-        const int n = f_item % w.tiles_n * BN + half * (BN / 2) + f_chunk * 32 + (lane & 3) * 8;
-        const int64_t m = (int64_t)(f_item / w.tiles_n % w.tiles_m) * S::kM + rank * 128 + quarter * 32 + (lane >> 2);
+        if (f_chunk == 0) {
+          f_n = f_item % w.tiles_n * BN + half * (BN / 2) + (lane & 3) * 8;
+          const int64_t m = (int64_t)(f_item / w.tiles_n % w.tiles_m) * S::kM + rank * 128 + quarter * 32 + (lane >> 2);
+          f_from = static_cast<const T*>(e.residual) + m * e.res_stride + f_n;
+          f_left = (int)min(e.M - m, (int64_t)32);
+        }
+        const uint32_t to = smem_u32(held + slot * 128 + lane);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          if (m + q * 8 < e.M && n < e.N)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(held + slot * 128 + q * 32 + lane)),
-                         "l"(static_cast<const T*>(e.residual) + (m + q * 8) * e.res_stride + n)
+          if (q * 8 < f_left && f_n < e.N)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + q * 512),
+                         "l"(f_from + q * 8 * e.res_stride)
                          : "memory");
+        f_from += 32;
+        f_n += 32;
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
       slot ^= 1;
@@ -581,18 +619,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         uint32_t r[2][16];
         tmem_ld16(src + j, r[0]);
         tmem_ld16(src + j + 16, r[1]);
-        const int nl = n + (lane & 3) * 8;
-        const bool in = nl < e.N;
-        float bias[8], res[4][8] = {};
-        int64_t m[4];
+        const int nl = n + (lane & 3) * 8, left = dense_left(e, m0, n, lane);
+        float bias[8];
         dense_bias8(e, c, nl, bias);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          m[q] = m0 + q * 8 + (lane >> 2);
-          if (m[q] >= e.M || !in) m[q] = -1;
-          if (e.residual && c.vec_res && !ahead && m[q] >= 0)
-            get8<T>(e.residual, m[q] * e.res_stride + nl, 8, true, res[q]);
-        }
         tmem_wait_ld();
         __syncwarp();
 #pragma unroll
@@ -603,19 +632,23 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         float v[4][8];
         st.get(v);
         if (e.partial) {
+          float* p = e.partial + ((int64_t)split * e.M + m0 + (lane >> 2)) * (e.per_row * 8) + nl;
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            if (m[q] >= 0) store8(e.partial + ((int64_t)split * e.M + m[q]) * (e.per_row * 8) + nl, v[q]);
+            if (q * 8 < left) store8(p + (int64_t)(q * 64) * e.per_row, v[q]);
         } else {
-          if (ahead) {
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
+          dense_epilogue<T, 4>(
+              e, c, m0 + (lane >> 2), left, nl, bias, v,
+              [&](float (&res)[4][8]) {
+                if (ahead) {
+                  asm volatile("cp.async.wait_group 1;" ::: "memory");
 #pragma unroll
-            for (int q = 0; q < 4; ++q) unpack8(held[slot * 128 + q * 32 + lane], res[q]);
-          } else if (e.residual && !c.vec_res) {
-            dense_stage_rows<T>(e, st, m0, n, res);
-          }
-          dense_epilogue<T, 4>(e, c, m, nl, bias, res, v,
-                               [&](void* base, const float (&u)[4][8]) { dense_put_chunk<T>(e, c, st, base, m0, n, m, nl, u); });
+                  for (int q = 0; q < 4; ++q) unpack8(held[slot * 128 + q * 32 + lane], res[q]);
+                } else {
+                  dense_get_chunk<T>(e, c, st, m0, n, left, res);
+                }
+              },
+              [&](void* base, const float (&u)[4][8]) { dense_put_chunk<T>(e, c, st, base, m0, n, left, u); });
           fetch();
         }
       }
@@ -654,27 +687,22 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   const int64_t m0 = i / chunks_n * 32;
   const int n = (int)(i % chunks_n) * 32, nl = n + (st.lane & 3) * 8;
   if (m0 >= e.M) return;
-  float v[4][8] = {}, bias[8], res[4][8] = {};
-  int64_t m[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    m[q] = m0 + q * 8 + (st.lane >> 2);
-    if (m[q] >= e.M || nl >= e.N) m[q] = -1;
-    if (e.residual && c.vec_res && m[q] >= 0) get8<T>(e.residual, m[q] * e.res_stride + nl, 8, true, res[q]);
-  }
+  const int left = dense_left(e, m0, n, st.lane);
+  float v[4][8] = {}, bias[8];
   for (int s = 0; s < splits; ++s) {
+    const float* p = part + ((int64_t)s * e.M + m0 + (st.lane >> 2)) * ld + nl;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       float t[8] = {};
-      if (m[q] >= 0) load8(part + ((int64_t)s * e.M + m[q]) * ld + nl, t);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[q][j] += t[j];
+      if (q * 8 < left) load8(p + q * 8 * ld, t);
+      add8(v[q], t);
     }
   }
-  if (e.residual && !c.vec_res) dense_stage_rows<T>(e, st, m0, n, res);
   dense_bias8(e, c, nl, bias);
-  dense_epilogue<T, 4>(e, c, m, nl, bias, res, v,
-                       [&](void* base, const float (&u)[4][8]) { dense_put_chunk<T>(e, c, st, base, m0, n, m, nl, u); });
+  dense_epilogue<T, 4>(
+      e, c, m0 + (st.lane >> 2), left, nl, bias, v,
+      [&](float (&res)[4][8]) { dense_get_chunk<T>(e, c, st, m0, n, left, res); },
+      [&](void* base, const float (&u)[4][8]) { dense_put_chunk<T>(e, c, st, base, m0, n, left, u); });
 }
 
 }  // namespace ssm
