@@ -7,10 +7,12 @@ The library links the CUDA runtime statically and resolves the driver's
 
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -45,18 +47,24 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
     """Compile the library unless it is newer than all its sources; returns its path."""
     if not force and up_to_date():
         return LIB
-    cmd = [nvcc_path(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr",
-           "-DSSM_BUILD", "-o", LIB + ".tmp"]
+    flags = [nvcc_path(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
+             "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr", "-DSSM_BUILD"]
     if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += list(extra_flags or [])
-    cmd += [os.path.join(CSRC, f) for f in SOURCES]
-    res = subprocess.run(cmd, cwd=CSRC, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
-    if verbose:
-        sys.stderr.write(res.stdout + res.stderr)
+        flags += ["-Xptxas", "-v"]
+    flags += list(extra_flags or [])
+
+    def run(cmd):
+        res = subprocess.run(cmd, cwd=CSRC, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+        if verbose:
+            sys.stderr.write(res.stdout + res.stderr)
+
+    # one compiler process per source, then one link
+    with tempfile.TemporaryDirectory() as tmp, concurrent.futures.ThreadPoolExecutor(os.cpu_count()) as pool:
+        objects = [os.path.join(tmp, f + ".o") for f in SOURCES]
+        list(pool.map(lambda p: run([*flags, "-c", os.path.join(CSRC, p[0]), "-o", p[1]]), zip(SOURCES, objects)))
+        run([*flags, "-shared", "-o", LIB + ".tmp", *objects])
     os.replace(LIB + ".tmp", LIB)
     return LIB
 

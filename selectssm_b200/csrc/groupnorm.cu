@@ -76,9 +76,8 @@ struct GnPlace {
 };
 __device__ __forceinline__ GnPlace gn_place(const GnGeom& g, bool reversed) {
   GnPlace q;
-  const unsigned n = gridDim.x * gridDim.y;
-  unsigned id = blockIdx.y * gridDim.x + blockIdx.x;  // (batch, chunk)
-  if (reversed) id = n - 1 - id;
+  unsigned id = blockIdx.x;  // (batch, chunk)
+  if (reversed) id = gridDim.x - 1 - id;
   q.b = id / g.chunks;
   q.chunk = id - q.b * g.chunks;
   q.vec = blockIdx.z * g.ct + threadIdx.x % g.ct;
@@ -517,11 +516,12 @@ __global__ void __launch_bounds__(1024) gn_param_kernel(const float2* sums, int 
 
 // ---------------------------------------------------------------- held form
 // A job: `gpj` groups (W channels) of one batch row, `ctas` CTAs with `rows`
-// rows each.  nv vectors of V channels by rt row lanes; each thread keeps
+// rows each; a cluster takes the same groups of every `turns`-th batch row, so
+// that many short rows (a norm per token) need few sums for dscale and dbias.  nv vectors of V channels by rt row lanes; each thread keeps
 // `slots` vectors of its own in shared memory.
 constexpr int kHoldThreads = 256;  // at most
 struct GnHold {
-  int32_t threads, W, gpj, jobs, ctas, nv, rt, slots;
+  int32_t threads, W, gpj, jobs, ctas, turns, nv, rt, slots;
   int64_t rows;
   size_t smem;
 };
@@ -556,7 +556,10 @@ __device__ __forceinline__ float2 gn_peer(const float2* p, int cta) {
   return v;
 }
 
-template <typename T, int V, int ACT, bool BWD>
+// SHORT: more batch rows than turns, or rows so short that the sums over a group
+// are a thread's work.  (The loop and the other form of the sums cost a call that
+// has no need of them up to a fifth of its time, in registers.)
+template <typename T, int V, int ACT, bool BWD, bool SHORT>
 __global__ void __launch_bounds__(kHoldThreads, 3) gn_hold_kernel(const GnArgs p, const GnHold h) {
   using Vec = GnVec<T, V>;
   extern __shared__ __align__(16) uint8_t raw[];
@@ -567,35 +570,39 @@ __global__ void __launch_bounds__(kHoldThreads, 3) gn_hold_kernel(const GnArgs p
   Vec* hd = hx + (BWD ? h.slots * threads : 0);
   float* red = reinterpret_cast<float*>(raw + ((size_t)h.slots * threads * sizeof(Vec) * (BWD ? 2 : 1) + 15) / 16 * 16);
   float2* chan = reinterpret_cast<float2*>(red + threads * (BWD || g.cg % V ? V : 2));  // backward: sums per channel
-  float2* own = chan + (BWD ? h.W : 0);  // this CTA's pair of each group
-  float2* all = own + h.gpj;                                                       // the job's
+  float2* acc = chan + (BWD ? h.W : 0);  // backward: those of all the batch rows so far
+  float2* own = acc + (BWD ? h.W : 0);   // this CTA's pair of each group
+  float2* all = own + h.gpj;            // the job's
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int rank = 0;
   if (h.ctas > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  const int job = blockIdx.x / h.ctas, b = job / h.jobs, g0 = job % h.jobs * h.gpj;
+  const int job = blockIdx.x / h.ctas, turn = job / h.jobs, g0 = job % h.jobs * h.gpj;
   const int ng = min(h.gpj, g.G - g0), width = ng * g.cg, c0 = g0 * g.cg;
   const int cv = tid % h.nv, rl = tid / h.nv;
   const bool active = rl < h.rt && cv * V < width;
   const int64_t l0 = rank * h.rows, l1 = min(l0 + h.rows, g.L);
   const int mine = active && l0 + rl < l1 ? (int)((l1 - l0 - rl + h.rt - 1) / h.rt) : 0;  // vectors of this thread
-  const int64_t base = ((int64_t)b * g.L + l0 + rl) * g.D + c0 + cv * V, step = (int64_t)h.rt * g.D;
-  const T* x = static_cast<const T*>(p.x) + base;
-  const T* dy = BWD ? static_cast<const T*>(p.dy) + base : nullptr;
-
+  const int64_t step = (int64_t)h.rt * g.D;
+  const auto fetch = [&](int64_t b) {
+    const int64_t base = (b * g.L + l0 + rl) * g.D + c0 + cv * V;
+    const T* x = static_cast<const T*>(p.x) + base;
+    const T* dy = BWD ? static_cast<const T*>(p.dy) + base : nullptr;
 #pragma unroll 4
-  for (int i = 0; i < mine; ++i) {
-    if constexpr (sizeof(Vec) == 16) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hx + i * threads + tid)), "l"(x + i * step)
-                   : "memory");
-      if (BWD)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hd + i * threads + tid)),
-                     "l"(dy + i * step)
+    for (int i = 0; i < mine; ++i) {
+      if constexpr (sizeof(Vec) == 16) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hx + i * threads + tid)), "l"(x + i * step)
                      : "memory");
-    } else {
-      hx[i * threads + tid].r = x[i * step];
-      if (BWD) hd[i * threads + tid].r = dy[i * step];
+        if (BWD)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(hd + i * threads + tid)),
+                       "l"(dy + i * step)
+                       : "memory");
+      } else {
+        hx[i * threads + tid].r = x[i * step];
+        if (BWD) hd[i * threads + tid].r = dy[i * step];
+      }
     }
-  }
+  };
+  fetch(turn);
   int grp[V];  // of the job's groups
 #pragma unroll
   for (int j = 0, q = cv * V / g.cg, left = (q + 1) * g.cg - cv * V; j < V; ++j) {
@@ -611,230 +618,252 @@ __global__ void __launch_bounds__(kHoldThreads, 3) gn_hold_kernel(const GnArgs p
     scale[i] = active && p.scale ? p.scale[c0 + cv * V + i] : 1.f;
     bias[i] = active && p.bias ? p.bias[c0 + cv * V + i] : 0.f;
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");  // a thread reads only what it fetched itself
-
   const float per_group = 1.f / ((float)g.L * (float)g.cg);
-  T* out = static_cast<T*>(p.out) + base;
-  // Per-thread values to sums over each group, in a fixed order, handed to
-  // finish(group, sum).  Vectors that lie in one group are summed first.  A
-  // group's values lie together, so that as many warps as there are for each
-  // group walk over them without a division.
-  const bool single = g.cg % V == 0;
-  const int unit = single ? V : 1, entries = g.cg / unit * h.rt;
-  const int share = max(warps / ng, 1);  // warps for a group
-  const auto group_sums = [&](const float (&s)[V], auto finish) {
-    if (active) {
-      if (single) {
-        float t = 0.f;
+  const int step_c = h.rt <= 8 ? 1 : 32;  // backward: lanes for a channel's sum
+  // The job's groups of every h.turns-th batch row, one after another.
+  for (int64_t b = turn; SHORT ? b < g.B : b == turn; b += SHORT ? h.turns : g.B) {
+    const int64_t base = (b * g.L + l0 + rl) * g.D + c0 + cv * V;
+    T* out = static_cast<T*>(p.out) + base;
+    if (SHORT && b != turn) fetch(b);
+    asm volatile("cp.async.wait_all;" ::: "memory");  // a thread reads only what it fetched itself
+
+    // Per-thread values to sums over each group, in a fixed order, handed to
+    // finish(group, sum).  Vectors that lie in one group are summed first.  A
+    // group's values lie together, so that as many warps as there are for each
+    // group walk over them without a division.
+    const bool single = g.cg % V == 0;
+    const int unit = single ? V : 1, entries = g.cg / unit * h.rt;
+    const int share = max(warps / ng, 1);  // warps for a group
+    const auto group_sums = [&](const float (&s)[V], auto finish) {
+      if (active) {
+        if (single) {
+          float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) t += s[i];
-        red[cv * h.rt + rl] = t;
-      } else {
+          for (int i = 0; i < V; ++i) t += s[i];
+          red[cv * h.rt + rl] = t;
+        } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) red[(cv * V + i) * h.rt + rl] = s[i];
-      }
-    }
-    __syncthreads();
-    for (int w = warp; w < ng * share; w += warps) {
-      const int q = w / share, part = w - q * share;
-      const float* from = red + q * entries;
-      float t = 0.f;
-      for (int i = part * 32 + lane; i < entries; i += 32 * share) t += from[i];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      if (lane == 0) {
-        if (share == 1) finish(q, t);
-        else parts[w] = t;
-      }
-    }
-    __syncthreads();
-    if (share > 1) {
-      if (tid < ng) {
-        float t = 0.f;
-        for (int i = 0; i < share; ++i) t += parts[tid * share + i];
-        finish(tid, t);
+          for (int i = 0; i < V; ++i) red[(cv * V + i) * h.rt + rl] = s[i];
+        }
       }
       __syncthreads();
-    }
-  };
-
-  if constexpr (!BWD) {
-    const float n = (float)max(l1 - l0, (int64_t)0) * (float)g.cg;  // this CTA's values of a group
-    float s[V] = {}, mean[V];
-#pragma unroll 4
-    for (int i = 0; i < mine; ++i) {
-      float v[V];
-      hx[i * threads + tid].get(v);
-      gn_add<V>(s, v);
-    }
-    group_sums(s, [&](int q, float t) { own[q].x = n > 0.f ? t / n : 0.f; });
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      mean[j] = own[grp[j]].x;
-      s[j] = 0.f;
-    }
-#pragma unroll 4
-    for (int i = 0; i < mine; ++i) {
-      float v[V];
-      hx[i * threads + tid].get(v);
-      gn_sub<V>(v, mean);
-      gn_fma<V>(s, v, v);
-    }
-    group_sums(s, [&](int q, float t) { own[q].y = t; });
-    // the CTAs' means and squared deviations, merged about the common mean
-    if (h.ctas > 1) {
-      gn_cluster_arrive();
-      gn_cluster_wait();
-    }
-    // (from the first one's mean, so that equal means merge to themselves); a
-    // lane for each CTA
-    for (int q = warp; q < ng; q += warps) {
-      float2 each = own[q];
-      float cnt = n;
-      if (h.ctas > 1) {
-        const int r = min(lane, h.ctas - 1);
-        each = gn_peer(own + q, r);
-        cnt = lane < h.ctas ? (float)((int)max(min((r + 1) * h.rows, g.L) - r * h.rows, (int64_t)0) * g.cg) : 0.f;
-      } else if (lane) {
-        cnt = 0.f;
+      if (SHORT && entries <= 32) {  // a thread a group
+        for (int q = tid; q < ng; q += threads) {
+          float t = 0.f;
+          for (int i = 0; i < entries; ++i) t += red[q * entries + i];
+          finish(q, t);
+        }
+        __syncthreads();
+        return;
       }
-      const float ref = __shfl_sync(0xffffffffu, each.x, 0);
-      float mu = cnt * (each.x - ref);
+      for (int w = warp; w < ng * share; w += warps) {
+        const int q = w / share, part = w - q * share;
+        const float* from = red + q * entries;
+        float t = 0.f;
+        for (int i = part * 32 + lane; i < entries; i += 32 * share) t += from[i];
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) mu += __shfl_xor_sync(0xffffffffu, mu, o, 8);
-      mu = fmaf(mu, per_group, ref);
-      const float d = each.x - mu;
-      float m2 = cnt > 0.f ? fmaf(cnt * d, d, each.y) : 0.f;
+        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        if (lane == 0) {
+          if (share == 1) finish(q, t);
+          else parts[w] = t;
+        }
+      }
+      __syncthreads();
+      if (share > 1) {
+        if (tid < ng) {
+          float t = 0.f;
+          for (int i = 0; i < share; ++i) t += parts[tid * share + i];
+          finish(tid, t);
+        }
+        __syncthreads();
+      }
+    };
+
+    if constexpr (!BWD) {
+      const float n = (float)max(l1 - l0, (int64_t)0) * (float)g.cg;  // this CTA's values of a group
+      float s[V] = {}, mean[V], gain[V];
+#pragma unroll 4
+      for (int i = 0; i < mine; ++i) {
+        float v[V];
+        hx[i * threads + tid].get(v);
+        gn_add<V>(s, v);
+      }
+      group_sums(s, [&](int q, float t) { own[q].x = n > 0.f ? t / n : 0.f; });
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o, 8);
-      if (lane == 0) {
+      for (int j = 0; j < V; ++j) {
+        mean[j] = own[grp[j]].x;
+        s[j] = 0.f;
+      }
+#pragma unroll 4
+      for (int i = 0; i < mine; ++i) {
+        float v[V];
+        hx[i * threads + tid].get(v);
+        gn_sub<V>(v, mean);
+        gn_fma<V>(s, v, v);
+      }
+      group_sums(s, [&](int q, float t) { own[q].y = t; });
+      // the CTAs' means and squared deviations, merged about the common mean
+      if (h.ctas > 1) {
+        gn_cluster_arrive();
+        gn_cluster_wait();
+      }
+      // (from the first one's mean, so that equal means merge to themselves); a
+      // lane for each CTA
+      const auto settle = [&](int q, float mu, float m2) {
         const float2 st = make_float2(mu, rsqrtf(fmaf(m2, per_group, p.eps)));
         all[q] = st;
         if (rank == 0) reinterpret_cast<float2*>(p.stats)[(int64_t)b * g.G + g0 + q] = st;
-      }
-    }
-    __syncthreads();
-    if (h.ctas > 1) gn_cluster_arrive();
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float2 st = all[grp[j]];
-      mean[j] = st.x;
-      scale[j] *= st.y;
-    }
-#pragma unroll 4
-    for (int i = 0; i < mine; ++i) {
-      float v[V];
-      hx[i * threads + tid].get(v);
-      gn_sub<V>(v, mean);
-      gn_muladd<V>(v, scale, bias);
-      gn_pairs<V>(v, [](float2 x, int) { return act2<ACT>(x); });
-      Vec::put(out + i * step, v);
-    }
-  } else {
-    float mean[V], rstd[V], s1[V] = {}, s2[V] = {};
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float2 st = reinterpret_cast<const float2*>(p.stats)[(int64_t)b * g.G + g0 + grp[j]];
-      mean[j] = st.x;
-      rstd[j] = st.y;
-    }
-#pragma unroll 4
-    for (int i = 0; i < mine; ++i) {
-      float xh[V], d[V];
-      hx[i * threads + tid].get(xh);
-      hd[i * threads + tid].get(d);
-      gn_sub<V>(xh, mean);
-      gn_mul<V>(xh, rstd);
-      gn_du<V, ACT>(d, xh, scale, bias);
-      gn_add<V>(s1, d);
-      gn_fma<V>(s2, d, xh);
-    }
-    // sums per channel, for dscale and dbias, and from them the groups' means; a
-    // thread a channel where its row lanes are few, a warp where they are many
-    const int step_c = h.rt <= 8 ? 1 : 32;
-    const auto channel_sums = [&](const float (&s)[V], auto finish) {
-      if (active)
-#pragma unroll
-        for (int j = 0; j < V; ++j) red[(cv * V + j) * h.rt + rl] = s[j];
-      __syncthreads();
-      for (int c = step_c == 1 ? tid : warp; c < width; c += step_c == 1 ? threads : warps) {
-        float t = 0.f;
-        for (int r = step_c == 1 ? 0 : lane; r < h.rt; r += step_c) t += red[c * h.rt + r];
-        if (step_c > 1)
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        if (step_c == 1 || lane == 0) finish(c, t);
-      }
-      __syncthreads();
-    };
-    channel_sums(s1, [&](int c, float t) { chan[c].x = t; });
-    channel_sums(s2, [&](int c, float t) {
-      p.sums[((int64_t)b * h.ctas + rank) * g.D + c0 + c] = make_float2(chan[c].x, t);
-      chan[c].y = t;
-    });
-    for (int q = warp; q < ng; q += warps) {
-      float t1 = 0.f, t2 = 0.f;
-      for (int c = lane; c < g.cg; c += 32) {
-        const float w = p.scale ? p.scale[c0 + q * g.cg + c] : 1.f;
-        t1 = fmaf(w, chan[q * g.cg + c].x, t1);
-        t2 = fmaf(w, chan[q * g.cg + c].y, t2);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        t1 += __shfl_xor_sync(0xffffffffu, t1, o);
-        t2 += __shfl_xor_sync(0xffffffffu, t2, o);
-      }
-      if (lane == 0) own[q] = make_float2(t1, t2);
-    }
-    __syncthreads();
-    if (h.ctas > 1) {
-      gn_cluster_arrive();
-      gn_cluster_wait();
-    }
-    for (int q = warp; q < ng; q += warps) {
-      float2 t = own[q];
-      if (h.ctas > 1) {
-        t = lane < h.ctas ? gn_peer(own + q, lane) : make_float2(0.f, 0.f);
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-          t.x += __shfl_xor_sync(0xffffffffu, t.x, o, 8);
-          t.y += __shfl_xor_sync(0xffffffffu, t.y, o, 8);
+      };
+      if (SHORT && h.ctas == 1)
+        for (int q = tid; q < ng; q += threads) settle(q, own[q].x, own[q].y);
+      for (int q = warp; (!SHORT || h.ctas > 1) && q < ng; q += warps) {
+        float2 each = own[q];
+        float cnt = lane ? 0.f : n;
+        if (h.ctas > 1) {
+          const int r = min(lane, h.ctas - 1);
+          each = gn_peer(own + q, r);
+          cnt = lane < h.ctas ? (float)((int)max(min((r + 1) * h.rows, g.L) - r * h.rows, (int64_t)0) * g.cg) : 0.f;
         }
-      }
-      if (lane == 0) all[q] = make_float2(t.x * per_group, t.y * per_group);
-    }
-    __syncthreads();
-    if (h.ctas > 1) gn_cluster_arrive();
-    float m1[V], m2[V];
+        const float ref = __shfl_sync(0xffffffffu, each.x, 0);
+        float mu = cnt * (each.x - ref);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float2 m = all[grp[j]];
-      m1[j] = m.x;
-      m2[j] = -m.y;
-    }
+        for (int o = 4; o > 0; o >>= 1) mu += __shfl_xor_sync(0xffffffffu, mu, o, 8);
+        mu = fmaf(mu, per_group, ref);
+        const float d = each.x - mu;
+        float m2 = cnt > 0.f ? fmaf(cnt * d, d, each.y) : 0.f;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o, 8);
+        if (lane == 0) settle(q, mu, m2);
+      }
+      __syncthreads();
+      if (h.ctas > 1) gn_cluster_arrive();
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float2 st = all[grp[j]];
+        mean[j] = st.x;
+        gain[j] = scale[j] * st.y;
+      }
 #pragma unroll 4
-    for (int i = 0; i < mine; ++i) {
-      float xh[V], d[V];
-      hx[i * threads + tid].get(xh);
-      hd[i * threads + tid].get(d);
-      gn_sub<V>(xh, mean);
-      gn_mul<V>(xh, rstd);
-      gn_du<V, ACT>(d, xh, scale, bias);
-      gn_mul<V>(d, scale);
-      gn_sub<V>(d, m1);
-      gn_fma<V>(d, xh, m2);  // m2 holds its negative
-      gn_mul<V>(d, rstd);
-      Vec::put(out + i * step, d);
+      for (int i = 0; i < mine; ++i) {
+        float v[V];
+        hx[i * threads + tid].get(v);
+        gn_sub<V>(v, mean);
+        gn_muladd<V>(v, gain, bias);
+        gn_pairs<V>(v, [](float2 x, int) { return act2<ACT>(x); });
+        Vec::put(out + i * step, v);
+      }
+    } else {
+      float mean[V], rstd[V], s1[V] = {}, s2[V] = {};
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float2 st = reinterpret_cast<const float2*>(p.stats)[(int64_t)b * g.G + g0 + grp[j]];
+        mean[j] = st.x;
+        rstd[j] = st.y;
+      }
+#pragma unroll 4
+      for (int i = 0; i < mine; ++i) {
+        float xh[V], d[V];
+        hx[i * threads + tid].get(xh);
+        hd[i * threads + tid].get(d);
+        gn_sub<V>(xh, mean);
+        gn_mul<V>(xh, rstd);
+        gn_du<V, ACT>(d, xh, scale, bias);
+        gn_add<V>(s1, d);
+        gn_fma<V>(s2, d, xh);
+      }
+      // sums per channel, for dscale and dbias, and from them the groups' means; a
+      // thread a channel where its row lanes are few, a warp where they are many
+      const auto channel_sums = [&](const float (&s)[V], auto finish) {
+        if (active)
+#pragma unroll
+          for (int j = 0; j < V; ++j) red[(cv * V + j) * h.rt + rl] = s[j];
+        __syncthreads();
+        for (int c = step_c == 1 ? tid : warp; c < width; c += step_c == 1 ? threads : warps) {
+          float t = 0.f;
+          for (int r = step_c == 1 ? 0 : lane; r < h.rt; r += step_c) t += red[c * h.rt + r];
+          if (step_c > 1)
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+          if (step_c == 1 || lane == 0) finish(c, t);
+        }
+        __syncthreads();
+      };
+      channel_sums(s1, [&](int c, float t) { chan[c].x = t; });
+      channel_sums(s2, [&](int c, float t) {
+        const float2 v = make_float2(chan[c].x, t);
+        acc[c] = !SHORT || b == turn ? v : fadd2(acc[c], v);  // a channel is always the same thread's
+        chan[c] = fmul2(v, dup2(p.scale ? p.scale[c0 + c] : 1.f));
+      });
+      const int lanes = SHORT && g.cg <= 32 && ng > warps ? 1 : 32;  // for a group: a thread where its channels are few
+      for (int q = lanes == 1 ? tid : warp; q < ng; q += lanes == 1 ? threads : warps) {
+        float t1 = 0.f, t2 = 0.f;
+        for (int c = lanes == 1 ? 0 : lane; c < g.cg; c += lanes) {
+          t1 += chan[q * g.cg + c].x;
+          t2 += chan[q * g.cg + c].y;
+        }
+        if (lanes > 1)
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            t1 += __shfl_xor_sync(0xffffffffu, t1, o);
+            t2 += __shfl_xor_sync(0xffffffffu, t2, o);
+          }
+        if (lanes == 1 || lane == 0) own[q] = make_float2(t1, t2);
+      }
+      __syncthreads();
+      if (h.ctas > 1) {
+        gn_cluster_arrive();
+        gn_cluster_wait();
+      }
+      if (SHORT && h.ctas == 1)
+        for (int q = tid; q < ng; q += threads) all[q] = make_float2(own[q].x * per_group, own[q].y * per_group);
+      for (int q = warp; (!SHORT || h.ctas > 1) && q < ng; q += warps) {
+        float2 t = own[q];
+        if (h.ctas > 1) {
+          t = lane < h.ctas ? gn_peer(own + q, lane) : make_float2(0.f, 0.f);
+#pragma unroll
+          for (int o = 4; o > 0; o >>= 1) {
+            t.x += __shfl_xor_sync(0xffffffffu, t.x, o, 8);
+            t.y += __shfl_xor_sync(0xffffffffu, t.y, o, 8);
+          }
+        }
+        if (lane == 0) all[q] = make_float2(t.x * per_group, t.y * per_group);
+      }
+      __syncthreads();
+      if (h.ctas > 1) gn_cluster_arrive();
+      float m1[V], m2[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float2 m = all[grp[j]];
+        m1[j] = m.x;
+        m2[j] = -m.y;
+      }
+#pragma unroll 4
+      for (int i = 0; i < mine; ++i) {
+        float xh[V], d[V];
+        hx[i * threads + tid].get(xh);
+        hd[i * threads + tid].get(d);
+        gn_sub<V>(xh, mean);
+        gn_mul<V>(xh, rstd);
+        gn_du<V, ACT>(d, xh, scale, bias);
+        gn_mul<V>(d, scale);
+        gn_sub<V>(d, m1);
+        gn_fma<V>(d, xh, m2);  // m2 holds its negative
+        gn_mul<V>(d, rstd);
+        Vec::put(out + i * step, d);
+      }
     }
+    __syncwarp();
+    if (h.ctas > 1) gn_cluster_wait();  // the others read this CTA's pairs
   }
-  __syncwarp();
-  if (h.ctas > 1) gn_cluster_wait();  // the others read this CTA's pairs
+  if (BWD)
+    for (int c = step_c == 1 ? tid : warp; c < width; c += step_c == 1 ? threads : warps)
+      if (step_c == 1 || lane == 0) p.sums[((int64_t)turn * h.ctas + rank) * g.D + c0 + c] = acc[c];
 }
 
 static int check_gn(const ssm_group_norm_params_t* p) {
   if (!p) return SSM_ERR_NULL;
   if (p->batch < 0 || p->seqlen < 0 || p->dim < 1 || p->groups < 1 || p->dim % p->groups || p->dim > (1 << 20) ||
-      p->batch > 65535 || p->seqlen > (1ll << 40) || p->act < SSM_ACT_NONE || p->act > SSM_ACT_RELU)
+      p->batch > 0x7fffffff / p->groups || p->seqlen > (1ll << 40) || p->act < SSM_ACT_NONE || p->act > SSM_ACT_RELU)
     return SSM_ERR_SHAPE;
   if (p->dtype != SSM_F32 && p->dtype != SSM_BF16) return SSM_ERR_DTYPE;
   return SSM_OK;
@@ -869,6 +898,7 @@ static GnGeom gn_geom(const ssm_group_norm_params_t* p) {
 // rows read 64 bytes or more (with 16 a call of 16 x 4096 x 256 bf16 took 39 us
 // for 24), and that small calls spread over the SMs.
 constexpr size_t kHoldSmem = 74 * 1024;
+constexpr int kHoldCtas = 32 * 148;  // at most, where there are that many batch rows
 static bool gn_hold(const ssm_group_norm_params_t* p, bool bwd, GnHold* h, int* V) {
   const int es = p->dtype == SSM_BF16 ? 2 : 4, cg = p->dim / p->groups;
   const int wide = 16 / es;
@@ -902,9 +932,10 @@ static bool gn_hold(const ssm_group_norm_params_t* p, bool bwd, GnHold* h, int* 
       c.rt = c.threads / c.nv;
       c.slots = (int)((rows + c.rt - 1) / c.rt);
       c.smem = ((size_t)c.slots * c.threads * *V * es * (bwd ? 2 : 1) + 15) / 16 * 16 +
-               (size_t)c.threads * 4 * (bwd || cg % *V ? *V : 2) + (bwd ? (size_t)c.W : 0) * sizeof(float2) +
+               (size_t)c.threads * 4 * (bwd || cg % *V ? *V : 2) + (bwd ? 2 * (size_t)c.W : 0) * sizeof(float2) +
                2 * (size_t)gpj * sizeof(float2);
-      return c.smem <= kHoldSmem && (int64_t)c.jobs * p->batch * ctas <= 0x7fffffff;
+      c.turns = (int)std::min<int64_t>(p->batch, std::max(1, kHoldCtas / (c.jobs * ctas)));
+      return c.smem <= kHoldSmem && (int64_t)c.jobs * c.turns * ctas <= 0x7fffffff;
     };
     if (!cut(least)) continue;
     int gpj = least;
@@ -927,7 +958,7 @@ static size_t gn_means_bytes(const GnGeom& g) { return gn_round((size_t)g.B * g.
 template <typename T, int V, int ACT>
 static void gn_fwd_launch(const GnArgs& a, cudaStream_t s) {
   const GnGeom& g = a.g;
-  const dim3 grid(g.chunks, g.B, g.tiles);
+  const dim3 grid((unsigned)(g.chunks * g.B), 1, g.tiles);
   constexpr size_t ring = kGnRing<T, V, 1>;
   const size_t smem = std::max(ring, (2 * (size_t)g.rt * g.ct * V + g.rt) * sizeof(float));
   if (ring > 48 * 1024) {
@@ -945,7 +976,7 @@ static void gn_fwd_launch(const GnArgs& a, cudaStream_t s) {
 template <typename T, int V, int ACT, bool ONE>
 static void gn_bwd_launch_one(const GnArgs& a, cudaStream_t s) {
   const GnGeom& g = a.g;
-  const dim3 grid(g.chunks, g.B, g.tiles);
+  const dim3 grid((unsigned)(g.chunks * g.B), 1, g.tiles);
   constexpr size_t ring = kGnRing<T, V, 2>;
   const size_t smem = std::max(ring, 2 * (size_t)g.rt * g.ct * V * sizeof(float));
   if (ring > 48 * 1024) {
@@ -974,15 +1005,15 @@ static void gn_launch(const GnArgs& a, int act, bool bwd, cudaStream_t s) {
   }
 }
 
-template <typename T, int V, int ACT, bool BWD>
+template <typename T, int V, int ACT, bool BWD, bool SHORT>
 static cudaError_t gn_hold_launch(const GnArgs& a, const GnHold& h, cudaStream_t s) {
-  const auto kernel = gn_hold_kernel<T, V, ACT, BWD>;
+  const auto kernel = gn_hold_kernel<T, V, ACT, BWD, SHORT>;
   if (h.smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)h.smem);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.g.B * h.jobs * h.ctas));
+  cfg.gridDim = dim3((unsigned)(h.turns * h.jobs * h.ctas));
   cfg.blockDim = dim3(h.threads);
   cfg.dynamicSmemBytes = h.smem;
   cfg.stream = s;
@@ -995,18 +1026,22 @@ static cudaError_t gn_hold_launch(const GnArgs& a, const GnHold& h, cudaStream_t
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, h);
   note_launches(1);
   if (BWD && e == cudaSuccess && (a.dscale || a.dbias)) {
-    gn_param_kernel<<<(a.g.D + 31) / 32, 1024, 0, s>>>(a.sums, a.g.B * h.ctas, a.g.D, a.dscale, a.dbias);
+    gn_param_kernel<<<(a.g.D + 31) / 32, 1024, 0, s>>>(a.sums, h.turns * h.ctas, a.g.D, a.dscale, a.dbias);
     note_launches(1);
   }
   return e;
 }
+template <typename T, int V, int ACT, bool BWD>
+static cudaError_t gn_hold_length(const GnArgs& a, const GnHold& h, cudaStream_t s) {
+  return h.turns < a.g.B || h.rows <= 4 ? gn_hold_launch<T, V, ACT, BWD, true>(a, h, s) : gn_hold_launch<T, V, ACT, BWD, false>(a, h, s);
+}
 template <typename T, int V, bool BWD>
 static cudaError_t gn_hold_act(const GnArgs& a, const GnHold& h, int act, cudaStream_t s) {
   switch (act) {
-    case SSM_ACT_SILU: return gn_hold_launch<T, V, SSM_ACT_SILU, BWD>(a, h, s);
-    case SSM_ACT_GELU: return gn_hold_launch<T, V, SSM_ACT_GELU, BWD>(a, h, s);
-    case SSM_ACT_RELU: return gn_hold_launch<T, V, SSM_ACT_RELU, BWD>(a, h, s);
-    default: return gn_hold_launch<T, V, SSM_ACT_NONE, BWD>(a, h, s);
+    case SSM_ACT_SILU: return gn_hold_length<T, V, SSM_ACT_SILU, BWD>(a, h, s);
+    case SSM_ACT_GELU: return gn_hold_length<T, V, SSM_ACT_GELU, BWD>(a, h, s);
+    case SSM_ACT_RELU: return gn_hold_length<T, V, SSM_ACT_RELU, BWD>(a, h, s);
+    default: return gn_hold_length<T, V, SSM_ACT_NONE, BWD>(a, h, s);
   }
 }
 template <bool BWD>
@@ -1054,8 +1089,13 @@ size_t ssm_group_norm_fwd_workspace_bytes(const ssm_group_norm_params_t* p) {
 size_t ssm_group_norm_bwd_workspace_bytes(const ssm_group_norm_params_t* p) {
   if (check_gn(p) || p->batch == 0 || p->seqlen == 0) return 0;
   const GnGeom g = gn_geom(p);
+  GnHold h;
+  int V;
+  if (p->x && p->dy && p->dx && gn_hold(p, true, &h, &V))
+    return gn_round((size_t)h.turns * h.ctas * g.D * sizeof(float2));
+  // without the pointers their alignment, which has a say in the form, is unknown
   const size_t split = gn_part_bytes(g) + gn_sums_bytes(g) + gn_means_bytes(g);
-  return std::max(split, gn_round((size_t)g.B * 8 * g.D * sizeof(float2)));  // of either form, whatever its cut
+  return std::max(split, gn_round((size_t)std::min<int64_t>(8 * p->batch, kHoldCtas + 8) * g.D * sizeof(float2)));
 }
 
 int ssm_group_norm_act_fwd(const ssm_group_norm_params_t* p, ssm_stream_t stream) {

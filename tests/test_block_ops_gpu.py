@@ -261,6 +261,24 @@ def test_group_norm_with_a_large_mean_and_one_outlier(cuda, shape):
     assert_within(y.reshape(want["y"].shape), want["y"], tol["y"] + 1e-30)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_group_norm_of_many_short_rows(cuda, dtype):
+    """A norm per token: far more batch rows than clusters, each taking several."""
+    from selectssm_b200 import group_norm_act
+    torch.manual_seed(10)
+    shape, groups = (70001, 1, 48), 6
+    x = torch.randn(shape, device=cuda).to(dtype).requires_grad_()
+    scale, bias = (t.requires_grad_() for t in (1 + 0.1 * torch.randn(48, device=cuda), torch.randn(48, device=cuda)))
+    dy = torch.randn(shape, device=cuda).to(dtype)
+    y = group_norm_act(x, scale, bias, groups=groups, activation="silu")
+    y.backward(dy)
+    want, tol = gn64(x, scale.detach().double(), bias.detach().double(), groups, 1e-6, "silu", dy)
+    for name, got in (("y", y.detach()), ("dx", x.grad)):
+        assert_within(got, want[name], tol[name] + stored(want[name], dtype), name)
+    for name, got in (("dscale", scale.grad), ("dbias", bias.grad)):
+        assert_within(got, want[name], tol[name] + 1e-30, name)
+
+
 def test_group_norm_constant_input(cuda):
     """No spread: xhat is 0 and y the activated bias."""
     from selectssm_b200 import group_norm_act
