@@ -294,31 +294,38 @@ constexpr uint32_t mma_idesc(int m, int n, bool a_mn, bool b_mn) {
 // cluster of two) that share one product: the pair's first CTA issues for both.
 template <bool PAIR>
 struct Mma {
-  __device__ __forceinline__ static void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  // `one`: nonzero in the lane that issues.  The whole warp comes here with the
+  // same operands.
+  __device__ __forceinline__ static void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate,
+                                             uint32_t one) {
     if constexpr (PAIR)
       asm volatile(
-          "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-          "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-          "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+          "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+          "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
           : "memory");
     else
       asm volatile(
-          "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-          "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-          "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+          "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+          "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
           : "memory");
   }
   // arrives on `bar` (of both CTAs of a pair) when the products issued so far are done
-  __device__ __forceinline__ static void commit(uint64_t* bar) {
+  __device__ __forceinline__ static void commit(uint64_t* bar, uint32_t one) {
     if constexpr (PAIR)
       asm volatile(
-          "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-              smem_u32(bar)),
-          "h"((uint16_t)3)
+          "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+          "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::
+              "r"(smem_u32(bar)),
+          "h"((uint16_t)3), "r"(one)
           : "memory");
     else
-      asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                   : "memory");
+      asm volatile(
+          "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+          "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+          "r"(one)
+          : "memory");
   }
   __device__ __forceinline__ static void alloc(uint32_t* dst, uint32_t ncols) {
     if constexpr (PAIR) {
@@ -337,21 +344,31 @@ struct Mma {
   }
   // a box to this CTA's `dst`, counted on `bar`: an address in the cluster's
   // shared memory, for a pair that of the first CTA's barrier
-  __device__ __forceinline__ static void load(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  __device__ __forceinline__ static void load(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
+                                              uint32_t one) {
     if constexpr (PAIR)
       asm volatile(
-          "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-          " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
-          "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+          "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+          "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+          " [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(smem_u32(dst)),
+          "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar), "r"(one)
           : "memory");
     else
       asm volatile(
-          "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-          " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
-          "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+          "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+          "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+          " [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(smem_u32(dst)),
+          "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar), "r"(one)
           : "memory");
   }
 };
+__device__ __forceinline__ void expect_bytes(uint64_t* bar, uint32_t bytes, uint32_t one) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+      "r"(bytes), "r"(one)
+      : "memory");
+}
 // the same shared-memory address in the cluster's CTA 0
 __device__ __forceinline__ uint32_t in_first_cta(const void* p) {
   uint32_t r;
@@ -368,6 +385,26 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
+}
+
+// nonzero in one lane of the warp
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+// A bounded wait as one stretch of code: at most `polls` polls, then `polls`
+// becomes 1, so that the waits after one that gave up do not wait.  Nothing
+// branches on the outcome, and the code around it stays the same for the warp.
+__device__ __forceinline__ void wait_through(uint64_t* bar, uint32_t parity, uint32_t& polls) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, %0;\n\t"
+      "POLL_%=:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE_%=;\n\t"
+      "sub.u32 n, n, 1;\n\tsetp.ne.u32 q, n, 0;\n\t@q bra POLL_%=;\n\tmov.u32 %0, 1;\n\t"
+      "DONE_%=:\n\t}"
+      : "+r"(polls)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
 }
 
 struct DenseWork {
@@ -458,14 +495,19 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     return false;
   };
 
-  if ((warp == 0 || warp == 3) && lane == 0) {
-    // Warp 0 loads A, warp 3 loads B: the time from a slice's release to its
-    // next load is on the path that bounds the products.
+  // The warps that load and that issue products walk their loops whole and one
+  // lane issues: in a branch of one lane every operand (descriptors, addresses)
+  // passes through vector registers, and what stands between two steps' products
+  // or loads then takes longer than the queue of products lasts.  (131072 x 1536
+  // x 768 without its epilogue: 329 thousand cycles that way, 312 with only the
+  // products' warp whole, 264 with all three; the products alone take 256.)
+  if (warp == 0 || warp == 3) {
+    // Warp 0 loads A, warp 3 loads B.
     const bool of_a = warp == 0;
+    const uint32_t one = elect_one();
     int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int item = first; ok && item < items; item += stride) {
+    uint32_t phase = 0, polls = kMmaSpin;
+    for (int item = first; item < items; item += stride) {
       const int rest = item / w.tiles_n, split = rest / w.tiles_m;
       const int n0 = item % w.tiles_n * BN + (PAIR ? rank * 128 : 0);
       const int m0 = rest % w.tiles_m * S::kM + (PAIR ? rank * 128 : 0);
@@ -473,27 +515,25 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       int seg = 0, kb = kb0, pa, pb;
       plane_pair(e.planes, seg, pa, pb);
       for (int t = (kb1 - kb0) * w.pairs; t > 0; --t) {
-        if (!wait(&empty[stage], phase ^ 1)) {
-          ok = false;
-          break;
-        }
+        wait_through(&empty[stage], phase ^ 1, polls);
+        if (polls == 1) break;  // what it would overwrite may still be read
         const int k0 = kb * kBK;
         uint8_t* sa = tiles + stage * S::kStage;
         uint8_t* sb = sa + S::kA;
         const uint32_t bar = PAIR ? in_first_cta(&full[stage]) : smem_u32(&full[stage]);
-        if (rank == 0 && of_a) mbar_arrive_expect_tx(&full[stage], PAIR ? 2 * S::kStage : S::kStage);
         if (of_a) {
+          if (rank == 0) expect_bytes(&full[stage], PAIR ? 2 * S::kStage : S::kStage, one);
           if (A_MN) {
 #pragma unroll
-            for (int j = 0; j < S::kBoxA / 64; ++j) I::load(sa + j * 8192, &map_a, bar, m0 + 64 * j, k0, pa);
+            for (int j = 0; j < S::kBoxA / 64; ++j) I::load(sa + j * 8192, &map_a, bar, m0 + 64 * j, k0, pa, one);
           } else {
-            I::load(sa, &map_a, bar, k0, m0, pa);
+            I::load(sa, &map_a, bar, k0, m0, pa, one);
           }
         } else if (B_MN) {
 #pragma unroll
-          for (int j = 0; j < S::kBoxB / 64; ++j) I::load(sb + j * 8192, &map_b, bar, n0 + 64 * j, k0, pb);
+          for (int j = 0; j < S::kBoxB / 64; ++j) I::load(sb + j * 8192, &map_b, bar, n0 + 64 * j, k0, pb, one);
         } else {
-          I::load(sb, &map_b, bar, k0, n0, pb);
+          I::load(sb, &map_b, bar, k0, n0, pb, one);
         }
         if (++kb == kb1) {
           kb = kb0;
@@ -504,58 +544,59 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           phase ^= 1;
         }
       }
+      if (polls == 1) break;
     }
-    // Loads still in flight when the products stopped early: wait for the last
-    // ones so that none lands after the CTA has gone.
-    if (!ok && rank == 0)
-      for (int i = 0; i < stages; ++i) {
-        mbar_wait_bounded(&full[stage], phase ^ 1, 1u << 16);
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1;
+    if (polls == 1) {
+      dead = 1;
+      if (one) report(status, kStatusTimeout);
+      // Loads still in flight: wait for the last ones so that none lands after
+      // the CTA has gone.
+      if (rank == 0)
+        for (int i = 0; i < stages; ++i) {
+          mbar_wait_bounded(&full[stage], phase ^ 1, 1u << 16);
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+          }
         }
-      }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+    }
+  } else if (warp == 1 && rank == 0) {
     constexpr uint32_t idesc = mma_idesc(S::kM, BN, A_MN, B_MN);
     constexpr uint32_t kStepA = (A_MN ? 2048 : 32) >> 4, kStepB = (B_MN ? 2048 : 32) >> 4;
+    const uint32_t one = elect_one();
+    const uint64_t da0 = smem_desc(smem_u32(tiles)), db0 = smem_desc(smem_u32(tiles + S::kA));
     int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    bool ok = true;
-    for (int item = first; ok && item < items; item += stride) {
+    uint32_t phase = 0, acc_phase = 0, polls = kMmaSpin;
+    for (int item = first; item < items; item += stride) {
       const int split = item / w.tiles_n / w.tiles_m;
       const int t1 = (w.block(split + 1) - w.block(split)) * w.pairs;
-      if (!wait(&acc_empty[acc], acc_phase ^ 1)) break;
+      wait_through(&acc_empty[acc], acc_phase ^ 1, polls);
       tmem_fence_after_sync();
       const uint32_t d = tmem + acc * BN;
-      bool ready = false;
+      wait_through(&full[stage], phase, polls);
       for (int t = 0; t < t1; ++t) {
-        if (!ready && !wait(&full[stage], phase)) {
-          ok = false;
-          break;
-        }
         tmem_fence_after_sync();
-        const uint32_t sa = smem_u32(tiles + stage * S::kStage);
-        const uint64_t da = smem_desc(sa), db = smem_desc(sa + S::kA);
+        const uint64_t da = da0 + stage * (S::kStage >> 4), db = db0 + stage * (S::kStage >> 4);
         uint64_t* const used = &empty[stage];
         if (++stage == stages) {
           stage = 0;
           phase ^= 1;
         }
-        // The queue of products is short: a barrier asked about after the last
-        // one is issued leaves the tensor core idle for the answer's 250
-        // cycles of every 510, so the next step's is asked about before.
-        I::mma(d, da, db, idesc, t > 0);
-        ready = t + 1 < t1 && mbar_try_wait(&full[stage], phase);
 #pragma unroll
-        for (int k = 1; k < kBK / 16; ++k) I::mma(d, da + k * kStepA, db + k * kStepB, idesc, 1);
-        I::commit(used);
+        for (int k = 0; k < kBK / 16; ++k) I::mma(d, da + k * kStepA, db + k * kStepB, idesc, t > 0 || k > 0, one);
+        I::commit(used, one);
+        if (t + 1 < t1) wait_through(&full[stage], phase, polls);
       }
-      I::commit(&acc_full[acc]);
-      if (!ok) mbar_wait_bounded(&acc_full[acc], acc_phase, 1u << 16);  // products still running use the buffers
+      I::commit(&acc_full[acc], one);
       if (++acc == 2) {
         acc = 0;
         acc_phase ^= 1;
       }
+    }
+    if (polls == 1) {
+      dead = 1;
+      if (one) report(status, kStatusTimeout);
+      mbar_wait_bounded(&acc_full[acc ^ 1], acc_phase ^ (acc == 0), 1u << 16);  // products still running use the buffers
     }
   } else if (warp >= 4) {
     const EpiConst c(e);
