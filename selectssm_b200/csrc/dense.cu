@@ -337,7 +337,7 @@ static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
   int st = q.pair ? launch_mma<A_MN, B_MN, true, T>(first, q, ma, mb, status, s)
                   : launch_mma<A_MN, B_MN, false, T>(first, q, ma, mb, status, s);
   if (st || q.w.splits == 1) return st;
-  const int64_t grid = ceil_div(ceil_div(e.M, 32) * ceil_div(e.N, 32), kJoinWarps);
+  const int64_t grid = ceil_div(ceil_div(e.M, 32) * ceil_div(e.N, kCW), kJoinWarps);
   if (grid > 0x7fffffff) return SSM_ERR_SHAPE;
   dense_join_kernel<T><<<(unsigned)grid, 32 * kJoinWarps, 0, s>>>(part, q.w.splits, e);
   return launched("launch dense join kernel", 1);

@@ -116,9 +116,9 @@ __device__ __forceinline__ void dense_bias8(const DenseEpi& e, const EpiConst& c
   else get8<float>(e.bias, n, e.N - n, c.vec_bias, b);
 }
 
-// What an epilogue does to columns n .. n+7 of R rows (row, row + 8, ...) from
-// the summed products v.  Only the first `left` / 8 of the rows exist, and only
-// stores look at that: written stage by stage over all rows, the rows' chains
+// What an epilogue does to columns n .. n+7 of R rows (row, row + 32 / R, ...)
+// from the summed products v.  Only those less than `left` below `row` exist, and
+// only stores look at that: written stage by stage over all rows, the rows' chains
 // (ten dependent rounds of the generator, the activation) overlap.  The
 // instructions of this function are what an epilogue costs: issued beside the
 // warp that starts the tensor core's products, they delay it one for one.
@@ -126,6 +126,7 @@ __device__ __forceinline__ void dense_bias8(const DenseEpi& e, const EpiConst& c
 template <typename T, int R, typename RES, typename PUT>
 __device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst& c, int64_t row, int left, int n,
                                                const float (&bias)[8], float (&v)[R][8], RES get_res, PUT put) {
+  constexpr int RS = 32 / R;
   if (sizeof(T) == 4 && e.planes == 3) {
     // An infinite operand has no finite planes besides its first, and infinity
     // times the other operand's planes gives NaN where the product is infinite.
@@ -140,7 +141,7 @@ __device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst
       for (int q = 0; q < R; ++q)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (isnan(v[q][i]) && q * 8 < left && n + i < e.N) v[q][i] = dense_again(e, row + q * 8, n + i);
+          if (isnan(v[q][i]) && q * RS < left && n + i < e.N) v[q][i] = dense_again(e, row + q * RS, n + i);
     }
   }
   if (e.bias)
@@ -152,10 +153,10 @@ __device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst
     const int64_t block = row * e.per_row + n / 8;
     if (c.low) {  // no counter passes 32 bits: the generator's first products are common to all
 #pragma unroll
-      for (int q = 0; q < R; ++q) w[q] = philox4x32_10((uint32_t)block + (uint32_t)(q * 8 * e.per_row), 0u, c.key);
+      for (int q = 0; q < R; ++q) w[q] = philox4x32_10((uint32_t)block + (uint32_t)(q * RS * e.per_row), 0u, c.key);
     } else {
 #pragma unroll
-      for (int q = 0; q < R; ++q) w[q] = philox4x32_10((uint64_t)(block + (int64_t)q * 8 * e.per_row), c.key);
+      for (int q = 0; q < R; ++q) w[q] = philox4x32_10((uint64_t)(block + (int64_t)q * RS * e.per_row), c.key);
     }
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -184,95 +185,106 @@ __device__ __forceinline__ void dense_put(const DenseEpi& e, const EpiConst& c, 
   T* p = static_cast<T*>(base) + row * e.N + n;
 #pragma unroll
   for (int q = 0; q < R; ++q)
-    if (q * 8 < left) put8<T>(p, (int64_t)(q * 8) * e.N, min(8, e.N - n), c.vec_out, v[q]);
+    if (q * (32 / R) < left) put8<T>(p, (int64_t)(q * (32 / R)) * e.N, min(8, e.N - n), c.vec_out, v[q]);
 }
 
-// A warp's 32 x 32 values in shared memory: 16-byte pieces, swizzled by row.
-// `put` and `get` move the epilogue's arrangement (eight columns of rows
-// lane / 4 + 8 q), `at` addresses a lane's own column.
-struct Stage32 {
+// A warp's chunk of an epilogue: 32 rows by kCW columns.  kCW / 8 lanes cover a
+// row, each with eight columns of kCR rows, kCStep apart.  (16 warps with chunks
+// of 16 columns have half the registers each: 131072 x 1536 x 768 with residual
+// and dropout 250 us for 242, 32768 x 768 x 1536 with silu and dropout 110 for 115.)
+constexpr int kCW = 32, kCLanes = kCW / 8, kCR = kCLanes, kCStep = 32 / kCLanes;
+
+// The chunk in shared memory: 16-byte pieces, swizzled by row so that a lane's
+// own row (as the accumulator has it) and the arrangement above both reach it
+// without conflicts.
+struct Stage {
   uint4* s;
   int lane;
-  __device__ __forceinline__ uint4& piece(int row, int p) const { return s[row * 8 + (p ^ (row & 7))]; }
-  __device__ __forceinline__ float& at(int row) const {
-    return reinterpret_cast<float*>(&piece(row, lane >> 2))[lane & 3];
+  static constexpr int kPieces = kCW / 4;  // of a row
+  __device__ __forceinline__ int row() const { return lane / kCLanes; }
+  __device__ __forceinline__ int col() const { return lane % kCLanes * 8; }
+  __device__ __forceinline__ uint4& piece(int row, int p) const {
+    return s[row * kPieces + (p ^ (kPieces == 8 ? row & 7 : row >> 1 & 3))];
   }
-  // this lane's two pieces of row lane / 4; those of the rows 8, 16 and 24 below are 64 pieces on
-  __device__ __forceinline__ uint4* mine(int half) const { return &piece(lane >> 2, (lane & 3) * 2 + half); }
-  __device__ __forceinline__ void get(float (&v)[4][8]) const {
+  __device__ __forceinline__ float& at(int row, int c) const { return reinterpret_cast<float*>(&piece(row, c >> 2))[c & 3]; }
+  // this lane's two pieces of its first row; kCStep rows below they have the same swizzle
+  __device__ __forceinline__ uint4* mine(int half) const { return &piece(row(), lane % kCLanes * 2 + half); }
+  __device__ __forceinline__ void get(float (&v)[kCR][8]) const {
     const uint4 *a = mine(0), *b = mine(1);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const uint4 lo = a[q * 64], hi = b[q * 64];
+    for (int q = 0; q < kCR; ++q) {
+      const uint4 lo = a[q * kCStep * kPieces], hi = b[q * kCStep * kPieces];
       v[q][0] = __uint_as_float(lo.x); v[q][1] = __uint_as_float(lo.y);
       v[q][2] = __uint_as_float(lo.z); v[q][3] = __uint_as_float(lo.w);
       v[q][4] = __uint_as_float(hi.x); v[q][5] = __uint_as_float(hi.y);
       v[q][6] = __uint_as_float(hi.z); v[q][7] = __uint_as_float(hi.w);
     }
   }
-  __device__ __forceinline__ void put(const float (&v)[4][8]) const {
+  __device__ __forceinline__ void put(const float (&v)[kCR][8]) const {
     uint4 *a = mine(0), *b = mine(1);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      a[q * 64] = make_uint4(__float_as_uint(v[q][0]), __float_as_uint(v[q][1]), __float_as_uint(v[q][2]),
-                             __float_as_uint(v[q][3]));
-      b[q * 64] = make_uint4(__float_as_uint(v[q][4]), __float_as_uint(v[q][5]), __float_as_uint(v[q][6]),
-                             __float_as_uint(v[q][7]));
+    for (int q = 0; q < kCR; ++q) {
+      a[q * kCStep * kPieces] = make_uint4(__float_as_uint(v[q][0]), __float_as_uint(v[q][1]), __float_as_uint(v[q][2]),
+                                           __float_as_uint(v[q][3]));
+      b[q * kCStep * kPieces] = make_uint4(__float_as_uint(v[q][4]), __float_as_uint(v[q][5]), __float_as_uint(v[q][6]),
+                                           __float_as_uint(v[q][7]));
     }
   }
 };
 
-// For rows that start anywhere: a warp's 32 x 32 chunk from row m0, column n,
-// one row at a time with a lane a column, so that its accesses lie together, and
-// through shared memory to or from the epilogue's arrangement.
+// For rows that start anywhere: a chunk from row m0, column n, with a lane a
+// column, so that its accesses lie together, and through shared memory to or
+// from the epilogue's arrangement.
 template <typename T>
-__device__ __forceinline__ void dense_stage_rows(const DenseEpi& e, const Stage32& st, int64_t m0, int n, float (&res)[4][8]) {
+__device__ __forceinline__ void dense_stage_rows(const DenseEpi& e, const Stage& st, int64_t m0, int n, float (&res)[kCR][8]) {
+  const int c = st.lane % kCW;
   __syncwarp();
-  if (n + st.lane < e.N)
-    for (int row = 0; row < 32 && m0 + row < e.M; ++row)
-      st.at(row) = Cvt<T>::to_f(static_cast<const T*>(e.residual)[(m0 + row) * e.res_stride + n + st.lane]);
+  if (n + c < e.N)
+    for (int row = st.lane / kCW; row < 32 && m0 + row < e.M; row += 32 / kCW)
+      st.at(row, c) = Cvt<T>::to_f(static_cast<const T*>(e.residual)[(m0 + row) * e.res_stride + n + c]);
   __syncwarp();
   st.get(res);
 }
 template <typename T>
-__device__ __forceinline__ void dense_put_chunk(const DenseEpi& e, const EpiConst& c, const Stage32& st, void* base,
-                                                int64_t m0, int n, int left, const float (&v)[4][8]) {
+__device__ __forceinline__ void dense_put_chunk(const DenseEpi& e, const EpiConst& c, const Stage& st, void* base, int64_t m0,
+                                                int n, int left, const float (&v)[kCR][8]) {
   if (c.vec_out) {
-    dense_put<T, 4>(e, c, base, m0 + (st.lane >> 2), left, n + (st.lane & 3) * 8, v);
+    dense_put<T, kCR>(e, c, base, m0 + st.row(), left, n + st.col(), v);
     return;
   }
+  const int k = st.lane % kCW;
   __syncwarp();
   st.put(v);
   __syncwarp();
-  if (n + st.lane < e.N)
-    for (int row = 0; row < 32 && m0 + row < e.M; ++row)
-      static_cast<T*>(base)[(m0 + row) * e.N + n + st.lane] = Cvt<T>::from_f(st.at(row));
+  if (n + k < e.N)
+    for (int row = st.lane / kCW; row < 32 && m0 + row < e.M; row += 32 / kCW)
+      static_cast<T*>(base)[(m0 + row) * e.N + n + k] = Cvt<T>::from_f(st.at(row, k));
 }
 // The residual of a chunk by plain loads.
 template <typename T>
-__device__ __forceinline__ void dense_get_chunk(const DenseEpi& e, const EpiConst& c, const Stage32& st, int64_t m0, int n,
-                                                int left, float (&res)[4][8]) {
+__device__ __forceinline__ void dense_get_chunk(const DenseEpi& e, const EpiConst& c, const Stage& st, int64_t m0, int n,
+                                                int left, float (&res)[kCR][8]) {
   if (!c.vec_res) {
     dense_stage_rows<T>(e, st, m0, n, res);
     return;
   }
-  const T* p = static_cast<const T*>(e.residual) + (m0 + (st.lane >> 2)) * e.res_stride + n + (st.lane & 3) * 8;
+  const T* p = static_cast<const T*>(e.residual) + (m0 + st.row()) * e.res_stride + n + st.col();
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < kCR; ++q) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) res[q][i] = 0.f;
-    if (q * 8 < left) get8<T>(p, q * 8 * e.res_stride, 8, true, res[q]);
+    if (q * kCStep < left) get8<T>(p, q * kCStep * e.res_stride, 8, true, res[q]);
   }
 }
-// rows of a chunk from m0 that this lane's places reach, times 8; 0 beyond the last column
-__device__ __forceinline__ int dense_left(const DenseEpi& e, int64_t m0, int n, int lane) {
-  return n + (lane & 3) * 8 < e.N ? (int)min(e.M - m0 - (lane >> 2), (int64_t)32) : 0;
+// rows of a chunk from m0, counted from this lane's first; 0 beyond the last column
+__device__ __forceinline__ int dense_left(const DenseEpi& e, int64_t m0, int n, const Stage& st) {
+  return n + st.col() < e.N ? (int)min(e.M - m0 - st.row(), (int64_t)32) : 0;
 }
 
 // ---------------------------------------------------------------- tensor-core pieces
 constexpr int kBK = 64;  // depth of a step
-constexpr int kMmaThreads = 384;
 constexpr int kEpiWarps = 8;
+constexpr int kMmaThreads = 32 * (4 + kEpiWarps);
 // Polls before a wait gives up; a tile takes microseconds, so this is far above any wait that ends.
 constexpr uint32_t kMmaSpin = 1u << 20;
 
@@ -425,12 +437,13 @@ struct Tile {
   static constexpr int kBoxA = 128, kBoxB = 128;                      // rows or columns one CTA loads
   static constexpr int kA = kBoxA * kBK * 2, kB = kBoxB * kBK * 2, kStage = kA + kB;
   static constexpr int kStages = 6;
-  static constexpr int kEpi = kEpiWarps * 4096;  // 32 x 32 fp32 for each epilogue warp
-  static constexpr int kChunks = kN / 64;        // of 32 columns, for an epilogue warp
-  // Two chunks of residual, 32 x 32 bf16 each, in the place of the last stage
-  // (not for fp32, where an item's products take six times as long).
+  static constexpr int kEpi = kEpiWarps * 32 * kCW * 4;  // a chunk of fp32 for each epilogue warp
+  static constexpr int kCols = kN / (kEpiWarps / 4);     // columns of an epilogue warp
+  static constexpr int kChunks = kCols / kCW;
+  // Two chunks of bf16 residual a warp, in the place of the last stage (not for
+  // fp32, where an item's products take six times as long).
   static constexpr int kAhead = sizeof(T) == 2 ? 2 : 0;
-  static_assert(kEpiWarps * kAhead * 2048 <= kStage);
+  static_assert(kEpiWarps * kAhead * 32 * kCW * 2 <= kStage);
   static constexpr int kBytes = kStages * kStage + kEpi + 1024;  // and alignment
 };
 
@@ -600,13 +613,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     }
   } else if (warp >= 4) {
     const EpiConst c(e);
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const Stage32 st = {reinterpret_cast<uint4*>(tiles + S::kStages * S::kStage) + (warp - 4) * 256, lane};
+    const int quarter = warp & 3, col0 = ((warp - 4) >> 2) * S::kCols;
+    const Stage st = {reinterpret_cast<uint4*>(tiles + S::kStages * S::kStage) + (warp - 4) * (8 * kCW), lane};
     // The slices that TMA has asked for keep the SM's way from L2 busy: a plain
     // load issued now is answered some 4000 cycles later, as long as a chunk
     // takes.  So the residual is fetched to shared memory two chunks ahead, each
     // lane its own pieces.
-    uint4* held = reinterpret_cast<uint4*>(tiles + (S::kStages - 1) * S::kStage) + (warp - 4) * 256;
+    uint4* held = reinterpret_cast<uint4*>(tiles + (S::kStages - 1) * S::kStage) + (warp - 4) * (8 * kCW);
     int f_item = first, f_chunk = 0, slot = 0;  // next to fetch; where it goes and the oldest one is
     const T* f_from = nullptr;                  // this lane's first piece of the item
     int f_left = 0, f_n = 0;
@@ -614,20 +627,20 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       if (!ahead) return;
       if (f_item < items) {
         if (f_chunk == 0) {
-          f_n = f_item % w.tiles_n * BN + half * (BN / 2) + (lane & 3) * 8;
-          const int64_t m = (int64_t)(f_item / w.tiles_n % w.tiles_m) * S::kM + rank * 128 + quarter * 32 + (lane >> 2);
+          f_n = f_item % w.tiles_n * BN + col0 + st.col();
+          const int64_t m = (int64_t)(f_item / w.tiles_n % w.tiles_m) * S::kM + rank * 128 + quarter * 32 + st.row();
           f_from = static_cast<const T*>(e.residual) + m * e.res_stride + f_n;
           f_left = (int)min(e.M - m, (int64_t)32);
         }
-        const uint32_t to = smem_u32(held + slot * 128 + lane);
+        const uint32_t to = smem_u32(held + slot * (4 * kCW) + lane);
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (q * 8 < f_left && f_n < e.N)
+        for (int q = 0; q < kCR; ++q)
+          if (q * kCStep < f_left && f_n < e.N)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + q * 512),
-                         "l"(f_from + q * 8 * e.res_stride)
+                         "l"(f_from + q * kCStep * e.res_stride)
                          : "memory");
-        f_from += 32;
-        f_n += 32;
+        f_from += kCW;
+        f_n += kCW;
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
       slot ^= 1;
@@ -641,55 +654,55 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     uint32_t acc_phase = 0;
     for (int item = first; item < items; item += stride) {
       const int rest = item / w.tiles_n, split = rest / w.tiles_m;
-      const int n0 = item % w.tiles_n * BN + half * (BN / 2);
+      const int n0 = item % w.tiles_n * BN + col0;
       const int64_t m0 = (int64_t)(rest % w.tiles_m) * S::kM + rank * 128 + quarter * 32;
       if (!__all_sync(0xffffffffu, wait(&acc_full[acc], acc_phase))) break;
       tmem_fence_after_sync();
-      const uint32_t src = tmem + acc * BN + half * (BN / 2) + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t src = tmem + acc * BN + col0 + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
       for (int chunk = 0; chunk < S::kChunks; ++chunk) {
-        const int j = chunk * 32, n = n0 + j;
+        const int j = chunk * kCW, n = n0 + j;
         if (n >= e.N) {
           fetch();
           continue;
         }
-        // A lane reads 32 columns of its own row of the accumulator; through
-        // shared memory (16-byte pieces, swizzled by row) it gets eight
-        // columns of four rows, so that four lanes cover 32 columns of a row
-        // in global memory and the eight share one dropout counter.
-        uint32_t r[2][16];
-        tmem_ld16(src + j, r[0]);
-        tmem_ld16(src + j + 16, r[1]);
-        const int nl = n + (lane & 3) * 8, left = dense_left(e, m0, n, lane);
+        // A lane reads the columns of its own row of the accumulator; through
+        // shared memory it gets eight columns of a few rows, so that
+        // neighbouring lanes cover a row's columns in global memory and the
+        // eight share one dropout counter.
+        uint32_t r[kCW / 16][16];
+#pragma unroll
+        for (int q = 0; q < kCW / 16; ++q) tmem_ld16(src + j + 16 * q, r[q]);
+        const int nl = n + st.col(), left = dense_left(e, m0, n, st);
         float bias[8];
         dense_bias8(e, c, nl, bias);
         tmem_wait_ld();
         __syncwarp();
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
+        for (int q = 0; q < kCW / 4; ++q)
           st.piece(lane, q) = make_uint4(r[q >> 2][(q & 3) * 4], r[q >> 2][(q & 3) * 4 + 1], r[q >> 2][(q & 3) * 4 + 2],
                                          r[q >> 2][(q & 3) * 4 + 3]);
         __syncwarp();
-        float v[4][8];
+        float v[kCR][8];
         st.get(v);
         if (e.partial) {
-          float* p = e.partial + ((int64_t)split * e.M + m0 + (lane >> 2)) * (e.per_row * 8) + nl;
+          float* p = e.partial + ((int64_t)split * e.M + m0 + st.row()) * (e.per_row * 8) + nl;
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (q * 8 < left) store8(p + (int64_t)(q * 64) * e.per_row, v[q]);
+          for (int q = 0; q < kCR; ++q)
+            if (q * kCStep < left) store8(p + (int64_t)(q * kCStep * 8) * e.per_row, v[q]);
         } else {
-          dense_epilogue<T, 4>(
-              e, c, m0 + (lane >> 2), left, nl, bias, v,
-              [&](float (&res)[4][8]) {
+          dense_epilogue<T, kCR>(
+              e, c, m0 + st.row(), left, nl, bias, v,
+              [&](float (&res)[kCR][8]) {
                 if (ahead) {
                   asm volatile("cp.async.wait_group 1;" ::: "memory");
 #pragma unroll
-                  for (int q = 0; q < 4; ++q) unpack8(held[slot * 128 + q * 32 + lane], res[q]);
+                  for (int q = 0; q < kCR; ++q) unpack8(held[slot * (4 * kCW) + q * 32 + lane], res[q]);
                 } else {
                   dense_get_chunk<T>(e, c, st, m0, n, left, res);
                 }
               },
-              [&](void* base, const float (&u)[4][8]) { dense_put_chunk<T>(e, c, st, base, m0, n, left, u); });
+              [&](void* base, const float (&u)[kCR][8]) { dense_put_chunk<T>(e, c, st, base, m0, n, left, u); });
           fetch();
         }
       }
@@ -715,35 +728,35 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 }
 
 // The epilogue of a product whose K loop was cut: the parts summed in order, a
-// 32 x 32 chunk a warp.
+// chunk a warp.
 constexpr int kJoinWarps = 4;
 template <typename T>
 __global__ void __launch_bounds__(32 * kJoinWarps)
     dense_join_kernel(const float* part, int splits, const __grid_constant__ DenseEpi e) {
-  __shared__ uint4 staged[kJoinWarps][256];
+  __shared__ uint4 staged[kJoinWarps][8 * kCW];
   const EpiConst c(e);
-  const Stage32 st = {staged[threadIdx.x >> 5], (int)threadIdx.x & 31};
-  const int64_t ld = (int64_t)e.per_row * 8, chunks_n = (e.N + 31) / 32;
+  const Stage st = {staged[threadIdx.x >> 5], (int)threadIdx.x & 31};
+  const int64_t ld = (int64_t)e.per_row * 8, chunks_n = (e.N + kCW - 1) / kCW;
   const int64_t i = (int64_t)blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
   const int64_t m0 = i / chunks_n * 32;
-  const int n = (int)(i % chunks_n) * 32, nl = n + (st.lane & 3) * 8;
+  const int n = (int)(i % chunks_n) * kCW, nl = n + st.col();
   if (m0 >= e.M) return;
-  const int left = dense_left(e, m0, n, st.lane);
-  float v[4][8] = {}, bias[8];
+  const int left = dense_left(e, m0, n, st);
+  float v[kCR][8] = {}, bias[8];
   for (int s = 0; s < splits; ++s) {
-    const float* p = part + ((int64_t)s * e.M + m0 + (st.lane >> 2)) * ld + nl;
+    const float* p = part + ((int64_t)s * e.M + m0 + st.row()) * ld + nl;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < kCR; ++q) {
       float t[8] = {};
-      if (q * 8 < left) load8(p + q * 8 * ld, t);
+      if (q * kCStep < left) load8(p + q * kCStep * ld, t);
       add8(v[q], t);
     }
   }
   dense_bias8(e, c, nl, bias);
-  dense_epilogue<T, 4>(
-      e, c, m0 + (st.lane >> 2), left, nl, bias, v,
-      [&](float (&res)[4][8]) { dense_get_chunk<T>(e, c, st, m0, n, left, res); },
-      [&](void* base, const float (&u)[4][8]) { dense_put_chunk<T>(e, c, st, base, m0, n, left, u); });
+  dense_epilogue<T, kCR>(
+      e, c, m0 + st.row(), left, nl, bias, v,
+      [&](float (&res)[kCR][8]) { dense_get_chunk<T>(e, c, st, m0, n, left, res); },
+      [&](void* base, const float (&u)[kCR][8]) { dense_put_chunk<T>(e, c, st, base, m0, n, left, u); });
 }
 
 }  // namespace ssm
