@@ -90,7 +90,7 @@ def _stream_of(t):
 
 
 def _workspace(nbytes, t):
-    return torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
+    return t.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def _residual_of(residual, shape, dtype):
@@ -113,7 +113,7 @@ def _records(*tensors):
 
 # ----------------------------------------------------------------------------- dropout
 def _dropout_forward(x, residual, drop, rng, act):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     if not x.numel():
         return y
     x, xs = _rows_of(x)
@@ -139,7 +139,7 @@ class _DropoutActFn(torch.autograd.Function):
         drop, rng, act = ctx.cfg
         dx = None
         if ctx.needs_input_grad[0]:
-            dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+            dx = dy.new_empty(dy.shape)
             if dx.numel():
                 d, ds = _rows_of(dy)
                 x, xs = _rows_of(x) if act else (None, 0)
@@ -179,8 +179,8 @@ def _gn_params(x, scale, bias, y, stats, groups, eps, act):
 
 def _group_norm_forward(x, scale, bias, groups, eps, act):
     """y and the statistics; x, scale and bias are dense, the latter float32."""
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
+    y = x.new_empty(x.shape)
+    stats = x.new_empty((x.shape[0], groups, 2), dtype=torch.float32)
     if x.numel():
         p = _gn_params(x, scale, bias, y, stats, groups, eps, act)
         lib, ref = _lib.load(), ctypes_byref(p)
@@ -207,8 +207,8 @@ class _GroupNormActFn(torch.autograd.Function):
         groups, eps, act = ctx.cfg
         dim = x.shape[-1]
         dy = _dense(dy)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        sums = torch.empty((2, dim), dtype=torch.float32, device=x.device)
+        dx = x.new_empty(x.shape)
+        sums = x.new_empty((2, dim), dtype=torch.float32)
         p = _gn_params(x, scale, bias, None, stats, groups, eps, act)
         p.dy, p.dx, p.dscale, p.dbias = dy.data_ptr(), dx.data_ptr(), sums.data_ptr(), sums.data_ptr() + 4 * dim
         lib, ref = _lib.load(), ctypes_byref(p)
@@ -254,8 +254,8 @@ def _dense_params(x, xs, w, b, drop, rng, act):
 def _dense_forward(x, w, bias, residual, act, drop, rng, keep_pre):
     """y and, with keep_pre, the activation's input; w and bias are dense, w of x's type."""
     shape = (*x.shape[:-1], w.shape[1])
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    pre = torch.empty(shape, dtype=x.dtype, device=x.device) if keep_pre else None
+    y = x.new_empty(shape)
+    pre = x.new_empty(shape) if keep_pre else None
     if y.numel():
         x, xs = _rows_of(x)
         p = _dense_params(x, xs, w, bias, drop, rng, act)
@@ -297,8 +297,8 @@ class _DenseActFn(torch.autograd.Function):
         p = _dense_params(xc, xs, w, bias, drop, (*rng, rng_t), act)
         p.pre, p.dy, p.dy_stride = _ptr(pre), d.data_ptr(), ds
         p.dkernel_dtype = _DT[kdtype]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
-        dw = torch.empty(w.shape, dtype=kdtype, device=x.device) if ctx.needs_input_grad[1] else None
+        dx = x.new_empty(x.shape) if ctx.needs_input_grad[0] else None
+        dw = w.new_empty(w.shape, dtype=kdtype) if ctx.needs_input_grad[1] else None
         db = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
         p.dx, p.dkernel, p.dbias = _ptr(dx), _ptr(dw), _ptr(db)
         lib, ref = _lib.load(), ctypes_byref(p)

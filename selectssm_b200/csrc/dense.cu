@@ -54,19 +54,57 @@ __device__ __forceinline__ void store_planes(__nv_bfloat16* dst, int64_t plane, 
   }
 }
 
-// (rows, cols) at row stride `stride` to planes of row length ld, a multiple of
-// 8; columns beyond cols become zeros.  Eight columns a thread.
+// What has to be ready before the products, in one launch (a small call's time is
+// its launches'): up to two operands as planes, and dbias from its runs' sums.
+struct Pack {  // (rows, cols) at row stride `stride` to planes of row length ld, a multiple of 8; zeros beyond cols
+  const void* src;
+  __nv_bfloat16* dst;
+  int64_t stride, rows;
+  int cols, ld;
+  bool vec;
+};
+struct Ready {
+  Pack pack[2];
+  int64_t blocks[2];  // CTAs of each, 0 where it is read in place
+  const float* sums;  // (parts, n)
+  int parts, n;
+  void* dbias;
+  bool dbias_bf16;
+  int64_t all() const { return blocks[0] + blocks[1] + (dbias ? (n + 7) / 8 : 0); }
+};
+
 template <typename T, int PLANES>
-__global__ void __launch_bounds__(256) dense_pack_kernel(const T* src, int64_t stride, int64_t rows, int cols, int ld,
-                                                         __nv_bfloat16* dst, bool vec) {
-  const int per = ld / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * per) return;
-  const int64_t r = i / per;
-  const int c = (int)(i - r * per) * 8;
-  float v[8];
-  get8<T>(src, r * stride + c, cols - c, vec && c + 8 <= cols, v);
-  store_planes<PLANES>(dst + r * ld + c, rows * ld, v);
+__global__ void __launch_bounds__(256) dense_ready_kernel(const __grid_constant__ Ready g) {
+  int64_t blk = blockIdx.x;
+  if (blk < g.blocks[0] + g.blocks[1]) {  // eight columns a thread
+    const Pack& o = g.pack[blk >= g.blocks[0]];
+    if (blk >= g.blocks[0]) blk -= g.blocks[0];
+    const int per = o.ld / 8;
+    const int64_t i = blk * 256 + threadIdx.x;
+    if (i >= o.rows * per) return;
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * 8;
+    float v[8];
+    get8<T>(static_cast<const T*>(o.src), r * o.stride + c, o.cols - c, o.vec && c + 8 <= o.cols, v);
+    store_planes<PLANES>(o.dst + r * o.ld + c, o.rows * o.ld, v);
+    return;
+  }
+  blk -= g.blocks[0] + g.blocks[1];
+  __shared__ float red[32][9];  // eight columns a CTA, 32 threads a column, in a fixed order
+  const int col = threadIdx.x & 7, lane = threadIdx.x >> 3, n = (int)blk * 8 + col;
+  float s = 0.f;
+  if (n < g.n)
+#pragma unroll 4
+    for (int i = lane; i < g.parts; i += 32) s += g.sums[(int64_t)i * g.n + n];
+  red[lane][col] = s;
+  __syncthreads();
+  if (lane == 0 && n < g.n) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t += red[i][col];
+    if (g.dbias_bf16) static_cast<__nv_bfloat16*>(g.dbias)[n] = __float2bfloat16_rn(t);
+    else static_cast<float*>(g.dbias)[n] = t;
+  }
 }
 
 template <typename T>
@@ -153,24 +191,6 @@ __global__ void __launch_bounds__(256, 3)
   }
 }
 
-// dbias: the runs' sums in a fixed order, 32 lanes a column
-__global__ void __launch_bounds__(1024) dense_dbias_kernel(const float* part, int parts, int N, void* dbias, int dtype) {
-  __shared__ float red[32][33];
-  const int col = threadIdx.x & 31, lane = threadIdx.x >> 5, n = blockIdx.x * 32 + col;
-  float s = 0.f;
-  if (n < N)
-    for (int i = lane; i < parts; i += 32) s += part[(int64_t)i * N + n];
-  red[lane][col] = s;
-  __syncthreads();
-  if (lane == 0 && n < N) {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) t += red[i][col];
-    if (dtype == SSM_BF16) static_cast<__nv_bfloat16*>(dbias)[n] = __float2bfloat16_rn(t);
-    else static_cast<float*>(dbias)[n] = t;
-  }
-}
-
 // ---------------------------------------------------------------- checks and sizes
 static bool known(int dtype) { return dtype == SSM_F32 || dtype == SSM_BF16; }
 
@@ -218,27 +238,23 @@ static Operand kernel_operand(const ssm_dense_params_t* p) {
   return {p->kernel, p->fout, p->fin, p->fout, p->dtype == SSM_BF16};
 }
 
-// The planes of an operand, packed into `*ws` (advanced) where it cannot be read in place.
-static int planes(const Operand& o, bool k_major, char** ws, cudaStream_t s, Planes* out) {
-  out->k_major = k_major;
-  if (o.direct()) {
-    *out = {static_cast<const __nv_bfloat16*>(o.src), 0, o.stride, k_major};
-    return SSM_OK;
-  }
+// The planes of an operand: read in place, or packed into `ws` by pack `slot` of `ready`.
+static Planes planes(const Operand& o, bool k_major, char* ws, Ready* ready, int slot) {
+  if (o.direct()) return {static_cast<const __nv_bfloat16*>(o.src), 0, o.stride, k_major};
   const int ld = pad8(o.cols);
-  __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(*ws);
-  *ws += o.bytes();
-  *out = {dst, o.rows * ld, ld, k_major};
-  const int64_t grid = ceil_div(o.rows * (ld / 8), 256);
+  __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(ws);
+  ready->pack[slot] = {o.src, dst, o.stride, o.rows, o.cols, ld, aligned16(o.src) && o.stride % (o.bf16 ? 8 : 4) == 0};
+  ready->blocks[slot] = ceil_div(o.rows * (ld / 8), 256);
+  return {dst, o.rows * ld, ld, k_major};
+}
+
+static int launch_ready(const Ready& g, bool bf16, cudaStream_t s) {
+  const int64_t grid = g.all();
+  if (grid == 0) return SSM_OK;
   if (grid > 0x7fffffff) return SSM_ERR_SHAPE;
-  const bool vec = aligned16(o.src) && o.stride % (o.bf16 ? 8 : 4) == 0;
-  if (o.bf16)
-    dense_pack_kernel<__nv_bfloat16, 1><<<(unsigned)grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(o.src), o.stride,
-                                                                      o.rows, o.cols, ld, dst, vec);
-  else
-    dense_pack_kernel<float, 3><<<(unsigned)grid, 256, 0, s>>>(static_cast<const float*>(o.src), o.stride, o.rows, o.cols,
-                                                               ld, dst, vec);
-  return launched("launch dense pack kernel", 1);
+  if (bf16) dense_ready_kernel<__nv_bfloat16, 1><<<(unsigned)grid, 256, 0, s>>>(g);
+  else dense_ready_kernel<float, 3><<<(unsigned)grid, 256, 0, s>>>(g);
+  return launched("launch dense ready kernel", 1);
 }
 
 // ---------------------------------------------------------------- one product
@@ -391,9 +407,12 @@ static int dense_fwd(const ssm_dense_params_t* p, cudaStream_t s) {
   int st = SSM_OK;
   const bool few = few_rows(p);
   if (!few) {
-    st = planes(x_operand(p), true, &ws, s, &e.a);
-    if (st) return st;
-    st = planes(kernel_operand(p), false, &ws, s, &e.b);
+    const Operand x = x_operand(p), w = kernel_operand(p);
+    Ready ready = {};
+    e.a = planes(x, true, ws, &ready, 0);
+    e.b = planes(w, false, ws + x.bytes(), &ready, 1);
+    ws += x.bytes() + w.bytes();
+    st = launch_ready(ready, p->dtype == SSM_BF16, s);
     if (st) return st;
   }
   e.M = p->rows;
@@ -494,40 +513,43 @@ static int dense_bwd(const ssm_dense_params_t* p, cudaStream_t s) {
     st = pl == 1 ? launch_dpre<__nv_bfloat16, 1>(p, same ? nullptr : dpre, p->dbias ? sums : nullptr, s)
                  : launch_dpre<float, 3>(p, dpre, p->dbias ? sums : nullptr, s);
   if (st) return st;
+  Ready ready = {};
   if (p->dbias) {
-    dense_dbias_kernel<<<(unsigned)ceil_div(N, 32), 1024, 0, s>>>(sums, dpre_geom(p).parts, N, p->dbias, p->bias_dtype);
-    st = launched("launch dense dbias kernel", 1);
-    if (st) return st;
+    ready.sums = sums;
+    ready.parts = dpre_geom(p).parts;
+    ready.n = N;
+    ready.dbias = p->dbias;
+    ready.dbias_bf16 = p->bias_dtype == SSM_BF16;
   }
+  Planes x = {}, kernel = {};
+  if (p->dkernel) x = planes(x_operand(p), false, ws, &ready, 0);
+  if (p->dx) kernel = planes(kernel_operand(p), true, ws + bytes.x, &ready, 1);
+  st = launch_ready(ready, p->dtype == SSM_BF16, s);
+  if (st) return st;
   const Planes d = same ? Planes{static_cast<const __nv_bfloat16*>(p->dy), 0, stride_or(p->dy_stride, N), true}
                         : Planes{dpre, p->rows * ld, ld, true};
+  float* part = reinterpret_cast<float*>(ws + bytes.x + bytes.kernel);
   DenseEpi e = {};
   e.planes = pl;
   if (p->dx) {  // (rows, fout) (fin, fout)^T
-    char* w = ws + bytes.x;
     e.a = d;
-    st = planes(kernel_operand(p), true, &w, s, &e.b);
-    if (st) return st;
+    e.b = kernel;
     e.M = p->rows;
     e.N = K;
     e.K = N;
     e.out = p->dx;
-    float* part = reinterpret_cast<float*>(w);
     st = p->dtype == SSM_BF16 ? product<false, false, __nv_bfloat16>(e, part, p->status, s)
                               : product<false, false, float>(e, part, p->status, s);
     if (st) return st;
   }
   if (p->dkernel) {  // (rows, fin)^T (rows, fout)
-    char* w = ws;
-    st = planes(x_operand(p), false, &w, s, &e.a);
-    if (st) return st;
+    e.a = x;
     e.b = d;
     e.b.k_major = false;
     e.M = K;
     e.N = N;
     e.K = p->rows;
     e.out = p->dkernel;
-    float* part = reinterpret_cast<float*>(ws + bytes.x + bytes.kernel);
     st = p->dkernel_dtype == SSM_BF16 ? product<true, true, __nv_bfloat16>(e, part, p->status, s)
                                       : product<true, true, float>(e, part, p->status, s);
   }

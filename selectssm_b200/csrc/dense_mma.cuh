@@ -103,7 +103,7 @@ __device__ __forceinline__ void act_rows(float (&v)[R][8]) {
 
 __device__ __noinline__ float dense_again(const DenseEpi& e, int64_t m, int n) {
   float s = 0.f;
-  for (int64_t k = 0; k < e.K; ++k) s = fmaf(e.a.at(m, k), e.b.at(n, k), s);
+  for (int64_t k = 0; k < e.K && !isnan(s); ++k) s = fmaf(e.a.at(m, k), e.b.at(n, k), s);
   return s;
 }
 

@@ -424,6 +424,39 @@ def test_dense_dropped_infinities_leave_no_trace(cuda):
     assert bool(torch.isfinite(y).all()) and bool((y[0][~keep] == 0).all())
 
 
+@pytest.mark.parametrize("sizes", [(3, 96, 72), (200, 700, 130), (300, 96, 257), (700, 333, 64)])
+def test_dense_fp32_infinities_and_the_largest_values(cuda, sizes):
+    """An infinite operand makes what it makes in fp32 arithmetic, in each of the
+    three products, and leaves the other rows and columns alone; values next to
+    the type's largest keep fp32 accuracy."""
+    from selectssm_b200 import dense_act
+    M, K, N = sizes
+    inf = float("inf")
+    torch.manual_seed(12)
+    x = torch.randn(M, K, device=cuda)
+    w = torch.randn(K, N, device=cuda) / K ** 0.5
+    dy = torch.randn(M, N, device=cuda)
+    x[0, 5], x[1, K - 1], x[2, 17] = inf, -inf, 3.0e38
+    w[5, 3] = 0.0  # infinity times nothing is NaN
+    dy[1, 2] = inf
+    dy[2] *= 0.125  # (products with 3e38 stay finite)
+    x.requires_grad_(), w.requires_grad_()
+    y = dense_act(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    x64, w64, d64 = (t.detach().double() for t in (x, w, dy))
+    for name, got, a, b in (("y", y.detach(), x64, w64), ("dx", dx, d64, w64.t()), ("dw", dw, x64.t(), d64)):
+        want = (a @ b)
+        clean = torch.isfinite(a).all(1)[:, None] & torch.isfinite(b).all(0)[None, :]
+        # (inf * finite summed by hand: a 64-bit product may order its sums either way, its class is the same)
+        assert torch.equal(torch.isnan(got)[~clean], torch.isnan(want)[~clean]), name
+        odd = ~clean & ~torch.isnan(want)
+        assert torch.equal(got[odd].double(), want[odd]), name
+        # additions to the tensor core's accumulator are cut at 2^-23 of it, 32 in a row, and a
+        # few roundings more; the planes leave 3 * 2^-24 of a product out
+        bound = 40 * 2.0 ** -23 * (a.abs() @ b.abs())
+        assert_within(got[clean], want[clean], bound[clean], name)
+
+
 def test_no_rows(cuda):
     from selectssm_b200 import dense_act, dropout_act, group_norm_act
     x = torch.empty(0, 16, device=cuda, requires_grad=True)
