@@ -315,7 +315,9 @@ typedef struct ssm_dense_params {
   void* dx;
   void* dkernel;
   void* dbias;
-  void* workspace;                      /* 256-byte aligned; the queries below give its bytes */
+  void* workspace;                      /* 256-byte aligned; the queries below give its bytes, and
+                                           read the other fields, pointers included (NULL counts
+                                           as aligned)                                     */
   size_t workspace_bytes;
   int32_t* status;                      /* optional device word: nonzero after a device-side
                                            failure (bounded wait gave up)                 */

@@ -56,6 +56,8 @@ __device__ __forceinline__ void store_planes(__nv_bfloat16* dst, int64_t plane, 
 
 // What has to be ready before the products, in one launch (a small call's time is
 // its launches'): up to two operands as planes, and dbias from its runs' sums.
+// (300 x 500) @ (500 x 400), fp32, forward and backward: 150 us of the host's time,
+// 163 with a launch for each.
 struct Pack {  // (rows, cols) at row stride `stride` to planes of row length ld, a multiple of 8; zeros beyond cols
   const void* src;
   __nv_bfloat16* dst;
@@ -113,8 +115,9 @@ constexpr int kDpreRows = sizeof(T) == 2 ? 4 : 2;
 // dpre as planes for the two products that follow, and the column sums of its
 // unrounded values over a run of rows.  A thread keeps eight columns (one
 // dropout counter each row) and takes ROWS rows at a time, whose loads it issues
-// together: the pass is bound by memory, and a loop that loads, computes and
-// stores row by row left it at half the rate.
+// together: a loop that loads, computes and stores row by row ran at half the
+// rate.  32768 x 1536 bf16, silu, dropout, dbias, cold: 70 us for 302 MB, 4.3 TB/s,
+// issue on 54% of cycles at 80 registers; HBM alone would take 46.
 template <typename T, int PLANES, bool WRITE, int ACT>
 __global__ void __launch_bounds__(256, 3)
     dense_dpre_kernel(const T* dy, int64_t dy_stride, const T* pre, __nv_bfloat16* dpre, int ld, float* part, int64_t M,

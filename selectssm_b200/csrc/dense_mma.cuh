@@ -11,6 +11,14 @@
 // swizzle), warp 1 issues the products, and warps 4 to 11 read the finished
 // accumulator from tensor memory, apply the epilogue and store; two
 // accumulators let the epilogue of one tile overlap the products of the next.
+//
+// Measured in bf16.  131072 x 1536 x 768, residual and dropout: 240 us, 1.29
+// PFLOP/s; without the epilogue 197 us, 1.57 PFLOP/s, the rate of a plain library
+// product at these sizes (203 us), with the clock held down by the power limit.
+// 32768 x 768 x 1536, silu, dropout and `pre`: 115 us, where the epilogue's issue is
+// the bound (the tensor cores work 32% of the time), and its two gradients 57 and 55
+// us, 1.35 and 1.4 PFLOP/s (68 and 70%).  In fp32 2042 x 515 x 1001, forward and
+// both gradients: 23 to 26 us each, 0.55 PFLOP/s of bf16 products.
 #pragma once
 
 #include <cstdint>
@@ -728,7 +736,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 }
 
 // The epilogue of a product whose K loop was cut: the parts summed in order, a
-// chunk a warp.
+// chunk a warp.  768 x 1536 of 4 parts (19 MB, mostly in L2): 6 us.
 constexpr int kJoinWarps = 4;
 template <typename T>
 __global__ void __launch_bounds__(32 * kJoinWarps)
