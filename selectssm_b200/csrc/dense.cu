@@ -271,32 +271,24 @@ struct Plan {
 
 // Tile (128 x 128 by one CTA, 256 x 256 by a pair) and cuts of the K loop: the
 // choice with the least estimated time.  The terms are measured: a 64-deep step
-// takes about 0.3 us of a single CTA's and 0.38 of a pair's, an item about 3 us
-// around its steps, and joining cut products a launch and their partials' way
-// through memory.
-//
-// The tensor cores cut, not round, what an addition to the accumulator cannot
-// hold, so an error grows with the number of additions.  For fp32 operands the K
-// loop is therefore cut at 512: partial sums of 32 additions each are then added
-// in rounded fp32 (a sum of 2042 products is good to 6e-7 so, 2.4e-6 without).
+// takes about 0.3 us of a single CTA's and 0.38 of a pair's, all six products of
+// three planes 1.2 us, an item about 3 us around its steps, and joining cut
+// products a launch and their partials' way through memory.
 static Plan plan_product(int64_t M, int64_t N, int64_t K, int planes) {
   Plan best = {};
   double least = 0;
-  for (int pair = 0; pair < 2; ++pair) {
+  for (int pair = 0; pair < (planes == 3 ? 1 : 2); ++pair) {
+    const double step = planes == 3 ? 1.2 : pair ? 0.38 : 0.3;
     DenseWork w;
     w.tiles_m = (int)ceil_div(M, pair ? Tile<true, float>::kM : Tile<false, float>::kM);
     w.tiles_n = (int)ceil_div(N, pair ? Tile<true, float>::kN : Tile<false, float>::kN);
     w.kblocks = (int)ceil_div(K, kBK);
-    w.pairs = planes == 3 ? 6 : 1;
     const int64_t tiles = (int64_t)w.tiles_m * w.tiles_n, teams = pair ? kSms / 2 : kSms;
-    // (in at most 1 GB of partial sums)
-    const int64_t room = std::max<int64_t>(1, ((int64_t)1 << 28) / (M * pad8((int)N)));
-    const int fewest = planes == 3 ? (int)std::min<int64_t>(ceil_div(w.kblocks, 8), room) : 1;
-    for (w.splits = fewest; w.splits == fewest || (w.splits * tiles <= 2 * teams &&
-                                                   w.splits * 4 <= w.kblocks * w.pairs && w.splits <= w.kblocks);
+    for (w.splits = 1; w.splits == 1 || (w.splits * tiles <= 2 * teams && w.splits <= w.kblocks &&
+                                         (planes == 3 || w.splits * 4 <= w.kblocks));
          ++w.splits) {
       const double rounds = (double)ceil_div(tiles * w.splits, teams);
-      double us = rounds * (ceil_div(w.kblocks, w.splits) * w.pairs * (pair ? 0.38 : 0.3) + 3);
+      double us = rounds * (ceil_div(w.kblocks, w.splits) * step + 3);
       if (w.splits > 1) us += 4.0 + 2.0 * w.splits * (double)M * N * 4 / 5e6;
       if (least == 0 || us < least) {
         best.pair = pair;
@@ -315,10 +307,10 @@ static bool operand_map(CUtensorMap* m, const Planes& o, int64_t rows, int64_t c
                   o.k_major ? 128 : kBK, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <bool A_MN, bool B_MN, bool PAIR, typename T>
+template <bool A_MN, bool B_MN, bool PAIR, int PLANES, typename T>
 static int launch_mma(const DenseEpi& e, const Plan& q, const CUtensorMap& ma, const CUtensorMap& mb, int32_t* status,
                       cudaStream_t s) {
-  const auto kernel = dense_mma_kernel<A_MN, B_MN, PAIR, T>;
+  const auto kernel = dense_mma_kernel<A_MN, B_MN, PAIR, PLANES, T>;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<PAIR, T>::kBytes);
   if (err != cudaSuccess) return launch_error("cudaFuncSetAttribute(dense)", err);
   const int items = q.w.tiles_m * q.w.tiles_n * q.w.splits;
@@ -353,8 +345,15 @@ static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
     first.partial = part;
     first.residual = first.bias = nullptr;
   }
-  int st = q.pair ? launch_mma<A_MN, B_MN, true, T>(first, q, ma, mb, status, s)
-                  : launch_mma<A_MN, B_MN, false, T>(first, q, ma, mb, status, s);
+  // only a kernel's gradient has another type than the operands
+  constexpr bool kAny = A_MN && B_MN;
+  int st = SSM_ERR_DTYPE;
+  if constexpr (sizeof(T) == 4 || kAny)
+    if (e.planes == 3) st = launch_mma<A_MN, B_MN, false, 3, T>(first, q, ma, mb, status, s);
+  if constexpr (sizeof(T) == 2 || kAny)
+    if (e.planes == 1)
+      st = q.pair ? launch_mma<A_MN, B_MN, true, 1, T>(first, q, ma, mb, status, s)
+                  : launch_mma<A_MN, B_MN, false, 1, T>(first, q, ma, mb, status, s);
   if (st || q.w.splits == 1) return st;
   const int64_t grid = ceil_div(ceil_div(e.M, 32) * ceil_div(e.N, kCW), kJoinWarps);
   if (grid > 0x7fffffff) return SSM_ERR_SHAPE;

@@ -3,8 +3,14 @@
 // A is (M, K), B is (K, N), each as one bf16 plane or, for fp32 operands, as
 // three whose sum is the fp32 value exactly (8 + 8 + 8 significant bits).  The
 // product of two such sums is formed from the six plane pairs of weight above
-// 2^-24, smallest first, so the accumulator is small while the corrections go
-// in and only the last K / 16 steps round at the size of the result.
+// 2^-24: the leading planes' in one accumulator, the other five, 2^-8 of it and
+// less, in another.
+//
+// The tensor core cuts, not rounds, what an addition to an accumulator cannot
+// hold, so an error grows with the number of additions.  For fp32 operands the
+// leading accumulator therefore starts afresh every 512 of K (32 additions) and
+// the other every 4096, and what they held is added in rounded fp32 to a sum that
+// stays in tensor memory: a sum of 2042 products is good to 6e-7 so, 2.4e-6 without.
 //
 // A persistent CTA walks over items (tile of 128 x BN, part of the K loop).
 // Warps 0 and 3 move 64-deep slices of A and of B to shared memory by TMA (128-byte
@@ -131,11 +137,11 @@ __device__ __forceinline__ void dense_bias8(const DenseEpi& e, const EpiConst& c
 // instructions of this function are what an epilogue costs: issued beside the
 // warp that starts the tensor core's products, they delay it one for one.
 // get_res() gives the residual's values, put(base, v) stores to `pre` or `out`.
-template <typename T, int R, typename RES, typename PUT>
+template <typename T, int R, bool PLANES3, typename RES, typename PUT>
 __device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst& c, int64_t row, int left, int n,
                                                const float (&bias)[8], float (&v)[R][8], RES get_res, PUT put) {
   constexpr int RS = 32 / R;
-  if (sizeof(T) == 4 && e.planes == 3) {
+  if (PLANES3 && e.planes == 3) {
     // An infinite operand has no finite planes besides its first, and infinity
     // times the other operand's planes gives NaN where the product is infinite.
     // Such elements are summed again from the fp32 values.
@@ -430,8 +436,7 @@ __device__ __forceinline__ void wait_through(uint64_t* bar, uint32_t parity, uin
 struct DenseWork {
   int32_t tiles_m, tiles_n, splits;
   int32_t kblocks;  // ceil(K / 64)
-  int32_t pairs;    // plane pairs: 1 or 6
-  // the 64-deep blocks of a split: each runs through all plane pairs
+  // the 64-deep blocks of a split
   __device__ __forceinline__ int block(int split) const { return (int)((int64_t)kblocks * split / splits); }
 };
 
@@ -439,6 +444,11 @@ struct DenseWork {
 // of it holds 128 rows of A and 128 columns of B and accumulates its 128 rows
 // of all 256 columns, so a step moves 32 KB into each SM for twice the products
 // that 32 KB give a single CTA.
+//
+// Three planes take a CTA of its own.  A block's planes are loaded once, one of A
+// and one of B a stage, and its six products made from three stages: 16 KB a
+// product (32 when each product had its own stage, and its time was L2's).  Tensor
+// memory holds two leading accumulators in turn, the other one and the sum.
 template <bool PAIR, typename T>
 struct Tile {
   static constexpr int kM = PAIR ? 256 : 128, kN = PAIR ? 256 : 128;  // of the item
@@ -455,23 +465,23 @@ struct Tile {
   static constexpr int kBytes = kStages * kStage + kEpi + 1024;  // and alignment
 };
 
-// plane pairs (of A, of B), smallest products first
-__device__ __forceinline__ void plane_pair(int planes, int seg, int& pa, int& pb) {
-  if (planes == 1) {
-    pa = pb = 0;
-    return;
-  }
-  pa = 0x001012 >> (4 * seg) & 15;  // 2 1 0 1 0 0
-  pb = 0x010210 >> (4 * seg) & 15;  // 0 1 2 0 1 0
+constexpr int kCut = 512 / kBK;  // most blocks that the leading accumulator of three planes takes
+constexpr int kCutsOfRest = 8;   // cuts that the other one takes
+// cuts of a split as even as they go
+__device__ __forceinline__ int even_cut(int blocks) {
+  const int cuts = (blocks + kCut - 1) / kCut;
+  return (blocks + cuts - 1) / cuts;
 }
 
-template <bool A_MN, bool B_MN, bool PAIR, typename T>
+template <bool A_MN, bool B_MN, bool PAIR, int PLANES, typename T>
 __global__ void __launch_bounds__(kMmaThreads, 1)
     dense_mma_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                      const __grid_constant__ DenseEpi e, const DenseWork w, int32_t* status) {
   using S = Tile<PAIR, T>;
   using I = Mma<PAIR>;
   constexpr int BN = S::kN;
+  static_assert(PLANES == 1 || (PLANES == 3 && !PAIR && S::kStages % 3 == 0));
+  constexpr int kTmem = PLANES == 3 ? 4 * BN : 2 * BN;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base;
@@ -495,13 +505,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   }
   __syncthreads();
   if constexpr (PAIR) cluster_barrier();
-  if (warp == 2) I::alloc(&tmem_base, 2 * BN);
+  if (warp == 2) I::alloc(&tmem_base, kTmem);
   tmem_fence_before_sync();
   __syncthreads();
   tmem_fence_after_sync();
   const uint32_t tmem = tmem_base;
   const int items = w.tiles_m * w.tiles_n * w.splits;
-  const bool ahead = S::kAhead && e.residual && EpiConst(e).vec_res;
+  const bool ahead = PLANES == 1 && S::kAhead && e.residual && EpiConst(e).vec_res;
   const int stages = ahead ? S::kStages - 1 : S::kStages;
   const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
 
@@ -533,9 +543,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const int n0 = item % w.tiles_n * BN + (PAIR ? rank * 128 : 0);
       const int m0 = rest % w.tiles_m * S::kM + (PAIR ? rank * 128 : 0);
       const int kb0 = w.block(split), kb1 = w.block(split + 1);
-      int seg = 0, kb = kb0, pa, pb;
-      plane_pair(e.planes, seg, pa, pb);
-      for (int t = (kb1 - kb0) * w.pairs; t > 0; --t) {
+      // three planes in the order 1 0 2, in which their products need them
+      int plane = PLANES == 3 ? 1 : 0, kb = kb0;
+      for (int t = (kb1 - kb0) * PLANES; t > 0; --t) {
         wait_through(&empty[stage], phase ^ 1, polls);
         if (polls == 1) break;  // what it would overwrite may still be read
         const int k0 = kb * kBK;
@@ -546,19 +556,21 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           if (rank == 0) expect_bytes(&full[stage], PAIR ? 2 * S::kStage : S::kStage, one);
           if (A_MN) {
 #pragma unroll
-            for (int j = 0; j < S::kBoxA / 64; ++j) I::load(sa + j * 8192, &map_a, bar, m0 + 64 * j, k0, pa, one);
+            for (int j = 0; j < S::kBoxA / 64; ++j) I::load(sa + j * 8192, &map_a, bar, m0 + 64 * j, k0, plane, one);
           } else {
-            I::load(sa, &map_a, bar, k0, m0, pa, one);
+            I::load(sa, &map_a, bar, k0, m0, plane, one);
           }
         } else if (B_MN) {
 #pragma unroll
-          for (int j = 0; j < S::kBoxB / 64; ++j) I::load(sb + j * 8192, &map_b, bar, n0 + 64 * j, k0, pb, one);
+          for (int j = 0; j < S::kBoxB / 64; ++j) I::load(sb + j * 8192, &map_b, bar, n0 + 64 * j, k0, plane, one);
         } else {
-          I::load(sb, &map_b, bar, k0, n0, pb, one);
+          I::load(sb, &map_b, bar, k0, n0, plane, one);
         }
-        if (++kb == kb1) {
-          kb = kb0;
-          plane_pair(e.planes, ++seg, pa, pb);
+        if (PLANES == 3) {
+          kb += plane == 2;
+          plane = plane == 2 ? 1 : plane == 1 ? 0 : 2;
+        } else {
+          ++kb;
         }
         if (++stage == stages) {
           stage = 0;
@@ -588,30 +600,75 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     const uint64_t da0 = smem_desc(smem_u32(tiles)), db0 = smem_desc(smem_u32(tiles + S::kA));
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0, polls = kMmaSpin;
+    // the four products of one plane of A with one of B, from stages sa and sb
+    const auto block = [&](uint32_t d, int sa, int sb, bool add) {
+      const uint64_t da = da0 + sa * (S::kStage >> 4), db = db0 + sb * (S::kStage >> 4);
+#pragma unroll
+      for (int k = 0; k < kBK / 16; ++k) I::mma(d, da + k * kStepA, db + k * kStepB, idesc, add || k > 0, one);
+    };
     for (int item = first; item < items; item += stride) {
       const int split = item / w.tiles_n / w.tiles_m;
-      const int t1 = (w.block(split + 1) - w.block(split)) * w.pairs;
-      wait_through(&acc_empty[acc], acc_phase ^ 1, polls);
-      tmem_fence_after_sync();
-      const uint32_t d = tmem + acc * BN;
-      wait_through(&full[stage], phase, polls);
-      for (int t = 0; t < t1; ++t) {
-        tmem_fence_after_sync();
-        const uint64_t da = da0 + stage * (S::kStage >> 4), db = db0 + stage * (S::kStage >> 4);
-        uint64_t* const used = &empty[stage];
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1;
+      const int blocks = w.block(split + 1) - w.block(split);
+      if constexpr (PLANES == 3) {
+        const uint32_t rest = tmem + 2 * BN;
+        const int cut = even_cut(blocks);
+        for (int b0 = 0; b0 < blocks; b0 += cut) {
+          const int b1 = min(b0 + cut, blocks);
+          const bool fresh = b0 % (cut * kCutsOfRest) == 0;
+          wait_through(&acc_empty[acc], acc_phase ^ 1, polls);
+          // the last cut has been taken, the accumulator of the rest with it
+          if (fresh && (b0 > 0 || item != first)) wait_through(&acc_empty[acc ^ 1], acc ? acc_phase : acc_phase ^ 1, polls);
+          tmem_fence_after_sync();
+          const uint32_t lead = tmem + acc * BN;
+          for (int b = b0; b < b1; ++b) {
+            const int s1 = stage, s0 = stage + 1, s2 = stage + 2;  // of planes 1, 0, 2
+            wait_through(&full[s1], phase, polls);
+            tmem_fence_after_sync();
+            block(rest, s1, s1, !fresh || b > b0);
+            wait_through(&full[s0], phase, polls);
+            tmem_fence_after_sync();
+            block(rest, s0, s1, true);
+            block(rest, s1, s0, true);
+            I::commit(&empty[s1], one);
+            block(lead, s0, s0, b > b0);
+            wait_through(&full[s2], phase, polls);
+            tmem_fence_after_sync();
+            block(rest, s0, s2, true);
+            block(rest, s2, s0, true);
+            I::commit(&empty[s0], one);
+            I::commit(&empty[s2], one);
+            if ((stage += 3) == S::kStages) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+          I::commit(&acc_full[acc], one);
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1;
+          }
         }
-#pragma unroll
-        for (int k = 0; k < kBK / 16; ++k) I::mma(d, da + k * kStepA, db + k * kStepB, idesc, t > 0 || k > 0, one);
-        I::commit(used, one);
-        if (t + 1 < t1) wait_through(&full[stage], phase, polls);
-      }
-      I::commit(&acc_full[acc], one);
-      if (++acc == 2) {
-        acc = 0;
-        acc_phase ^= 1;
+      } else {
+        wait_through(&acc_empty[acc], acc_phase ^ 1, polls);
+        tmem_fence_after_sync();
+        const uint32_t d = tmem + acc * BN;
+        wait_through(&full[stage], phase, polls);
+        for (int b = 0; b < blocks; ++b) {
+          tmem_fence_after_sync();
+          const int used = stage;
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+          }
+          block(d, used, used, b > 0);
+          I::commit(&empty[used], one);
+          if (b + 1 < blocks) wait_through(&full[stage], phase, polls);
+        }
+        I::commit(&acc_full[acc], one);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
       }
     }
     if (polls == 1) {
@@ -664,9 +721,58 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const int rest = item / w.tiles_n, split = rest / w.tiles_m;
       const int n0 = item % w.tiles_n * BN + col0;
       const int64_t m0 = (int64_t)(rest % w.tiles_m) * S::kM + rank * 128 + quarter * 32;
-      if (!__all_sync(0xffffffffu, wait(&acc_full[acc], acc_phase))) break;
-      tmem_fence_after_sync();
-      const uint32_t src = tmem + acc * BN + col0 + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t at = tmem + col0 + ((uint32_t)(quarter * 32) << 16);
+      // of both, what the products' warp waits for before it uses the accumulator again
+      const auto release = [&]() {
+        tmem_fence_before_sync();
+        if (lane == 0) {
+          if constexpr (PAIR) arrive_cluster(in_first_cta(&acc_empty[acc]));
+          else mbar_arrive(&acc_empty[acc]);
+        }
+        __syncwarp();
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+      };
+      uint32_t src = at + acc * BN;
+      if constexpr (PLANES == 3) {
+        // each cut is added to the sum and its accumulator given back; what
+        // follows reads the sum
+        src = at + 3 * BN;
+        const int blocks = w.block(split + 1) - w.block(split), cut = even_cut(blocks);
+        bool ended = false;
+        for (int b0 = 0; b0 < blocks; b0 += cut) {
+          if (!__all_sync(0xffffffffu, wait(&acc_full[acc], acc_phase))) {
+            ended = true;
+            break;
+          }
+          tmem_fence_after_sync();
+          const bool rest = b0 + cut >= blocks || (b0 + cut) % (cut * kCutsOfRest) == 0;
+#pragma unroll 1
+          for (int j = 0; j < S::kCols; j += 16) {
+            uint32_t lead[16], more[16], sum[16];
+            tmem_ld16(at + acc * BN + j, lead);
+            if (rest) tmem_ld16(at + 2 * BN + j, more);
+            if (b0 > 0) tmem_ld16(src + j, sum);
+            tmem_wait_ld();
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              v[i] = __uint_as_float(lead[i]);
+              if (rest) v[i] += __uint_as_float(more[i]);
+              if (b0 > 0) v[i] += __uint_as_float(sum[i]);
+            }
+            tmem_st16(src + j, v);
+          }
+          tmem_wait_st();
+          release();
+        }
+        if (ended) break;
+      } else {
+        if (!__all_sync(0xffffffffu, wait(&acc_full[acc], acc_phase))) break;
+        tmem_fence_after_sync();
+      }
 #pragma unroll 1
       for (int chunk = 0; chunk < S::kChunks; ++chunk) {
         const int j = chunk * kCW, n = n0 + j;
@@ -699,7 +805,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           for (int q = 0; q < kCR; ++q)
             if (q * kCStep < left) store8(p + (int64_t)(q * kCStep * 8) * e.per_row, v[q]);
         } else {
-          dense_epilogue<T, kCR>(
+          dense_epilogue<T, kCR, PLANES == 3>(
               e, c, m0 + st.row(), left, nl, bias, v,
               [&](float (&res)[kCR][8]) {
                 if (ahead) {
@@ -714,16 +820,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           fetch();
         }
       }
-      tmem_fence_before_sync();
-      if (lane == 0) {
-        if constexpr (PAIR) arrive_cluster(in_first_cta(&acc_empty[acc]));
-        else mbar_arrive(&acc_empty[acc]);
-      }
-      __syncwarp();
-      if (++acc == 2) {
-        acc = 0;
-        acc_phase ^= 1;
-      }
+      if constexpr (PLANES == 1) release();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
@@ -732,7 +829,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   __syncthreads();
   if constexpr (PAIR) cluster_barrier();  // the other CTA's products, loads and arrivals reach into this one
   tmem_fence_after_sync();
-  if (warp == 2) I::dealloc(tmem, 2 * BN);
+  if (warp == 2) I::dealloc(tmem, kTmem);
 }
 
 // The epilogue of a product whose K loop was cut: the parts summed in order, a
@@ -761,7 +858,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
     }
   }
   dense_bias8(e, c, nl, bias);
-  dense_epilogue<T, kCR>(
+  dense_epilogue<T, kCR, true>(
       e, c, m0 + st.row(), left, nl, bias, v,
       [&](float (&res)[kCR][8]) { dense_get_chunk<T>(e, c, st, m0, n, left, res); },
       [&](void* base, const float (&u)[kCR][8]) { dense_put_chunk<T>(e, c, st, base, m0, n, left, u); });

@@ -457,6 +457,38 @@ def test_dense_fp32_infinities_and_the_largest_values(cuda, sizes):
         assert_within(got[clean], want[clean], bound[clean], name)
 
 
+def test_dense_infinities_under_a_bf16_kernel(cuda):
+    """The gradient of a bf16 kernel under fp32 activations is summed from the same planes."""
+    from selectssm_b200 import dense_act
+    torch.manual_seed(13)
+    x = torch.randn(150, 72, device=cuda)
+    x[4, 7] = float("inf")
+    w = torch.randn(72, 96, device=cuda).bfloat16().requires_grad_()
+    dy = torch.randn(150, 96, device=cuda).bfloat16().float()  # (whose lower planes are zeros)
+    dw, = torch.autograd.grad(dense_act(x, w), w, dy)
+    want = x.double().t() @ dy.double()
+    assert dw.dtype == torch.bfloat16 and torch.equal(dw[7].double(), want[7])
+    rest = [i for i in range(72) if i != 7]
+    bound = 40 * 2.0 ** -23 * (x[:, rest].double().abs().t() @ dy.double().abs())
+    assert_within(dw[rest], want[rest], bound + stored(want[rest], torch.bfloat16), "dw")
+
+
+@pytest.mark.parametrize("sizes", [(129, 5000, 136), (2000, 520, 390), (513, 1032, 4200)])
+def test_dense_fp32_over_long_sums(cuda, sizes):
+    """Sums that pass through several accumulators, in whole and in cut K loops."""
+    from selectssm_b200 import dense_act
+    M, K, N = sizes
+    torch.manual_seed(14)
+    x = torch.rand(M, K, device=cuda).requires_grad_()  # of one sign: every addition is at the size of the result
+    w = torch.rand(K, N, device=cuda).requires_grad_()
+    dy = torch.rand(M, N, device=cuda)
+    y = dense_act(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    x64, w64, d64 = x.detach().double(), w.detach().double(), dy.double()
+    for name, got, want in (("y", y.detach(), x64 @ w64), ("dx", dx, d64 @ w64.t()), ("dw", dw, x64.t() @ d64)):
+        assert_within(got, want, 40 * 2.0 ** -23 * want, name)
+
+
 def test_no_rows(cuda):
     from selectssm_b200 import dense_act, dropout_act, group_norm_act
     x = torch.empty(0, 16, device=cuda, requires_grad=True)
