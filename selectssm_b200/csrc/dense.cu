@@ -273,7 +273,8 @@ struct Plan {
 // choice with the least estimated time.  The terms are measured: a 64-deep step
 // takes about 0.3 us of a single CTA's and 0.38 of a pair's, all six products of
 // three planes 1.2 us, an item about 3 us around its steps, and joining cut
-// products a launch and their partials' way through memory.
+// products a launch, a share of a round trip for each part, and the parts' way
+// through memory.
 static Plan plan_product(int64_t M, int64_t N, int64_t K, int planes) {
   Plan best = {};
   double least = 0;
@@ -289,7 +290,7 @@ static Plan plan_product(int64_t M, int64_t N, int64_t K, int planes) {
          ++w.splits) {
       const double rounds = (double)ceil_div(tiles * w.splits, teams);
       double us = rounds * (ceil_div(w.kblocks, w.splits) * step + 3);
-      if (w.splits > 1) us += 4.0 + 2.0 * w.splits * (double)M * N * 4 / 5e6;
+      if (w.splits > 1) us += 3.5 + w.splits * (0.35 + 2.0 * (double)M * N * 4 / 5e6);
       if (least == 0 || us < least) {
         best.pair = pair;
         best.w = w;

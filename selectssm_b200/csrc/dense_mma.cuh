@@ -848,14 +848,20 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   if (m0 >= e.M) return;
   const int left = dense_left(e, m0, n, st);
   float v[kCR][8] = {}, bias[8];
-  for (int s = 0; s < splits; ++s) {
-    const float* p = part + ((int64_t)s * e.M + m0 + st.row()) * ld + nl;
+  // two parts' loads together: one after another each is a round trip
+  for (int s = 0; s < splits; s += 2) {
+    float t[2][kCR][8] = {};
 #pragma unroll
-    for (int q = 0; q < kCR; ++q) {
-      float t[8] = {};
-      if (q * kCStep < left) load8(p + q * kCStep * ld, t);
-      add8(v[q], t);
+    for (int u = 0; u < 2; ++u) {
+      const float* p = part + ((int64_t)(s + u) * e.M + m0 + st.row()) * ld + nl;
+#pragma unroll
+      for (int q = 0; q < kCR; ++q)
+        if (q * kCStep < left && s + u < splits) load8(p + q * kCStep * ld, t[u][q]);
     }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int q = 0; q < kCR; ++q) add8(v[q], t[u][q]);
   }
   dense_bias8(e, c, nl, bias);
   dense_epilogue<T, kCR, true>(
