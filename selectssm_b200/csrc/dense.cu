@@ -271,15 +271,17 @@ struct Plan {
 
 // Tile (128 x 128 by one CTA, 256 x 256 by a pair) and cuts of the K loop: the
 // choice with the least estimated time.  The terms are measured: a 64-deep step
-// takes about 0.3 us of a single CTA's and 0.38 of a pair's, all six products of
-// three planes 1.2 us, an item about 3 us around its steps, and joining cut
+// takes 0.22 us of a single CTA's and 0.36 of a pair's, all six products of three
+// planes 1.2 us; an item 3 us around its steps, a pair's 4.5; and joining cut
 // products a launch, a share of a round trip for each part, and the parts' way
-// through memory.
+// through memory.  (bf16, one way against the other: 8192 x 768 x 768 14 us by
+// single CTAs and 16 by pairs, 16384 x 768 x 1536 38 and 35, 768 x 1536 of
+// K 32768 67 and 59.)
 static Plan plan_product(int64_t M, int64_t N, int64_t K, int planes) {
   Plan best = {};
   double least = 0;
   for (int pair = 0; pair < (planes == 3 ? 1 : 2); ++pair) {
-    const double step = planes == 3 ? 1.2 : pair ? 0.38 : 0.3;
+    const double step = planes == 3 ? 1.2 : pair ? 0.36 : 0.22, item = pair ? 4.5 : 3;
     DenseWork w;
     w.tiles_m = (int)ceil_div(M, pair ? Tile<true, float>::kM : Tile<false, float>::kM);
     w.tiles_n = (int)ceil_div(N, pair ? Tile<true, float>::kN : Tile<false, float>::kN);
@@ -289,7 +291,7 @@ static Plan plan_product(int64_t M, int64_t N, int64_t K, int planes) {
                                          (planes == 3 || w.splits * 4 <= w.kblocks));
          ++w.splits) {
       const double rounds = (double)ceil_div(tiles * w.splits, teams);
-      double us = rounds * (ceil_div(w.kblocks, w.splits) * step + 3);
+      double us = rounds * (ceil_div(w.kblocks, w.splits) * step + item);
       if (w.splits > 1) us += 3.5 + w.splits * (0.35 + 2.0 * (double)M * N * 4 / 5e6);
       if (least == 0 || us < least) {
         best.pair = pair;
