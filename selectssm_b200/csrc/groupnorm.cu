@@ -568,9 +568,10 @@ __device__ __forceinline__ float2 gn_peer(const float2* p, int cta) {
 // SHORT: more batch rows than turns, or rows so short that the sums over a group
 // are a thread's work.  (The loop and the other form of the sums cost a call that
 // has no need of them up to a fifth of its time, in registers.)
-// 64 x 2048 x 768 bf16: 106 us for 403 MB, 3.8 TB/s.  A CTA reads its part, meets its
-// cluster, and writes; with three CTAs an SM (80 registers; issue 47% of cycles, HBM
-// a third of its peak) these phases overlap only in part.
+// 64 x 2048 x 768 bf16: 95 us for 403 MB, 4.2 TB/s.  A CTA reads its part, meets its
+// cluster, and writes, and what a thread does once (80 registers of constants, two
+// sums over the CTA) stands against 26 vectors of its own: the phases of four CTAs
+// an SM overlap only in part.
 template <typename T, int V, int ACT, bool BWD, bool SHORT>
 __global__ void __launch_bounds__(kHoldThreads, 3) gn_hold_kernel(const GnArgs p, const GnHold h) {
   using Vec = GnVec<T, V>;
@@ -939,7 +940,12 @@ static bool gn_hold(const ssm_group_norm_params_t* p, bool bwd, GnHold* h, int* 
       c.jobs = (p->groups + gpj - 1) / gpj;
       c.nv = c.W / *V;
       if (c.nv > kHoldThreads) return false;
-      c.threads = bytes > 4096 ? 256 : 128;
+      // Half the threads, each with twice the rows, where four CTAs then share an SM
+      // and there are several rounds of them: what a thread does once weighs less, and
+      // a fourth CTA's loads are under way (64 x 2048 x 768 bf16 forward 95 us for 108,
+      // 64 x 1024 x 768 53 for 55; with jobs of 64 KB, three to an SM, 35 for 32).
+      const bool many = !bwd && *V > 1 && bytes <= 52 * 1024 && p->batch * c.jobs * ctas >= 8 * 148;
+      c.threads = bytes > 4096 && !many ? 256 : 128;
       while (c.threads < c.nv) c.threads *= 2;
       c.rt = c.threads / c.nv;
       c.slots = (int)((rows + c.rt - 1) / c.rt);
