@@ -401,8 +401,11 @@ __device__ __forceinline__ uint32_t in_first_cta(const void* p) {
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
   return r;
 }
+// Relaxed: what the waiting side relies on are reads of tensor memory, which
+// tcgen05.wait::ld has completed.  A release at the cluster's scope would first wait
+// for all the warp's stores to global memory (4% of 32768 x 768 x 1536).
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
