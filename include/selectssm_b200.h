@@ -272,7 +272,8 @@ typedef struct ssm_group_norm_params {
   const float* scale;                   /* (dim) or NULL: ones */
   const float* bias;                    /* (dim) or NULL: zeros */
   void* y;
-  float* stats;                         /* (batch, groups, 2) mean and rstd: forward output, backward input */
+  float* stats;                         /* (batch, groups, 2) mean and rstd: forward output (NULL: not
+                                           kept), backward input                          */
   const void* dy;
   void* dx;
   float* dscale;                        /* (dim) */

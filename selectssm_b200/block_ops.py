@@ -174,13 +174,13 @@ def _gn_params(x, scale, bias, y, stats, groups, eps, act):
     batch, dim = x.shape[0], x.shape[-1]
     seqlen = x.numel() // (batch * dim) if batch else 0
     return _lib.SSMGroupNormParams(batch, seqlen, dim, groups, _DT[x.dtype], act, eps, x.data_ptr(), _ptr(scale),
-                                   _ptr(bias), _ptr(y), stats.data_ptr())
+                                   _ptr(bias), _ptr(y), _ptr(stats))
 
 
-def _group_norm_forward(x, scale, bias, groups, eps, act):
-    """y and the statistics; x, scale and bias are dense, the latter float32."""
+def _group_norm_forward(x, scale, bias, groups, eps, act, keep_stats):
+    """y and, with keep_stats, the statistics; x, scale and bias are dense, the latter float32."""
     y = x.new_empty(x.shape)
-    stats = x.new_empty((x.shape[0], groups, 2), dtype=torch.float32)
+    stats = x.new_empty((x.shape[0], groups, 2), dtype=torch.float32) if keep_stats else None
     if x.numel():
         p = _gn_params(x, scale, bias, y, stats, groups, eps, act)
         lib, ref = _lib.load(), ctypes_byref(p)
@@ -195,7 +195,7 @@ class _GroupNormActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, scale, bias, groups, eps, act):
         x = _dense(x)
-        y, stats = _group_norm_forward(x, scale, bias, groups, eps, act)
+        y, stats = _group_norm_forward(x, scale, bias, groups, eps, act, True)
         ctx.save_for_backward(x, scale, bias, stats)
         ctx.cfg = (groups, eps, act)
         return y
@@ -240,7 +240,7 @@ def group_norm_act(x, scale=None, bias=None, groups=32, eps=1e-6, activation=Non
     bias = bias if bias is None else _dense(bias.float())
     if _records(x, scale, bias):
         return _GroupNormActFn.apply(x, scale, bias, groups, eps, _act_code(activation))
-    return _group_norm_forward(_dense(x), scale, bias, groups, eps, _act_code(activation))[0]
+    return _group_norm_forward(_dense(x), scale, bias, groups, eps, _act_code(activation), False)[0]
 
 
 # ----------------------------------------------------------------------------- dense layer
@@ -334,4 +334,5 @@ def dense_act(x, kernel, bias=None, activation=None, residual=None, rate=0.0, rn
         residual = _residual_of(residual, (*x.shape[:-1], fout), x.dtype)
     if _records(x, kernel, bias, residual):
         return _DenseActFn.apply(x, kernel, bias, residual, act, drop, rng)
-    return _dense_forward(x, _dense(kernel.to(x.dtype)), bias, residual, act, drop, rng, False)[0]
+    kernel = kernel if kernel.dtype == x.dtype else kernel.to(x.dtype)
+    return _dense_forward(x, _dense(kernel), bias, residual, act, drop, rng, False)[0]

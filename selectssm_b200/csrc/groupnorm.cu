@@ -725,7 +725,7 @@ __global__ void __launch_bounds__(kHoldThreads, 3) gn_hold_kernel(const GnArgs p
       const auto settle = [&](int q, float mu, float m2) {
         const float2 st = make_float2(mu, rsqrtf(fmaf(m2, per_group, p.eps)));
         all[q] = st;
-        if (rank == 0) reinterpret_cast<float2*>(p.stats)[(int64_t)b * g.G + g0 + q] = st;
+        if (rank == 0 && p.stats) reinterpret_cast<float2*>(p.stats)[(int64_t)b * g.G + g0 + q] = st;
       };
       if (SHORT && h.ctas == 1)
         for (int q = tid; q < ng; q += threads) settle(q, own[q].x, own[q].y);
@@ -969,6 +969,9 @@ static bool gn_hold(const ssm_group_norm_params_t* p, bool bwd, GnHold* h, int* 
 }
 
 static size_t gn_round(size_t v) { return (v + 255) / 256 * 256; }
+static size_t gn_stats_bytes(const ssm_group_norm_params_t* p) {  // of statistics that the caller does not keep
+  return p->stats ? 0 : gn_round((size_t)p->batch * p->groups * sizeof(float2));
+}
 static size_t gn_part_bytes(const GnGeom& g) { return gn_round((size_t)g.B * g.chunks * g.D * sizeof(float2)); }
 static size_t gn_sums_bytes(const GnGeom& g) { return gn_round((size_t)g.B * g.D * sizeof(float2)); }
 static size_t gn_means_bytes(const GnGeom& g) { return gn_round((size_t)g.B * g.G * sizeof(float2)); }
@@ -1101,7 +1104,9 @@ size_t ssm_group_norm_fwd_workspace_bytes(const ssm_group_norm_params_t* p) {
   GnHold h;
   int V;
   // without the pointers their alignment, which has a say in the form, is unknown
-  return p->x && p->y && gn_hold(p, false, &h, &V) ? 0 : gn_part_bytes(gn_geom(p));
+  return p->x && p->y && gn_hold(p, false, &h, &V)
+             ? 0
+             : gn_part_bytes(gn_geom(p)) + gn_stats_bytes(p);
 }
 
 size_t ssm_group_norm_bwd_workspace_bytes(const ssm_group_norm_params_t* p) {
@@ -1120,7 +1125,7 @@ int ssm_group_norm_act_fwd(const ssm_group_norm_params_t* p, ssm_stream_t stream
   int st = check_gn(p);
   if (st) return st;
   if (p->batch == 0 || p->seqlen == 0) return SSM_OK;
-  if (!p->x || !p->y || !p->stats) return SSM_ERR_NULL;
+  if (!p->x || !p->y) return SSM_ERR_NULL;
   if (gn_vector(p) && (!aligned16(p->x) || !aligned16(p->y))) return SSM_ERR_ALIGN;
   const size_t need = ssm_group_norm_fwd_workspace_bytes(p);
   if (need && (!p->workspace || p->workspace_bytes < need)) return SSM_ERR_WORKSPACE;
@@ -1134,6 +1139,8 @@ int ssm_group_norm_act_fwd(const ssm_group_norm_params_t* p, ssm_stream_t stream
   a.bias = p->bias;
   a.stats = p->stats;
   a.part = static_cast<float2*>(p->workspace);
+  // the split form's second pass reads the statistics; the held one keeps them itself
+  if (!a.stats && need) a.stats = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + gn_part_bytes(a.g));
   a.out = p->y;
   return gn_dispatch(p, a, false, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -563,3 +563,13 @@ def test_captured_step_follows_the_device_rng(cuda):
         torch.cuda.synchronize()
         got = [t.clone() for t in captured]
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.parametrize("shape,groups", [((3, 50, 64), 8), ((1, 60000, 32), 2)])
+def test_group_norm_with_and_without_statistics(cuda, shape, groups):
+    """A call that records no gradient keeps no statistics, in either form, and gives the same bits."""
+    from selectssm_b200 import group_norm_act
+    torch.manual_seed(15)
+    x = torch.randn(shape, device=cuda)
+    y = group_norm_act(x, groups=groups, activation="silu")
+    assert torch.equal(y, group_norm_act(x.clone().requires_grad_(), groups=groups, activation="silu"))
