@@ -42,6 +42,32 @@ __device__ __forceinline__ void store_planes(__nv_bfloat16* dst, int64_t plane, 
   if (PLANES == 1) {
     store8(dst, v);
   } else {
+    // Pairs are converted together and need no second conversion to be stored;
+    // values that would round to infinity, and infinities, take the long way.
+    float rest[8];
+    bool large = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      rest[i] = v[i];
+      large |= fabsf(v[i]) > __uint_as_float(0x7f7f0000u);  // the largest bf16 value
+    }
+    if (!large) {
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(rest[2 * i], rest[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&b);
+          const float2 left = fsub2(make_float2(rest[2 * i], rest[2 * i + 1]),
+                                    make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)));
+          rest[2 * i] = left.x;
+          rest[2 * i + 1] = left.y;
+        }
+        *reinterpret_cast<uint4*>(dst + p * plane) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      return;
+    }
     float h[8][3], t[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) split3(v[i], h[i]);
@@ -57,7 +83,7 @@ __device__ __forceinline__ void store_planes(__nv_bfloat16* dst, int64_t plane, 
 // What has to be ready before the products, in one launch (a small call's time is
 // its launches'): up to two operands as planes, and dbias from its runs' sums.
 // (300 x 500) @ (500 x 400), fp32, forward and backward: 150 us of the host's time,
-// 163 with a launch for each.
+// 163 with a launch for each.  16384 x 768 twice in fp32: 36 us for 252 MB, 7 TB/s.
 struct Pack {  // (rows, cols) at row stride `stride` to planes of row length ld, a multiple of 8; zeros beyond cols
   const void* src;
   __nv_bfloat16* dst;

@@ -18,13 +18,14 @@
 // accumulator from tensor memory, apply the epilogue and store; two
 // accumulators let the epilogue of one tile overlap the products of the next.
 //
-// Measured in bf16.  131072 x 1536 x 768, residual and dropout: 240 us, 1.29
+// Measured in bf16.  131072 x 1536 x 768, residual and dropout: 232 us, 1.33
 // PFLOP/s; without the epilogue 197 us, 1.57 PFLOP/s, the rate of a plain library
 // product at these sizes (203 us), with the clock held down by the power limit.
-// 32768 x 768 x 1536, silu, dropout and `pre`: 115 us, where the epilogue's issue is
-// the bound (the tensor cores work 32% of the time), and its two gradients 57 and 55
-// us, 1.35 and 1.4 PFLOP/s (68 and 70%).  In fp32 2042 x 515 x 1001, forward and
-// both gradients: 23 to 26 us each, 0.55 PFLOP/s of bf16 products.
+// 32768 x 768 x 1536, silu, dropout and `pre`: 106 us, where the epilogue's issue is
+// the bound (66 us without it), and its two gradients 59 and 55 us, 1.3 and 1.4
+// PFLOP/s.  In fp32 8192 x 768 x 1536: 107 us with the planes' pass, 66% of the rate
+// of six bf16 products; 2042 x 515 x 1001, forward and both gradients: 24, 25 and 21
+// us, bound by the latency of the loads of one round of tiles.
 #pragma once
 
 #include <cstdint>
