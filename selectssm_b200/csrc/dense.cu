@@ -137,15 +137,16 @@ __global__ void __launch_bounds__(256) dense_ready_kernel(const __grid_constant_
 
 template <typename T>
 constexpr int kDpreRows = sizeof(T) == 2 ? 4 : 2;
+constexpr int kDpreCtas = 3;  // on an SM
 
 // dpre as planes for the two products that follow, and the column sums of its
 // unrounded values over a run of rows.  A thread keeps eight columns (one
 // dropout counter each row) and takes ROWS rows at a time, whose loads it issues
 // together: a loop that loads, computes and stores row by row ran at half the
-// rate.  32768 x 1536 bf16, silu, dropout, dbias, cold: 70 us for 302 MB, 4.3 TB/s,
-// issue on 54% of cycles at 80 registers; HBM alone would take 46.
+// rate.  32768 x 1536 bf16, silu, dropout, dbias: 62 us for 302 MB, 4.9 TB/s; issue (54%
+// of cycles) and latency at 80 registers, where HBM alone would take 46.
 template <typename T, int PLANES, bool WRITE, int ACT>
-__global__ void __launch_bounds__(256, 3)
+__global__ void __launch_bounds__(256, kDpreCtas)
     dense_dpre_kernel(const T* dy, int64_t dy_stride, const T* pre, __nv_bfloat16* dpre, int ld, float* part, int64_t M,
                       int N, int64_t run, int cb, DropRng rng, bool vec) {
   constexpr int ROWS = kDpreRows<T>;
@@ -476,9 +477,13 @@ static DpreGeom dpre_geom(const ssm_dense_params_t* p) {
   g.tiles = (int)ceil_div(per_row, 32);
   g.cb = (int)ceil_div(per_row, g.tiles);
   const int rl = 256 / g.cb;
-  // one round of the rows' loads a CTA, more where that made over 256 parts of each column's sum
+  // bf16: as many CTAs as the SMs hold at once, with long runs (131072 x 768 120 us, 133 with
+  // 256 parts of each column's sum; 32768 x 1536 62 for 67).  fp32, whose rounds are twice as
+  // long, is better off with more (32768 x 1536 119 and 112): one round of the rows' loads a
+  // CTA, more where that made over 256 parts.
   const int64_t round = (int64_t)rl * (p->dtype == SSM_BF16 ? kDpreRows<__nv_bfloat16> : kDpreRows<float>);
-  g.run = round * ceil_div(p->rows, 256 * round);
+  if (p->dtype == SSM_BF16) g.run = std::max(round, ceil_div(p->rows, std::max(1, kDpreCtas * kSms / g.tiles)));
+  else g.run = round * ceil_div(p->rows, 256 * round);
   g.parts = (int)ceil_div(p->rows, g.run);
   return g;
 }
