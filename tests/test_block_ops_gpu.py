@@ -573,3 +573,14 @@ def test_group_norm_with_and_without_statistics(cuda, shape, groups):
     x = torch.randn(shape, device=cuda)
     y = group_norm_act(x, groups=groups, activation="silu")
     assert torch.equal(y, group_norm_act(x.clone().requires_grad_(), groups=groups, activation="silu"))
+
+
+def test_dense_fp32_sums_that_start_the_small_products_afresh(cuda):
+    """More tiles than CTAs, so that the K loop stays whole, and more than 4096 of K."""
+    from selectssm_b200 import dense_act
+    torch.manual_seed(16)
+    x, w = torch.rand(1530, 4700, device=cuda), torch.rand(4700, 1660, device=cuda)
+    want = x.double() @ w.double()
+    # a sum of one sign grows from nothing, so its additions are cut at half of 2^-23 of the result
+    # on average: 16 of the leading products, 3 of the small ones, 5 of ten cuts joined in fp32
+    assert_within(dense_act(x, w), want, 25 * 2.0 ** -23 * want, "y")
