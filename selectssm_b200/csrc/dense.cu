@@ -319,7 +319,8 @@ static Plan plan_product(int64_t M, int64_t N, int64_t K, int planes) {
          ++w.splits) {
       const double rounds = (double)ceil_div(tiles * w.splits, teams);
       double us = rounds * (ceil_div(w.kblocks, w.splits) * step + item);
-      if (w.splits > 1) us += 3.5 + w.splits * (0.35 + 2.0 * (double)M * N * 4 / 5e6);
+      if (w.splits > 1) us += 3.5 + (w.splits < kJoinShared ? 0.35 * w.splits : 2 + 0.09 * w.splits) +
+                              w.splits * 2.0 * (double)M * N * 4 / 5e6;
       if (least == 0 || us < least) {
         best.pair = pair;
         best.w = w;
@@ -385,7 +386,8 @@ static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
       st = q.pair ? launch_mma<A_MN, B_MN, true, 1, T>(first, q, ma, mb, status, s)
                   : launch_mma<A_MN, B_MN, false, 1, T>(first, q, ma, mb, status, s);
   if (st || q.w.splits == 1) return st;
-  const int64_t grid = ceil_div(ceil_div(e.M, 32) * ceil_div(e.N, kCW), kJoinWarps);
+  const int64_t chunks = ceil_div(e.M, 32) * ceil_div(e.N, kCW);
+  const int64_t grid = q.w.splits >= kJoinShared ? chunks : ceil_div(chunks, kJoinWarps);
   if (grid > 0x7fffffff) return SSM_ERR_SHAPE;
   dense_join_kernel<T><<<(unsigned)grid, 32 * kJoinWarps, 0, s>>>(part, q.w.splits, e);
   return launched("launch dense join kernel", 1);

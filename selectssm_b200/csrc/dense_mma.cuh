@@ -250,13 +250,18 @@ struct Stage {
 // For rows that start anywhere: a chunk from row m0, column n, with a lane a
 // column, so that its accesses lie together, and through shared memory to or
 // from the epilogue's arrangement.
+static_assert(kCW == 32);
 template <typename T>
 __device__ __forceinline__ void dense_stage_rows(const DenseEpi& e, const Stage& st, int64_t m0, int n, float (&res)[kCR][8]) {
-  const int c = st.lane % kCW;
   __syncwarp();
-  if (n + c < e.N)
-    for (int row = st.lane / kCW; row < 32 && m0 + row < e.M; row += 32 / kCW)
-      st.at(row, c) = Cvt<T>::to_f(static_cast<const T*>(e.residual)[(m0 + row) * e.res_stride + n + c]);
+  if (n + st.lane < e.N) {
+    const int rows = (int)min(e.M - m0, (int64_t)32);
+    const T* p = static_cast<const T*>(e.residual) + m0 * e.res_stride + n + st.lane;
+    for (int r0 = 0; r0 < 32; r0 += 8, p += 8 * e.res_stride)
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (r0 + u < rows) st.at(r0 + u, st.lane) = Cvt<T>::to_f(p[u * e.res_stride]);
+  }
   __syncwarp();
   st.get(res);
 }
@@ -267,13 +272,17 @@ __device__ __forceinline__ void dense_put_chunk(const DenseEpi& e, const EpiCons
     dense_put<T, kCR>(e, c, base, m0 + st.row(), left, n + st.col(), v);
     return;
   }
-  const int k = st.lane % kCW;
   __syncwarp();
   st.put(v);
   __syncwarp();
-  if (n + k < e.N)
-    for (int row = st.lane / kCW; row < 32 && m0 + row < e.M; row += 32 / kCW)
-      static_cast<T*>(base)[(m0 + row) * e.N + n + k] = Cvt<T>::from_f(st.at(row, k));
+  if (n + st.lane < e.N) {
+    const int rows = (int)min(e.M - m0, (int64_t)32);
+    T* p = static_cast<T*>(base) + m0 * e.N + n + st.lane;
+    for (int r0 = 0; r0 < 32; r0 += 8, p += 8 * (int64_t)e.N)
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (r0 + u < rows) p[u * (int64_t)e.N] = Cvt<T>::from_f(st.at(r0 + u, st.lane));
+  }
 }
 // The residual of a chunk by plain loads.
 template <typename T>
@@ -837,35 +846,51 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 }
 
 // The epilogue of a product whose K loop was cut: the parts summed in order, a
-// chunk a warp.  768 x 1536 of 4 parts (19 MB, mostly in L2): 6 us.
+// chunk a warp or, of many parts (then there are few chunks, and one part after
+// another is a round trip each), a chunk a CTA and a run of the parts a warp.  768 x 1536 of 4 parts (19 MB, mostly in L2): 6 us.
 constexpr int kJoinWarps = 4;
+constexpr int kJoinShared = 8;  // parts from which a CTA's warps share a chunk's
 template <typename T>
 __global__ void __launch_bounds__(32 * kJoinWarps)
     dense_join_kernel(const float* part, int splits, const __grid_constant__ DenseEpi e) {
   __shared__ uint4 staged[kJoinWarps][8 * kCW];
   const EpiConst c(e);
-  const Stage st = {staged[threadIdx.x >> 5], (int)threadIdx.x & 31};
+  const int warp = threadIdx.x >> 5;
+  const bool share = splits >= kJoinShared;
+  const Stage st = {staged[warp], (int)threadIdx.x & 31};
   const int64_t ld = (int64_t)e.per_row * 8, chunks_n = (e.N + kCW - 1) / kCW;
-  const int64_t i = (int64_t)blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+  const int64_t i = share ? blockIdx.x : (int64_t)blockIdx.x * kJoinWarps + warp;
+  const int s0 = share ? splits * warp / kJoinWarps : 0, s1 = share ? splits * (warp + 1) / kJoinWarps : splits;
   const int64_t m0 = i / chunks_n * 32;
   const int n = (int)(i % chunks_n) * kCW, nl = n + st.col();
   if (m0 >= e.M) return;
   const int left = dense_left(e, m0, n, st);
   float v[kCR][8] = {}, bias[8];
   // two parts' loads together: one after another each is a round trip
-  for (int s = 0; s < splits; s += 2) {
+  for (int s = s0; s < s1; s += 2) {
     float t[2][kCR][8] = {};
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const float* p = part + ((int64_t)(s + u) * e.M + m0 + st.row()) * ld + nl;
 #pragma unroll
       for (int q = 0; q < kCR; ++q)
-        if (q * kCStep < left && s + u < splits) load8(p + q * kCStep * ld, t[u][q]);
+        if (q * kCStep < left && s + u < s1) load8(p + q * kCStep * ld, t[u][q]);
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int q = 0; q < kCR; ++q) add8(v[q], t[u][q]);
+  }
+  if (share) {
+    if (warp) st.put(v);
+    __syncthreads();
+    if (warp) return;
+    for (int w = 1; w < kJoinWarps; ++w) {
+      float t[kCR][8];
+      Stage{staged[w], st.lane}.get(t);
+#pragma unroll
+      for (int q = 0; q < kCR; ++q) add8(v[q], t[q]);
+    }
   }
   dense_bias8(e, c, nl, bias);
   dense_epilogue<T, kCR, true>(
