@@ -526,8 +526,9 @@ __global__ void __launch_bounds__(1024) gn_param_kernel(const float2* sums, int 
 // ---------------------------------------------------------------- held form
 // A job: `gpj` groups (W channels) of one batch row, `ctas` CTAs with `rows`
 // rows each; a cluster takes the same groups of every `turns`-th batch row, so
-// that many short rows (a norm per token) need few sums for dscale and dbias.  nv vectors of V channels by rt row lanes; each thread keeps
-// `slots` vectors of its own in shared memory.
+// that many short rows (a norm per token) need few sums for dscale and dbias.  nv
+// vectors of V channels by rt row lanes; each thread keeps `slots` vectors of its
+// own in shared memory.
 constexpr int kHoldThreads = 256;  // at most
 struct GnHold {
   int32_t threads, W, gpj, jobs, ctas, turns, nv, rt, slots;
