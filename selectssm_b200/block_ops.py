@@ -8,7 +8,8 @@ projection and the MLP with its dropout:
 * :func:`dropout_act`     residual + activation(dropout(x))
 * :func:`dense_act`       residual + activation(dropout(x @ kernel + bias))
 
-Each is differentiable once.  PyTorch holds the memory, the stream and the
+Each is differentiable once, in reverse mode; forward-mode tangents are refused
+with autograd's NotImplementedError.  PyTorch holds the memory, the stream and the
 autograd graph; the arithmetic runs in the kernels of ``libselectssm_b200.so``.
 
 Dropout takes its random bits from ``rng = (seed, offset)``, two integers or an
@@ -22,6 +23,7 @@ another offset.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -103,13 +105,19 @@ def _residual_of(residual, shape, dtype):
 
 
 def _records(*tensors):
-    """Whether autograd will ask for a gradient."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether the call is autograd's business: it will ask for a gradient, or an
+    operand carries a forward-mode tangent, which autograd refuses (a direct call
+    would lose it)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    # outside every dual level (the usual case) no operand is looked at
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 # Each operator has a plain function that makes the call and an autograd
-# function around it; without a gradient to record the former is called
-# directly, which halves the host's time for a single token.
+# function around it; without a gradient to record or a tangent to refuse the
+# former is called directly, which halves the host's time for a single token.
 
 # ----------------------------------------------------------------------------- dropout
 def _dropout_forward(x, residual, drop, rng, act):

@@ -117,3 +117,19 @@ def test_row_views():
         m, step = block_ops._rows_of(view)
         rows = view.reshape(-1, view.shape[-1])
         assert step >= view.shape[-1] and torch.equal(m.as_strided(rows.shape, (step, 1)), rows)
+
+
+def test_a_forward_mode_tangent_goes_through_autograd():
+    """Which has no rule for it and says so; a call past autograd would return no tangent."""
+    from torch.autograd import forward_ad
+    x, t = torch.zeros(3), torch.ones(3)
+    assert not block_ops._records(x, None)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, t)
+        assert block_ops._records(None, dual) and block_ops._records(dual)
+        assert not block_ops._records(x, None)
+        with torch.no_grad():
+            assert block_ops._records(x, dual)
+    assert block_ops._records(x.clone().requires_grad_())
+    with torch.no_grad():
+        assert not block_ops._records(x.clone().requires_grad_())

@@ -584,3 +584,25 @@ def test_dense_fp32_sums_that_start_the_small_products_afresh(cuda):
     # a sum of one sign grows from nothing, so its additions are cut at half of 2^-23 of the result
     # on average: 16 of the leading products, 3 of the small ones, 5 of ten cuts joined in fp32
     assert_within(dense_act(x, w), want, 25 * 2.0 ** -23 * want, "y")
+
+
+@pytest.mark.parametrize("which", ["x", "scale", "kernel", "bias", "residual"])
+def test_forward_mode_tangents_are_refused(cuda, which):
+    from torch.autograd import forward_ad
+    from selectssm_b200 import dense_act, dropout_act, group_norm_act
+    a = dict(x=torch.randn(20, 5, 16, device=cuda), scale=torch.ones(16, device=cuda), kernel=torch.randn(16, 16, device=cuda),
+             bias=torch.zeros(16, device=cuda), residual=torch.zeros(20, 5, 16, device=cuda))
+    calls = [("x residual", lambda p: dropout_act(p["x"], 0.5, (1, 2), residual=p["residual"])),
+             ("x scale bias", lambda p: group_norm_act(p["x"], p["scale"], p["bias"], groups=4)),
+             ("x kernel bias residual", lambda p: dense_act(p["x"], p["kernel"], p["bias"], residual=p["residual"]))]
+    for names, call in calls:
+        with forward_ad.dual_level():
+            p = dict(a)
+            p[which] = forward_ad.make_dual(a[which], torch.ones_like(a[which]))
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad):
+                    if which in names.split():
+                        with pytest.raises(NotImplementedError):
+                            call(p)
+                    else:
+                        call(p)
