@@ -244,8 +244,8 @@ def group_norm_act(x, scale=None, bias=None, groups=32, eps=1e-6, activation=Non
         if t is not None and t.shape != (dim,):
             raise ValueError(f"{name} must be ({dim},), got {tuple(t.shape)}")
     # converted outside, so that autograd returns the gradients in their types
-    scale = scale if scale is None else _dense(scale.float())
-    bias = bias if bias is None else _dense(bias.float())
+    scale = scale if scale is None else scale.float().contiguous()
+    bias = bias if bias is None else bias.float().contiguous()
     if _records(x, scale, bias):
         return _GroupNormActFn.apply(x, scale, bias, groups, eps, _act_code(activation))
     return _group_norm_forward(_dense(x), scale, bias, groups, eps, _act_code(activation), False)[0]
@@ -284,7 +284,7 @@ def _dense_forward(x, w, bias, residual, act, drop, rng, keep_pre):
 class _DenseActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, kernel, bias, residual, act, drop, rng):
-        w = _dense(kernel.to(x.dtype))
+        w = kernel.to(x.dtype).contiguous()
         need = any(ctx.needs_input_grad[:3])
         y, pre = _dense_forward(x, w, bias, residual, act, drop, rng, need and act != 0)
         if need:
@@ -343,4 +343,4 @@ def dense_act(x, kernel, bias=None, activation=None, residual=None, rate=0.0, rn
     if _records(x, kernel, bias, residual):
         return _DenseActFn.apply(x, kernel, bias, residual, act, drop, rng)
     kernel = kernel if kernel.dtype == x.dtype else kernel.to(x.dtype)
-    return _dense_forward(x, _dense(kernel), bias, residual, act, drop, rng, False)[0]
+    return _dense_forward(x, kernel.contiguous(), bias, residual, act, drop, rng, False)[0]

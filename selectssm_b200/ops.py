@@ -60,7 +60,10 @@ def _rows(t: torch.Tensor, width: int):
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
-    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.contiguous()
+    """t, contiguous from a 16-byte aligned address, for kernels with wide accesses
+    (contiguous() alone returns a contiguous view into a larger buffer as it stands)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _stream() -> int:
@@ -123,8 +126,8 @@ class _Prepared:
             B, C2 = B.contiguous(), C2.contiguous()
             self.bc_stride = N
         self.B, self.C = B, C2
-        self.D = None if D is None else _dense(D.float())
-        self.delta_bias = None if delta_bias is None else _dense(delta_bias.float())
+        self.D = None if D is None else D.float().contiguous()
+        self.delta_bias = None if delta_bias is None else delta_bias.float().contiguous()
         if z is not None:
             z, self.z_stride = _rows(z.to(u.dtype), Dm)
         else:
@@ -357,7 +360,7 @@ class _Conv1dActFn(torch.autograd.Function):
         K = w.shape[0]
         w_shape = w.shape
         x, xs = _rows(x, Dm)
-        w = _dense(w.float().reshape(K, Dm))
+        w = w.float().reshape(K, Dm).contiguous()
         u = torch.empty((Bsz, L, Dm), dtype=x.dtype, device=x.device)
         p = _conv_params(x, xs, w, act, reverse, complement)
         p.u = u.data_ptr()
@@ -371,7 +374,7 @@ class _Conv1dActFn(torch.autograd.Function):
     def backward(ctx, du):
         x, w = ctx.saved_tensors
         xs, act, reverse, complement = ctx.cfg
-        du = _dense(du.to(x.dtype))
+        du = du.to(x.dtype).contiguous()
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         dw = torch.empty_like(w)
         p = _conv_params(x, xs, w, act, reverse, complement)
@@ -415,13 +418,13 @@ class _RMSNormResidualFn(torch.autograd.Function):
     def forward(ctx, x, scale, res_bias, eps):
         _require_cuda(x, scale)
         dim = x.shape[-1]
-        x2 = _dense(x).reshape(-1, dim)
-        scale = _dense(scale.float())
+        x2 = x.contiguous().reshape(-1, dim)
+        scale = scale.float().contiguous()
         y = torch.empty_like(x2)
         base = torch.empty_like(x2)
         rstd = torch.empty(x2.shape[0], dtype=torch.float32, device=x.device)
         p = _norm_params(x2, scale, eps, rstd)
-        bias = None if res_bias is None else _dense(res_bias.float())
+        bias = None if res_bias is None else res_bias.float().contiguous()
         p.y, p.res_base = y.data_ptr(), base.data_ptr()
         p.res_bias = 0 if bias is None else bias.data_ptr()
         _lib.check(_lib.load().ssm_rmsnorm_fwd(ctypes_byref(p), _stream()), "ssm_rmsnorm_fwd")
@@ -433,8 +436,8 @@ class _RMSNormResidualFn(torch.autograd.Function):
     def backward(ctx, dy, dbase):
         x2, scale, rstd = ctx.saved_tensors
         dim = x2.shape[1]
-        dy = torch.zeros_like(x2) if dy is None else _dense(dy.to(x2.dtype)).reshape(-1, dim)
-        dres = None if dbase is None else _dense(dbase.to(x2.dtype)).reshape(-1, dim)
+        dy = torch.zeros_like(x2) if dy is None else dy.to(x2.dtype).contiguous().reshape(-1, dim)
+        dres = None if dbase is None else dbase.to(x2.dtype).contiguous().reshape(-1, dim)
         dx = torch.empty_like(x2)
         dscale = torch.empty(dim, dtype=torch.float32, device=x2.device)
         p = _norm_params(x2, scale, ctx.eps, rstd)

@@ -133,3 +133,13 @@ def test_a_forward_mode_tangent_goes_through_autograd():
     assert block_ops._records(x.clone().requires_grad_())
     with torch.no_grad():
         assert not block_ops._records(x.clone().requires_grad_())
+
+
+def test_dense_operands_are_aligned():
+    """A contiguous view may start anywhere; the kernels' 16-byte accesses may not."""
+    from selectssm_b200.ops import _dense
+    flat = torch.arange(200.0)
+    for t in (flat[3:67].view(2, 4, 8), flat[1:], flat.view(10, 20).t(), flat[4:20].view(4, 4)):
+        d = _dense(t)
+        assert d.is_contiguous() and d.data_ptr() % 16 == 0 and torch.equal(d, t)
+    assert _dense(flat) is flat and _dense(flat[4:20]).data_ptr() == flat[4:20].data_ptr()

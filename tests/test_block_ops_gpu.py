@@ -606,3 +606,26 @@ def test_forward_mode_tangents_are_refused(cuda, which):
                             call(p)
                     else:
                         call(p)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", [((3, 50, 64), 8), ((1, 60000, 32), 2), ((4, 1, 96), 32)])
+def test_group_norm_of_operands_at_any_address(cuda, dtype, shape, groups):
+    """Contiguous views into a flat buffer, of x and (by the gradient of a concatenation) of dy."""
+    from selectssm_b200 import group_norm_act
+    torch.manual_seed(17)
+    n = int(np.prod(shape))
+    flat = torch.randn(n + 3, device=cuda).to(dtype)
+    dy = torch.randn(n + 3, device=cuda).to(dtype)
+    x = flat[3:].view(shape)
+    assert x.is_contiguous() and x.data_ptr() % 16
+    runs = []
+    for xi, di in ((x.detach().requires_grad_(), dy), (x.clone().requires_grad_(), dy)):
+        y = group_norm_act(xi, groups=groups, activation="silu")
+        runs.append((y.detach(), *torch.autograd.grad(torch.cat([y.new_zeros(3), y.flatten()]), xi, di)))
+    xa = x.clone().requires_grad_()
+    ya = group_norm_act(xa, groups=groups, activation="silu")
+    runs.append((ya.detach(), *torch.autograd.grad(ya, xa, dy[3:].clone().view(shape))))
+    for other in runs[:2]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[2], other))
+    assert torch.equal(group_norm_act(x, groups=groups), group_norm_act(x.clone(), groups=groups))
