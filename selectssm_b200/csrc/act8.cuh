@@ -19,11 +19,18 @@ __device__ __forceinline__ float2 inv1p_ex2(float2 t) {
 // -2 z log2(e) as x (c1 + c3 x^2)
 constexpr float kGelu1 = -2.f * kGeluC * kLog2e, kGelu3 = kGelu1 * 0.044715f;
 
+// relu: NaN stays NaN (fmaxf would return the 0)
+__device__ __forceinline__ float relu1(float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 template <int ACT>
 __device__ __forceinline__ float2 act2(float2 x) {
   if constexpr (ACT == 1) return fmul2(x, inv1p_ex2(fmul2(x, dup2(-kLog2e))));
   if constexpr (ACT == 2) return fmul2(x, inv1p_ex2(fmul2(x, ffma2(fmul2(x, x), dup2(kGelu3), dup2(kGelu1)))));
-  if constexpr (ACT == 3) return make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f));
+  if constexpr (ACT == 3) return make_float2(relu1(x.x), relu1(x.y));
   return x;
 }
 
@@ -39,7 +46,7 @@ __device__ __forceinline__ float2 slope2(float2 x) {
     const float2 dz = ffma2(q, dup2(6.f * kGeluC * 0.044715f), dup2(2.f * kGeluC));
     return ffma2(fmul2(fmul2(x, s), fsub2(dup2(1.f), s)), dz, s);
   }
-  if constexpr (ACT == 3) return make_float2(x.x > 0.f ? 1.f : 0.f, x.y > 0.f ? 1.f : 0.f);
+  if constexpr (ACT == 3) return make_float2(x.x <= 0.f ? 0.f : 1.f, x.y <= 0.f ? 0.f : 1.f);  // 1 at NaN, as PyTorch's
   return dup2(1.f);
 }
 

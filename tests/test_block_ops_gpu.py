@@ -629,3 +629,56 @@ def test_group_norm_of_operands_at_any_address(cuda, dtype, shape, groups):
     for other in runs[:2]:
         assert all(torch.equal(a, b) for a, b in zip(runs[2], other))
     assert torch.equal(group_norm_act(x, groups=groups), group_norm_act(x.clone(), groups=groups))
+
+
+def _same(a, b):
+    return torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.nan_to_num(a), torch.nan_to_num(b))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [64, 61])
+def test_dropout_relu_passes_nan_on(cuda, dtype, cols):
+    """What is NaN where it is kept stays NaN, and its gradient is what torch's relu gives there."""
+    from selectssm_b200 import dropout_act
+    torch.manual_seed(18)
+    x = torch.randn(20, cols, device=cuda).to(dtype)
+    x[3, 5] = x[7, cols - 1] = x[19, 0] = float("nan")
+    x[4, 4], x[4, 5] = float("inf"), -float("inf")
+    dy = torch.randn(20, cols, device=cuda).to(dtype)
+    a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
+    ya, yb = dropout_act(a, 0.0, None, activation="relu"), torch.relu(b)
+    ga, gb = torch.autograd.grad(ya, a, dy)[0], torch.autograd.grad(yb, b, dy)[0]
+    assert _same(ya, yb) and _same(ga, gb)
+    keep = keep_mask(20, cols, 0.5, 6, 1)
+    y = dropout_act(x, 0.5, (6, 1), activation="relu")
+    assert torch.equal(torch.isnan(y), torch.isnan(x) & keep)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 9, 200])
+def test_dense_relu_passes_nan_on(cuda, dtype, rows):
+    from selectssm_b200 import dense_act
+    torch.manual_seed(19)
+    x, w = torch.randn(rows, 72, device=cuda).to(dtype), torch.randn(72, 40, device=cuda).to(dtype)
+    x[rows // 2, 7] = float("nan")
+    y = dense_act(x, w, activation="relu")
+    assert bool(torch.isnan(y[rows // 2]).all())
+    rest = [r for r in range(rows) if r != rows // 2]
+    assert bool(torch.isfinite(y[rest]).all()) and bool((y[rest] >= 0).all())
+    # torch's relu lets the gradient of a NaN through
+    xg = x.clone().requires_grad_()
+    g, = torch.autograd.grad(dense_act(xg, w, activation="relu"), xg, torch.ones_like(y))
+    want, = torch.autograd.grad(torch.relu(xg @ w), xg, torch.ones_like(y))
+    assert torch.equal(torch.isnan(g), torch.isnan(want))
+
+
+@pytest.mark.parametrize("shape,groups", [((2, 50, 64), 8), ((1, 60000, 32), 2), ((6, 1, 33), 11)])
+def test_group_norm_relu_passes_nan_on(cuda, shape, groups):
+    from selectssm_b200 import group_norm_act
+    x = torch.randn(shape, device=cuda)
+    x[0, -1, 5] = float("nan")
+    y = group_norm_act(x, groups=groups, activation="relu")
+    cg = shape[-1] // groups
+    hit = torch.zeros(shape, dtype=torch.bool, device=cuda)
+    hit[0, :, 5 // cg * cg:(5 // cg + 1) * cg] = True
+    assert torch.equal(torch.isnan(y), hit)
