@@ -396,18 +396,23 @@ static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
 // ---------------------------------------------------------------- forward and backward
 static bool few_rows(const ssm_dense_params_t* p) { return p->rows <= kFewRows && p->fin <= kFewMaxFin; }
 
+constexpr size_t kFewPart = 128 * 1024;  // most bytes of x a CTA holds
+
 template <typename T, int R, int CT, int V>
 static int launch_few(const ssm_dense_params_t* p, const DenseEpi& e, cudaStream_t s) {
   const int tiles = (int)ceil_div(p->fout, CT);
   // parts of fin: enough CTAs for the SMs, and at least 64 rows of the kernel each
   // (and few enough for x's part to fit: 16384 rows of 16 values need all eight)
   const int64_t useful = std::min<int64_t>({8, ceil_div(kSms, tiles), p->fin / 64});
-  const int parts = (int)std::max<int64_t>({1, useful, ceil_div((int64_t)p->fin * R * sizeof(float), 128 * 1024)});
+  const int parts = (int)std::max<int64_t>({1, useful, ceil_div((int64_t)p->fin * R * sizeof(float), kFewPart)});
   const size_t smem = (size_t)ceil_div(p->fin, parts) * R * sizeof(float) + R * sizeof(float);
   const auto kernel = dense_few_kernel<T, R, CT, V>;
   cudaError_t err;
   if (smem > 16 * 1024) {
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // The limit belongs to the kernel, not to this launch: always the same one (a part's, and
+    // a row for its rounding up and one behind it), as another thread may be launching too.
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)(kFewPart + 2 * R * sizeof(float)));
     if (err != cudaSuccess) return launch_error("cudaFuncSetAttribute(dense few rows)", err);
   }
   cudaLaunchConfig_t cfg = {};

@@ -1030,8 +1030,8 @@ static void gn_launch(const GnArgs& a, int act, bool bwd, cudaStream_t s) {
 template <typename T, int V, int ACT, bool BWD, bool SHORT>
 static cudaError_t gn_hold_launch(const GnArgs& a, const GnHold& h, cudaStream_t s) {
   const auto kernel = gn_hold_kernel<T, V, ACT, BWD, SHORT>;
-  if (h.smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)h.smem);
+  if (h.smem > 48 * 1024) {  // the kernel's limit, always the same: another thread may be launching it too
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kHoldSmem);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};

@@ -682,3 +682,52 @@ def test_group_norm_relu_passes_nan_on(cuda, shape, groups):
     hit = torch.zeros(shape, dtype=torch.bool, device=cuda)
     hit[0, :, 5 // cg * cg:(5 // cg + 1) * cg] = True
     assert torch.equal(torch.isnan(y), hit)
+
+
+@pytest.mark.parametrize("op", ["dense", "norm"])
+def test_threads_with_different_shapes(cuda, op):
+    """Launches of one kernel with different amounts of shared memory, from two host threads
+    at once: the C entries' calls alone, so that they overlap."""
+    import ctypes
+    import sys
+    import threading
+    from selectssm_b200 import _lib
+    torch.manual_seed(20)
+    lib, calls = _lib.load(), []
+    stream = torch.cuda.current_stream().cuda_stream
+    if op == "dense":  # 16 rows of fin / 8 values: 128 and 32 KB of shared memory
+        w = torch.randn(16384, 512, device=cuda)
+        for fin in (16384, 4096):
+            x, y = torch.randn(16, fin, device=cuda), torch.empty(16, 512, device=cuda)
+            p = _lib.SSMDenseParams()
+            p.rows, p.fin, p.fout = 16, fin, 512
+            p.x, p.kernel, p.y = x.data_ptr(), w.data_ptr(), y.data_ptr()
+            calls.append((lib.ssm_dense_act_fwd, p, x, y))
+    else:  # a batch row a CTA: 70 and 50 KB
+        for length in (260, 190):
+            x = torch.randn(512, length, 64, device=cuda)
+            y = torch.empty_like(x)
+            p = _lib.SSMGroupNormParams()
+            p.batch, p.seqlen, p.dim, p.groups, p.eps = 512, length, 64, 1, 1e-6
+            p.x, p.y = x.data_ptr(), y.data_ptr()
+            calls.append((lib.ssm_group_norm_act_fwd, p, x, y))
+    codes = [set(), set()]
+
+    def work(i):
+        f, p = calls[i][:2]
+        ref = ctypes.byref(p)
+        for _ in range(20000):
+            codes[i].add(f(ref, stream))
+
+    before = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(before)
+    torch.cuda.synchronize()
+    assert codes == [{_lib.SSM_OK}, {_lib.SSM_OK}]
