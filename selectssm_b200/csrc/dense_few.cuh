@@ -142,8 +142,8 @@ __global__ void __launch_bounds__(kFewThreads)
       add8(v[0], t);
     }
     dense_bias8(e, c, n0 + col, bias);
-    dense_epilogue<T, 1, false>(
-        e, c, m, 1, n0 + col, bias, v,
+    dense_epilogue<T, 1>(
+        e, c, m, n0 + col, bias, v,
         [&](float (&res)[1][8]) {
           get8<T>(e.residual, m * e.res_stride + n0 + col, e.N - n0 - col, c.vec_res, res[0]);
         },

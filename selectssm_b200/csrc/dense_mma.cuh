@@ -43,10 +43,6 @@ struct Planes {
   const __nv_bfloat16* base;
   int64_t plane, ld;
   bool k_major;  // rows are M (or N) and columns K; otherwise rows are K
-  __device__ __forceinline__ float at(int64_t mn, int64_t k) const {
-    const __nv_bfloat16* q = base + (k_major ? mn * ld + k : k * ld + mn);
-    return __bfloat162float(q[0]) + __bfloat162float(q[plane]) + __bfloat162float(q[2 * plane]);
-  }
 };
 
 struct DenseEpi {
@@ -116,12 +112,6 @@ __device__ __forceinline__ void act_rows(float (&v)[R][8]) {
   for (int q = 0; q < R; ++q) act8<ACT>(v[q]);
 }
 
-__device__ __noinline__ float dense_again(const DenseEpi& e, int64_t m, int n) {
-  float s = 0.f;
-  for (int64_t k = 0; k < e.K && !isnan(s); ++k) s = fmaf(e.a.at(m, k), e.b.at(n, k), s);
-  return s;
-}
-
 // bias of columns n .. n+7, zeros where there is none
 __device__ __forceinline__ void dense_bias8(const DenseEpi& e, const EpiConst& c, int n, float (&b)[8]) {
 #pragma unroll
@@ -132,33 +122,16 @@ __device__ __forceinline__ void dense_bias8(const DenseEpi& e, const EpiConst& c
 }
 
 // What an epilogue does to columns n .. n+7 of R rows (row, row + 32 / R, ...)
-// from the summed products v.  Only those less than `left` below `row` exist, and
-// only stores look at that: written stage by stage over all rows, the rows' chains
+// from the summed products v.  Not all of the rows exist, and only get_res and put
+// look at that: written stage by stage over all rows, the rows' chains
 // (ten dependent rounds of the generator, the activation) overlap.  The
 // instructions of this function are what an epilogue costs: issued beside the
 // warp that starts the tensor core's products, they delay it one for one.
 // get_res() gives the residual's values, put(base, v) stores to `pre` or `out`.
-template <typename T, int R, bool PLANES3, typename RES, typename PUT>
-__device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst& c, int64_t row, int left, int n,
+template <typename T, int R, typename RES, typename PUT>
+__device__ __forceinline__ void dense_epilogue(const DenseEpi& e, const EpiConst& c, int64_t row, int n,
                                                const float (&bias)[8], float (&v)[R][8], RES get_res, PUT put) {
   constexpr int RS = 32 / R;
-  if (PLANES3 && e.planes == 3) {
-    // An infinite operand has no finite planes besides its first, and infinity
-    // times the other operand's planes gives NaN where the product is infinite.
-    // Such elements are summed again from the fp32 values.
-    bool bad = false;
-#pragma unroll
-    for (int q = 0; q < R; ++q)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) bad |= isnan(v[q][i]);
-    if (bad) {
-#pragma unroll
-      for (int q = 0; q < R; ++q)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (isnan(v[q][i]) && q * RS < left && n + i < e.N) v[q][i] = dense_again(e, row + q * RS, n + i);
-    }
-  }
   if (e.bias)
 #pragma unroll
     for (int q = 0; q < R; ++q) add8(v[q], bias);
@@ -453,6 +426,15 @@ struct DenseWork {
   __device__ __forceinline__ int block(int split) const { return (int)((int64_t)kblocks * split / splits); }
 };
 
+__device__ __forceinline__ bool any_nan(const float (&v)[kCR][8]) {
+  bool bad = false;
+#pragma unroll
+  for (int q = 0; q < kCR; ++q)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bad |= isnan(v[q][i]);
+  return bad;
+}
+
 // A CTA of its own makes a tile of 128 x 128, a pair one of 256 x 256: each CTA
 // of it holds 128 rows of A and 128 columns of B and accumulates its 128 rows
 // of all 256 columns, so a step moves 32 KB into each SM for twice the products
@@ -477,6 +459,150 @@ struct Tile {
   static_assert(kEpiWarps * kAhead * 32 * kCW * 2 <= kStage);
   static constexpr int kBytes = kStages * kStage + kEpi + 1024;  // and alignment
 };
+
+// An infinite operand has no finite planes besides its first, and infinity times
+// the other operand's planes gives NaN where the product is infinite; so do
+// products of finite values that pass the type's largest.  A warp that met NaN in
+// a sum of three planes comes here after its last item, when nothing waits for it
+// any more, finds its chunks that hold NaN as they were stored, and sums them again
+// in fp32 from the operands' values: a rank-one step for each k, with a row of A
+// and a column of B a lane.  What was not NaN stays.  Where all sums of a chunk have
+// become NaN the rest of K changes nothing.  dW of 20011 x 2056 -> 2000, 0.93 ms: 4.6 with
+// an infinity in dy, 23 with a row of them, which makes every sum anew.
+constexpr int kDeep = 16;  // of K at a time: A's and B's values fill a warp's staged chunk
+
+// 32 rows (or columns) from `mn` by kDeep of K from `k` of one operand's planes, on
+// their way; `limit` rows exist, k ends at `end`.  Rows along K: a lane holds its own
+// row's.  Rows along mn: four lanes hold a k's 32 values.  Starts are multiples of 8
+// values, as are plane and ld, so that 16 bytes are loaded at a time.
+struct RepairLoad {
+  uint4 r[2][3];
+  __device__ __forceinline__ void load(const Planes& o, int lane, int64_t mn, int64_t limit, int64_t k, int64_t end) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int64_t row = o.k_major ? mn + lane : k + lane / 4 + 8 * j, col = o.k_major ? k + 8 * j : mn + lane % 4 * 8;
+      const bool in = o.k_major ? row < limit && col < end : row < end && col < limit;
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        r[j][p] = in ? *reinterpret_cast<const uint4*>(o.base + p * o.plane + row * o.ld + col) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  // the fp32 values to v[k][mn], zeros where k has ended
+  __device__ __forceinline__ void put(float* v, bool k_major, int lane, int64_t k, int64_t end) const {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float t[8], u[8];
+      unpack8(r[j][2], t);
+#pragma unroll
+      for (int p = 1; p >= 0; --p) {
+        unpack8(r[j][p], u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] += u[i];
+      }
+      if (k_major) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[(8 * j + i) * 32 + lane] = k + 8 * j + i < end ? t[i] : 0.f;
+      } else {
+        store8(v + (lane / 4 + 8 * j) * 32 + lane % 4 * 8, t);
+      }
+    }
+  }
+};
+
+// The sums of a chunk (its first row m of `rows`, column n of `cols`) over k .. end - 1,
+// left in its staged form.  A function of its own, and its operands by value: its loop
+// has no registers to spare for anything else.
+__device__ __noinline__ void dense_sum_again(const Planes pa, const Planes pb, const Stage st, int64_t m, int64_t rows,
+                                             int64_t n, int64_t cols, int64_t k, int64_t end) {
+  float acc[32] = {};
+  float* va = reinterpret_cast<float*>(st.s);  // [kDeep][32] of A, then of B
+  float* vb = va + kDeep * 32;
+  RepairLoad a, b;
+  a.load(pa, st.lane, m, rows, k, end);
+  b.load(pb, st.lane, n, cols, k, end);
+#pragma unroll 1
+  for (; k < end; k += kDeep) {
+    __syncwarp();
+    a.put(va, pa.k_major, st.lane, k, end);
+    b.put(vb, pb.k_major, st.lane, k, end);
+    a.load(pa, st.lane, m, rows, k + kDeep, end);
+    b.load(pb, st.lane, n, cols, k + kDeep, end);
+    __syncwarp();
+#pragma unroll 2
+    for (int i = 0; i < kDeep; ++i) {
+      const float y = vb[i * 32 + st.lane];
+#pragma unroll
+      for (int r = 0; r < 32; r += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(va + i * 32 + r);
+        acc[r] = fmaf(x.x, y, acc[r]);
+        acc[r + 1] = fmaf(x.y, y, acc[r + 1]);
+        acc[r + 2] = fmaf(x.z, y, acc[r + 2]);
+        acc[r + 3] = fmaf(x.w, y, acc[r + 3]);
+      }
+    }
+    bool all = true;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) all &= isnan(acc[r]) || m + r >= rows || n + st.lane >= cols;
+    if (__all_sync(0xffffffffu, all)) break;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int r = 0; r < 32; ++r) st.at(r, st.lane) = acc[r];
+  __syncwarp();
+}
+
+template <typename T>
+__device__ __noinline__ void dense_repair(const DenseEpi& e, const DenseWork w, const Stage st, int quarter, int col0) {
+  using S = Tile<false, T>;
+  const EpiConst c(e);
+  for (int item = blockIdx.x; item < w.tiles_m * w.tiles_n * w.splits; item += gridDim.x) {
+    const int rest = item / w.tiles_n, split = rest / w.tiles_m;
+    const int64_t m0 = (int64_t)(rest % w.tiles_m) * S::kM + quarter * 32;
+    const int64_t k0 = (int64_t)w.block(split) * kBK, k1 = min((int64_t)w.block(split + 1) * kBK, e.K);
+    for (int chunk = 0; chunk < S::kChunks; ++chunk) {
+      const int n = item % w.tiles_n * S::kN + col0 + chunk * kCW, nl = n + st.col();
+      if (n >= e.N || m0 >= e.M) break;
+      const int left = dense_left(e, m0, n, st);
+      // f(row, column) of this lane's elements
+      const auto each = [&](auto f) {
+#pragma unroll
+        for (int q = 0; q < kCR; ++q)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (q * kCStep < left && nl + i < e.N) f(q, i);
+      };
+      float* part = e.partial ? e.partial + ((int64_t)split * e.M + m0 + st.row()) * (e.per_row * 8) + nl : nullptr;
+      const auto stored = [&](void* base, int q, int i) -> T& {
+        return static_cast<T*>(base)[(m0 + st.row() + q * kCStep) * e.N + nl + i];
+      };
+      bool bad = false;
+      each([&](int q, int i) {
+        bad |= isnan(part ? part[(int64_t)(q * kCStep * 8) * e.per_row + i] : Cvt<T>::to_f(stored(e.pre ? e.pre : e.out, q, i)));
+      });
+      if (!__any_sync(0xffffffffu, bad)) continue;
+      dense_sum_again(e.a, e.b, st, m0, e.M, n, e.N, k0, k1);
+      float v[kCR][8], bias[8];
+      st.get(v);
+      if (part) {
+        each([&](int q, int i) {
+          float& p = part[(int64_t)(q * kCStep * 8) * e.per_row + i];
+          if (isnan(p)) p = v[q][i];
+        });
+        continue;
+      }
+      dense_bias8(e, c, nl, bias);
+      dense_epilogue<T, kCR>(
+          e, c, m0 + st.row(), nl, bias, v,
+          [&](float (&res)[kCR][8]) { dense_get_chunk<T>(e, c, st, m0, n, left, res); },
+          [&](void* base, const float (&u)[kCR][8]) {
+            each([&](int q, int i) {
+              T& p = stored(base, q, i);
+              if (isnan(Cvt<T>::to_f(p))) p = Cvt<T>::from_f(u[q][i]);
+            });
+          });
+    }
+  }
+}
 
 constexpr int kCut = 512 / kBK;  // most blocks that the leading accumulator of three planes takes
 constexpr int kCutsOfRest = 8;   // cuts that the other one takes
@@ -730,6 +856,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     for (int i = 0; i < S::kAhead; ++i) fetch();
     int acc = 0;
     uint32_t acc_phase = 0;
+    bool bad = false, ended = false;
     for (int item = first; item < items; item += stride) {
       const int rest = item / w.tiles_n, split = rest / w.tiles_m;
       const int n0 = item % w.tiles_n * BN + col0;
@@ -754,7 +881,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         // follows reads the sum
         src = at + 3 * BN;
         const int blocks = w.block(split + 1) - w.block(split), cut = even_cut(blocks);
-        bool ended = false;
         for (int b0 = 0; b0 < blocks; b0 += cut) {
           if (!__all_sync(0xffffffffu, wait(&acc_full[acc], acc_phase))) {
             ended = true;
@@ -812,14 +938,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         __syncwarp();
         float v[kCR][8];
         st.get(v);
+        if (PLANES == 3) bad |= any_nan(v);
         if (e.partial) {
           float* p = e.partial + ((int64_t)split * e.M + m0 + st.row()) * (e.per_row * 8) + nl;
 #pragma unroll
           for (int q = 0; q < kCR; ++q)
             if (q * kCStep < left) store8(p + (int64_t)(q * kCStep * 8) * e.per_row, v[q]);
         } else {
-          dense_epilogue<T, kCR, PLANES == 3>(
-              e, c, m0 + st.row(), left, nl, bias, v,
+          dense_epilogue<T, kCR>(
+              e, c, m0 + st.row(), nl, bias, v,
               [&](float (&res)[kCR][8]) {
                 if (ahead) {
                   asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -836,6 +963,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       if constexpr (PLANES == 1) release();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    if constexpr (PLANES == 3)
+      if (__any_sync(0xffffffffu, bad) && !ended) dense_repair<T>(e, w, st, quarter, col0);
   }
   __syncwarp();
   tmem_fence_before_sync();
@@ -893,8 +1022,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
     }
   }
   dense_bias8(e, c, nl, bias);
-  dense_epilogue<T, kCR, true>(
-      e, c, m0 + st.row(), left, nl, bias, v,
+  dense_epilogue<T, kCR>(
+      e, c, m0 + st.row(), nl, bias, v,
       [&](float (&res)[kCR][8]) { dense_get_chunk<T>(e, c, st, m0, n, left, res); },
       [&](void* base, const float (&u)[kCR][8]) { dense_put_chunk<T>(e, c, st, base, m0, n, left, u); });
 }

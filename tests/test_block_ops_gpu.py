@@ -731,3 +731,65 @@ def test_threads_with_different_shapes(cuda, op):
         sys.setswitchinterval(before)
     torch.cuda.synchronize()
     assert codes == [{_lib.SSM_OK}, {_lib.SSM_OK}]
+
+
+def _classes_agree(got, want, what=""):
+    """NaN where want is NaN, the same infinity where it is infinite."""
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    odd = torch.isinf(want)
+    assert torch.equal(got[odd].double(), want[odd]) and not bool(torch.isinf(got[~odd]).any()), what
+
+
+def test_dense_infinities_over_a_long_whole_sum(cuda):
+    """More tiles than CTAs, so that a kernel's gradient is summed over all rows by one CTA
+    each: with one infinity the other rows and columns keep their bits; with an infinite row,
+    which reaches every sum, each is infinite or NaN as its terms say; a NaN row is NaN throughout."""
+    from selectssm_b200 import dense_act
+    torch.manual_seed(21)
+    rows, fin, fout = 20011, 2056, 2000
+    x, dy = torch.randn(rows, fin, device=cuda), torch.randn(rows, fout, device=cuda)
+    w = torch.zeros(fin, fout, device=cuda, requires_grad=True)
+
+    def dw(x, dy):
+        return torch.autograd.grad(dense_act(x, w), w, dy)[0]
+
+    clean = dw(x, dy)
+    one = dy.clone()
+    one[19000, 7] = float("inf")
+    g = dw(x, one)
+    assert torch.equal(g[:, 7], torch.sign(x[19000]) * float("inf"))
+    rest = torch.arange(fout, device=cuda) != 7
+    assert torch.equal(g[:, rest], clean[:, rest])
+    dy[19990] = float("inf")
+    dy[5, 3] = -float("inf")
+    _classes_agree(dw(x, dy), x.double().t() @ dy.double())
+    dy[40] = float("nan")
+    assert bool(torch.isnan(dw(x, dy)).all())
+
+
+@pytest.mark.parametrize("sizes", [(300, 96, 257), (129, 5000, 136), (20000, 72, 40)])
+@pytest.mark.parametrize("act", ACTS)
+def test_dense_fp32_infinities_through_the_epilogue(cuda, sizes, act):
+    """Sums made again pass through bias, dropout, activation and residual like the others,
+    with and without `pre` kept; what no infinity reaches keeps its bits."""
+    from selectssm_b200 import dense_act
+    M, K, N = sizes
+    torch.manual_seed(22)
+    x, w = torch.randn(M, K, device=cuda), torch.randn(K, N, device=cuda) / K ** 0.5
+    b, res = torch.randn(N, device=cuda), torch.randn(M, N, device=cuda)
+    call = lambda x, w: dense_act(x, w, b, activation=act, residual=res, rate=0.3, rng=(8, 9))
+    clean = call(x, w)
+    x[2, 17], x[M - 1, K - 1], x[9, 0] = float("inf"), -float("inf"), 3.0e38
+    w[3, N - 1] = float("inf")
+    w[0, 5] = 1.0e6  # a product of finite values beyond the largest
+    keep = keep_mask(M, N, 0.3, 8, 9)
+    pre = x.double() @ w.double() + b.double()
+    u = drop64(torch.where(pre.abs() > 3.5e38, pre * float("inf"), pre), 0.3, keep)
+    want = act64(u, act) + res.double()
+    for y in (call(x, w), call(x.clone().requires_grad_(), w).detach()):
+        hit = torch.zeros(M, N, dtype=torch.bool, device=cuda)
+        hit[[2, 9, M - 1]] = True
+        hit[:, [5, N - 1]] = True
+        assert torch.equal(y[~hit], clean[~hit])
+        sure = hit & ~((u.abs() > 1e30) & torch.isfinite(u))  # (a sum next to the largest value may pass it)
+        _classes_agree(y[sure], want[sure])
