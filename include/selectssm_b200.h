@@ -321,7 +321,8 @@ typedef struct ssm_dense_params {
                                            as aligned)                                     */
   size_t workspace_bytes;
   int32_t* status;                      /* optional device word: nonzero after a device-side
-                                           failure (bounded wait gave up)                 */
+                                           failure (bounded wait gave up; the outputs that it
+                                           kept from being computed are NaN)              */
 } ssm_dense_params_t;
 
 SSM_API size_t ssm_dense_fwd_workspace_bytes(const ssm_dense_params_t* p);
@@ -344,6 +345,16 @@ SSM_API int ssm_selftest_wait_timeout(int32_t* status, uint32_t spin_limit, ssm_
  * stays usable.  The gradients it writes are undefined.  No counterpart in the
  * reference. */
 SSM_API int ssm_selftest_lookback_timeout(const ssm_params_t* p, uint32_t spin_limit, ssm_stream_t stream);
+
+/* Failure-path self-test of the dense products: runs ssm_dense_act_fwd on p
+ * (more than 16 rows, p->status set; otherwise SSM_ERR_SHAPE / SSM_ERR_NULL) but
+ * leaves out the loads of the last tile (of its last part, where the K loop is
+ * cut), so that its products wait for slices that never come.  Every wait gives
+ * up after spin_limit polls (2 .. 2^20), the kernel writes SSM_ERR_TIMEOUT to
+ * *p->status and returns, and the context stays usable.  That tile of y is NaN;
+ * with spin_limit above the polls that an ordinary wait takes the others are
+ * right.  */
+SSM_API int ssm_selftest_dense_timeout(const ssm_dense_params_t* p, uint32_t spin_limit, ssm_stream_t stream);
 
 /* Message for a status code (static storage). */
 SSM_API const char* ssm_strerror(int status);

@@ -49,6 +49,7 @@ EXPORTED_SYMBOLS = (
     "ssm_group_norm_fwd_workspace_bytes", "ssm_group_norm_bwd_workspace_bytes",
     "ssm_group_norm_act_fwd", "ssm_group_norm_act_bwd",
     "ssm_dense_fwd_workspace_bytes", "ssm_dense_bwd_workspace_bytes", "ssm_dense_act_fwd", "ssm_dense_act_bwd",
+    "ssm_selftest_dense_timeout",
 )
 
 
@@ -189,6 +190,7 @@ def load(path: str | None = None) -> ctypes.CDLL:
         "ssm_dense_act_bwd": (ctypes.c_int, [LP, ctypes.c_void_p]),
         "ssm_selftest_wait_timeout": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p]),
         "ssm_selftest_lookback_timeout": (ctypes.c_int, [ctypes.POINTER(SSMParams), ctypes.c_uint32, ctypes.c_void_p]),
+        "ssm_selftest_dense_timeout": (ctypes.c_int, [LP, ctypes.c_uint32, ctypes.c_void_p]),
         "ssm_strerror": (ctypes.c_char_p, [ctypes.c_int]),
         "ssm_last_error": (ctypes.c_char_p, []),
         "ssm_version": (ctypes.c_char_p, []),

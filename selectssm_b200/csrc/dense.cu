@@ -361,12 +361,22 @@ static int launch_mma(const DenseEpi& e, const Plan& q, const CUtensorMap& ma, c
   return err == cudaSuccess ? SSM_OK : launch_error("launch dense product kernel", err);
 }
 
+// The bounds of a product's waits; `omit` leaves the last item's loads out (the self-test).
+struct DenseWait {
+  int32_t* status;
+  uint32_t spin;
+  bool omit;
+};
+
 // e.M, e.N, e.K, e.a, e.b and the epilogue are set; `part` holds plan_product's part_bytes.
 template <bool A_MN, bool B_MN, typename T>
-static int product(DenseEpi e, float* part, int32_t* status, cudaStream_t s) {
-  const Plan q = plan_product(e.M, e.N, e.K, e.planes);
+static int product(DenseEpi e, float* part, const DenseWait& wait, cudaStream_t s) {
+  Plan q = plan_product(e.M, e.N, e.K, e.planes);
+  int32_t* status = wait.status;
   e.per_row = (e.N + 7) / 8;
   if ((int64_t)q.w.tiles_m * q.w.tiles_n * q.w.splits > 0x7fffffff) return SSM_ERR_SHAPE;
+  q.w.loaded = q.w.tiles_m * q.w.tiles_n * q.w.splits - (wait.omit ? 1 : 0);
+  q.w.spin = wait.spin;
   CUtensorMap ma, mb;
   if (!operand_map(&ma, e.a, A_MN ? e.K : e.M, A_MN ? e.M : e.K, e.planes) ||
       !operand_map(&mb, e.b, B_MN ? e.K : e.N, B_MN ? e.N : e.K, e.planes))
@@ -440,7 +450,7 @@ static int dense_few(const ssm_dense_params_t* p, const DenseEpi& e, cudaStream_
   return ceil_div(p->fout, 64) * 8 >= kSms ? launch_few<T, 1, 64, 8>(p, e, s) : launch_few<T, 1, 32, 8>(p, e, s);
 }
 
-static int dense_fwd(const ssm_dense_params_t* p, cudaStream_t s) {
+static int dense_fwd(const ssm_dense_params_t* p, const DenseWait& wait, cudaStream_t s) {
   char* ws = static_cast<char*>(p->workspace);
   DenseEpi e = {};
   int st = SSM_OK;
@@ -469,8 +479,8 @@ static int dense_fwd(const ssm_dense_params_t* p, cudaStream_t s) {
   e.rng = drop_rng(p);
   if (few) return p->dtype == SSM_BF16 ? dense_few<__nv_bfloat16>(p, e, s) : dense_few<float>(p, e, s);
   float* part = reinterpret_cast<float*>(ws);
-  return p->dtype == SSM_BF16 ? product<false, true, __nv_bfloat16>(e, part, p->status, s)
-                              : product<false, true, float>(e, part, p->status, s);
+  return p->dtype == SSM_BF16 ? product<false, true, __nv_bfloat16>(e, part, wait, s)
+                              : product<false, true, float>(e, part, wait, s);
 }
 
 // How the dpre pass cuts (rows, fout): cb blocks of eight columns a CTA, `run` rows.
@@ -543,7 +553,7 @@ static BwdBytes bwd_bytes(const ssm_dense_params_t* p) {
   return b;
 }
 
-static int dense_bwd(const ssm_dense_params_t* p, cudaStream_t s) {
+static int dense_bwd(const ssm_dense_params_t* p, const DenseWait& wait, cudaStream_t s) {
   const int pl = planes_of(p), N = p->fout, K = p->fin, ld = pad8(N);
   const BwdBytes bytes = bwd_bytes(p);
   char* ws = static_cast<char*>(p->workspace);
@@ -581,8 +591,8 @@ static int dense_bwd(const ssm_dense_params_t* p, cudaStream_t s) {
     e.N = K;
     e.K = N;
     e.out = p->dx;
-    st = p->dtype == SSM_BF16 ? product<false, false, __nv_bfloat16>(e, part, p->status, s)
-                              : product<false, false, float>(e, part, p->status, s);
+    st = p->dtype == SSM_BF16 ? product<false, false, __nv_bfloat16>(e, part, wait, s)
+                              : product<false, false, float>(e, part, wait, s);
     if (st) return st;
   }
   if (p->dkernel) {  // (rows, fin)^T (rows, fout)
@@ -593,8 +603,8 @@ static int dense_bwd(const ssm_dense_params_t* p, cudaStream_t s) {
     e.N = N;
     e.K = p->rows;
     e.out = p->dkernel;
-    st = p->dkernel_dtype == SSM_BF16 ? product<true, true, __nv_bfloat16>(e, part, p->status, s)
-                                      : product<true, true, float>(e, part, p->status, s);
+    st = p->dkernel_dtype == SSM_BF16 ? product<true, true, __nv_bfloat16>(e, part, wait, s)
+                                      : product<true, true, float>(e, part, wait, s);
   }
   return st;
 }
@@ -602,6 +612,18 @@ static int dense_bwd(const ssm_dense_params_t* p, cudaStream_t s) {
 }  // namespace ssm
 
 using namespace ssm;
+
+static int dense_fwd_call(const ssm_dense_params_t* p, const DenseWait& wait, ssm_stream_t stream) {
+  int st = check_dense(p);
+  if (st) return st;
+  if (p->rows == 0) return SSM_OK;
+  if (!p->x || !p->kernel || !p->y) return SSM_ERR_NULL;
+  const size_t need = ssm_dense_fwd_workspace_bytes(p);
+  if (need && (!p->workspace || p->workspace_bytes < need)) return SSM_ERR_WORKSPACE;
+  st = bind_device(p->x);
+  if (st) return st;
+  return dense_fwd(p, wait, reinterpret_cast<cudaStream_t>(stream));
+}
 
 extern "C" {
 
@@ -617,16 +639,15 @@ size_t ssm_dense_bwd_workspace_bytes(const ssm_dense_params_t* p) {
 }
 
 int ssm_dense_act_fwd(const ssm_dense_params_t* p, ssm_stream_t stream) {
+  return dense_fwd_call(p, {p ? p->status : nullptr, kMmaSpin, false}, stream);
+}
+
+int ssm_selftest_dense_timeout(const ssm_dense_params_t* p, uint32_t spin_limit, ssm_stream_t stream) {
   int st = check_dense(p);
   if (st) return st;
-  if (p->rows == 0) return SSM_OK;
-  if (!p->x || !p->kernel || !p->y) return SSM_ERR_NULL;
-  const size_t need = ssm_dense_fwd_workspace_bytes(p);
-  if (need && (!p->workspace || p->workspace_bytes < need)) return SSM_ERR_WORKSPACE;
-  st = bind_device(p->x);
-  if (st) return st;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return dense_fwd(p, s);
+  if (!p->status) return SSM_ERR_NULL;
+  if (p->rows == 0 || few_rows(p) || spin_limit < 2 || spin_limit > kMmaSpin) return SSM_ERR_SHAPE;
+  return dense_fwd_call(p, {p->status, spin_limit, true}, stream);
 }
 
 int ssm_dense_act_bwd(const ssm_dense_params_t* p, ssm_stream_t stream) {
@@ -651,7 +672,7 @@ int ssm_dense_act_bwd(const ssm_dense_params_t* p, ssm_stream_t stream) {
   if (!p->workspace || p->workspace_bytes < ssm_dense_bwd_workspace_bytes(p)) return SSM_ERR_WORKSPACE;
   st = bind_device(p->dy);
   if (st) return st;
-  return dense_bwd(p, s);
+  return dense_bwd(p, {p->status, kMmaSpin, false}, s);
 }
 
 }  // extern "C"

@@ -284,6 +284,8 @@ constexpr int kEpiWarps = 8;
 constexpr int kMmaThreads = 32 * (4 + kEpiWarps);
 // Polls before a wait gives up; a tile takes microseconds, so this is far above any wait that ends.
 constexpr uint32_t kMmaSpin = 1u << 20;
+// Polls for what is still under way when one has given up.
+constexpr uint32_t kDrainSpin = 1u << 16;
 
 // Shared-memory operand descriptor, 128-byte swizzle.  K-major rows of 128
 // bytes: groups of 8 rows are 1024 bytes apart.  MN-major rows (one k each, 64
@@ -320,14 +322,14 @@ struct Mma {
           "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
           : "memory");
   }
-  // arrives on `bar` (of both CTAs of a pair) when the products issued so far are done
-  __device__ __forceinline__ static void commit(uint64_t* bar, uint32_t one) {
+  // arrives on `bar` (of a pair's CTAs in `mask`) when the products issued so far are done
+  __device__ __forceinline__ static void commit(uint64_t* bar, uint32_t one, uint16_t mask = 3) {
     if constexpr (PAIR)
       asm volatile(
           "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
           "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::
               "r"(smem_u32(bar)),
-          "h"((uint16_t)3), "r"(one)
+          "h"(mask), "r"(one)
           : "memory");
     else
       asm volatile(
@@ -422,6 +424,8 @@ __device__ __forceinline__ void wait_through(uint64_t* bar, uint32_t parity, uin
 struct DenseWork {
   int32_t tiles_m, tiles_n, splits;
   int32_t kblocks;  // ceil(K / 64)
+  int32_t loaded;   // items whose slices are loaded: all, except in the self-test of a wait that gives up
+  uint32_t spin;    // polls before a wait gives up, 2 at least
   // the 64-deep blocks of a split
   __device__ __forceinline__ int block(int split) const { return (int)((int64_t)kblocks * split / splits); }
 };
@@ -604,6 +608,31 @@ __device__ __noinline__ void dense_repair(const DenseEpi& e, const DenseWork w, 
   }
 }
 
+// NaN for a warp's 32 rows by `cols` columns of the items from `item` on, whose products never came.
+template <typename T>
+__device__ __noinline__ void dense_poison(const DenseEpi& e, const DenseWork w, int lane, int item, int stride, int tile_m,
+                                          int row0, int tile_n, int col0, int cols) {
+  const float nan = __uint_as_float(0x7fc00000u);
+  for (; item < w.tiles_m * w.tiles_n * w.splits; item += stride) {
+    const int rest = item / w.tiles_n, split = rest / w.tiles_m;
+    const int64_t m0 = (int64_t)(rest % w.tiles_m) * tile_m + row0;
+    const int rows = (int)min(e.M - m0, (int64_t)32);
+    for (int j = lane; j < cols; j += 32) {
+      const int64_t n = (int64_t)(item % w.tiles_n) * tile_n + col0 + j;
+      if (n >= e.N) break;
+      for (int r = 0; r < rows; ++r) {
+        const int64_t at = (m0 + r) * e.N + n;
+        if (e.partial) {
+          e.partial[((int64_t)split * e.M + m0 + r) * (e.per_row * 8) + n] = nan;
+        } else {
+          static_cast<T*>(e.out)[at] = Cvt<T>::from_f(nan);
+          if (e.pre) static_cast<T*>(e.pre)[at] = Cvt<T>::from_f(nan);
+        }
+      }
+    }
+  }
+}
+
 constexpr int kCut = 512 / kBK;  // most blocks that the leading accumulator of three planes takes
 constexpr int kCutsOfRest = 8;   // cuts that the other one takes
 // cuts of a split as even as they go
@@ -622,7 +651,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   static_assert(PLANES == 1 || (PLANES == 3 && !PAIR && S::kStages % 3 == 0));
   constexpr int kTmem = PLANES == 3 ? 4 * BN : 2 * BN;
   extern __shared__ uint8_t raw[];
-  __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2], drained;
   __shared__ uint32_t tmem_base;
   __shared__ volatile int dead;
   uint8_t* tiles = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
@@ -637,6 +666,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], PAIR ? 2 * kEpiWarps : kEpiWarps);
     }
+    mbar_init(&drained, 1);
     dead = 0;
     fence_mbar_init();
     tma_prefetch_desc(&map_a);
@@ -654,9 +684,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   const int stages = ahead ? S::kStages - 1 : S::kStages;
   const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
 
-  // Bounded wait; a role that gives up (or sees that another did) stops.
+  // Bounded wait; a role that gives up (or sees that another did) stops.  Outputs
+  // whose products never came are NaN then, and what is under way (loads, products)
+  // is waited for before the CTA leaves.
   const auto wait = [&](uint64_t* bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kMmaSpin; ++i) {
+    for (uint32_t i = 0; i < w.spin; ++i) {
       if (mbar_try_wait(bar, parity)) return true;
       if ((i & 63) == 63 && dead) return false;
     }
@@ -676,8 +708,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     const bool of_a = warp == 0;
     const uint32_t one = elect_one();
     int stage = 0;
-    uint32_t phase = 0, polls = kMmaSpin;
-    for (int item = first; item < items; item += stride) {
+    uint32_t phase = 0, polls = w.spin;
+    for (int item = first; item < w.loaded; item += stride) {
       const int rest = item / w.tiles_n, split = rest / w.tiles_m;
       const int n0 = item % w.tiles_n * BN + (PAIR ? rank * 128 : 0);
       const int m0 = rest % w.tiles_m * S::kM + (PAIR ? rank * 128 : 0);
@@ -721,24 +753,27 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     if (polls == 1) {
       dead = 1;
       if (one) report(status, kStatusTimeout);
-      // Loads still in flight: wait for the last ones so that none lands after
-      // the CTA has gone.
-      if (rank == 0)
-        for (int i = 0; i < stages; ++i) {
-          mbar_wait_bounded(&full[stage], phase ^ 1, 1u << 16);
-          if (++stage == stages) {
-            stage = 0;
-            phase ^= 1;
-          }
-        }
     }
+    // No load may land after the CTA has gone: the last one of each stage is waited
+    // for, whoever gave up (otherwise the products have waited for them).
+    if (of_a && rank == 0)
+      for (int i = 0; i < stages; ++i) {
+        mbar_wait_bounded(&full[stage], phase ^ 1, kDrainSpin);
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
   } else if (warp == 1 && rank == 0) {
     constexpr uint32_t idesc = mma_idesc(S::kM, BN, A_MN, B_MN);
     constexpr uint32_t kStepA = (A_MN ? 2048 : 32) >> 4, kStepB = (B_MN ? 2048 : 32) >> 4;
     const uint32_t one = elect_one();
     const uint64_t da0 = smem_desc(smem_u32(tiles)), db0 = smem_desc(smem_u32(tiles + S::kA));
     int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0, polls = kMmaSpin;
+    uint32_t phase = 0, acc_phase = 0, polls = w.spin;
+    // asked once an item (or cut), of the whole warp: a branch on one lane's count would
+    // cost the loop its uniform operands
+    const auto gave_up = [&] { return __any_sync(0xffffffffu, polls == 1); };
     // the four products of one plane of A with one of B, from stages sa and sb
     const auto block = [&](uint32_t d, int sa, int sb, bool add) {
       const uint64_t da = da0 + sa * (S::kStage >> 4), db = db0 + sb * (S::kStage >> 4);
@@ -757,6 +792,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           wait_through(&acc_empty[acc], acc_phase ^ 1, polls);
           // the last cut has been taken, the accumulator of the rest with it
           if (fresh && (b0 > 0 || item != first)) wait_through(&acc_empty[acc ^ 1], acc ? acc_phase : acc_phase ^ 1, polls);
+          if (gave_up()) break;  // what the products would overwrite may still be read
           tmem_fence_after_sync();
           const uint32_t lead = tmem + acc * BN;
           for (int b = b0; b < b1; ++b) {
@@ -781,14 +817,17 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
               phase ^= 1;
             }
           }
+          if (gave_up()) break;  // these are products of what was never loaded
           I::commit(&acc_full[acc], one);
           if (++acc == 2) {
             acc = 0;
             acc_phase ^= 1;
           }
         }
+        if (gave_up()) break;
       } else {
         wait_through(&acc_empty[acc], acc_phase ^ 1, polls);
+        if (gave_up()) break;
         tmem_fence_after_sync();
         const uint32_t d = tmem + acc * BN;
         wait_through(&full[stage], phase, polls);
@@ -803,6 +842,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           I::commit(&empty[used], one);
           if (b + 1 < blocks) wait_through(&full[stage], phase, polls);
         }
+        if (gave_up()) break;
         I::commit(&acc_full[acc], one);
         if (++acc == 2) {
           acc = 0;
@@ -810,10 +850,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         }
       }
     }
-    if (polls == 1) {
+    if (gave_up()) {
       dead = 1;
       if (one) report(status, kStatusTimeout);
-      mbar_wait_bounded(&acc_full[acc ^ 1], acc_phase ^ (acc == 0), 1u << 16);  // products still running use the buffers
+      I::commit(&drained, one, 1);  // products still running use the buffers
+      mbar_wait_bounded(&drained, 0, kDrainSpin);
     }
   } else if (warp >= 4) {
     const EpiConst c(e);
@@ -857,7 +898,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     int acc = 0;
     uint32_t acc_phase = 0;
     bool bad = false, ended = false;
-    for (int item = first; item < items; item += stride) {
+    int item = first;
+    for (; item < items; item += stride) {
       const int rest = item / w.tiles_n, split = rest / w.tiles_m;
       const int n0 = item % w.tiles_n * BN + col0;
       const int64_t m0 = (int64_t)(rest % w.tiles_m) * S::kM + rank * 128 + quarter * 32;
@@ -909,7 +951,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         }
         if (ended) break;
       } else {
-        if (!__all_sync(0xffffffffu, wait(&acc_full[acc], acc_phase))) break;
+        if (!__all_sync(0xffffffffu, wait(&acc_full[acc], acc_phase))) {
+          ended = true;
+          break;
+        }
         tmem_fence_after_sync();
       }
 #pragma unroll 1
@@ -963,6 +1008,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       if constexpr (PLANES == 1) release();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    if (ended) dense_poison<T>(e, w, lane, item, stride, S::kM, rank * 128 + quarter * 32, BN, col0, S::kCols);
     if constexpr (PLANES == 3)
       if (__any_sync(0xffffffffu, bad) && !ended) dense_repair<T>(e, w, st, quarter, col0);
   }
