@@ -22,6 +22,8 @@ another offset.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
@@ -252,11 +254,32 @@ def group_norm_act(x, scale=None, bias=None, groups=32, eps=1e-6, activation=Non
 
 
 # ----------------------------------------------------------------------------- dense layer
+_status = {}  # device index -> (pinned word, the same as a C integer)
+
+
+def _status_word(index):
+    """Address of the word in which the device's dense kernels say that a bounded
+    wait gave up (the outputs that it held up are NaN).  It lies in host memory, so
+    that asking for it waits for nothing: what an earlier call has left there by
+    now is raised here."""
+    word = _status.get(index)
+    if word is None:
+        t = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+        word = _status.setdefault(index, (t, ctypes.c_int32.from_address(t.data_ptr())))
+    code = word[1].value
+    if code:
+        word[1].value = 0
+        _lib.check(code, f"an earlier dense_act call on cuda:{index}")
+    return word[0].data_ptr()
+
+
 def _dense_params(x, xs, w, b, drop, rng, act):
     code = _DT[x.dtype]
     fin, fout = w.shape
-    return _lib.SSMDenseParams(x.numel() // fin, fin, fout, code, code if b is None else _DT[b.dtype], code, act, drop,
-                               rng[0], rng[1], _ptr(rng[2]), xs, 0, 0, x.data_ptr(), w.data_ptr(), _ptr(b))
+    p = _lib.SSMDenseParams(x.numel() // fin, fin, fout, code, code if b is None else _DT[b.dtype], code, act, drop,
+                            rng[0], rng[1], _ptr(rng[2]), xs, 0, 0, x.data_ptr(), w.data_ptr(), _ptr(b))
+    p.status = _status_word(x.get_device())
+    return p
 
 
 def _dense_forward(x, w, bias, residual, act, drop, rng, keep_pre):
@@ -325,7 +348,10 @@ def dense_act(x, kernel, bias=None, activation=None, residual=None, rate=0.0, rn
     to the (..., fout) output.  Products are summed in fp32; float32 operands
     keep fp32 accuracy.  ``rate`` and ``rng`` as in :func:`dropout_act`, over
     rows of fout columns.  For the backward an activation's input is kept in
-    x's type."""
+    x's type.
+
+    The kernels' waits are bounded.  Should one give up, the outputs that it held
+    up are NaN and the next dense call on the device raises SSMLibraryError."""
     _check_devices(x, kernel, bias, residual)
     _dtype_code(x), _dtype_code(kernel)
     if kernel.dim() != 2 or x.dim() < 1 or x.shape[-1] != kernel.shape[0] or min(kernel.shape) < 1:

@@ -143,3 +143,13 @@ def test_dense_operands_are_aligned():
         d = _dense(t)
         assert d.is_contiguous() and d.data_ptr() % 16 == 0 and torch.equal(d, t)
     assert _dense(flat) is flat and _dense(flat[4:20]).data_ptr() == flat[4:20].data_ptr()
+
+
+def test_a_wait_that_gave_up_is_raised_once(monkeypatch):
+    word = torch.zeros(1, dtype=torch.int32)
+    monkeypatch.setitem(block_ops._status, 7, (word, ctypes.c_int32.from_address(word.data_ptr())))
+    assert block_ops._status_word(7) == word.data_ptr()
+    word[0] = _lib.SSM_ERR_TIMEOUT
+    with pytest.raises(_lib.SSMLibraryError, match="an earlier dense_act call on cuda:7.*wait"):
+        block_ops._status_word(7)
+    assert block_ops._status_word(7) == word.data_ptr() and int(word) == 0

@@ -65,3 +65,40 @@ def test_refusals_of_the_self_test():
     assert lib.ssm_selftest_dense_timeout(ctypes.byref(p), (1 << 20) + 1, None) == _lib.SSM_ERR_SHAPE
     p.rows = 16
     assert lib.ssm_selftest_dense_timeout(ctypes.byref(p), 100, None) == _lib.SSM_ERR_SHAPE
+
+
+@pytest.mark.parametrize("where", ["forward", "backward"])
+def test_dense_act_raises_what_an_earlier_call_left(cuda, where):
+    from selectssm_b200 import _lib, block_ops, dense_act
+    x, w = torch.randn(200, 64, device=cuda, requires_grad=True), torch.randn(64, 72, device=cuda)
+    want = dense_act(x, w)  # its status word is the device's
+    p, ws = _params(x, w, torch.empty_like(want), torch.empty_like(want), want)
+    p.status = block_ops._status_word(x.get_device())
+    assert _lib.load().ssm_selftest_dense_timeout(ctypes.byref(p), 1 << 14, torch.cuda.current_stream().cuda_stream) == _lib.SSM_OK
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.SSMLibraryError, match="earlier dense_act call"):
+        dense_act(x, w) if where == "forward" else torch.autograd.grad(want.sum(), x, retain_graph=True)
+    assert torch.equal(dense_act(x, w), want)
+    torch.autograd.grad(want.sum(), x)
+
+
+def test_first_call_under_capture(cuda):
+    """In a process of its own, where no call has made the status word yet."""
+    import os
+    import subprocess
+    import sys
+    code = """if True:
+        import torch
+        from selectssm_b200 import dense_act
+        x, w = torch.randn(200, 64, device="cuda"), torch.randn(64, 72, device="cuda")
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = dense_act(x, w)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, dense_act(x, w))
+        """
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
