@@ -338,6 +338,9 @@ class BidirectionalMamba(nn.Module):
         if rate > 0:
             first = dropout_rng
             if first is None:  # as PyTorch's dropout: from its default (CPU) generator
+                if x.is_cuda and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("a captured graph would replay one dropout mask for ever: give dropout_rng, an "
+                                       "int64 CUDA tensor (seed, offset) that the program changes between replays")
                 first = tuple(torch.randint(0, 2 ** 62, (2,)).tolist())
             if torch.is_tensor(first):
                 second = torch.stack((first[0], first[1] + 1))
@@ -350,7 +353,7 @@ class BidirectionalMamba(nn.Module):
         """x: (B, L, features).  ``dropout_rng``: (seed, offset) of this call's MLP
         dropout with ``fused_block``, two integers or an int64 CUDA tensor of
         them; a call uses offset and offset + 1.  Without it they are drawn from
-        PyTorch's default generator."""
+        PyTorch's default generator on the host, which a graph's capture refuses."""
         skip = x                                                                 # :300
         base = None
         if self.norm_type == "rms":  # one kernel: the norm and the residual base skip + out_proj.bias

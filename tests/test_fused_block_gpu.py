@@ -72,3 +72,30 @@ def test_example_learns(cuda, monkeypatch):
     monkeypatch.setattr(sys, "argv", ["train_block.py", "--steps", "60", "--length", "128", "--width", "64"])
     first, last = example.main()
     assert first > 1.0 and last < 0.8 * first  # chance is log 4
+
+
+def test_a_captured_step_needs_a_device_rng(cuda):
+    """Seeds drawn on the host would be frozen into the graph with their mask."""
+    _, m = _pair(cuda, norm_type="group", mlp_dropout_rate=0.3)
+    x = torch.randn(2, 50, 64, device=cuda)
+    rng = torch.tensor([1, 2], dtype=torch.int64, device=cuda)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad(), torch.cuda.stream(side):
+        m(x, train=True)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="dropout_rng"):
+            m(x, train=True)
+        y = m(x, train=True, dropout_rng=rng)
+        m(x)  # nothing is drawn
+    outs = []
+    for offset in (2, 4):
+        rng[1] = offset
+        graph.replay()
+        torch.cuda.synchronize()
+        outs.append(y.clone())
+        with torch.no_grad():
+            assert torch.equal(y, m(x, train=True, dropout_rng=(1, offset)))
+    assert not torch.equal(*outs)
