@@ -354,6 +354,8 @@ class BidirectionalMamba(nn.Module):
         dropout with ``fused_block``, two integers or an int64 CUDA tensor of
         them; a call uses offset and offset + 1.  Without it they are drawn from
         PyTorch's default generator on the host, which a graph's capture refuses."""
+        if dropout_rng is not None and not self.fused_block:
+            raise ValueError("dropout_rng needs fused_block=True; without it dropout draws from PyTorch's generator")
         skip = x                                                                 # :300
         base = None
         if self.norm_type == "rms":  # one kernel: the norm and the residual base skip + out_proj.bias

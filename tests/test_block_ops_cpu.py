@@ -153,3 +153,11 @@ def test_a_wait_that_gave_up_is_raised_once(monkeypatch):
     with pytest.raises(_lib.SSMLibraryError, match="an earlier dense_act call on cuda:7.*wait"):
         block_ops._status_word(7)
     assert block_ops._status_word(7) == word.data_ptr() and int(word) == 0
+
+
+def test_dropout_rng_without_the_fused_block_is_refused():
+    """The unfused block's dropout draws from torch's generator and would ignore it."""
+    from selectssm_b200 import BidirectionalMamba
+    m = BidirectionalMamba(32, hidden_features=16, expansion_factor=1, mlp_layer=True)
+    with pytest.raises(ValueError, match="fused_block"):
+        m(torch.zeros(1, 8, 32), train=True, dropout_rng=(1, 2))
