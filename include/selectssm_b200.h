@@ -57,7 +57,8 @@ enum ssm_status {
   SSM_ERR_LAUNCH = 3,           /* CUDA launch / driver error */
   SSM_ERR_TIMEOUT = 4,          /* a bounded device-side wait gave up (status word) */
   SSM_ERR_NULL = 5,             /* a required pointer is NULL */
-  SSM_ERR_ALIGN = 6,            /* pointer / stride alignment not met (16 bytes) */
+  SSM_ERR_ALIGN = 6,            /* pointer / stride alignment not met (16 bytes; workspaces 256, and where
+                                   a struct says less, an element's own size)  */
   SSM_ERR_WORKSPACE = 7         /* workspace missing or too small */
 };
 
@@ -236,7 +237,8 @@ SSM_API int ssm_rmsnorm_bwd(const ssm_norm_params_t* p, ssm_stream_t stream);
  * column c of row r takes the 16 bits number c % 8 of the 128 bits that
  * Philox4x32-10 gives for the counter (r * ceil(dim / 8) + c / 8, offset)
  * under the key seed, and is kept when they are >= drop.  A dropped element
- * contributes act(0) and no gradient, whatever x holds there.  */
+ * contributes act(0) and no gradient, whatever x holds there.  Tensors may start
+ * at any element, rng at 8 bytes; rows that start at 16 bytes move faster.  */
 typedef struct ssm_dropout_params {
   int64_t rows;
   int32_t dim;                          /* columns, >= 1 */
@@ -261,7 +263,8 @@ SSM_API int ssm_dropout_act_bwd(const ssm_dropout_params_t* p, ssm_stream_t stre
  * "group") over x (batch, seqlen, dim): mean and variance of each of `groups`
  * runs of dim / groups channels over the whole sequence, then
  * y = act((x - mean) * rstd * scale + bias).  The backward writes dx, dscale
- * and dbias; every sum is formed in a fixed order.  */
+ * and dbias; every sum is formed in a fixed order.  x, y, dy and dx start at 16
+ * bytes where dim is a multiple of 8 and at any element otherwise, stats at 8.  */
 typedef struct ssm_group_norm_params {
   int64_t batch, seqlen;
   int32_t dim, groups;                  /* groups divides dim */
@@ -293,7 +296,7 @@ SSM_API int ssm_group_norm_act_bwd(const ssm_group_norm_params_t* p, ssm_stream_
  * The backward writes those of dx, dkernel and dbias that are not NULL; the
  * residual's gradient is dy itself.  Sums are held in fp32; with bf16 the
  * operands of the products (x, W, and in the backward the gradient of the
- * pre-activation) are bf16.  */
+ * pre-activation) are bf16.  Tensors may start at any element, rng at 8 bytes.  */
 typedef struct ssm_dense_params {
   int64_t rows;
   int32_t fin, fout;                    /* >= 1 */

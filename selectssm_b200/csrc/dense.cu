@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(256, kDpreCtas)
 
 // ---------------------------------------------------------------- checks and sizes
 static bool known(int dtype) { return dtype == SSM_F32 || dtype == SSM_BF16; }
+static size_t elem_bytes(int dtype) { return dtype == SSM_BF16 ? 2 : 4; }
 
 static int check_dense(const ssm_dense_params_t* p) {
   if (!p) return SSM_ERR_NULL;
@@ -233,11 +234,15 @@ static int check_dense(const ssm_dense_params_t* p) {
       (p->dy_stride && p->dy_stride < p->fout))
     return SSM_ERR_SHAPE;
   if (!known(p->dtype) || !known(p->bias_dtype) || !known(p->dkernel_dtype)) return SSM_ERR_DTYPE;
+  if (!all_aligned(elem_bytes(p->dtype), {p->x, p->kernel, p->residual, p->y, p->pre, p->dy, p->dx}) ||
+      !all_aligned(elem_bytes(p->bias_dtype), {p->bias, p->dbias}) || !all_aligned(elem_bytes(p->dkernel_dtype), {p->dkernel}) ||
+      !all_aligned(sizeof(uint64_t), {p->rng}) || !all_aligned(sizeof(int32_t), {p->status}) ||
+      !all_aligned(kWorkspaceAlign, {p->workspace}))
+    return SSM_ERR_ALIGN;
   return SSM_OK;
 }
 
 static size_t round256(size_t v) { return (v + 255) / 256 * 256; }
-static size_t elem_bytes(int dtype) { return dtype == SSM_BF16 ? 2 : 4; }
 static DropRng drop_rng(const ssm_dense_params_t* p) { return {p->seed, p->offset, p->rng, (uint32_t)p->drop}; }
 static int pad8(int n) { return (n + 7) / 8 * 8; }
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }

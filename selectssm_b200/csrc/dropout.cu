@@ -200,6 +200,9 @@ static int check_drop(const ssm_dropout_params_t* p) {
       (p->dy_stride && p->dy_stride < p->dim))
     return SSM_ERR_SHAPE;
   if (p->dtype != SSM_F32 && p->dtype != SSM_BF16) return SSM_ERR_DTYPE;
+  if (!all_aligned(p->dtype == SSM_BF16 ? 2 : 4, {p->x, p->residual, p->y, p->dy, p->dx}) ||
+      !all_aligned(sizeof(uint64_t), {p->rng}))
+    return SSM_ERR_ALIGN;
   return SSM_OK;
 }
 

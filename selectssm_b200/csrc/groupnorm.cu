@@ -880,6 +880,11 @@ static int check_gn(const ssm_group_norm_params_t* p) {
       p->batch > 0x7fffffff / p->groups || p->seqlen > (1ll << 40) || p->act < SSM_ACT_NONE || p->act > SSM_ACT_RELU)
     return SSM_ERR_SHAPE;
   if (p->dtype != SSM_F32 && p->dtype != SSM_BF16) return SSM_ERR_DTYPE;
+  // x, y, dy and dx of whole vectors a row are accessed by vectors
+  if (!all_aligned(p->dim % 8 == 0 ? 16 : p->dtype == SSM_BF16 ? 2 : 4, {p->x, p->y, p->dy, p->dx}) ||
+      !all_aligned(sizeof(float), {p->scale, p->bias, p->dscale, p->dbias}) || !all_aligned(sizeof(float2), {p->stats}) ||
+      !all_aligned(kWorkspaceAlign, {p->workspace}))
+    return SSM_ERR_ALIGN;
   return SSM_OK;
 }
 
@@ -1127,7 +1132,6 @@ int ssm_group_norm_act_fwd(const ssm_group_norm_params_t* p, ssm_stream_t stream
   if (st) return st;
   if (p->batch == 0 || p->seqlen == 0) return SSM_OK;
   if (!p->x || !p->y) return SSM_ERR_NULL;
-  if (gn_vector(p) && (!aligned16(p->x) || !aligned16(p->y))) return SSM_ERR_ALIGN;
   const size_t need = ssm_group_norm_fwd_workspace_bytes(p);
   if (need && (!p->workspace || p->workspace_bytes < need)) return SSM_ERR_WORKSPACE;
   st = bind_device(p->x);
@@ -1161,7 +1165,6 @@ int ssm_group_norm_act_bwd(const ssm_group_norm_params_t* p, ssm_stream_t stream
     return SSM_OK;
   }
   if (!p->x || !p->dy || !p->dx || !p->stats) return SSM_ERR_NULL;
-  if (gn_vector(p) && (!aligned16(p->x) || !aligned16(p->dy) || !aligned16(p->dx))) return SSM_ERR_ALIGN;
   if (!p->workspace || p->workspace_bytes < ssm_group_norm_bwd_workspace_bytes(p)) return SSM_ERR_WORKSPACE;
   st = bind_device(p->x);
   if (st) return st;

@@ -3,6 +3,8 @@
 #pragma once
 
 #include <cstdint>
+#include <initializer_list>
+
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -11,6 +13,13 @@
 namespace ssm {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// whether all start at a multiple of `bytes`, a power of two (null pointers do)
+inline bool all_aligned(size_t bytes, std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) return false;
+  return true;
+}
+constexpr size_t kWorkspaceAlign = 256;
 
 __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
   const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);

@@ -161,3 +161,51 @@ def test_dropout_rng_without_the_fused_block_is_refused():
     m = BidirectionalMamba(32, hidden_features=16, expansion_factor=1, mlp_layer=True)
     with pytest.raises(ValueError, match="fused_block"):
         m(torch.zeros(1, 8, 32), train=True, dropout_rng=(1, 2))
+
+
+def test_abi_refuses_misaligned_pointers():
+    """Which would fault in the kernels' wide accesses."""
+    lib = _lib.load()
+
+    def code(f, p):
+        return f(ctypes.byref(p), None)
+
+    d = _lib.SSMDenseParams()
+    d.rows, d.fin, d.fout = 40, 8, 8
+    d.x = d.kernel = d.y = d.dy = d.dx = 0x1000
+    for f, query in ((lib.ssm_dense_act_fwd, lib.ssm_dense_fwd_workspace_bytes),
+                     (lib.ssm_dense_act_bwd, lib.ssm_dense_bwd_workspace_bytes)):
+        d.workspace, d.workspace_bytes = 0x1010, query(ctypes.byref(d)) + 4096
+        assert code(f, d) == _lib.SSM_ERR_ALIGN
+        d.workspace = None
+        for field in ("x", "kernel", "residual", "y", "pre", "dy", "dx", "bias", "dkernel", "dbias", "status"):
+            before = getattr(d, field)
+            setattr(d, field, 0x1002)
+            assert code(f, d) == _lib.SSM_ERR_ALIGN, field
+            setattr(d, field, before)
+        d.rng = 0x1004
+        assert code(f, d) == _lib.SSM_ERR_ALIGN
+        d.rng = None
+    g = _lib.SSMGroupNormParams()
+    g.batch, g.seqlen, g.dim, g.groups = 2, 5, 33, 3
+    g.x = g.y = g.dy = g.dx = g.stats = 0x1000
+    for f, query in ((lib.ssm_group_norm_act_fwd, lib.ssm_group_norm_fwd_workspace_bytes),
+                     (lib.ssm_group_norm_act_bwd, lib.ssm_group_norm_bwd_workspace_bytes)):
+        g.workspace, g.workspace_bytes = 0x1010, query(ctypes.byref(g)) + 4096
+        assert code(f, g) == _lib.SSM_ERR_ALIGN
+        g.workspace = None
+        for field, bad in (("x", 0x1002), ("y", 0x1002), ("dy", 0x1002), ("dx", 0x1002), ("scale", 0x1002),
+                           ("bias", 0x1002), ("stats", 0x1004), ("dscale", 0x1002), ("dbias", 0x1002)):
+            before = getattr(g, field)
+            setattr(g, field, bad)
+            assert code(f, g) == _lib.SSM_ERR_ALIGN, field
+            setattr(g, field, before)
+    p = _lib.SSMDropoutParams()
+    p.rows, p.dim = 2, 8
+    p.x = p.y = p.dy = p.dx = 0x1000
+    for f in (lib.ssm_dropout_act_fwd, lib.ssm_dropout_act_bwd):
+        for field, bad in (("x", 0x1002), ("residual", 0x1002), ("y", 0x1002), ("dy", 0x1002), ("dx", 0x1002), ("rng", 0x1004)):
+            before = getattr(p, field)
+            setattr(p, field, bad)
+            assert code(f, p) == _lib.SSM_ERR_ALIGN, field
+            setattr(p, field, before)
