@@ -793,3 +793,84 @@ def test_dense_fp32_infinities_through_the_epilogue(cuda, sizes, act):
         assert torch.equal(y[~hit], clean[~hit])
         sure = hit & ~((u.abs() > 1e30) & torch.isfinite(u))  # (a sum next to the largest value may pass it)
         _classes_agree(y[sure], want[sure])
+
+
+# Sizes of which the product kernels make pairs of CTAs, several tiles a CTA (or pair) in a row, and
+# cut K loops in bf16, all with ragged edges (tiles are 128 x 128 a CTA, of 148, or 256 x 256 a pair, of 74):
+#   20001 x 1536 -> 776   y: pairs, 4.3 tiles each, last column tile 8 wide; dx: pairs, 6.4; dW: pairs, K in 3 parts
+#   16500 x 264 -> 1000   y: pairs, 3.5; dx: single CTAs, 2.6; dW: single, K in 6 parts
+#   20001 x 1031 -> 777   y and dx: pairs, rows that start anywhere; dW: single, K in 2 parts
+#   40000 x 304 -> 304    y and dx: single CTAs, 6.3 tiles each; dW: K in 16 parts
+#   768 x 32000 -> 1536   y: pairs, K in 4 parts joined with the epilogue; dx: pairs, 5.1; dW: pairs, 10.1
+@pytest.mark.parametrize("sizes,act,rate,res_stride", [
+    ((20001, 1536, 776), None, 0.1, 776), ((20001, 1536, 776), "silu", 0.0, 779), ((16500, 264, 1000), "silu", 0.1, None),
+    ((20001, 1031, 777), "gelu", 0.3, 777), ((40000, 304, 304), None, 0.2, 312), ((768, 32000, 1536), "silu", 0.1, 1536)])
+def test_dense_bf16_of_many_tiles(cuda, sizes, act, rate, res_stride):
+    from selectssm_b200 import dense_act
+    M, K, N = sizes
+    dtype = torch.bfloat16
+    torch.manual_seed(23)
+    x = torch.randn(M, K, device=cuda).to(dtype).requires_grad_()
+    w = (torch.randn(K, N, device=cuda) / K ** 0.5).to(dtype).requires_grad_()
+    b = torch.randn(N, device=cuda).to(dtype).requires_grad_()
+    res = torch.randn(M, res_stride, device=cuda).to(dtype)[:, :N] if res_stride else None
+    dy = torch.randn(M, N, device=cuda).to(dtype)
+    keep = keep_mask(M, N, rate, 31, 7) if rate else None
+    runs = []
+    for _ in range(2):
+        y = dense_act(x, w, b, activation=act, residual=res, rate=rate, rng=(31, 7))
+        runs.append((y.detach(), *torch.autograd.grad(y, (x, w, b), dy)))
+    assert all(torch.equal(p, q) for p, q in zip(*runs))
+    want, tol = dense64(x, w, b, res, act, rate, keep, dy, dtype)
+    for name, got in zip(("y", "dx", "dw", "db"), runs[0]):
+        assert_within(got, want[name], tol[name], name)
+
+
+def _needs(gigabytes):
+    if torch.cuda.mem_get_info()[0] < gigabytes << 30:
+        pytest.skip(f"needs {gigabytes} GB of the GPU's memory")
+
+
+def test_dense_counters_beyond_32_bits(cuda):
+    """Three dropout counters a row, more than 2^32 of them, and 24e9 outputs."""
+    from selectssm_b200 import dense_act
+    torch.cuda.empty_cache()
+    _needs(90)
+    torch.manual_seed(24)
+    rows, fin, fout, tail = (1 << 32) // 3 + 60, 8, 17, 100
+    x = torch.zeros(rows, fin, device=cuda, dtype=torch.bfloat16)
+    x[-tail:] = torch.randn(tail, fin, device=cuda).bfloat16()
+    w, b = torch.randn(fin, fout, device=cuda).bfloat16(), torch.randn(fout, device=cuda).bfloat16()
+    y = dense_act(x, w, b, rate=0.5, rng=(11, 12))[-tail:].double()
+    idx = np.arange((rows - tail) * 3, rows * 3, dtype=np.uint64)
+    assert idx[0] < 1 << 32 < idx[-1]
+    c = philox4x32_10([idx & np.uint64(0xFFFFFFFF), idx >> np.uint64(32), np.full_like(idx, 12), np.zeros_like(idx)], (11, 0))
+    bits = np.stack([(c[j // 2] >> np.uint64(16 * (j % 2))) & np.uint64(0xFFFF) for j in range(8)], axis=1)
+    keep = torch.from_numpy(np.ascontiguousarray(bits.reshape(tail, 24)[:, :fout] >= 32768)).to(cuda)
+    want = drop64(x[-tail:].double() @ w.double() + b.double(), 0.5, keep)
+    assert_within(y, want, 32 * U32 * (x[-tail:].double().abs() @ w.double().abs() + b.double().abs()) + stored(want, torch.bfloat16))
+    del x, y
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape,groups", [((3, 1500001, 512), 64), ((70000001, 1, 32), 4)])
+def test_group_norm_beyond_32_bit_offsets(cuda, shape, groups):
+    """More than 2^31 elements, in the split and in the held form: the last channels' group of the last rows."""
+    from selectssm_b200 import group_norm_act
+    torch.cuda.empty_cache()
+    _needs(60)
+    torch.manual_seed(25)
+    B, L, D = shape
+    cg = D // groups
+    x = torch.empty(shape, device=cuda, dtype=torch.bfloat16).normal_().requires_grad_()
+    dy = torch.empty(shape, device=cuda, dtype=torch.bfloat16).normal_()
+    scale, bias = 1 + 0.2 * torch.randn(D, device=cuda), 0.3 * torch.randn(D, device=cuda)
+    y = group_norm_act(x, scale, bias, groups=groups, activation="silu")
+    dx, = torch.autograd.grad(y, x, dy)
+    last = (slice(-2, None), slice(None), slice(-cg, None))
+    want, tol = gn64(x[last], scale[-cg:].double(), bias[-cg:].double(), 1, 1e-6, "silu", dy[last].contiguous())
+    for name, got in (("y", y), ("dx", dx)):
+        got = got.detach()[last]
+        assert_within(got, want[name], tol[name] + stored(want[name], torch.bfloat16), name)
+    del x, y, dx, dy
+    torch.cuda.empty_cache()
