@@ -1,4 +1,4 @@
-"""Trains one BidirectionalMamba block with group norm and an MLP with dropout, every part in this package's kernels.
+"""Trains one BidirectionalMamba block with group norm and an MLP with dropout in its fused form.
 
 The task is synthetic: from a one-hot DNA sequence, predict at each position the base three to the left.
 

@@ -294,7 +294,9 @@ SSM_API int ssm_group_norm_act_bwd(const ssm_group_norm_params_t* p, ssm_stream_
  * y = residual + act(drop(x W + bias)), x (rows, fin), W (fin, fout) as Flax's
  * Dense kernel, drop() as in ssm_dropout_act_fwd over rows of fout columns.
  * The backward writes those of dx, dkernel and dbias that are not NULL; the
- * residual's gradient is dy itself.  Sums are held in fp32; with bf16 the
+ * residual's gradient is dy itself.  Sums are held in fp32 (the tensor cores cut
+ * what an addition cannot hold; fp32 operands' sums start afresh often enough to
+ * keep fp32 accuracy); with bf16 the
  * operands of the products (x, W, and in the backward the gradient of the
  * pre-activation) are bf16.  Tensors may start at any element, rng at 8 bytes.  */
 typedef struct ssm_dense_params {

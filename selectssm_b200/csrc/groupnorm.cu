@@ -572,7 +572,8 @@ __device__ __forceinline__ float2 gn_peer(const float2* p, int cta) {
 // 64 x 2048 x 768 bf16: 95 us for 403 MB, 4.2 TB/s.  A CTA reads its part, meets its
 // cluster, and writes, and what a thread does once (80 registers of constants, two
 // sums over the CTA) stands against 26 vectors of its own: the phases of four CTAs
-// an SM overlap only in part.
+// an SM overlap only in part.  The backward in bf16 with an activation has too few
+// registers (88 to 124 bytes spilled).
 template <typename T, int V, int ACT, bool BWD, bool SHORT>
 __global__ void __launch_bounds__(kHoldThreads, 3) gn_hold_kernel(const GnArgs p, const GnHold h) {
   using Vec = GnVec<T, V>;

@@ -277,10 +277,11 @@ class BidirectionalMamba(nn.Module):
     With ``concatenate_fwd_rev`` both SSM scans, their D skips and the gates run
     in one kernel launch writing the concatenated (B, L, 2*ED) result.
 
-    With ``fused_block`` the rest of the block runs in this package's kernels
-    too: the group norm (``norm_type="group"``), the projections with their
-    biases and residuals, and the MLP with dropout and activation in the
-    products' epilogues (:mod:`selectssm_b200.block_ops`).  Values agree with the
+    With ``fused_block`` these run in this package's kernels too: the group norm
+    (``norm_type="group"``), in_proj and out_proj with their biases and the
+    residual, and the MLP with dropout and activation in the products' epilogues
+    (:mod:`selectssm_b200.block_ops`); layer and batch norm and the projections
+    inside SelectiveSSM stay as they are.  Values agree with the
     unfused block up to rounding; the dropout masks come from ``dropout_rng`` of
     the call instead of PyTorch's generator."""
 
