@@ -347,9 +347,10 @@ def dense_act(x, kernel, bias=None, activation=None, residual=None, rate=0.0, rn
     x: (..., fin), float32 or bfloat16, rows at any stride; kernel: Flax's
     (fin, fout), converted to x's type; bias: (fout,); ``residual`` broadcasts
     to the (..., fout) output and is converted to x's type, in which the sum is
-    returned.  Products are summed in fp32; float32 operands keep fp32 accuracy.  ``rate`` and ``rng`` as in :func:`dropout_act`, over
-    rows of fout columns.  For the backward an activation's input is kept in
-    x's type, and the gradient before the two products is rounded to it.
+    returned.  Products are summed in fp32; float32 operands keep fp32 accuracy.
+    ``rate`` and ``rng`` as in :func:`dropout_act`, over rows of fout columns.
+    For the backward an activation's input is kept in x's type, and the gradient
+    before the two products is rounded to it.
 
     The kernels' waits are bounded.  Should one give up, the outputs that it held
     up are NaN and the next dense call on the device raises SSMLibraryError."""

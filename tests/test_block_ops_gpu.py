@@ -874,3 +874,55 @@ def test_group_norm_beyond_32_bit_offsets(cuda, shape, groups):
         assert_within(got, want[name], tol[name] + stored(want[name], torch.bfloat16), name)
     del x, y, dx, dy
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("sizes", [(17, 1, 1), (33, 3, 1), (1000, 128, 1), (17, 1, 300), (50, 2, 7), (20000, 1, 9)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_dense_smallest_widths(cuda, dtype, sizes, wide):
+    """One column in or out past the few-row form, from rows of their own and from slices TMA can address."""
+    from selectssm_b200 import dense_act
+    M, K, N = sizes
+    torch.manual_seed(26)
+    x = torch.randn(M, (K + 15) // 8 * 8 if wide else K, device=cuda).to(dtype)[:, :K].requires_grad_()
+    w, b = torch.randn(K, N, device=cuda).to(dtype).requires_grad_(), torch.randn(N, device=cuda).to(dtype).requires_grad_()
+    dy = torch.randn(M, 24 if wide else N, device=cuda).to(dtype)[:, :N] if N < 24 else torch.randn(M, N, device=cuda).to(dtype)
+    for act, rate in (("silu", 0.25), (None, 0.0)):
+        keep = keep_mask(M, N, rate, 2, 3) if rate else None
+        y = dense_act(x, w, b, activation=act, rate=rate, rng=(2, 3))
+        grads = torch.autograd.grad(y, (x, w, b), dy)
+        want, tol = dense64(x, w, b, None, act, rate, keep, dy, dtype)
+        for name, got in zip(("y", "dx", "dw", "db"), (y.detach(), *grads)):
+            assert_within(got, want[name], tol[name], name)
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_dense_with_everything_dropped(cuda, dtype, rows):
+    from selectssm_b200 import dense_act
+    x, w = torch.randn(rows, 40, device=cuda).to(dtype), torch.randn(40, 24, device=cuda).to(dtype)
+    x[1, 1] = float("inf")
+    x.requires_grad_(), w.requires_grad_()
+    res = torch.randn(rows, 24, device=cuda).to(dtype)
+    y = dense_act(x, w, activation="silu", residual=res, rate=1.0, rng=(1, 1))
+    assert torch.equal(y, res)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert bool((dx == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", [((2, 50, 1), 1), ((5, 1, 1), 1), ((3, 1, 2), 2), ((1, 200001, 1), 1), ((2, 1), 1)])
+def test_group_norm_smallest_widths(cuda, dtype, shape, groups):
+    from selectssm_b200 import group_norm_act
+    torch.manual_seed(27)
+    D = shape[-1]
+    x = torch.randn(shape, device=cuda).to(dtype).requires_grad_()
+    scale, bias = torch.randn(D, device=cuda).requires_grad_(), torch.randn(D, device=cuda).requires_grad_()
+    dy = torch.randn(shape, device=cuda).to(dtype)
+    y = group_norm_act(x, scale, bias, groups=groups, activation="gelu")
+    y.backward(dy)
+    want, tol = gn64(x, scale.detach().double(), bias.detach().double(), groups, 1e-6, "gelu", dy)
+    for name, got in (("y", y.detach()), ("dx", x.grad)):
+        assert_within(got.reshape(want[name].shape), want[name], tol[name] + stored(want[name], dtype), name)
+    for name, got in (("dscale", scale.grad), ("dbias", bias.grad)):
+        assert_within(got, want[name], tol[name] + 1e-30, name)
